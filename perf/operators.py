@@ -10,7 +10,7 @@ Families ("kind"):
             gradient of a training step                 mrsa.rotary_qk
     append  rows of new tokens rotated and written into the pages of several
             sequences                                   mrsa.paged_cache_append
-    attend  the newest rows of each sequence against its pages
+    attend  a block of rows of each sequence against its pages
                                                         mrsa.paged_cached_attention
     pages   pages copied inside a pool, K and V of every layer
                                                         mrsa.copy_cache_pages
@@ -46,7 +46,7 @@ def _append(**more):
 def _attend(**more):
     return {"kind": "attend", "batch": 1, "rows": 1, "len": 1024, "heads": 28, "kv_heads": 4,
             "dim": 128, "page": 64, "window": -1, "causal": False, "type": "bf16",
-            "ragged": False, **more}
+            "ragged": False, "after": 0, **more}
 
 
 def _pages(**more):
@@ -75,9 +75,9 @@ def listed():
         _attend(name="attend_64x8k", batch=64, len=8192, ragged=True),
         # a decode block against a long cache: the matrix products
         _attend(name="attend_block_64k", rows=32, len=65503),
-        # decode blocks of a sliding-window layer, small pages
+        # decode blocks of a sliding-window layer with a block cached behind them, small pages
         _attend(name="attend_window", batch=8, rows=32, len=16384, window=1280, page=16,
-                ragged=True),
+                ragged=True, after=32),
         # the last, shared pages of eight forked sequences
         _pages(name="pages_fork", count=8),
         # a pool of many sequences made dense again
@@ -121,7 +121,7 @@ def draw(rng):
         return _attend(batch=batch, rows=rows, len=_log_int(rng, rows, most), heads=heads,
                        kv_heads=kv_heads, dim=dim, page=page,
                        window=rng.choice([-1, -1, -1, 319, 1280]), causal=rng.random() < 0.3,
-                       type=type_, ragged=rng.random() < 0.6)
+                       type=type_, ragged=rng.random() < 0.6, after=rng.choice([0, 0, 0, 100]))
     return _pages(layers=rng.choice([1, 7, 28]), count=_log_int(rng, 1, 300), kv_heads=kv_heads,
                   dim=dim, page=rng.choice([16, 32, 64]) if kv_heads < 8 else 16, type=type_)
 
@@ -193,7 +193,7 @@ def prepare(case, seed):
         s["q"], s["k"], s["v"] = normal(B, L, H, D), normal(B, L, Hkv, D), normal(B, L, Hkv, D)
         s["cos"], s["sin"] = _tables(c["reach"], c["part"], device)
         # the rows come after a cached prefix of another length for each sequence
-        prefix = [(37 * b + seed % 101) % 500 for b in range(B)]
+        prefix = [(37 * b + 61) % 500 for b in range(B)]
         pool, s["page_table"] = _paging([p + t for p, t in zip(prefix, tokens)], c["page"], gen,
                                         device, 3)
         s["k_pages"] = normal(pool, c["page"], Hkv, D)
@@ -210,6 +210,8 @@ def prepare(case, seed):
     s["v_pages"] = normal(pool, c["page"], Hkv, D)
     s["cache_lens"] = torch.tensor(lens, dtype=torch.int32, device=device)
     s["max_len"] = max(lens)
+    # the block is the newest rows, or has some rows cached behind it
+    s["query_starts"] = s["cache_lens"] - c["rows"] - c["after"] if c["after"] else None
     return s
 
 
@@ -281,20 +283,21 @@ def _run_attend(s):
 
         return mrsa.paged_cached_attention(s["q"], s["k_pages"], s["v_pages"], s["page_table"],
                                            s["cache_lens"], causal=c["causal"], window=window,
+                                           query_starts=s["query_starts"],
                                            max_len=s["max_len"])
     q, lens, page = s["q"], s["cache_lens"].long()[:, None], c["page"]
     B, R, H, D = q.shape
     Hkv, G = c["kv_heads"], H // c["kv_heads"]
     # the last rows of each sequence that any of its queries can see
-    span = s["max_len"] if window is None else min(s["max_len"], R + window)
+    span = s["max_len"] if window is None else min(s["max_len"], R + c["after"] + window)
     j = lens - span + torch.arange(span, device=q.device)                       # [B, span]
     there = j >= 0
     at = j.clamp(min=0)
     pages = s["page_table"].long().gather(1, at // page)
     k = s["k_pages"][pages, at % page].permute(0, 2, 3, 1).contiguous().float()  # [B, Hkv, D, span]
     v = s["v_pages"][pages, at % page].permute(0, 2, 1, 3).contiguous().float()  # [B, Hkv, span, D]
-    p = lens - R + torch.arange(R, device=q.device)                             # [B, R]
-    seen = there[:, None, :].expand(B, R, span)
+    p = lens - R - c["after"] + torch.arange(R, device=q.device)                # [B, R]
+    seen = there[:, None, :] & (p >= 0)[:, :, None]
     if c["causal"]:
         seen = seen & (j[:, None, :] <= p[:, :, None])
     if window is not None:
@@ -339,18 +342,18 @@ def _visible(c):
     """Keys that some query of each sequence sees, and pairs of a query and a key that it sees."""
     keys = pairs = 0
     for n in _lens(c):
-        first = n
+        first, last = n, 0
         for i in range(c["rows"]):
-            p = n - c["rows"] + i
-            lo, hi = 0, n - 1
+            p = n - c["rows"] - c["after"] + i
+            lo, hi = 0, n - 1 if p >= 0 else -1
             if c["causal"]:
                 hi = min(hi, p)
             if c["window"] >= 0:
                 lo, hi = max(lo, p - c["window"]), min(hi, p + c["window"])
             if hi >= lo:
                 pairs += hi - lo + 1
-                first = min(first, lo)
-        keys += n - first
+                first, last = min(first, lo), max(last, hi + 1)
+        keys += max(0, last - first)
     return keys, pairs
 
 
@@ -419,8 +422,9 @@ def exact(case, seed):
     for b, n in enumerate(_lens(c)):
         own_pages = s["page_table"][b, :-(-n // c["page"])].long()
         at = torch.arange(n, device=out.device)
-        far = at[None, :] - torch.arange(n - R, n, device=out.device)[:, None]   # j - p
-        seen = torch.ones_like(far, dtype=torch.bool)
+        p0 = n - R - c["after"]
+        far = at[None, :] - torch.arange(p0, p0 + R, device=out.device)[:, None]  # j - p
+        seen = (at[None, :] - far) >= 0
         if c["causal"]:
             seen &= far <= 0
         if c["window"] >= 0:
