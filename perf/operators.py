@@ -118,10 +118,13 @@ def draw(rng):
         # no more bytes than 64 sequences of 8192, no more products than a block at 64k
         most = min(131072, 64 * 8192 * 4 * 128 / (batch * kv_heads * dim),
                    32 * 65503 * 28 * 128 / (batch * rows * heads * dim))
-        return _attend(batch=batch, rows=rows, len=_log_int(rng, rows, most), heads=heads,
-                       kv_heads=kv_heads, dim=dim, page=page,
-                       window=rng.choice([-1, -1, -1, 319, 1280]), causal=rng.random() < 0.3,
-                       type=type_, ragged=rng.random() < 0.6, after=rng.choice([0, 0, 0, 100]))
+        length = _log_int(rng, rows, most)
+        # (the shortest of ragged sequences, an eighth as long, still holds its block)
+        after = rng.choice([0, 0, 0, 100]) if length > 8 * (rows + 100) else 0
+        return _attend(batch=batch, rows=rows, len=length, heads=heads, kv_heads=kv_heads, dim=dim,
+                       page=page, window=rng.choice([-1, -1, -1, 319, 1280]),
+                       causal=rng.random() < 0.3, type=type_, ragged=rng.random() < 0.6,
+                       after=after)
     return _pages(layers=rng.choice([1, 7, 28]), count=_log_int(rng, 1, 300), kv_heads=kv_heads,
                   dim=dim, page=rng.choice([16, 32, 64]) if kv_heads < 8 else 16, type=type_)
 
