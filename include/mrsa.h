@@ -31,6 +31,11 @@ extern "C" {
 #define MRSA_ERR_LAUNCH 3           /* the HIP runtime rejected a launch */
 #define MRSA_ERR_SCRATCH 4          /* exceeds a no-allocation entry point's static buffer */
 
+/* Element types of the entry points that take more than bf16. */
+#define MRSA_DTYPE_BF16 0
+#define MRSA_DTYPE_FP16 1
+#define MRSA_DTYPE_FP32 2
+
 /* Human-readable text for a status code (static storage). */
 const char* mrsa_status_string(int status);
 
@@ -895,6 +900,104 @@ int mrsa_candidate_token_scores_fwd(const void* q, const void* kv_frags, const i
                                     int64_t kv_len, int64_t q_heads, int64_t kv_heads,
                                     int64_t head_dim, int64_t topk, int64_t chunk_size,
                                     float sm_scale, float* scores, void* stream);
+
+/*
+ * Rotary positions of query and key heads (the rotation of rope_qkv, for any
+ * head layout): with c, s = row `position` of the tables, each pair (x1, x2)
+ * of a head's first rotary_dim dims becomes
+ *   (x1 c - x2 s, x2 c + x1 s);   inverse: s -> -s, the gradient.
+ * Pairs are dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved;
+ * dims past rotary_dim are copied.  fp32 arithmetic, one rounding.
+ *   q: [batch, seq_len, q_heads, head_dim], k: [.., kv_heads, ..] of `dtype`
+ *     (MRSA_DTYPE_*), with batch, row and head strides in elements and a dense
+ *     last dim (strides may be 0); a tensor with 0 heads may be NULL
+ *   cos_table, sin_table: fp32 [table_rows, rotary_dim / 2]
+ *   positions: optional int64 [batch, seq_len] with strides (NULL: row i is
+ *     at position i); a position outside [0, table_rows) makes its rows'
+ *     rotated dims NaN
+ *   q_out, k_out: dense, not overlapping the inputs
+ * Limits: batch * seq_len < 2^31, head_dim <= 4096.
+ */
+int mrsa_rotary_fwd(const void* q, int64_t q_batch_stride, int64_t q_row_stride,
+                    int64_t q_head_stride, const void* k, int64_t k_batch_stride,
+                    int64_t k_row_stride, int64_t k_head_stride, const float* cos_table,
+                    const float* sin_table, int64_t table_rows, const int64_t* positions,
+                    int64_t positions_batch_stride, int64_t positions_row_stride, int64_t batch,
+                    int64_t seq_len, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                    int64_t rotary_dim, int32_t dtype, int32_t interleaved, int32_t inverse,
+                    void* q_out, void* k_out, void* stream);
+
+/*
+ * New rows into the pages of a K/V cache, rotated on the way: k rows turned as
+ * by mrsa_rotary_fwd, v rows as they are, row (b, l) to slot s = slots[b, l]
+ * of sequence b, i.e. row s % page_size of page page_table[b, s / page_size].
+ * Rows whose slot is negative or past the table, or whose page lies outside
+ * [0, num_pages), are not written.  q (optional, 0 heads) is turned into q_out
+ * for every row.  rotary_dim 0: nothing is turned.
+ *   q, k, v, tables, positions: as in mrsa_rotary_fwd
+ *   slots: int64 [batch, seq_len] with strides; two rows of one call must not
+ *     name the same cache row (either's units remain)
+ *   page_table: int32 [batch, table_pages], row stride page_table_stride
+ *   k_pages, v_pages (in/out): [num_pages, page_size, kv_heads, head_dim] in
+ *     any order given by page, slot and head strides, dense last dim
+ * Limits: page_size a power of two, as mrsa_rotary_fwd otherwise.
+ */
+int mrsa_paged_append_fwd(
+    const void* q, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
+    const void* k, int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride,
+    const void* v, int64_t v_batch_stride, int64_t v_row_stride, int64_t v_head_stride,
+    const float* cos_table, const float* sin_table, int64_t table_rows, const int64_t* positions,
+    int64_t positions_batch_stride, int64_t positions_row_stride, const int64_t* slots,
+    int64_t slots_batch_stride, int64_t slots_row_stride, const int32_t* page_table,
+    int64_t page_table_stride, int64_t table_pages, int64_t num_pages, int64_t page_size,
+    void* k_pages, int64_t k_page_stride, int64_t k_slot_stride, int64_t k_pages_head_stride,
+    void* v_pages, int64_t v_page_stride, int64_t v_slot_stride, int64_t v_pages_head_stride,
+    int64_t batch, int64_t seq_len, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+    int64_t rotary_dim, int32_t dtype, int32_t interleaved, void* q_out, void* stream);
+
+/*
+ * Attention of a block of rows of each sequence against its pages, with
+ * natural-log LSE.  Sequence b has n = cache_lens[b] rows in the cache, the
+ * query rows' own among them (n is cut to max_len and to the table's rows); row
+ * i sits at position p = query_starts[b] + i (NULL: n - q_len + i, the newest
+ * rows) and sees the keys j of [0, n) in mapped pages (page_table entries of
+ * [0, num_pages)), j <= p if causal, |j - p| <= window if window >= 0.  A row
+ * at a position outside [0, n) is padding.  Padding, and a row that sees no
+ * key, give out = 0 and lse = -inf.
+ *   q: [batch, q_len, q_heads, head_dim] with strides, bf16 or fp16 (dtype)
+ *   k_pages, v_pages, page_table: as in mrsa_paged_append_fwd
+ *   cache_lens: int32 [batch]; query_starts: optional int32 [batch]
+ *   out: [batch, q_len, q_heads, head_dim]; lse: fp32 [batch, q_len, q_heads]
+ *   parts (1..1024): pieces that the visible span is cut into, joined by a
+ *     second kernel over fp32 partials in `workspace`
+ *     (mrsa_paged_attention_workspace_bytes; 16-byte aligned; unused for 1)
+ *   max_len: bound of cache_lens; sm_scale: finite and > 0
+ * Limits: head_dim 64 or 128, page_size a power of two from 16 on, pointers
+ * 16-byte aligned and strides multiples of 8 elements, max_len < 2^29.
+ */
+int64_t mrsa_paged_attention_workspace_bytes(int64_t batch, int64_t q_len, int64_t q_heads,
+                                             int64_t head_dim, int64_t parts);
+int mrsa_paged_attention_fwd(
+    const void* q, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
+    const void* k_pages, int64_t k_page_stride, int64_t k_slot_stride, int64_t k_head_stride,
+    const void* v_pages, int64_t v_page_stride, int64_t v_slot_stride, int64_t v_head_stride,
+    const int32_t* page_table, int64_t page_table_stride, int64_t table_pages, int64_t num_pages,
+    int64_t page_size, const int32_t* cache_lens, const int32_t* query_starts, int64_t max_len, int64_t batch, int64_t q_len,
+    int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t dtype, int32_t causal,
+    int64_t window, float sm_scale, int64_t parts, void* workspace, int64_t workspace_bytes,
+    void* out, float* lse, void* stream);
+
+/*
+ * Page src[i] copied to page dst[i], K and V, in every layer.  Strides and
+ * page_bytes in bytes, multiples of 16, a page's bytes contiguous; src and dst
+ * are host arrays of `count` page indices, read before the call returns.
+ * MRSA_ERR_INVALID_ARGUMENT, and nothing copied, for an index outside
+ * [0, num_pages), a destination named twice or one that is also a source.
+ */
+int mrsa_copy_pages(void* k_pages, int64_t k_layer_stride, int64_t k_page_stride, void* v_pages,
+                    int64_t v_layer_stride, int64_t v_page_stride, int64_t layers,
+                    int64_t num_pages, int64_t page_bytes, int64_t count, const int64_t* src,
+                    const int64_t* dst, void* stream);
 
 /*
  * Self-test of the matrix-core lane layout every kernel above relies on:

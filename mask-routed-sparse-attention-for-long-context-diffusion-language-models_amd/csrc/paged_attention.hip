@@ -1,0 +1,550 @@
+// Attention of the newest rows of several sequences against a paged K/V cache,
+// split over the cache's length and joined.
+//
+// Sequence b holds n = cache_lens[b] rows; its query row i sits at position
+// p = query_starts[b] + i (by default the query rows are the last ones).  A
+// row with p in [0, n) sees the keys j of [0, n) with j <= p if causal,
+// |j - p| <= window if windowed, that lie in a mapped page (an entry of the
+// page table outside [0, num_pages) holds no keys); other rows are padding:
+//   s_j = scale q . k_j,  lse = log sum_j exp s_j,  out = sum_j exp(s_j - lse) v_j,
+// and out = 0, lse = -inf for a row that sees none.
+//
+// The G query heads of a KV head and the q_len rows are matrix columns
+// (column m: row m / G, head m % G), 16 to a tile.  A wave streams tiles of 32
+// keys with a running maximum and sum per column:
+//   S^T = K . Q^T    K rows straight from HBM to registers (operand A)
+//   O^T += V^T . P^T P^T is S^T's own register layout (operand B); V goes
+//                    through the wave's own piece of LDS and comes back
+//                    transposed (gfx950's transposing reads).
+// Products of 16-bit inputs are exact, sums fp32; P is rounded to the inputs'
+// type as a matrix operand (the sum uses the unrounded values), which is half
+// a step of that type per term.  The maximum moves only when a score passes it
+// by more than 8 (base 2), so that P stays below 2^8 and the accumulators are
+// rarely rescaled.
+#include "chunk_tile.h"
+#include "mrsa_device.h"
+
+using namespace mrsa;
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kTile = 32;                  // keys of a wave's tile
+constexpr int kStep = kWaves * kTile;      // keys of a workgroup's round
+constexpr int kMaxParts = 1024;
+constexpr int kFar = 1 << 29;              // bound of positions and windows: their sums fit 32 bits
+constexpr float kSlack = 8.f;              // base-2 growth before the maximum moves
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+struct Bf16 {
+  static __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
+    return mfma_bf16_16x16x32(a, b, c);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  static __device__ __forceinline__ float value(uint32_t bits) { return bf16_to_f32(bits); }
+  static constexpr uint32_t kExp = 0x7f80u;
+};
+struct Fp16 {
+  static __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    f32x2_t v = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+  }
+  static __device__ __forceinline__ float value(uint32_t bits) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+  }
+  static constexpr uint32_t kExp = 0x7c00u;
+};
+
+struct PagedArgs {
+  const uint16_t* q;
+  int64_t q_sb, q_sl, q_sh;
+  const uint16_t* k;
+  int64_t k_sp, k_sr, k_sh;   // page, row, head strides
+  const uint16_t* v;
+  int64_t v_sp, v_sr, v_sh;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_width, page_shift, num_pages;
+  const int32_t* lens;
+  const int32_t* starts;      // optional
+  int max_len;
+  int B, Lq, Hq, Hkv, G, M;   // M = Lq G columns
+  int causal, window;         // window < 0: none
+  float scale_log2;
+  int parts, part_keys, col_tiles;
+  uint16_t* out;
+  float* lse;
+  float* part_out;            // parts > 1: [B, Hkv, M, parts, D]
+  float* part_ml;             // parts > 1: [B, Hkv, M, parts, 2]
+};
+
+// Rows in use of sequence b.
+__device__ __forceinline__ int length_of(const PagedArgs& a, int b) {
+  const int n = min(a.lens[b], a.max_len);
+  const int64_t room = (int64_t)a.table_width << a.page_shift;
+  return max(0, (int)min((int64_t)n, room));
+}
+// Position of query row 0 of sequence b.
+__device__ __forceinline__ int start_of(const PagedArgs& a, int b, int n) {
+  return a.starts ? max(-kFar, min(kFar, a.starts[b])) : n - a.Lq;
+}
+// Keys [lo, hi) that the row at position p of [0, n) may see, both rising with p.
+__device__ __forceinline__ void seen_by(const PagedArgs& a, int n, int p, int& lo, int& hi) {
+  lo = a.window >= 0 ? max(0, min(n, p - a.window)) : 0;
+  hi = n;
+  if (a.causal) hi = min(hi, p + 1);
+  if (a.window >= 0) hi = min(hi, p + a.window + 1);
+  hi = max(0, hi);
+}
+// Keys of a column tile: [start, end) that some column sees (start a multiple
+// of the tile), [inner_lo, inner_hi) that all see.
+struct Range {
+  int start, end, inner_lo, inner_hi, lo;
+};
+__device__ __forceinline__ Range tile_range(const PagedArgs& a, int n, int p0, int first_col,
+                                            int cols) {
+  // first and last position of the tile's rows that are not padding
+  const int pa = max(0, p0 + first_col / a.G);
+  const int pz = min(n - 1, p0 + min(a.M - 1, first_col + cols - 1) / a.G);
+  Range r = {0, 0, 0, 0, 0};
+  if (pz < pa) return r;
+  seen_by(a, n, pa, r.lo, r.inner_hi);
+  seen_by(a, n, pz, r.inner_lo, r.end);
+  r.start = r.lo & ~(kTile - 1);
+  return r;
+}
+
+// Swizzle of V's LDS rows in 16-byte units: the transposing read's rows of one
+// lane group meet different banks.
+template <int D>
+__device__ __forceinline__ int swizzle(int r) {
+  return D == 128 ? 2 * (r & 7) + ((r >> 3) & 1) : 2 * ((r >> 1) & 3) + ((r >> 3) & 1);
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
+  constexpr int KS = D / 32;             // reduction steps of S
+  constexpr int DT = D / 16;             // output tiles
+  constexpr int UNITS = D / 8;           // 16-byte units of a row
+  constexpr int VROWS = 64 / UNITS;      // rows of one V load
+  constexpr int VL = kTile / VROWS;      // V loads per lane
+  constexpr int ROWB = 2 * D;            // bytes of a row
+  constexpr int OPAD = D + 4;
+  constexpr int LDS_V = kWaves * kTile * ROWB;
+  constexpr int LDS_O = kWaves * 16 * OPAD * 4;
+  __shared__ __align__(256) unsigned char smem[LDS_V > LDS_O ? LDS_V : LDS_O];
+  __shared__ float red_m[kWaves][16], red_l[kWaves][16];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  int64_t id = blockIdx.x;
+  const int h = (int)(id % a.Hkv);
+  id /= a.Hkv;
+  const int part = (int)(id % a.parts);
+  id /= a.parts;
+  const int ct = (int)(id % a.col_tiles);
+  const int b = (int)(id / a.col_tiles);
+
+  const int n = length_of(a, b), p0 = start_of(a, b, n);
+  const Range r = tile_range(a, n, p0, ct * 16, 16);
+  const int first = r.start + part * a.part_keys;
+  const int last = min(r.end, first + a.part_keys);
+  if (part > 0 && first >= r.end) return;   // (part 0 also writes the empty rows)
+
+  // ---- this lane's column
+  const int m = ct * 16 + col;
+  const bool cok = m < a.M;
+  const int qi = cok ? m / a.G : 0, qg = cok ? m - qi * a.G : 0;
+  const int pos = p0 + qi;
+  const bool padding = !cok || pos < 0 || pos >= n;
+  int lo = 0, hi = 0;
+  if (!padding) seen_by(a, n, pos, lo, hi);
+  u32x4_t Q[KS];
+  {
+    const uint16_t* qp = a.q + b * a.q_sb + qi * a.q_sl + (h * a.G + qg) * a.q_sh + 8 * grp;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      Q[s] = u32x4_t{0, 0, 0, 0};
+      if (cok) Q[s] = *reinterpret_cast<const u32x4_t*>(qp + 32 * s);
+    }
+  }
+  f32x4_t O[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) O[t] = zero4();
+  float mx = neg_inf(), sum = 0.f;
+
+  const int32_t* table = a.table + b * a.table_stride;
+  const int page_mask = (1 << a.page_shift) - 1;
+  const uint16_t* kb = a.k + h * a.k_sh + col * a.k_sr + 8 * grp;
+  const int vrow = lane / UNITS, vunit = lane % UNITS;
+  const uint16_t* vb = a.v + h * a.v_sh + vrow * a.v_sr + 8 * vunit;
+  unsigned char* vl = smem + wave * kTile * ROWB;
+  const uint32_t vbase = lds_addr(vl);
+  // transposing reads: row 4 grp + (col >> 2), piece col & 3 of its 32 bytes
+  const int tr = 4 * grp + (col >> 2);
+  const uint32_t tr0 = vbase + tr * ROWB + ((((col & 3) >> 1) ^ swizzle<D>(tr)) << 4) + (col & 1) * 8;
+
+  u32x4_t K[2][KS], V[VL];
+  bool live[2];  // the tile's half lies in a mapped page
+  auto page_of = [&](int key) -> int {
+    const int e = key >> a.page_shift;
+    return e < a.table_width ? table[e] : -1;
+  };
+  const int page_half = 16;
+  for (int base = first + wave * kTile; base < last; base += kStep) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = base + t * page_half;
+      int pg = __builtin_amdgcn_readfirstlane(page_of(key));
+      live[t] = pg >= 0 && pg < a.num_pages;
+      if (!live[t]) pg = 0;  // a page that exists; its values are not used
+      const int row = key & page_mask;
+      const uint16_t* kp = kb + pg * a.k_sp + row * a.k_sr;
+      const uint16_t* vp = vb + pg * a.v_sp + row * a.v_sr;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) K[t][s] = *reinterpret_cast<const u32x4_t*>(kp + 32 * s);
+#pragma unroll
+      for (int i = 0; i < VL / 2; ++i)
+        V[t * (VL / 2) + i] = *reinterpret_cast<const u32x4_t*>(vp + i * VROWS * a.v_sr);
+    }
+    const bool whole = live[0] && live[1];
+    const bool edge = !whole || base < r.lo || base + kTile > r.end;           // V rows nobody sees
+    const bool mixed = !whole || base < r.inner_lo || base + kTile > r.inner_hi;  // masked scores
+    uint64_t dirty = 0;
+    if (mixed) {
+      // Keys that some columns see and others do not: a non-finite value
+      // must not reach the others as 0 x inf, so it is taken out here and its
+      // terms are added one by one below.  Rows nobody sees become zeros.
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        const int key = base + i * VROWS + vrow;
+        const bool there = live[i / (VL / 2)] && key >= r.lo && key < r.end;
+        if (edge && !there) V[i] = u32x4_t{0, 0, 0, 0};
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t w = V[i][e];
+          const bool b0 = (w & T::kExp) == T::kExp, b1 = ((w >> 16) & T::kExp) == T::kExp;
+          odd |= b0 || b1;
+          if (b0) w &= 0xffff0000u;
+          if (b1) w &= 0x0000ffffu;
+          V[i][e] = w;
+        }
+        dirty |= __builtin_amdgcn_ballot_w64(odd);
+      }
+    }
+    // ---- V to LDS
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int rr = i * VROWS + vrow;
+      *reinterpret_cast<u32x4_t*>(vl + rr * ROWB + ((vunit ^ swizzle<D>(rr)) << 4)) = V[i];
+    }
+    // ---- scores
+    f32x4_t S[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      S[t] = zero4();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) S[t] = T::mfma(K[t][s], Q[s], S[t]);
+    }
+    uint32_t seen = 0xffu;
+    if (mixed) {
+      seen = 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = base + 16 * t + 4 * grp + e;
+          const bool ok = live[t] && key >= lo && key < hi;
+          if (ok) seen |= 1u << (4 * t + e);
+          S[t][e] = ok ? S[t][e] : neg_inf();
+        }
+    }
+    float top = neg_inf();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        S[t][e] *= a.scale_log2;   // (-inf stays: the scale is positive)
+        top = __builtin_fmaxf(top, S[t][e]);
+      }
+    top = across4_max(top);
+    if (__builtin_amdgcn_ballot_w64(top > mx + kSlack) != 0) {
+      const float to = __builtin_fmaxf(mx, top);
+      const float f = to == neg_inf() ? 1.f : exp2_hw(mx - to);
+      mx = to;
+      sum *= f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[t][e] *= f;
+    }
+    const float off = mx == neg_inf() ? 0.f : mx;
+    float P[8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        P[4 * t + e] = exp2_hw(S[t][e] - off);
+        sum += P[4 * t + e];
+      }
+    const u32x4_t Pb = {T::pack(P[0], P[1]), T::pack(P[2], P[3]), T::pack(P[4], P[5]),
+                        T::pack(P[6], P[7])};
+    // ---- V^T . P^T
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      const uint32_t at = tr0 ^ (t << 5);
+      const u32x2_t x = read_transposed(at), y = read_transposed(at + 16 * ROWB);
+      O[t] = T::mfma(u32x4_t{x[0], x[1], y[0], y[1]}, Pb, O[t]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (dirty) {
+      for (int kk = 0; kk < kTile; ++kk) {
+        const int key = base + kk;
+        if (!live[kk >> 4] || key < r.lo || key >= r.end) continue;
+        const int from = 16 * ((kk & 15) >> 2) + col;
+        const int slot = 4 * (kk >> 4) + (kk & 3);
+        float pv = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pv = e == slot ? P[e] : pv;
+        const float pk = __shfl(pv, from, 64);
+        const bool ok = (__shfl(seen, from, 64) >> slot) & 1;
+        const int pg = __builtin_amdgcn_readfirstlane(page_of(key));
+        const uint16_t* vp = a.v + h * a.v_sh + pg * a.v_sp + (key & page_mask) * a.v_sr;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t w = vp[16 * t + 4 * grp + e];
+            if (ok && (w & T::kExp) == T::kExp) O[t][e] += pk * T::value(w);
+          }
+      }
+    }
+  }
+
+  // ---- join the four waves
+  if (padding) {  // (its scores were not masked in tiles that every row sees)
+    mx = neg_inf();
+    sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) O[t] = zero4();
+  }
+  sum = across4_sum(sum);
+  if (grp == 0) {
+    red_m[wave][col] = mx;
+    red_l[wave][col] = sum;
+  }
+  __syncthreads();
+  float M = neg_inf(), total = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) M = __builtin_fmaxf(M, red_m[w][col]);
+  const float f = M == neg_inf() ? 1.f : exp2_hw(mx - M);
+  float* ol = reinterpret_cast<float*>(smem) + wave * 16 * OPAD + col * OPAD;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+    *reinterpret_cast<f32x4_t*>(ol + 16 * t + 4 * grp) = O[t] * f;
+  __syncthreads();
+  // thread: column tid / (kThreads / 16), D / 16 dims
+  constexpr int TPC = kThreads / 16, DPT = D / TPC;
+  const int c2 = tid / TPC, d2 = (tid % TPC) * DPT;
+  const int m2 = ct * 16 + c2;
+  if (m2 >= a.M) return;
+  M = neg_inf();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) M = __builtin_fmaxf(M, red_m[w][c2]);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    total += red_l[w][c2] * (M == neg_inf() ? 1.f : exp2_hw(red_m[w][c2] - M));
+  float acc[DPT];
+#pragma unroll
+  for (int d = 0; d < DPT; ++d) acc[d] = 0.f;
+  for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+    for (int d = 0; d < DPT; ++d)
+      acc[d] += reinterpret_cast<float*>(smem)[w * 16 * OPAD + c2 * OPAD + d2 + d];
+  if (a.parts > 1) {
+    const int64_t at = (((int64_t)b * a.Hkv + h) * a.M + m2) * a.parts + part;
+#pragma unroll
+    for (int d = 0; d < DPT; ++d) a.part_out[at * D + d2 + d] = acc[d];
+    if (d2 == 0) {
+      a.part_ml[2 * at] = M;
+      a.part_ml[2 * at + 1] = total;
+    }
+    return;
+  }
+  const int i2 = m2 / a.G;
+  const int64_t row = ((int64_t)b * a.Lq + i2) * a.Hq + h * a.G + (m2 - i2 * a.G);
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+  for (int d = 0; d < DPT; d += 2)
+    *reinterpret_cast<uint32_t*>(a.out + row * D + d2 + d) =
+        total == 0.f ? 0u : T::pack(acc[d] * inv, acc[d + 1] * inv);
+  if (d2 == 0) a.lse[row] = total == 0.f ? neg_inf() : kLn2 * (M + log2_hw(total));
+}
+
+// One workgroup per column: the parts' maxima and sums, then their outputs.
+template <class T, int D>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(PagedArgs a) {
+  constexpr int TPR = D / 4;                 // threads of a row, four dims each
+  constexpr int LANES = kThreads / TPR;      // parts at a time
+  __shared__ float weight[kMaxParts];
+  __shared__ float red[kThreads / 64];
+  __shared__ f32x4_t acc_l[kThreads];
+  const int tid = threadIdx.x;
+  const int64_t c = blockIdx.x;              // (b Hkv + h) M + m
+  const int m = (int)(c % a.M);
+  const int64_t bh = c / a.M;
+  const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv);
+  const int n = length_of(a, b);
+  const Range r = tile_range(a, n, start_of(a, b, n), m & ~15, 16);
+  const int np = max(1, (r.end - r.start + a.part_keys - 1) / a.part_keys);
+  const float* ml = a.part_ml + 2 * c * a.parts;
+  float M = neg_inf();
+  for (int p = tid; p < np; p += kThreads) M = __builtin_fmaxf(M, ml[2 * p]);
+  M = wave_max(M);
+  if ((tid & 63) == 0) red[tid >> 6] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) M = __builtin_fmaxf(M, red[w]);
+  __syncthreads();
+  float total = 0.f;
+  for (int p = tid; p < np; p += kThreads) {
+    const float w = M == neg_inf() ? 1.f : exp2_hw(ml[2 * p] - M);
+    weight[p] = w;
+    total += w * ml[2 * p + 1];
+  }
+  total = wave_sum(total);
+  if ((tid & 63) == 0) red[tid >> 6] = total;
+  __syncthreads();
+  total = 0.f;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) total += red[w];
+  const int d4 = tid % TPR;
+  const f32x4_t* po = reinterpret_cast<const f32x4_t*>(a.part_out + c * a.parts * D) + d4;
+  f32x4_t acc = zero4();
+  for (int p = tid / TPR; p < np; p += LANES) acc += weight[p] * po[(int64_t)p * TPR];
+  acc_l[tid] = acc;
+  __syncthreads();
+  if (tid >= TPR) return;
+  for (int l = 1; l < LANES; ++l) acc += acc_l[l * TPR + tid];
+  const int i = m / a.G;
+  const int64_t row = ((int64_t)b * a.Lq + i) * a.Hq + h * a.G + (m - i * a.G);
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  u32x2_t o = {0u, 0u};
+  if (total != 0.f) o = u32x2_t{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
+  *reinterpret_cast<u32x2_t*>(a.out + row * D + 4 * d4) = o;
+  if (tid == 0) a.lse[row] = total == 0.f ? neg_inf() : kLn2 * (M + log2_hw(total));
+}
+
+// Most keys that one column tile's columns can see.
+int64_t span_bound(int64_t max_len, int64_t q_len, int64_t group, int64_t window, int causal) {
+  if (window < 0) return max_len;
+  const int64_t rows = std::min<int64_t>(q_len, 16 / group + 2);
+  return std::min(max_len, rows + (causal ? 1 : 2) * window + 1);
+}
+
+template <class T, int D>
+int launch(const PagedArgs& a, hipStream_t stream) {
+  const int64_t grid = (int64_t)a.B * a.Hkv * a.col_tiles * a.parts;
+  const int64_t cols = (int64_t)a.B * a.Hkv * a.M;
+  if (grid > 0x7fffffff || cols > 0x7fffffff) return MRSA_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+  int st = mrsa_launch_status();
+  if (st != MRSA_OK || a.parts == 1) return st;
+  hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)cols), dim3(kThreads), 0, stream, a);
+  return mrsa_launch_status();
+}
+
+}  // namespace
+
+extern "C" int64_t mrsa_paged_attention_workspace_bytes(int64_t batch, int64_t q_len,
+                                                        int64_t q_heads, int64_t head_dim,
+                                                        int64_t parts) {
+  const int64_t most = 1ll << 31;
+  if (batch < 0 || q_len < 0 || q_heads <= 0 || head_dim <= 0 || parts < 1 || batch > most ||
+      q_len > most || q_heads > 65536 || head_dim > 4096 || parts > kMaxParts)
+    return -1;
+  if (parts == 1 || batch == 0 || q_len == 0) return 0;
+  if (q_len > (1ll << 40) / batch / q_heads) return -1;
+  return batch * q_len * q_heads * parts * (head_dim + 2) * (int64_t)sizeof(float);
+}
+
+extern "C" int mrsa_paged_attention_fwd(
+    const void* q, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
+    const void* k_pages, int64_t k_page_stride, int64_t k_slot_stride, int64_t k_head_stride,
+    const void* v_pages, int64_t v_page_stride, int64_t v_slot_stride, int64_t v_head_stride,
+    const int32_t* page_table, int64_t page_table_stride, int64_t table_pages, int64_t num_pages,
+    int64_t page_size, const int32_t* cache_lens, const int32_t* query_starts, int64_t max_len, int64_t batch, int64_t q_len,
+    int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t dtype, int32_t causal,
+    int64_t window, float sm_scale, int64_t parts, void* workspace, int64_t workspace_bytes,
+    void* out, float* lse, void* stream) {
+  if (batch < 0 || q_len < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 ||
+      max_len < 0 || table_pages < 0 || num_pages < 0 || page_size <= 0 || parts < 1 ||
+      parts > kMaxParts)
+    return MRSA_ERR_INVALID_ARGUMENT;
+  if (!(sm_scale > 0.f) || !(sm_scale < __builtin_inff())) return MRSA_ERR_INVALID_ARGUMENT;
+  if (dtype != MRSA_DTYPE_BF16 && dtype != MRSA_DTYPE_FP16) return MRSA_ERR_UNSUPPORTED;
+  if (head_dim != 64 && head_dim != 128) return MRSA_ERR_UNSUPPORTED;
+  if ((page_size & (page_size - 1)) != 0 || page_size < 16 || page_size > (1 << 20))
+    return MRSA_ERR_UNSUPPORTED;
+  const int64_t most = kFar;
+  if (max_len >= most || q_len >= most || table_pages >= most || num_pages > 0x7fffffff ||
+      batch > most || q_heads > 65536 || (q_len > 0 && q_heads / kv_heads > most / q_len))
+    return MRSA_ERR_UNSUPPORTED;
+  if (batch == 0 || q_len == 0) return MRSA_OK;
+  if (!q || !cache_lens || !out || !lse) return MRSA_ERR_INVALID_ARGUMENT;
+  if (table_pages == 0 || num_pages == 0) max_len = 0;   // no keys anywhere
+  else if (!page_table || !k_pages || !v_pages) return MRSA_ERR_INVALID_ARGUMENT;
+  if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) % 16 != 0 ||
+      (q_batch_stride | q_row_stride | q_head_stride | k_page_stride | k_slot_stride |
+       k_head_stride | v_page_stride | v_slot_stride | v_head_stride) % 8 != 0)
+    return MRSA_ERR_UNSUPPORTED;
+  const int64_t need = mrsa_paged_attention_workspace_bytes(batch, q_len, q_heads, head_dim, parts);
+  if (need < 0) return MRSA_ERR_UNSUPPORTED;
+  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16 != 0))
+    return MRSA_ERR_INVALID_ARGUMENT;
+  PagedArgs a = {};
+  a.q = (const uint16_t*)q;
+  a.q_sb = q_batch_stride, a.q_sl = q_row_stride, a.q_sh = q_head_stride;
+  a.k = (const uint16_t*)k_pages;
+  a.k_sp = k_page_stride, a.k_sr = k_slot_stride, a.k_sh = k_head_stride;
+  a.v = (const uint16_t*)v_pages;
+  a.v_sp = v_page_stride, a.v_sr = v_slot_stride, a.v_sh = v_head_stride;
+  a.table = page_table;
+  a.table_stride = page_table_stride;
+  a.table_width = (int)table_pages;
+  a.page_shift = __builtin_ctzll((uint64_t)page_size);
+  a.num_pages = (int)num_pages;
+  a.lens = cache_lens;
+  a.starts = query_starts;
+  a.max_len = (int)max_len;
+  a.B = (int)batch, a.Lq = (int)q_len, a.Hq = (int)q_heads, a.Hkv = (int)kv_heads;
+  a.G = (int)(q_heads / kv_heads);
+  a.M = a.Lq * a.G;
+  a.causal = causal != 0;
+  a.window = window < 0 ? -1 : (int)std::min<int64_t>(window, most);
+  a.scale_log2 = sm_scale * kLog2e;
+  a.parts = (int)parts;
+  a.col_tiles = (a.M + 15) / 16;
+  const int64_t span = span_bound(max_len, q_len, a.G, a.window, a.causal) + kTile - 1;
+  a.part_keys = (int)(((span + parts - 1) / parts + kStep - 1) / kStep * kStep);
+  a.out = (uint16_t*)out;
+  a.lse = lse;
+  a.part_out = (float*)workspace;
+  if (parts > 1) a.part_ml = a.part_out + batch * q_len * q_heads * parts * head_dim;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == MRSA_DTYPE_BF16)
+    return head_dim == 128 ? launch<Bf16, 128>(a, s) : launch<Bf16, 64>(a, s);
+  return head_dim == 128 ? launch<Fp16, 128>(a, s) : launch<Fp16, 64>(a, s);
+}

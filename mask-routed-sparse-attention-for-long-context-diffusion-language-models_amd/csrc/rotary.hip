@@ -1,0 +1,417 @@
+// Rotary positions of query and key heads, and the same rotation fused with
+// the write of new rows into the pages of a K/V cache.
+//
+// A head's first 2 `half` dims hold pairs (x1, x2): dims i and i + half (half
+// layout) or 2 i and 2 i + 1 (interleaved).  With c, s = cos, sin of row
+// `position` of the tables:
+//     y1 = x1 c - x2 s,   y2 = x2 c + x1 s          (inverse: s -> -s,
+// the transpose, which is the gradient).  Dims past 2 half are copied.
+// Products and sums are fp32 with fp32 tables, rounded once to the tensors'
+// type.  A position outside the tables gives NaN rows: nothing is read there.
+//
+// Pure streams: every element is read once and written once, so the kernels
+// are bound by HBM for long inputs and by the launch for short ones.  A thread
+// takes one 16-byte unit (or the two units of a half-layout pair) of up to
+// kHeadsPerThread heads of one token, so that a token's table row is read once
+// per thread and not once per head, and all its loads are in flight together.
+#include "mrsa_device.h"
+
+using namespace mrsa;
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kHeadsPerThread = 4;
+
+// One stream of heads: [batch, row, head] strides in elements, last dim dense.
+struct Heads {
+  const void* src;
+  int64_t sb, sl, sh;
+  void* dst;          // paged: the page pool
+  int64_t db, dl, dh; // paged: page, row, head strides
+  int heads;
+};
+
+struct RotaryArgs {
+  Heads q, k, v;
+  const float* cos_t;
+  const float* sin_t;
+  int64_t table_rows;
+  const int64_t* positions;  // optional
+  int64_t ps_b, ps_l;
+  int tokens, L;             // tokens = batch * L
+  int D, half;
+  float sign;                // -1: inverse
+  // paged writes of k and v
+  const int64_t* slots;
+  int64_t sl_b, sl_l;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_width, page_shift;
+  int64_t num_pages;
+  int units, head_slots, tokens_per_block;
+};
+
+template <class T>
+struct Traits;
+template <>
+struct Traits<__bf16> {
+  static constexpr int kPer16 = 8;
+};
+template <>
+struct Traits<_Float16> {
+  static constexpr int kPer16 = 8;
+};
+template <>
+struct Traits<float> {
+  static constexpr int kPer16 = 4;
+};
+
+template <class T>
+struct alignas(16) Vec {
+  T e[Traits<T>::kPer16];
+};
+
+// Base of token (b, l)'s rows in a dense or paged destination; false if the
+// token has no place.
+template <class T, bool PAGED>
+__device__ __forceinline__ bool cache_row(const RotaryArgs& a, int b, int l, int64_t& page,
+                                          int64_t& row) {
+  const int64_t slot = a.slots[b * a.sl_b + l * a.sl_l];
+  if (slot < 0 || (slot >> a.page_shift) >= a.table_width) return false;
+  const int32_t p = a.table[b * a.table_stride + (slot >> a.page_shift)];
+  if (p < 0 || p >= a.num_pages) return false;
+  page = p;
+  row = slot & ((1ll << a.page_shift) - 1);
+  return true;
+}
+
+// One pair; the order of the roundings is fixed, so that every kernel here gives
+// the same bits.
+__device__ __forceinline__ void turn_pair(float& x1, float& x2, float c, float s) {
+  const float y1 = __builtin_fmaf(x1, c, -__fmul_rn(x2, s));
+  x2 = __builtin_fmaf(x2, c, __fmul_rn(x1, s));
+  x1 = y1;
+}
+
+template <class T, bool INTERLEAVED>
+__device__ __forceinline__ void turn(Vec<T>& x, Vec<T>& y, const float* c, const float* s) {
+  constexpr int E = Traits<T>::kPer16;
+  if constexpr (INTERLEAVED) {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      float x1 = (float)x.e[2 * i], x2 = (float)x.e[2 * i + 1];
+      turn_pair(x1, x2, c[i], s[i]);
+      x.e[2 * i] = (T)x1;
+      x.e[2 * i + 1] = (T)x2;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      float x1 = (float)x.e[i], x2 = (float)y.e[i];
+      turn_pair(x1, x2, c[i], s[i]);
+      x.e[i] = (T)x1;
+      y.e[i] = (T)x2;
+    }
+  }
+}
+
+// 16-byte units; PAGED: k and v go to pages (v is copied), else only q and k.
+template <class T, bool INTERLEAVED, bool PAGED>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
+  constexpr int E = Traits<T>::kPer16;
+  constexpr int TN = INTERLEAVED ? E / 2 : E;  // table values of a unit
+  const int per_token = a.units * a.head_slots;
+  const int total_heads = a.q.heads + a.k.heads + (PAGED ? a.v.heads : 0);
+  const int rot_units = a.half / TN;
+  const int tail_at = 2 * a.half;
+  for (int lid = threadIdx.x; lid < a.tokens_per_block * per_token; lid += kThreads) {
+    const int ti = lid / per_token;
+    const int64_t tok = (int64_t)blockIdx.x * a.tokens_per_block + ti;
+    if (tok >= a.tokens) return;
+    const int rem = lid - ti * per_token;
+    const int hs = rem / a.units;
+    const int u = rem - hs * a.units;
+    const int b = (int)tok / a.L, l = (int)tok - b * a.L;
+    int64_t page = 0, row = 0;
+    bool placed = false;
+    if constexpr (PAGED) placed = cache_row<T, PAGED>(a, b, l, page, row);
+    const bool rotate = u < rot_units;
+    float c[TN], s[TN];
+    if (rotate) {
+      const int64_t pos = a.positions ? a.positions[b * a.ps_b + l * a.ps_l] : l;
+      if (pos >= 0 && pos < a.table_rows) {
+        const float4* cp = reinterpret_cast<const float4*>(a.cos_t + pos * a.half + u * TN);
+        const float4* sp = reinterpret_cast<const float4*>(a.sin_t + pos * a.half + u * TN);
+        if constexpr (TN >= 4) {
+#pragma unroll
+          for (int i = 0; i < TN / 4; ++i) {
+            const float4 cv = cp[i], sv = sp[i];
+            c[4 * i] = cv.x, c[4 * i + 1] = cv.y, c[4 * i + 2] = cv.z, c[4 * i + 3] = cv.w;
+            s[4 * i] = sv.x, s[4 * i + 1] = sv.y, s[4 * i + 2] = sv.z, s[4 * i + 3] = sv.w;
+          }
+        } else {
+          const float2 cv = *reinterpret_cast<const float2*>(cp);
+          const float2 sv = *reinterpret_cast<const float2*>(sp);
+          c[0] = cv.x, c[1] = cv.y, s[0] = sv.x, s[1] = sv.y;
+        }
+#pragma unroll
+        for (int i = 0; i < TN; ++i) s[i] *= a.sign;
+      } else {
+#pragma unroll
+        for (int i = 0; i < TN; ++i) c[i] = s[i] = __builtin_nanf("");
+      }
+    }
+    // dims of this unit: [at, at + E) and, half layout, [at2, at2 + E)
+    const int at = rotate ? u * E : tail_at + (u - rot_units) * E;
+    const int at2 = at + a.half;
+    const bool two = !INTERLEAVED && rotate;
+    Vec<T> x[kHeadsPerThread], y[kHeadsPerThread];
+    T* out[kHeadsPerThread];
+    int kind[kHeadsPerThread];  // 0 none, 1 q or k, 2 v
+#pragma unroll
+    for (int i = 0; i < kHeadsPerThread; ++i) {
+      int h = hs + i * a.head_slots;
+      kind[i] = 0;
+      if (h >= total_heads) continue;
+      const Heads* seg = &a.q;
+      bool paged = false;
+      if (h >= a.q.heads) {
+        h -= a.q.heads;
+        seg = &a.k;
+        paged = PAGED;
+        if (PAGED && h >= a.k.heads) {
+          h -= a.k.heads;
+          seg = &a.v;
+          kind[i] = 2;
+        }
+      }
+      if (kind[i] == 0) kind[i] = 1;
+      if (paged && !placed) {
+        kind[i] = 0;
+        continue;
+      }
+      const T* in = (const T*)seg->src + b * seg->sb + l * seg->sl + h * seg->sh;
+      out[i] = (T*)seg->dst + (paged ? page * seg->db + row * seg->dl : b * seg->db + l * seg->dl) +
+               h * seg->dh;
+      x[i] = *reinterpret_cast<const Vec<T>*>(in + at);
+      if (two) y[i] = *reinterpret_cast<const Vec<T>*>(in + at2);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeadsPerThread; ++i) {
+      if (!kind[i]) continue;
+      if (rotate && kind[i] == 1) turn<T, INTERLEAVED>(x[i], y[i], c, s);
+      *reinterpret_cast<Vec<T>*>(out[i] + at) = x[i];
+      if (two) *reinterpret_cast<Vec<T>*>(out[i] + at2) = y[i];
+    }
+  }
+}
+
+// The same one value (a tail dim or a v dim) or pair at a time, for head parts
+// that 16-byte units do not divide and for unaligned tensors: units = half
+// pairs and D - 2 half tail dims.
+template <class T, bool INTERLEAVED, bool PAGED>
+__global__ void __launch_bounds__(kThreads) rotary_scalar_kernel(RotaryArgs a) {
+  const int per_token = a.units * a.head_slots;  // head_slots = every head
+  for (int lid = threadIdx.x; lid < a.tokens_per_block * per_token; lid += kThreads) {
+    const int ti = lid / per_token;
+    const int64_t tok = (int64_t)blockIdx.x * a.tokens_per_block + ti;
+    if (tok >= a.tokens) return;
+    const int rem = lid - ti * per_token;
+    int h = rem / a.units;
+    const int u = rem - h * a.units;
+    const int b = (int)tok / a.L, l = (int)tok - b * a.L;
+    const Heads* seg = &a.q;
+    bool paged = false, turned = true;
+    if (h >= a.q.heads) {
+      h -= a.q.heads;
+      seg = &a.k;
+      paged = PAGED;
+      if (PAGED && h >= a.k.heads) {
+        h -= a.k.heads;
+        seg = &a.v;
+        turned = false;
+      }
+    }
+    int64_t page = 0, row = 0;
+    if (PAGED && paged && !cache_row<T, PAGED>(a, b, l, page, row)) continue;
+    const T* in = (const T*)seg->src + b * seg->sb + l * seg->sl + h * seg->sh;
+    T* out = (T*)seg->dst + (paged ? page * seg->db + row * seg->dl : b * seg->db + l * seg->dl) +
+             h * seg->dh;
+    if (u >= a.half) {
+      const int at = u + a.half;
+      out[at] = in[at];
+      continue;
+    }
+    const int i1 = INTERLEAVED ? 2 * u : u, i2 = INTERLEAVED ? 2 * u + 1 : u + a.half;
+    const T x1 = in[i1], x2 = in[i2];
+    if (!turned) {
+      out[i1] = x1;
+      out[i2] = x2;
+      continue;
+    }
+    const int64_t pos = a.positions ? a.positions[b * a.ps_b + l * a.ps_l] : l;
+    float c = __builtin_nanf(""), s = c;
+    if (pos >= 0 && pos < a.table_rows) {
+      c = a.cos_t[pos * a.half + u];
+      s = a.sign * a.sin_t[pos * a.half + u];
+    }
+    float f1 = (float)x1, f2 = (float)x2;
+    turn_pair(f1, f2, c, s);
+    out[i1] = (T)f1;
+    out[i2] = (T)f2;
+  }
+}
+
+template <class T, bool PAGED>
+int launch(RotaryArgs a, bool interleaved, hipStream_t stream) {
+  constexpr int E = Traits<T>::kPer16;
+  const int heads = a.q.heads + a.k.heads + (PAGED ? a.v.heads : 0);
+  // 16-byte units need whole units of pairs and of tail dims, and every row aligned.
+  bool vec = a.D % E == 0 && (interleaved ? 2 * a.half : a.half) % E == 0 &&
+             ((uintptr_t)a.cos_t | (uintptr_t)a.sin_t) % 16 == 0;
+  const Heads* segs[3] = {&a.q, &a.k, &a.v};
+  for (const Heads* s : segs) {
+    if (s->heads == 0) continue;
+    vec = vec && ((uintptr_t)s->src | (uintptr_t)s->dst) % 16 == 0 &&
+          (s->sb | s->sl | s->sh | s->db | s->dl | s->dh) % E == 0;
+  }
+  if (vec) {
+    const int rot = a.half / (interleaved ? E / 2 : E);
+    a.units = rot + (a.D - 2 * a.half) / E;
+    // Few tokens: a head per thread, so that as many threads as there are work; many: the
+    // table row of a thread serves kHeadsPerThread heads.
+    const int64_t one = (int64_t)a.tokens * heads * a.units;
+    a.head_slots = one < 256 * 1024 ? heads : (heads + kHeadsPerThread - 1) / kHeadsPerThread;
+  } else {
+    a.units = a.D - a.half;
+    a.head_slots = heads;
+  }
+  const int per_token = a.units * a.head_slots;
+  a.tokens_per_block = std::max(1, kThreads / per_token);
+  const unsigned blocks = (unsigned)((a.tokens + a.tokens_per_block - 1) / a.tokens_per_block);
+  void (*kern)(RotaryArgs) =
+      vec ? (interleaved ? rotary_kernel<T, true, PAGED> : rotary_kernel<T, false, PAGED>)
+          : (interleaved ? rotary_scalar_kernel<T, true, PAGED>
+                         : rotary_scalar_kernel<T, false, PAGED>);
+  hipLaunchKernelGGL(kern, dim3(blocks), dim3(kThreads), 0, stream, a);
+  return mrsa_launch_status();
+}
+
+template <bool PAGED>
+int dispatch(const RotaryArgs& a, int dtype, int interleaved, void* stream) {
+  hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case MRSA_DTYPE_BF16: return launch<__bf16, PAGED>(a, interleaved != 0, s);
+    case MRSA_DTYPE_FP16: return launch<_Float16, PAGED>(a, interleaved != 0, s);
+    case MRSA_DTYPE_FP32: return launch<float, PAGED>(a, interleaved != 0, s);
+    default: return MRSA_ERR_INVALID_ARGUMENT;
+  }
+}
+
+// What both entry points check of the sizes; 0 tokens or heads pass.
+bool sizes_ok(int64_t batch, int64_t seq_len, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+              int64_t rotary_dim, int64_t table_rows) {
+  return batch >= 0 && seq_len >= 0 && q_heads >= 0 && kv_heads >= 0 && head_dim > 0 &&
+         rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim && table_rows >= 0;
+}
+bool sizes_fit(int64_t batch, int64_t seq_len, int64_t q_heads, int64_t kv_heads,
+               int64_t head_dim) {
+  const int64_t most = 0x7fffffff;
+  if (batch > most || seq_len > most || q_heads > 65536 || kv_heads > 65536 || head_dim > 4096)
+    return false;
+  return batch == 0 || seq_len <= most / batch;
+}
+
+}  // namespace
+
+extern "C" int mrsa_rotary_fwd(const void* q, int64_t q_batch_stride, int64_t q_row_stride,
+                               int64_t q_head_stride, const void* k, int64_t k_batch_stride,
+                               int64_t k_row_stride, int64_t k_head_stride,
+                               const float* cos_table, const float* sin_table, int64_t table_rows,
+                               const int64_t* positions, int64_t positions_batch_stride,
+                               int64_t positions_row_stride, int64_t batch, int64_t seq_len,
+                               int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                               int64_t rotary_dim, int32_t dtype, int32_t interleaved,
+                               int32_t inverse, void* q_out, void* k_out, void* stream) {
+  if (!sizes_ok(batch, seq_len, q_heads, kv_heads, head_dim, rotary_dim, table_rows))
+    return MRSA_ERR_INVALID_ARGUMENT;
+  if (dtype < MRSA_DTYPE_BF16 || dtype > MRSA_DTYPE_FP32) return MRSA_ERR_INVALID_ARGUMENT;
+  if (!sizes_fit(batch, seq_len, q_heads, kv_heads, head_dim)) return MRSA_ERR_UNSUPPORTED;
+  if (batch * seq_len == 0 || q_heads + kv_heads == 0) return MRSA_OK;
+  if ((q_heads && (!q || !q_out)) || (kv_heads && (!k || !k_out)))
+    return MRSA_ERR_INVALID_ARGUMENT;
+  if (rotary_dim && table_rows && (!cos_table || !sin_table)) return MRSA_ERR_INVALID_ARGUMENT;
+  RotaryArgs a = {};
+  a.q = {q, q_batch_stride, q_row_stride, q_head_stride, q_out, seq_len * q_heads * head_dim,
+         q_heads * head_dim, head_dim, (int)q_heads};
+  a.k = {k, k_batch_stride, k_row_stride, k_head_stride, k_out, seq_len * kv_heads * head_dim,
+         kv_heads * head_dim, head_dim, (int)kv_heads};
+  a.cos_t = cos_table;
+  a.sin_t = sin_table;
+  a.table_rows = table_rows;
+  a.positions = positions;
+  a.ps_b = positions_batch_stride;
+  a.ps_l = positions_row_stride;
+  a.tokens = (int)(batch * seq_len);
+  a.L = (int)seq_len;
+  a.D = (int)head_dim;
+  a.half = (int)(rotary_dim / 2);
+  a.sign = inverse ? -1.f : 1.f;
+  return dispatch<false>(a, dtype, interleaved, stream);
+}
+
+extern "C" int mrsa_paged_append_fwd(
+    const void* q, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
+    const void* k, int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride,
+    const void* v, int64_t v_batch_stride, int64_t v_row_stride, int64_t v_head_stride,
+    const float* cos_table, const float* sin_table, int64_t table_rows, const int64_t* positions,
+    int64_t positions_batch_stride, int64_t positions_row_stride, const int64_t* slots,
+    int64_t slots_batch_stride, int64_t slots_row_stride, const int32_t* page_table,
+    int64_t page_table_stride, int64_t table_pages, int64_t num_pages, int64_t page_size,
+    void* k_pages, int64_t k_page_stride, int64_t k_slot_stride, int64_t k_pages_head_stride,
+    void* v_pages, int64_t v_page_stride, int64_t v_slot_stride, int64_t v_pages_head_stride,
+    int64_t batch, int64_t seq_len, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+    int64_t rotary_dim, int32_t dtype, int32_t interleaved, void* q_out, void* stream) {
+  if (!sizes_ok(batch, seq_len, q_heads, kv_heads, head_dim, rotary_dim, table_rows) ||
+      table_pages < 0 || num_pages < 0 || page_size <= 0)
+    return MRSA_ERR_INVALID_ARGUMENT;
+  if (dtype < MRSA_DTYPE_BF16 || dtype > MRSA_DTYPE_FP32) return MRSA_ERR_INVALID_ARGUMENT;
+  if ((page_size & (page_size - 1)) != 0 || page_size > (1 << 20)) return MRSA_ERR_UNSUPPORTED;
+  if (!sizes_fit(batch, seq_len, q_heads, kv_heads, head_dim) || table_pages > 0x7fffffff)
+    return MRSA_ERR_UNSUPPORTED;
+  if (batch * seq_len == 0 || q_heads + kv_heads == 0) return MRSA_OK;
+  if ((q_heads && (!q || !q_out)) || !slots) return MRSA_ERR_INVALID_ARGUMENT;
+  if (kv_heads && (!k || !v)) return MRSA_ERR_INVALID_ARGUMENT;
+  if (kv_heads && table_pages && num_pages &&
+      (!page_table || !k_pages || !v_pages || k_pages == v_pages))
+    return MRSA_ERR_INVALID_ARGUMENT;
+  if (rotary_dim && table_rows && (!cos_table || !sin_table)) return MRSA_ERR_INVALID_ARGUMENT;
+  RotaryArgs a = {};
+  a.q = {q, q_batch_stride, q_row_stride, q_head_stride, q_out, seq_len * q_heads * head_dim,
+         q_heads * head_dim, head_dim, (int)q_heads};
+  a.k = {k, k_batch_stride, k_row_stride, k_head_stride,
+         k_pages, k_page_stride, k_slot_stride, k_pages_head_stride, (int)kv_heads};
+  a.v = {v, v_batch_stride, v_row_stride, v_head_stride,
+         v_pages, v_page_stride, v_slot_stride, v_pages_head_stride, (int)kv_heads};
+  a.cos_t = cos_table;
+  a.sin_t = sin_table;
+  a.table_rows = table_rows;
+  a.positions = positions;
+  a.ps_b = positions_batch_stride;
+  a.ps_l = positions_row_stride;
+  a.tokens = (int)(batch * seq_len);
+  a.L = (int)seq_len;
+  a.D = (int)head_dim;
+  a.half = (int)(rotary_dim / 2);
+  a.sign = 1.f;
+  a.slots = slots;
+  a.sl_b = slots_batch_stride;
+  a.sl_l = slots_row_stride;
+  a.table = page_table;
+  a.table_stride = page_table_stride;
+  a.table_width = num_pages ? (int)table_pages : 0;
+  a.num_pages = num_pages;
+  a.page_shift = __builtin_ctzll((uint64_t)page_size);
+  return dispatch<true>(a, dtype, interleaved, stream);
+}

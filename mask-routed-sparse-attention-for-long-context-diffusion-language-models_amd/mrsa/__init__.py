@@ -20,6 +20,9 @@ hand-written HIP kernels in ../csrc (C ABI: include/mrsa.h).  Module map:
     kernel_utils.py     remote_drop_mask(_rows), chunk_aligned_local_bounds, group_pad_to/unpad
     route_layer.py      route_attention, swa_attention  (attention.py route / SWA layers),
                         cached_route_attention + LayerKVCache (fastdllm_attention.py cached step)
+    rotary.py           rotary_qk (with its gradient), rotary_tables, rotary_frequencies
+    paged_cache.py      PagedKVCache, paged_cache_append, paged_cached_attention,
+                        copy_cache_pages: several sequences' K/V in shared pages
     ops.py              torch.ops.mrsa.* custom operators (schemas, CUDA and fake kernels)
 """
 
@@ -32,8 +35,11 @@ from .kernel_utils import (
     remote_drop_mask_rows,
 )
 from .local_attention import bidir_local_attention, cached_local_attention
+from .paged_cache import (PagedBatch, PagedKVCache, PagesExhausted, copy_cache_pages,
+                          paged_cache_append, paged_cached_attention)
 from .pool import (chunk_attn_pool_gqa, chunk_attn_pool_gqa_backward, chunk_attn_pool_gqa_prior,
                    kv_fragments_pool)
+from .rotary import rotary_frequencies, rotary_qk, rotary_tables
 from .route_layer import (
     CachedBlockStep,
     LayerKVCache,
@@ -62,6 +68,15 @@ from . import ops  # registers torch.ops.mrsa.* (after every module it wraps)
 
 __all__ = [
     "HiLS_block_M_head",
+    "PagedBatch",
+    "PagedKVCache",
+    "PagesExhausted",
+    "copy_cache_pages",
+    "paged_cache_append",
+    "paged_cached_attention",
+    "rotary_frequencies",
+    "rotary_qk",
+    "rotary_tables",
     "LIB_PATH",
     "MrsaLibraryError",
     "CachedBlockStep",

@@ -194,6 +194,27 @@ SIGNATURES = {
         _I,
         [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _P, _P],
     ),
+    "mrsa_rotary_fwd": (
+        _I,
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _I64,
+         _I64, _I64, _I64, _I64, _I, _I, _I, _P, _P, _P],
+    ),
+    "mrsa_paged_append_fwd": (
+        _I,
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P,
+         _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64,
+         _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _P, _P],
+    ),
+    "mrsa_paged_attention_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
+    "mrsa_paged_attention_fwd": (
+        _I,
+        [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
+         _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _I64, _F, _I64, _P, _I64, _P,
+         _P, _P],
+    ),
+    "mrsa_copy_pages": (
+        _I, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P],
+    ),
     "mrsa_selftest_mfma_layout": (_I, [_P, _P, _P, _P]),
 }
 
@@ -258,6 +279,15 @@ def stream_of(t: torch.Tensor) -> int:
 
 def call(name: str, *args) -> int:
     return getattr(load(), name)(*args)
+
+
+def call_on(device: torch.device, name: str, *args) -> int:
+    """call() with `device` current: a launch needs the device of its stream."""
+
+    if torch.cuda.current_device() == device.index:
+        return getattr(load(), name)(*args)
+    with torch.cuda.device(device):
+        return getattr(load(), name)(*args)
 
 
 def copy_buffers(dst: list, src: list) -> None:

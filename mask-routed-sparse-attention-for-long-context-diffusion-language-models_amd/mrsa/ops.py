@@ -23,7 +23,9 @@ from torch import Tensor
 from .fusion import _fuse_bwd_impl, _fuse_impl
 from .kernel_utils import _drop_mask_impl, _drop_mask_rows_impl
 from .local_attention import _local_attention_impl
+from .paged_cache import _copy_pages_impl, _paged_append_impl, _paged_attention_impl
 from .pool import _kv_fragments_pool_impl, _pool_bwd_impl, _pool_impl
+from .rotary import _rotary_impl
 from .route_weights import _route_weights_bwd_impl, _route_weights_impl
 from .local_attention import _local_attention_qf_impl
 from .sparse_attention import (FRAG_ELEMS, _kv_fragments_impl, _kv_fragments_rows_impl,
@@ -367,6 +369,51 @@ def _(entropy, indices):
     B, L, H, K = indices.shape
     return entropy.new_empty(B, L, H, K, dtype=torch.float32)
 
+
+
+# -- rotary positions, paged cache ----------------------------------------
+# Defined by schema: a call costs 4-5 us of host time against 14-16 us through
+# custom_op, which is most of the time of these operators at one new token.
+_lib = torch.library.Library("mrsa", "FRAGMENT")
+
+
+def _define(schema, impl):
+    name = schema.split("(")[0]
+    _lib.define(schema)
+    _lib.impl(name, impl, "CUDA")
+    return torch.library.register_fake(f"mrsa::{name}", lib=_lib)
+
+
+@_define("rotary(Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, "
+         "bool interleaved, bool inverse) -> (Tensor, Tensor)", _rotary_impl)
+def _(q, k, cos, sin, positions, interleaved, inverse):
+    B, L, _, D = q.shape
+    return q.new_empty(q.shape), q.new_empty((B, L, 0 if k is None else k.shape[2], D))
+
+
+@_define("paged_append_(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, "
+         "Tensor page_table, Tensor slots, Tensor? q, Tensor? cos, Tensor? sin, "
+         "Tensor? positions, bool interleaved) -> Tensor", _paged_append_impl)
+def _(k, v, k_pages, v_pages, page_table, slots, q, cos, sin, positions, interleaved):
+    B, L, _, D = k.shape
+    return k.new_empty((B, L, 0 if q is None else q.shape[2], D))
+
+
+@_define("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, "
+         "Tensor cache_lens, Tensor? query_starts, int max_len, bool causal, int window, "
+         "float sm_scale, int parts) -> (Tensor, Tensor)", _paged_attention_impl)
+def _(q, k_pages, v_pages, page_table, cache_lens, query_starts, max_len, causal, window,
+      sm_scale, parts):
+    B, Lq, Hq, _ = q.shape
+    return q.new_empty(q.shape), q.new_empty((B, Lq, Hq), dtype=torch.float32)
+
+
+@_define("copy_pages_(Tensor(a!) k_pages, Tensor(b!) v_pages, int[] src, int[] dst) -> ()",
+         _copy_pages_impl)
+def _(k_pages, v_pages, src, dst):
+    return None
+
+
 OPERATORS = (
     "kv_fragments", "kv_fragments_rows_", "q_fragments", "local_attention",
     "local_attention_qf", "chunk_attn_pool", "kv_fragments_pool",
@@ -374,5 +421,5 @@ OPERATORS = (
     "selected_attention", "selected_attention_bwd", "fuse_hils_outputs", "fuse_hils_outputs_bwd",
     "remote_drop_mask",
     "remote_drop_mask_rows", "candidate_token_scores", "token_keep", "token_keep_entropy",
-    "gather_selected_chunk_entropy",
+    "gather_selected_chunk_entropy", "rotary", "paged_append_", "paged_attention", "copy_pages_",
 )
