@@ -78,7 +78,7 @@ struct PagedArgs {
   int B, Lq, Hq, Hkv, G, M;   // M = Lq G columns
   int causal, window;         // window < 0: none
   float scale_log2;
-  int parts, part_keys, col_tiles;
+  int parts, part_keys, col_tiles, tile_cols;
   uint16_t* out;
   float* lse;
   float* part_out;            // parts > 1: [B, Hkv, M, parts, D]
@@ -268,15 +268,10 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
           S[t][e] = ok ? S[t][e] : neg_inf();
         }
     }
-    float top = neg_inf();
+    float top = S[0][0];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        S[t][e] *= a.scale_log2;   // (-inf stays: the scale is positive)
-        top = __builtin_fmaxf(top, S[t][e]);
-      }
-    top = across4_max(top);
+    for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, S[i >> 2][i & 3]);
+    top = across4_max(top) * a.scale_log2;   // (-inf stays: the scale is positive)
     if (__builtin_amdgcn_ballot_w64(top > mx + kSlack) != 0) {
       const float to = __builtin_fmaxf(mx, top);
       const float f = to == neg_inf() ? 1.f : exp2_hw(mx - to);
@@ -293,7 +288,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        P[4 * t + e] = exp2_hw(S[t][e] - off);
+        P[4 * t + e] = exp2_hw(__builtin_fmaf(S[t][e], a.scale_log2, -off));
         sum += P[4 * t + e];
       }
     const u32x4_t Pb = {T::pack(P[0], P[1]), T::pack(P[2], P[3]), T::pack(P[4], P[5]),
@@ -315,10 +310,6 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
         if (!live[kk >> 4] || key < r.lo || key >= r.end) continue;
         const int from = 16 * ((kk & 15) >> 2) + col;
         const int slot = 4 * (kk >> 4) + (kk & 3);
-        float pv = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pv = e == slot ? P[e] : pv;
-        const float pk = __shfl(pv, from, 64);
         const bool ok = (__shfl(seen, from, 64) >> slot) & 1;
         const int pg = __builtin_amdgcn_readfirstlane(page_of(key));
         const uint16_t* vp = a.v + h * a.v_sh + pg * a.v_sp + (key & page_mask) * a.v_sr;
@@ -327,7 +318,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t w = vp[16 * t + 4 * grp + e];
-            if (ok && (w & T::kExp) == T::kExp) O[t][e] += pk * T::value(w);
+            if (ok && (w & T::kExp) == T::kExp) O[t][e] += T::value(w);  // (p > 0: its size is no matter)
           }
       }
     }
@@ -393,6 +384,317 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
   if (d2 == 0) a.lse[row] = total == 0.f ? neg_inf() : kLn2 * (M + log2_hw(total));
 }
 
+// Many columns: a workgroup of up to eight waves, 32 columns each, over tiles of
+// 64 keys that all its waves read from LDS.  K and V rows come by global->LDS
+// DMA into a two-slot ring, one barrier per tile; K is read along the row
+// (operand A of S^T), V by transposing reads (operand A of O^T).
+constexpr int kBlockKeys = 64;
+constexpr int kBlockCols = 32;             // of a wave
+constexpr int kBlockWaves = 8;
+
+template <class T, int D>
+__global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs a) {
+  constexpr int KS = D / 32, DT = D / 16, NT = kBlockCols / 16;
+  constexpr int ROWB = 2 * D;
+  constexpr int UNITS = D / 8;
+  constexpr int PIECE = 64 / UNITS;        // rows of one DMA instruction (1 KB)
+  constexpr int PIECES = kBlockKeys / PIECE;  // of K, and as many of V
+  constexpr int TILEB = kBlockKeys * ROWB;
+  constexpr int SLOTB = 2 * TILEB;
+  extern __shared__ __align__(256) unsigned char ring[];
+  int* flag = reinterpret_cast<int*>(ring + 2 * SLOTB);  // last tile (+ 1) with a value not finite
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int waves = __builtin_amdgcn_readfirstlane((int)blockDim.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  int64_t id = blockIdx.x;
+  const int h = (int)(id % a.Hkv);
+  id /= a.Hkv;
+  const int part = (int)(id % a.parts);
+  id /= a.parts;
+  const int ct = (int)(id % a.col_tiles);
+  const int b = (int)(id / a.col_tiles);
+  const int cols = kBlockCols * waves;
+  const int n = length_of(a, b), p0 = start_of(a, b, n);
+  const Range r = tile_range(a, n, p0, ct * cols, cols);
+  const int first = r.start + part * a.part_keys;
+  const int last = min(r.end, first + a.part_keys);
+  if (part > 0 && first >= r.end) return;
+  const int c0 = ct * cols + kBlockCols * wave;   // this wave's columns
+  const Range w = tile_range(a, n, p0, min(c0, a.M), kBlockCols);
+
+  // ---- this lane's columns
+  bool padding[NT];
+  int lo[NT], hi[NT];
+  u32x4_t Q[NT][KS];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int m = c0 + 16 * t + col;
+    const bool cok = m < a.M;
+    const int qi = cok ? m / a.G : 0, qg = cok ? m - qi * a.G : 0;
+    const int pos = p0 + qi;
+    padding[t] = !cok || pos < 0 || pos >= n;
+    lo[t] = hi[t] = 0;
+    if (!padding[t]) seen_by(a, n, pos, lo[t], hi[t]);
+    const uint16_t* qp = a.q + b * a.q_sb + qi * a.q_sl + (h * a.G + qg) * a.q_sh + 8 * grp;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      Q[t][s] = u32x4_t{0, 0, 0, 0};
+      if (cok) Q[t][s] = *reinterpret_cast<const u32x4_t*>(qp + 32 * s);
+    }
+  }
+  f32x4_t O[NT][DT];
+  float mx[NT], sum[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    mx[t] = neg_inf();
+    sum[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) O[t][d] = zero4();
+  }
+  if (tid == 0) *flag = 0;
+
+  // ---- the stream.  DMA instruction x fills rows PIECE x .. of K (x < PIECES) or V: lane
+  // (row lane / UNITS, unit lane % UNITS) fetches the unit that belongs there.
+  const int32_t* table = a.table + b * a.table_stride;
+  const int page_mask = (1 << a.page_shift) - 1;
+  const int lrow = lane / UNITS, lunit = (lane % UNITS) ^ (swizzle<D>(lrow) & ~1);
+  // (row x + lrow's swizzle is lrow's with these bits of x flipped)
+  auto flips = [&](int x) { return D == 128 ? 2 * (x & 4) + ((x >> 3) & 1) : (x >> 3) & 1; };
+  const uint16_t* kb = a.k + h * a.k_sh + lrow * a.k_sr;
+  const uint16_t* vb = a.v + h * a.v_sh + lrow * a.v_sr;
+  auto page_at = [&](int key) -> int {
+    const int e = key >> a.page_shift;
+    return __builtin_amdgcn_readfirstlane(e < a.table_width ? table[e] : -1);
+  };
+  int pages[4], next_pages[4];             // of the tile's sixteens of keys
+  auto fetch_pages = [&](int (&to)[4], int base) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = page_at(base + 16 * i);
+  };
+  auto issue = [&](int slot, int base, const int (&pg)[4]) {
+    unsigned char* dst = ring + slot * SLOTB;
+    for (int x = wave; x < 2 * PIECES; x += waves) {
+      const bool is_v = x >= PIECES;
+      const int r0 = (is_v ? x - PIECES : x) * PIECE;
+      int page = r0 < 16 ? pg[0] : r0 < 32 ? pg[1] : r0 < 48 ? pg[2] : pg[3];
+      if (page < 0 || page >= a.num_pages) page = 0;  // a page that exists; its values are not used
+      const int64_t row = (base + r0) & page_mask;
+      const uint16_t* src = is_v ? vb + page * a.v_sp + row * a.v_sr : kb + page * a.k_sp + row * a.k_sr;
+      src += 8 * (lunit ^ flips(r0));
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) uint32_t*)src,
+          (lds_void_t*)(dst + (is_v ? TILEB : 0) + r0 * ROWB), 16, 0, 0);
+    }
+  };
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(Q[t][s]));
+  const int tiles = first < last ? (last - first + kBlockKeys - 1) / kBlockKeys : 0;
+  if (tiles > 0) {
+    fetch_pages(pages, first);
+    issue(0, first, pages);
+    if (tiles > 1) fetch_pages(next_pages, first + kBlockKeys);
+  }
+  const uint32_t arow = ROWB * col + 16u * (uint32_t)(grp ^ swizzle<D>(col));
+  const int rt = 4 * grp + (col >> 2);
+  const uint32_t trow = ROWB * rt + 16u * (uint32_t)(((col >> 1) & 1) ^ swizzle<D>(rt)) + 8u * (col & 1);
+
+  for (int t = 0; t < tiles; ++t) {
+    const int base = first + t * kBlockKeys;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    bool live[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) live[i] = pages[i] >= 0 && pages[i] < a.num_pages;
+    if (t + 1 < tiles) {
+      issue((t + 1) & 1, base + kBlockKeys, next_pages);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pages[i] = next_pages[i];
+      if (t + 2 < tiles) fetch_pages(next_pages, base + 2 * kBlockKeys);
+    }
+    asm volatile("" ::: "memory");
+    unsigned char* slot = ring + (t & 1) * SLOTB;
+    const uint32_t sbase = lds_addr(slot);
+    const bool whole = live[0] && live[1] && live[2] && live[3];
+    const bool mixed = !whole || base < r.inner_lo || base + kBlockKeys > r.inner_hi;
+    bool dirty = false;
+    if (mixed) {
+      // V rows that no column sees become zeros; values that are not finite
+      // are taken out (a column that does not see them must not get 0 x inf)
+      // and added one by one below.
+      bool odd = false;
+      for (int x = tid; x < kBlockKeys * UNITS; x += 64 * waves) {
+        const int row = x / UNITS, key = base + row;
+        u32x4_t* at = reinterpret_cast<u32x4_t*>(slot + TILEB + 16 * x);
+        const bool lv = row < 16 ? live[0] : row < 32 ? live[1] : row < 48 ? live[2] : live[3];
+        if (!lv || key < r.lo || key >= r.end) {
+          *at = u32x4_t{0, 0, 0, 0};
+          continue;
+        }
+        u32x4_t v = *at;
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool b0 = (v[e] & T::kExp) == T::kExp, b1 = ((v[e] >> 16) & T::kExp) == T::kExp;
+          bad |= b0 || b1;
+          if (b0) v[e] &= 0xffff0000u;
+          if (b1) v[e] &= 0x0000ffffu;
+        }
+        if (bad) *at = v;
+        odd |= bad;
+      }
+      if (odd) *flag = t + 1;
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      dirty = *(volatile int*)flag == t + 1;
+    }
+    // ---- scores
+    f32x4_t S[NT][4];
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+      for (int m = 0; m < 4; ++m) S[c][m] = zero4();
+    {
+      const uint32_t at = sbase + arow;
+      constexpr int AHEAD = 4;
+      u32x4_t x[4 * KS];
+      auto operand = [&](int o) {  // keys 16 (o & 3) .., dims 32 (o >> 2) ..
+        return lds_read16((at ^ (64u * (o >> 2))) + 16u * ROWB * (o & 3));
+      };
+#pragma unroll
+      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int o = 0; o < 4 * KS; ++o) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c) S[c][o & 3] = T::mfma(x[o], Q[c][o >> 2], S[c][o & 3]);
+        if (o + AHEAD < 4 * KS) x[o + AHEAD] = operand(o + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    uint32_t seen[NT];
+    u32x4_t Pb[NT][2];
+    if (!whole || base < w.inner_lo || base + kBlockKeys > w.inner_hi) {
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        seen[c] = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = base + 16 * (i >> 2) + 4 * grp + (i & 3);
+          const bool ok = live[i >> 2] && key >= lo[c] && key < hi[c];
+          if (ok) seen[c] |= 1u << i;
+          S[c][i >> 2][i & 3] = ok ? S[c][i >> 2][i & 3] : neg_inf();
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NT; ++c) seen[c] = 0xffffu;
+    }
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+      const float top = across4_max(max16_raw(S[c])) * a.scale_log2;
+      if (__builtin_amdgcn_ballot_w64(top > mx[c] + kSlack) != 0) {
+        const float to = __builtin_fmaxf(mx[c], top);
+        const float f = to == neg_inf() ? 1.f : exp2_hw(mx[c] - to);
+        mx[c] = to;
+        sum[c] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) O[c][d] *= f;
+      }
+      const float off = mx[c] == neg_inf() ? 0.f : mx[c];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = exp2_hw(__builtin_fmaf(S[c][i >> 2][i & 3], a.scale_log2, -off));
+        S[c][i >> 2][i & 3] = p;
+        sum[c] += p;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        Pb[c][k] = u32x4_t{T::pack(S[c][2 * k][0], S[c][2 * k][1]), T::pack(S[c][2 * k][2], S[c][2 * k][3]),
+                           T::pack(S[c][2 * k + 1][0], S[c][2 * k + 1][1]),
+                           T::pack(S[c][2 * k + 1][2], S[c][2 * k + 1][3])};
+    }
+    // ---- V^T . P^T
+    {
+      const uint32_t at = sbase + TILEB + trow;
+      constexpr int AHEAD = 4;
+      u32x4_t x[2 * DT];
+      auto operand = [&](int o) {  // dims 16 (o >> 1) .., keys 32 (o & 1) ..
+        const uint32_t ad = (at ^ (32u * (o >> 1))) + 32u * ROWB * (o & 1);
+        const u32x2_t y0 = read_transposed(ad), y1 = read_transposed(ad + 16u * ROWB);
+        return u32x4_t{y0[0], y0[1], y1[0], y1[1]};
+      };
+#pragma unroll
+      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int o = 0; o < 2 * DT; ++o) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c) O[c][o >> 1] = T::mfma(x[o], Pb[c][o & 1], O[c][o >> 1]);
+        if (o + AHEAD < 2 * DT) x[o + AHEAD] = operand(o + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (dirty) {
+      for (int kk = 0; kk < kBlockKeys; ++kk) {
+        const int key = base + kk;
+        const bool lv = kk < 16 ? live[0] : kk < 32 ? live[1] : kk < 48 ? live[2] : live[3];
+        if (!lv || key < r.lo || key >= r.end) continue;
+        const int from = 16 * ((kk & 15) >> 2) + col, slot_i = 4 * (kk >> 4) + (kk & 3);
+        const uint16_t* vp = a.v + h * a.v_sh + page_at(key) * a.v_sp + (int64_t)(key & page_mask) * a.v_sr;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          const bool ok = (__shfl(seen[c], from, 64) >> slot_i) & 1;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x = vp[16 * d + 4 * grp + e];
+              if (ok && (x & T::kExp) == T::kExp) O[c][d][e] += T::value(x);
+            }
+        }
+      }
+    }
+  }
+
+  // ---- out: lane (col, grp) holds dims 16 d + 4 grp .. of its columns
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int m = c0 + 16 * t + col;
+    float total = across4_sum(sum[t]);
+    if (padding[t]) {  // (its scores were not masked in tiles that every row sees)
+      mx[t] = neg_inf();
+      total = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) O[t][d] = zero4();
+    }
+    if (m >= a.M) continue;
+    if (a.parts > 1) {
+      const int64_t at = (((int64_t)b * a.Hkv + h) * a.M + m) * a.parts + part;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        *reinterpret_cast<f32x4_t*>(a.part_out + at * D + 16 * d + 4 * grp) = O[t][d];
+      if (grp == 0) {
+        a.part_ml[2 * at] = mx[t];
+        a.part_ml[2 * at + 1] = total;
+      }
+      continue;
+    }
+    const int qi = m / a.G;
+    const int64_t row = ((int64_t)b * a.Lq + qi) * a.Hq + h * a.G + (m - qi * a.G);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      u32x2_t o = {0u, 0u};
+      if (total != 0.f)
+        o = u32x2_t{T::pack(O[t][d][0] * inv, O[t][d][1] * inv), T::pack(O[t][d][2] * inv, O[t][d][3] * inv)};
+      *reinterpret_cast<u32x2_t*>(a.out + row * D + 16 * d + 4 * grp) = o;
+    }
+    if (grp == 0) a.lse[row] = total == 0.f ? neg_inf() : kLn2 * (mx[t] + log2_hw(total));
+  }
+}
+
 // One workgroup per column: the parts' maxima and sums, then their outputs.
 template <class T, int D>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(PagedArgs a) {
@@ -407,7 +709,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(PagedArgs a) {
   const int64_t bh = c / a.M;
   const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv);
   const int n = length_of(a, b);
-  const Range r = tile_range(a, n, start_of(a, b, n), m & ~15, 16);
+  const Range r = tile_range(a, n, start_of(a, b, n), m / a.tile_cols * a.tile_cols, a.tile_cols);
   const int np = max(1, (r.end - r.start + a.part_keys - 1) / a.part_keys);
   const float* ml = a.part_ml + 2 * c * a.parts;
   float M = neg_inf();
@@ -433,7 +735,15 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(PagedArgs a) {
   const int d4 = tid % TPR;
   const f32x4_t* po = reinterpret_cast<const f32x4_t*>(a.part_out + c * a.parts * D) + d4;
   f32x4_t acc = zero4();
-  for (int p = tid / TPR; p < np; p += LANES) acc += weight[p] * po[(int64_t)p * TPR];
+  // eight rows in flight per thread (a row past the last is the last one, with no part in the sum)
+  for (int p0 = tid / TPR; p0 < np; p0 += 8 * LANES) {
+    f32x4_t v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = po[(int64_t)min(p0 + u * LANES, np - 1) * TPR];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (p0 + u * LANES < np) acc += weight[p0 + u * LANES] * v[u];
+  }
   acc_l[tid] = acc;
   __syncthreads();
   if (tid >= TPR) return;
@@ -447,10 +757,20 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(PagedArgs a) {
   if (tid == 0) a.lse[row] = total == 0.f ? neg_inf() : kLn2 * (M + log2_hw(total));
 }
 
-// Most keys that one column tile's columns can see.
-int64_t span_bound(int64_t max_len, int64_t q_len, int64_t group, int64_t window, int causal) {
+// Columns of a workgroup: up to 16 the streaming kernel; more, whole waves of the
+// block kernel, as even as they come.
+int columns_of(int64_t M) {
+  if (M <= 16) return 16;
+  const int64_t groups = (M + kBlockCols - 1) / kBlockCols;
+  const int64_t tiles = (groups + kBlockWaves - 1) / kBlockWaves;
+  return (int)((groups + tiles - 1) / tiles * kBlockCols);
+}
+
+// Most keys that the columns of one workgroup can see.
+int64_t span_bound(int64_t max_len, int64_t q_len, int64_t group, int64_t cols, int64_t window,
+                   int causal) {
   if (window < 0) return max_len;
-  const int64_t rows = std::min<int64_t>(q_len, 16 / group + 2);
+  const int64_t rows = std::min<int64_t>(q_len, cols / group + 2);
   return std::min(max_len, rows + (causal ? 1 : 2) * window + 1);
 }
 
@@ -459,7 +779,16 @@ int launch(const PagedArgs& a, hipStream_t stream) {
   const int64_t grid = (int64_t)a.B * a.Hkv * a.col_tiles * a.parts;
   const int64_t cols = (int64_t)a.B * a.Hkv * a.M;
   if (grid > 0x7fffffff || cols > 0x7fffffff) return MRSA_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+  if (a.tile_cols == 16) {
+    hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+  } else {
+    const size_t lds = 4 * kBlockKeys * 2 * D + 16;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_block_kernel<T, D>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+      return MRSA_ERR_LAUNCH;
+    hipLaunchKernelGGL((paged_block_kernel<T, D>), dim3((unsigned)grid),
+                       dim3(64 * a.tile_cols / kBlockCols), lds, stream, a);
+  }
   int st = mrsa_launch_status();
   if (st != MRSA_OK || a.parts == 1) return st;
   hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)cols), dim3(kThreads), 0, stream, a);
@@ -536,8 +865,10 @@ extern "C" int mrsa_paged_attention_fwd(
   a.window = window < 0 ? -1 : (int)std::min<int64_t>(window, most);
   a.scale_log2 = sm_scale * kLog2e;
   a.parts = (int)parts;
-  a.col_tiles = (a.M + 15) / 16;
-  const int64_t span = span_bound(max_len, q_len, a.G, a.window, a.causal) + kTile - 1;
+  a.tile_cols = columns_of(a.M);
+  a.col_tiles = (a.M + a.tile_cols - 1) / a.tile_cols;
+  const int64_t span =
+      span_bound(max_len, q_len, a.G, a.tile_cols, a.window, a.causal) + kTile - 1;
   a.part_keys = (int)(((span + parts - 1) / parts + kStep - 1) / kStep * kStep);
   a.out = (uint16_t*)out;
   a.lse = lse;

@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kHeadsPerThread = 4;
+constexpr int64_t kManyUnits = 256 * 1024;  // head units from which a thread takes that many
 
 // One stream of heads: [batch, row, head] strides in elements, last dim dense.
 struct Heads {
@@ -72,8 +73,7 @@ struct alignas(16) Vec {
   T e[Traits<T>::kPer16];
 };
 
-// Base of token (b, l)'s rows in a dense or paged destination; false if the
-// token has no place.
+// Page and row of token (b, l); false if the token has no place.
 template <class T, bool PAGED>
 __device__ __forceinline__ bool cache_row(const RotaryArgs& a, int b, int l, int64_t& page,
                                           int64_t& row) {
@@ -116,8 +116,56 @@ __device__ __forceinline__ void turn(Vec<T>& x, Vec<T>& y, const float* c, const
   }
 }
 
+// The stream, place and rows of one head out of q, k and (paged) v.  Fields are
+// selected value by value: a pointer into the arguments would put them in
+// scratch memory.
+template <class T, bool PAGED>
+struct Rows {
+  const T *q_in, *k_in, *v_in;
+  T *q_out, *k_out, *v_out;
+  bool placed;
+
+  __device__ __forceinline__ Rows(const RotaryArgs& a, int b, int l) {
+    q_in = (const T*)a.q.src + b * a.q.sb + l * a.q.sl;
+    k_in = (const T*)a.k.src + b * a.k.sb + l * a.k.sl;
+    q_out = (T*)a.q.dst + b * a.q.db + l * a.q.dl;
+    placed = true;
+    if constexpr (PAGED) {
+      int64_t page = 0, row = 0;
+      placed = cache_row<T, PAGED>(a, b, l, page, row);
+      v_in = (const T*)a.v.src + b * a.v.sb + l * a.v.sl;
+      k_out = (T*)a.k.dst + page * a.k.db + row * a.k.dl;
+      v_out = (T*)a.v.dst + page * a.v.db + row * a.v.dl;
+    } else {
+      k_out = (T*)a.k.dst + b * a.k.db + l * a.k.dl;
+    }
+  }
+  // Head h of all; `turns`: q and k heads, `there`: it has a place to go.
+  __device__ __forceinline__ void head(const RotaryArgs& a, int h, const T*& in, T*& out,
+                                       bool& turns, bool& there) const {
+    const bool is_q = h < a.q.heads;
+    const bool is_v = PAGED && h >= a.q.heads + a.k.heads;
+    int hh = is_q ? h : h - a.q.heads;
+    in = is_q ? q_in : k_in;
+    out = is_q ? q_out : k_out;
+    int64_t sh = is_q ? a.q.sh : a.k.sh, dh = is_q ? a.q.dh : a.k.dh;
+    if constexpr (PAGED) {
+      hh = is_v ? hh - a.k.heads : hh;
+      in = is_v ? v_in : in;
+      out = is_v ? v_out : out;
+      sh = is_v ? a.v.sh : sh;
+      dh = is_v ? a.v.dh : dh;
+    }
+    in += hh * sh;
+    out += hh * dh;
+    turns = !is_v;
+    there = is_q || placed;
+  }
+};
+
 // 16-byte units; PAGED: k and v go to pages (v is copied), else only q and k.
-template <class T, bool INTERLEAVED, bool PAGED>
+// HEADS: heads of a thread.
+template <class T, bool INTERLEAVED, bool PAGED, int HEADS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
   constexpr int E = Traits<T>::kPer16;
   constexpr int TN = INTERLEAVED ? E / 2 : E;  // table values of a unit
@@ -133,74 +181,53 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
     const int hs = rem / a.units;
     const int u = rem - hs * a.units;
     const int b = (int)tok / a.L, l = (int)tok - b * a.L;
-    int64_t page = 0, row = 0;
-    bool placed = false;
-    if constexpr (PAGED) placed = cache_row<T, PAGED>(a, b, l, page, row);
+    const Rows<T, PAGED> rows(a, b, l);
     const bool rotate = u < rot_units;
+    // dims of this unit: [at, at + E) and, half layout, [at2, at2 + E)
+    const int at = rotate ? u * E : tail_at + (u - rot_units) * E;
+    const int at2 = at + a.half;
+    const bool two = !INTERLEAVED && rotate;
+    Vec<T> x[HEADS], y[HEADS];
+    T* out[HEADS];
+    bool turns[HEADS], there[HEADS];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+      const int h = hs + i * a.head_slots;
+      const T* in;
+      rows.head(a, min(h, total_heads - 1), in, out[i], turns[i], there[i]);
+      there[i] &= h < total_heads;
+      x[i] = *reinterpret_cast<const Vec<T>*>(in + at);
+      if (two) y[i] = *reinterpret_cast<const Vec<T>*>(in + at2);
+    }
     float c[TN], s[TN];
     if (rotate) {
       const int64_t pos = a.positions ? a.positions[b * a.ps_b + l * a.ps_l] : l;
       if (pos >= 0 && pos < a.table_rows) {
-        const float4* cp = reinterpret_cast<const float4*>(a.cos_t + pos * a.half + u * TN);
-        const float4* sp = reinterpret_cast<const float4*>(a.sin_t + pos * a.half + u * TN);
+        const float* cp = a.cos_t + pos * a.half + u * TN;
+        const float* sp = a.sin_t + pos * a.half + u * TN;
         if constexpr (TN >= 4) {
 #pragma unroll
           for (int i = 0; i < TN / 4; ++i) {
-            const float4 cv = cp[i], sv = sp[i];
-            c[4 * i] = cv.x, c[4 * i + 1] = cv.y, c[4 * i + 2] = cv.z, c[4 * i + 3] = cv.w;
-            s[4 * i] = sv.x, s[4 * i + 1] = sv.y, s[4 * i + 2] = sv.z, s[4 * i + 3] = sv.w;
+            const f32x4_t cv = reinterpret_cast<const f32x4_t*>(cp)[i];
+            const f32x4_t sv = reinterpret_cast<const f32x4_t*>(sp)[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[4 * i + j] = cv[j], s[4 * i + j] = a.sign * sv[j];
           }
         } else {
-          const float2 cv = *reinterpret_cast<const float2*>(cp);
-          const float2 sv = *reinterpret_cast<const float2*>(sp);
-          c[0] = cv.x, c[1] = cv.y, s[0] = sv.x, s[1] = sv.y;
-        }
+          const f32x2_t cv = *reinterpret_cast<const f32x2_t*>(cp);
+          const f32x2_t sv = *reinterpret_cast<const f32x2_t*>(sp);
 #pragma unroll
-        for (int i = 0; i < TN; ++i) s[i] *= a.sign;
+          for (int j = 0; j < 2; ++j) c[j] = cv[j], s[j] = a.sign * sv[j];
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < TN; ++i) c[i] = s[i] = __builtin_nanf("");
       }
     }
-    // dims of this unit: [at, at + E) and, half layout, [at2, at2 + E)
-    const int at = rotate ? u * E : tail_at + (u - rot_units) * E;
-    const int at2 = at + a.half;
-    const bool two = !INTERLEAVED && rotate;
-    Vec<T> x[kHeadsPerThread], y[kHeadsPerThread];
-    T* out[kHeadsPerThread];
-    int kind[kHeadsPerThread];  // 0 none, 1 q or k, 2 v
 #pragma unroll
-    for (int i = 0; i < kHeadsPerThread; ++i) {
-      int h = hs + i * a.head_slots;
-      kind[i] = 0;
-      if (h >= total_heads) continue;
-      const Heads* seg = &a.q;
-      bool paged = false;
-      if (h >= a.q.heads) {
-        h -= a.q.heads;
-        seg = &a.k;
-        paged = PAGED;
-        if (PAGED && h >= a.k.heads) {
-          h -= a.k.heads;
-          seg = &a.v;
-          kind[i] = 2;
-        }
-      }
-      if (kind[i] == 0) kind[i] = 1;
-      if (paged && !placed) {
-        kind[i] = 0;
-        continue;
-      }
-      const T* in = (const T*)seg->src + b * seg->sb + l * seg->sl + h * seg->sh;
-      out[i] = (T*)seg->dst + (paged ? page * seg->db + row * seg->dl : b * seg->db + l * seg->dl) +
-               h * seg->dh;
-      x[i] = *reinterpret_cast<const Vec<T>*>(in + at);
-      if (two) y[i] = *reinterpret_cast<const Vec<T>*>(in + at2);
-    }
-#pragma unroll
-    for (int i = 0; i < kHeadsPerThread; ++i) {
-      if (!kind[i]) continue;
-      if (rotate && kind[i] == 1) turn<T, INTERLEAVED>(x[i], y[i], c, s);
+    for (int i = 0; i < HEADS; ++i) {
+      if (!there[i]) continue;
+      if (rotate && turns[i]) turn<T, INTERLEAVED>(x[i], y[i], c, s);
       *reinterpret_cast<Vec<T>*>(out[i] + at) = x[i];
       if (two) *reinterpret_cast<Vec<T>*>(out[i] + at2) = y[i];
     }
@@ -218,26 +245,15 @@ __global__ void __launch_bounds__(kThreads) rotary_scalar_kernel(RotaryArgs a) {
     const int64_t tok = (int64_t)blockIdx.x * a.tokens_per_block + ti;
     if (tok >= a.tokens) return;
     const int rem = lid - ti * per_token;
-    int h = rem / a.units;
+    const int h = rem / a.units;
     const int u = rem - h * a.units;
     const int b = (int)tok / a.L, l = (int)tok - b * a.L;
-    const Heads* seg = &a.q;
-    bool paged = false, turned = true;
-    if (h >= a.q.heads) {
-      h -= a.q.heads;
-      seg = &a.k;
-      paged = PAGED;
-      if (PAGED && h >= a.k.heads) {
-        h -= a.k.heads;
-        seg = &a.v;
-        turned = false;
-      }
-    }
-    int64_t page = 0, row = 0;
-    if (PAGED && paged && !cache_row<T, PAGED>(a, b, l, page, row)) continue;
-    const T* in = (const T*)seg->src + b * seg->sb + l * seg->sl + h * seg->sh;
-    T* out = (T*)seg->dst + (paged ? page * seg->db + row * seg->dl : b * seg->db + l * seg->dl) +
-             h * seg->dh;
+    const Rows<T, PAGED> rows(a, b, l);
+    const T* in;
+    T* out;
+    bool turned, there;
+    rows.head(a, h, in, out, turned, there);
+    if (!there) continue;
     if (u >= a.half) {
       const int at = u + a.half;
       out[at] = in[at];
@@ -276,13 +292,15 @@ int launch(RotaryArgs a, bool interleaved, hipStream_t stream) {
     vec = vec && ((uintptr_t)s->src | (uintptr_t)s->dst) % 16 == 0 &&
           (s->sb | s->sl | s->sh | s->db | s->dl | s->dh) % E == 0;
   }
+  int heads_each = 1;
   if (vec) {
     const int rot = a.half / (interleaved ? E / 2 : E);
     a.units = rot + (a.D - 2 * a.half) / E;
     // Few tokens: a head per thread, so that as many threads as there are work; many: the
     // table row of a thread serves kHeadsPerThread heads.
     const int64_t one = (int64_t)a.tokens * heads * a.units;
-    a.head_slots = one < 256 * 1024 ? heads : (heads + kHeadsPerThread - 1) / kHeadsPerThread;
+    if (one >= kManyUnits) heads_each = kHeadsPerThread;
+    a.head_slots = (heads + heads_each - 1) / heads_each;
   } else {
     a.units = a.D - a.half;
     a.head_slots = heads;
@@ -290,10 +308,14 @@ int launch(RotaryArgs a, bool interleaved, hipStream_t stream) {
   const int per_token = a.units * a.head_slots;
   a.tokens_per_block = std::max(1, kThreads / per_token);
   const unsigned blocks = (unsigned)((a.tokens + a.tokens_per_block - 1) / a.tokens_per_block);
-  void (*kern)(RotaryArgs) =
-      vec ? (interleaved ? rotary_kernel<T, true, PAGED> : rotary_kernel<T, false, PAGED>)
-          : (interleaved ? rotary_scalar_kernel<T, true, PAGED>
-                         : rotary_scalar_kernel<T, false, PAGED>);
+  void (*kern)(RotaryArgs);
+  if (!vec)
+    kern = interleaved ? rotary_scalar_kernel<T, true, PAGED> : rotary_scalar_kernel<T, false, PAGED>;
+  else if (heads_each == 1)
+    kern = interleaved ? rotary_kernel<T, true, PAGED, 1> : rotary_kernel<T, false, PAGED, 1>;
+  else
+    kern = interleaved ? rotary_kernel<T, true, PAGED, kHeadsPerThread>
+                       : rotary_kernel<T, false, PAGED, kHeadsPerThread>;
   hipLaunchKernelGGL(kern, dim3(blocks), dim3(kThreads), 0, stream, a);
   return mrsa_launch_status();
 }

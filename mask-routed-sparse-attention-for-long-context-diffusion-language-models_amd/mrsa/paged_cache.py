@@ -138,10 +138,11 @@ def paged_cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
 def cache_parts(batch: int, q_len: int, q_heads: int, kv_heads: int, span: int) -> int:
     """Pieces that paged_cached_attention cuts the visible span into."""
 
-    tiles = batch * kv_heads * -(-q_len * (q_heads // kv_heads) // 16)
+    cols = q_len * (q_heads // kv_heads)
+    tiles = batch * kv_heads * -(-cols // (16 if cols <= 16 else 256))
     if tiles == 0 or span <= 0:
         return 1
-    keys = max(128, -(-span * tiles // 1536))
+    keys = max(128, -(-span * tiles // (1536 if cols <= 16 else 512)))
     keys = -(-keys // 128) * 128
     return max(1, min(MAX_PARTS, -(-span // keys)))
 
@@ -231,7 +232,8 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if parts is None:
         span = max_len
         if window >= 0:
-            span = min(span, 16 * Hkv // Hq + 3 + (1 if causal else 2) * window)
+            span = min(span, Lq, 256) + (1 if causal else 2) * window
+            span = min(span, max_len)
         parts = cache_parts(B, Lq, Hq, Hkv, span)
     return torch.ops.mrsa.paged_attention.default(q, k_pages, v_pages, page_table, cache_lens,
                                                   query_starts, max_len, bool(causal), window,
