@@ -28,8 +28,8 @@ using namespace mrsa;
 
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kThreads = 256;              // of the joining kernel
+constexpr int kWaves = 8;                  // of the streaming kernel
 constexpr int kTile = 32;                  // keys of a wave's tile
 constexpr int kStep = kWaves * kTile;      // keys of a workgroup's round
 constexpr int kMaxParts = 1024;
@@ -85,15 +85,29 @@ struct PagedArgs {
   float* part_ml;             // parts > 1: [B, Hkv, M, parts, 2]
 };
 
+// Page table and lengths are read through the constant address space, that is by
+// scalar loads (nothing writes them while the kernel runs): a vector load's
+// result would be waited for behind every K and V load in flight.
+typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
+__device__ __forceinline__ scalar_ints scalars(const int32_t* p) {
+  return (scalar_ints)(uintptr_t)p;
+}
+// The page of sixteen keys from `key` on (wave-uniform); -1 past the table.
+__device__ __forceinline__ int page_at(const PagedArgs& a, scalar_ints table, int key) {
+  const int e = key >> a.page_shift;
+  const int page = table[min(e, a.table_width - 1)];
+  return e < a.table_width ? page : -1;
+}
+
 // Rows in use of sequence b.
 __device__ __forceinline__ int length_of(const PagedArgs& a, int b) {
-  const int n = min(a.lens[b], a.max_len);
+  const int n = min(scalars(a.lens)[b], a.max_len);
   const int64_t room = (int64_t)a.table_width << a.page_shift;
   return max(0, (int)min((int64_t)n, room));
 }
 // Position of query row 0 of sequence b.
 __device__ __forceinline__ int start_of(const PagedArgs& a, int b, int n) {
-  return a.starts ? max(-kFar, min(kFar, a.starts[b])) : n - a.Lq;
+  return a.starts ? max(-kFar, min(kFar, scalars(a.starts)[b])) : n - a.Lq;
 }
 // Keys [lo, hi) that the row at position p of [0, n) may see, both rising with p.
 __device__ __forceinline__ void seen_by(const PagedArgs& a, int n, int p, int& lo, int& hi) {
@@ -129,7 +143,7 @@ __device__ __forceinline__ int swizzle(int r) {
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
+__global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedArgs a) {
   constexpr int KS = D / 32;             // reduction steps of S
   constexpr int DT = D / 16;             // output tiles
   constexpr int UNITS = D / 8;           // 16-byte units of a row
@@ -137,9 +151,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
   constexpr int VL = kTile / VROWS;      // V loads per lane
   constexpr int ROWB = 2 * D;            // bytes of a row
   constexpr int OPAD = D + 4;
-  constexpr int LDS_V = kWaves * kTile * ROWB;
-  constexpr int LDS_O = kWaves * 16 * OPAD * 4;
-  __shared__ __align__(256) unsigned char smem[LDS_V > LDS_O ? LDS_V : LDS_O];
+  extern __shared__ __align__(256) unsigned char smem[];
   __shared__ float red_m[kWaves][16], red_l[kWaves][16];
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -181,7 +193,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
   for (int t = 0; t < DT; ++t) O[t] = zero4();
   float mx = neg_inf(), sum = 0.f;
 
-  const int32_t* table = a.table + b * a.table_stride;
+  const scalar_ints table = scalars(a.table + b * a.table_stride);
   const int page_mask = (1 << a.page_shift) - 1;
   const uint16_t* kb = a.k + h * a.k_sh + col * a.k_sr + 8 * grp;
   const int vrow = lane / UNITS, vunit = lane % UNITS;
@@ -192,28 +204,47 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
   const int tr = 4 * grp + (col >> 2);
   const uint32_t tr0 = vbase + tr * ROWB + ((((col & 3) >> 1) ^ swizzle<D>(tr)) << 4) + (col & 1) * 8;
 
+  // Every load is issued a tile ahead: V's as soon as the registers have gone
+  // to LDS, K's after the products, page indices one tile before those.
   u32x4_t K[2][KS], V[VL];
-  bool live[2];  // the tile's half lies in a mapped page
-  auto page_of = [&](int key) -> int {
-    const int e = key >> a.page_shift;
-    return e < a.table_width ? table[e] : -1;
-  };
-  const int page_half = 16;
-  for (int base = first + wave * kTile; base < last; base += kStep) {
+  int pages[2], next_pages[2];  // of the tile's sixteens of keys
+  auto page_of = [&](int key) { return page_at(a, table, key); };
+  auto is_live = [&](int page) { return page >= 0 && page < a.num_pages; };
+  auto safe = [&](int page) { return is_live(page) ? page : 0; };  // a page that exists
+  auto load_k = [&](int base, const int (&pg)[2]) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int key = base + t * page_half;
-      int pg = __builtin_amdgcn_readfirstlane(page_of(key));
-      live[t] = pg >= 0 && pg < a.num_pages;
-      if (!live[t]) pg = 0;  // a page that exists; its values are not used
-      const int row = key & page_mask;
-      const uint16_t* kp = kb + pg * a.k_sp + row * a.k_sr;
-      const uint16_t* vp = vb + pg * a.v_sp + row * a.v_sr;
+      const uint16_t* kp = kb + safe(pg[t]) * a.k_sp + ((base + 16 * t) & page_mask) * a.k_sr;
 #pragma unroll
       for (int s = 0; s < KS; ++s) K[t][s] = *reinterpret_cast<const u32x4_t*>(kp + 32 * s);
+    }
+  };
+  auto load_v = [&](int base, const int (&pg)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint16_t* vp = vb + safe(pg[t]) * a.v_sp + ((base + 16 * t) & page_mask) * a.v_sr;
 #pragma unroll
       for (int i = 0; i < VL / 2; ++i)
         V[t * (VL / 2) + i] = *reinterpret_cast<const u32x4_t*>(vp + i * VROWS * a.v_sr);
+    }
+  };
+  const int begin = first + wave * kTile;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    pages[t] = begin < last ? page_of(begin + 16 * t) : -1;
+    next_pages[t] = begin + kStep < last ? page_of(begin + kStep + 16 * t) : -1;
+  }
+  if (begin < last) {
+    load_v(begin, pages);
+    load_k(begin, pages);
+  }
+  for (int base = begin; base < last; base += kStep) {
+    const bool live[2] = {is_live(pages[0]), is_live(pages[1])};
+    const bool more = base + kStep < last;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      pages[t] = next_pages[t];
+      next_pages[t] = base + 2 * kStep < last ? page_of(base + 2 * kStep + 16 * t) : -1;
     }
     const bool whole = live[0] && live[1];
     const bool edge = !whole || base < r.lo || base + kTile > r.end;           // V rows nobody sees
@@ -247,6 +278,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
       const int rr = i * VROWS + vrow;
       *reinterpret_cast<u32x4_t*>(vl + rr * ROWB + ((vunit ^ swizzle<D>(rr)) << 4)) = V[i];
     }
+    if (more) load_v(base + kStep, pages);
     // ---- scores
     f32x4_t S[2];
 #pragma unroll
@@ -255,6 +287,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) S[t] = T::mfma(K[t][s], Q[s], S[t]);
     }
+    if (more) load_k(base + kStep, pages);
     uint32_t seen = 0xffu;
     if (mixed) {
       seen = 0;
@@ -311,8 +344,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
         const int from = 16 * ((kk & 15) >> 2) + col;
         const int slot = 4 * (kk >> 4) + (kk & 3);
         const bool ok = (__shfl(seen, from, 64) >> slot) & 1;
-        const int pg = __builtin_amdgcn_readfirstlane(page_of(key));
-        const uint16_t* vp = a.v + h * a.v_sh + pg * a.v_sp + (key & page_mask) * a.v_sr;
+        const uint16_t* vp =
+            a.v + h * a.v_sh + page_of(key) * a.v_sp + (key & page_mask) * a.v_sr;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -346,8 +379,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(PagedArgs a) {
   for (int t = 0; t < DT; ++t)
     *reinterpret_cast<f32x4_t*>(ol + 16 * t + 4 * grp) = O[t] * f;
   __syncthreads();
-  // thread: column tid / (kThreads / 16), D / 16 dims
-  constexpr int TPC = kThreads / 16, DPT = D / TPC;
+  // thread: column tid / TPC, DPT dims
+  constexpr int TPC = 64 * kWaves / 16, DPT = D / TPC;
   const int c2 = tid / TPC, d2 = (tid % TPC) * DPT;
   const int m2 = ct * 16 + c2;
   if (m2 >= a.M) return;
@@ -397,11 +430,11 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   constexpr int KS = D / 32, DT = D / 16, NT = kBlockCols / 16;
   constexpr int ROWB = 2 * D;
   constexpr int UNITS = D / 8;
-  constexpr int PIECE = 64 / UNITS;        // rows of one DMA instruction (1 KB)
-  constexpr int PIECES = kBlockKeys / PIECE;  // of K, and as many of V
+  constexpr int ROWS = 64 / UNITS;         // of one DMA instruction (1 KB)
   constexpr int TILEB = kBlockKeys * ROWB;
   constexpr int SLOTB = 2 * TILEB;
-  extern __shared__ __align__(256) unsigned char ring[];
+  extern __shared__ __align__(256) unsigned char smem[];
+  unsigned char* ring = smem;
   int* flag = reinterpret_cast<int*>(ring + 2 * SLOTB);  // last tile (+ 1) with a value not finite
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -455,37 +488,46 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   }
   if (tid == 0) *flag = 0;
 
-  // ---- the stream.  DMA instruction x fills rows PIECE x .. of K (x < PIECES) or V: lane
-  // (row lane / UNITS, unit lane % UNITS) fetches the unit that belongs there.
-  const int32_t* table = a.table + b * a.table_stride;
+  // ---- the stream.  A tile is eight pieces of sixteen rows, K's four and V's
+  // four, each inside one page; wave w brings pieces w, w + waves, ...  A DMA
+  // instruction fills ROWS rows (1 KB): lane (row lane / UNITS, unit lane % UNITS)
+  // fetches the unit that the swizzle puts there.
+  const scalar_ints table = scalars(a.table + b * a.table_stride);
   const int page_mask = (1 << a.page_shift) - 1;
-  const int lrow = lane / UNITS, lunit = (lane % UNITS) ^ (swizzle<D>(lrow) & ~1);
-  // (row x + lrow's swizzle is lrow's with these bits of x flipped)
-  auto flips = [&](int x) { return D == 128 ? 2 * (x & 4) + ((x >> 3) & 1) : (x >> 3) & 1; };
-  const uint16_t* kb = a.k + h * a.k_sh + lrow * a.k_sr;
-  const uint16_t* vb = a.v + h * a.v_sh + lrow * a.v_sr;
-  auto page_at = [&](int key) -> int {
-    const int e = key >> a.page_shift;
-    return __builtin_amdgcn_readfirstlane(e < a.table_width ? table[e] : -1);
+  const int lrow = lane / UNITS, lunit = (lane % UNITS) ^ swizzle<D>(lrow);
+  const int64_t k_lane = 2 * ((int64_t)h * a.k_sh + lrow * a.k_sr);  // bytes
+  const int64_t v_lane = 2 * ((int64_t)h * a.v_sh + lrow * a.v_sr);
+  struct Pages {
+    int p0, p1, p2, p3;                    // of the tile's sixteens of keys
+    __device__ __forceinline__ int at(int i) const {
+      const int lo = i & 1 ? p1 : p0, hi = i & 1 ? p3 : p2;
+      return i & 2 ? hi : lo;
+    }
   };
-  int pages[4], next_pages[4];             // of the tile's sixteens of keys
-  auto fetch_pages = [&](int (&to)[4], int base) {
+  auto fetch_pages = [&](int base) {
+    return Pages{page_at(a, table, base), page_at(a, table, base + 16), page_at(a, table, base + 32),
+                 page_at(a, table, base + 48)};
+  };
+  auto is_live = [&](int page) { return (uint32_t)page < (uint32_t)a.num_pages; };
+  auto issue = [&](int slot, int base, const Pages& pg) {
+    for (int x = wave; x < 8; x += waves) {
+      const bool is_v = x >= 4;
+      const int page = pg.at(x & 3);
+      const int64_t at = is_live(page) ? page : 0;  // a page that exists; its values are not used
+      const int row = (base + 16 * (x & 3)) & page_mask;
+      const int64_t sr = is_v ? a.v_sr : a.k_sr;
+      const uint8_t* src = (const uint8_t*)(is_v ? a.v : a.k) +
+                           2 * (at * (is_v ? a.v_sp : a.k_sp) + row * sr) + (is_v ? v_lane : k_lane);
+      unsigned char* dst = ring + slot * SLOTB + (is_v ? TILEB : 0) + (x & 3) * 16 * ROWB;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) to[i] = page_at(base + 16 * i);
-  };
-  auto issue = [&](int slot, int base, const int (&pg)[4]) {
-    unsigned char* dst = ring + slot * SLOTB;
-    for (int x = wave; x < 2 * PIECES; x += waves) {
-      const bool is_v = x >= PIECES;
-      const int r0 = (is_v ? x - PIECES : x) * PIECE;
-      int page = r0 < 16 ? pg[0] : r0 < 32 ? pg[1] : r0 < 48 ? pg[2] : pg[3];
-      if (page < 0 || page >= a.num_pages) page = 0;  // a page that exists; its values are not used
-      const int64_t row = (base + r0) & page_mask;
-      const uint16_t* src = is_v ? vb + page * a.v_sp + row * a.v_sr : kb + page * a.k_sp + row * a.k_sr;
-      src += 8 * (lunit ^ flips(r0));
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) uint32_t*)src,
-          (lds_void_t*)(dst + (is_v ? TILEB : 0) + r0 * ROWB), 16, 0, 0);
+      for (int i = 0; i < 16 / ROWS; ++i) {
+        constexpr int kFlipHi = D == 128 ? 8 : 0;   // row 4's part of the swizzle
+        const int flip = ((i * ROWS) & 4 ? kFlipHi : 0) + ((i * ROWS) >> 3 & 1);
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) uint32_t*)(src + 16 * (lunit ^ flip)),
+            (lds_void_t*)(dst + 1024 * i), 16, 0, 0);
+        src += 2 * ROWS * sr;
+      }
     }
   };
 #pragma unroll
@@ -493,43 +535,152 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(Q[t][s]));
   const int tiles = first < last ? (last - first + kBlockKeys - 1) / kBlockKeys : 0;
+  Pages pages = {0, 0, 0, 0}, next = pages;
   if (tiles > 0) {
-    fetch_pages(pages, first);
+    pages = fetch_pages(first);
     issue(0, first, pages);
-    if (tiles > 1) fetch_pages(next_pages, first + kBlockKeys);
+    next = tiles > 1 ? fetch_pages(first + kBlockKeys) : pages;
   }
-  const uint32_t arow = ROWB * col + 16u * (uint32_t)(grp ^ swizzle<D>(col));
+  const uint32_t lds0 = lds_addr(ring);
+  const uint32_t arow = lds0 + ROWB * col + 16u * (uint32_t)(grp ^ swizzle<D>(col));
   const int rt = 4 * grp + (col >> 2);
-  const uint32_t trow = ROWB * rt + 16u * (uint32_t)(((col >> 1) & 1) ^ swizzle<D>(rt)) + 8u * (col & 1);
+  const uint32_t trow = lds0 + TILEB + ROWB * rt +
+                        16u * (uint32_t)(((col >> 1) & 1) ^ swizzle<D>(rt)) + 8u * (col & 1);
+
+  // One tile's products; MASKED: some column of the wave does not see all of it, DIRTY: and
+  // V holds values that are not finite (taken out of LDS: added here).
+  auto compute = [&](int base, uint32_t slot_off, const Pages& pg, auto masked, bool dirty) {
+    constexpr bool MASKED = decltype(masked)::value;
+    f32x4_t S[NT][4];
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+      for (int m = 0; m < 4; ++m) S[c][m] = zero4();
+    {
+      const uint32_t at = arow + slot_off;
+      constexpr int AHEAD = 4;
+      u32x4_t x[4 * KS];
+      auto operand = [&](int o) {  // keys 16 (o & 3) .., dims 32 (o >> 2) ..
+        return lds_read16((at ^ (64u * (o >> 2))) + 16u * ROWB * (o & 3));
+      };
+#pragma unroll
+      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int o = 0; o < 4 * KS; ++o) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c) S[c][o & 3] = T::mfma(x[o], Q[c][o >> 2], S[c][o & 3]);
+        if (o + AHEAD < 4 * KS) x[o + AHEAD] = operand(o + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    uint32_t seen[NT];
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        seen[c] = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = base + 16 * (i >> 2) + 4 * grp + (i & 3);
+          const bool ok = is_live(pg.at(i >> 2)) && key >= lo[c] && key < hi[c];
+          if (ok) seen[c] |= 1u << i;
+          S[c][i >> 2][i & 3] = ok ? S[c][i >> 2][i & 3] : neg_inf();
+        }
+      }
+    }
+    u32x4_t Pb[NT][2];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+      const float top = across4_max(max16_raw(S[c])) * a.scale_log2;
+      if (__builtin_amdgcn_ballot_w64(top > mx[c] + kSlack) != 0) {
+        const float to = __builtin_fmaxf(mx[c], top);
+        const float f = to == neg_inf() ? 1.f : exp2_hw(mx[c] - to);
+        mx[c] = to;
+        sum[c] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) O[c][d] *= f;
+      }
+      const float off = mx[c] == neg_inf() ? 0.f : mx[c];
+      float part_sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = exp2_hw(__builtin_fmaf(S[c][i >> 2][i & 3], a.scale_log2, -off));
+        S[c][i >> 2][i & 3] = p;
+        part_sum[i & 3] += p;
+      }
+      sum[c] += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        Pb[c][k] = u32x4_t{T::pack(S[c][2 * k][0], S[c][2 * k][1]), T::pack(S[c][2 * k][2], S[c][2 * k][3]),
+                           T::pack(S[c][2 * k + 1][0], S[c][2 * k + 1][1]),
+                           T::pack(S[c][2 * k + 1][2], S[c][2 * k + 1][3])};
+    }
+    // ---- V^T . P^T
+    {
+      const uint32_t at = trow + slot_off;
+      constexpr int AHEAD = 4;
+      u32x4_t x[2 * DT];
+      auto operand = [&](int o) {  // dims 16 (o >> 1) .., keys 32 (o & 1) ..
+        const uint32_t ad = (at ^ (32u * (o >> 1))) + 32u * ROWB * (o & 1);
+        const u32x2_t y0 = read_transposed(ad), y1 = read_transposed(ad + 16u * ROWB);
+        return u32x4_t{y0[0], y0[1], y1[0], y1[1]};
+      };
+#pragma unroll
+      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int o = 0; o < 2 * DT; ++o) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c) O[c][o >> 1] = T::mfma(x[o], Pb[c][o & 1], O[c][o >> 1]);
+        if (o + AHEAD < 2 * DT) x[o + AHEAD] = operand(o + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (MASKED) {
+      if (!dirty) return;
+      for (int kk = 0; kk < kBlockKeys; ++kk) {
+        const int key = base + kk;
+        if (!is_live(pg.at(kk >> 4)) || key < r.lo || key >= r.end) continue;
+        const int from = 16 * ((kk & 15) >> 2) + col, slot_i = 4 * (kk >> 4) + (kk & 3);
+        const uint16_t* vp = a.v + h * a.v_sh + page_at(a, table, key) * a.v_sp +
+                             (int64_t)(key & page_mask) * a.v_sr;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          const bool ok = (__shfl(seen[c], from, 64) >> slot_i) & 1;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x = vp[16 * d + 4 * grp + e];
+              if (ok && (x & T::kExp) == T::kExp) O[c][d][e] += T::value(x);
+            }
+        }
+      }
+    }
+  };
 
   for (int t = 0; t < tiles; ++t) {
     const int base = first + t * kBlockKeys;
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    bool live[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) live[i] = pages[i] >= 0 && pages[i] < a.num_pages;
+    const Pages pg = pages;
     if (t + 1 < tiles) {
-      issue((t + 1) & 1, base + kBlockKeys, next_pages);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pages[i] = next_pages[i];
-      if (t + 2 < tiles) fetch_pages(next_pages, base + 2 * kBlockKeys);
+      issue((t + 1) & 1, base + kBlockKeys, next);
+      pages = next;
+      if (t + 2 < tiles) next = fetch_pages(base + 2 * kBlockKeys);
     }
     asm volatile("" ::: "memory");
-    unsigned char* slot = ring + (t & 1) * SLOTB;
-    const uint32_t sbase = lds_addr(slot);
-    const bool whole = live[0] && live[1] && live[2] && live[3];
-    const bool mixed = !whole || base < r.inner_lo || base + kBlockKeys > r.inner_hi;
+    const uint32_t slot_off = (t & 1) * SLOTB;
+    const bool whole = is_live(pg.p0) && is_live(pg.p1) && is_live(pg.p2) && is_live(pg.p3);
     bool dirty = false;
-    if (mixed) {
+    if (!whole || base < r.inner_lo || base + kBlockKeys > r.inner_hi) {
       // V rows that no column sees become zeros; values that are not finite
       // are taken out (a column that does not see them must not get 0 x inf)
-      // and added one by one below.
+      // and added one by one in compute().
       bool odd = false;
       for (int x = tid; x < kBlockKeys * UNITS; x += 64 * waves) {
         const int row = x / UNITS, key = base + row;
-        u32x4_t* at = reinterpret_cast<u32x4_t*>(slot + TILEB + 16 * x);
-        const bool lv = row < 16 ? live[0] : row < 32 ? live[1] : row < 48 ? live[2] : live[3];
-        if (!lv || key < r.lo || key >= r.end) {
+        u32x4_t* at = reinterpret_cast<u32x4_t*>(ring + slot_off + TILEB + 16 * x);
+        if (!is_live(pg.at(row >> 4)) || key < r.lo || key >= r.end) {
           *at = u32x4_t{0, 0, 0, 0};
           continue;
         }
@@ -549,113 +700,10 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       dirty = *(volatile int*)flag == t + 1;
     }
-    // ---- scores
-    f32x4_t S[NT][4];
-#pragma unroll
-    for (int c = 0; c < NT; ++c)
-#pragma unroll
-      for (int m = 0; m < 4; ++m) S[c][m] = zero4();
-    {
-      const uint32_t at = sbase + arow;
-      constexpr int AHEAD = 4;
-      u32x4_t x[4 * KS];
-      auto operand = [&](int o) {  // keys 16 (o & 3) .., dims 32 (o >> 2) ..
-        return lds_read16((at ^ (64u * (o >> 2))) + 16u * ROWB * (o & 3));
-      };
-#pragma unroll
-      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int o = 0; o < 4 * KS; ++o) {
-#pragma unroll
-        for (int c = 0; c < NT; ++c) S[c][o & 3] = T::mfma(x[o], Q[c][o >> 2], S[c][o & 3]);
-        if (o + AHEAD < 4 * KS) x[o + AHEAD] = operand(o + AHEAD);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    uint32_t seen[NT];
-    u32x4_t Pb[NT][2];
-    if (!whole || base < w.inner_lo || base + kBlockKeys > w.inner_hi) {
-#pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        seen[c] = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = base + 16 * (i >> 2) + 4 * grp + (i & 3);
-          const bool ok = live[i >> 2] && key >= lo[c] && key < hi[c];
-          if (ok) seen[c] |= 1u << i;
-          S[c][i >> 2][i & 3] = ok ? S[c][i >> 2][i & 3] : neg_inf();
-        }
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < NT; ++c) seen[c] = 0xffffu;
-    }
-#pragma unroll
-    for (int c = 0; c < NT; ++c) {
-      const float top = across4_max(max16_raw(S[c])) * a.scale_log2;
-      if (__builtin_amdgcn_ballot_w64(top > mx[c] + kSlack) != 0) {
-        const float to = __builtin_fmaxf(mx[c], top);
-        const float f = to == neg_inf() ? 1.f : exp2_hw(mx[c] - to);
-        mx[c] = to;
-        sum[c] *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) O[c][d] *= f;
-      }
-      const float off = mx[c] == neg_inf() ? 0.f : mx[c];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = exp2_hw(__builtin_fmaf(S[c][i >> 2][i & 3], a.scale_log2, -off));
-        S[c][i >> 2][i & 3] = p;
-        sum[c] += p;
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        Pb[c][k] = u32x4_t{T::pack(S[c][2 * k][0], S[c][2 * k][1]), T::pack(S[c][2 * k][2], S[c][2 * k][3]),
-                           T::pack(S[c][2 * k + 1][0], S[c][2 * k + 1][1]),
-                           T::pack(S[c][2 * k + 1][2], S[c][2 * k + 1][3])};
-    }
-    // ---- V^T . P^T
-    {
-      const uint32_t at = sbase + TILEB + trow;
-      constexpr int AHEAD = 4;
-      u32x4_t x[2 * DT];
-      auto operand = [&](int o) {  // dims 16 (o >> 1) .., keys 32 (o & 1) ..
-        const uint32_t ad = (at ^ (32u * (o >> 1))) + 32u * ROWB * (o & 1);
-        const u32x2_t y0 = read_transposed(ad), y1 = read_transposed(ad + 16u * ROWB);
-        return u32x4_t{y0[0], y0[1], y1[0], y1[1]};
-      };
-#pragma unroll
-      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int o = 0; o < 2 * DT; ++o) {
-#pragma unroll
-        for (int c = 0; c < NT; ++c) O[c][o >> 1] = T::mfma(x[o], Pb[c][o & 1], O[c][o >> 1]);
-        if (o + AHEAD < 2 * DT) x[o + AHEAD] = operand(o + AHEAD);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    if (dirty) {
-      for (int kk = 0; kk < kBlockKeys; ++kk) {
-        const int key = base + kk;
-        const bool lv = kk < 16 ? live[0] : kk < 32 ? live[1] : kk < 48 ? live[2] : live[3];
-        if (!lv || key < r.lo || key >= r.end) continue;
-        const int from = 16 * ((kk & 15) >> 2) + col, slot_i = 4 * (kk >> 4) + (kk & 3);
-        const uint16_t* vp = a.v + h * a.v_sh + page_at(key) * a.v_sp + (int64_t)(key & page_mask) * a.v_sr;
-#pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          const bool ok = (__shfl(seen[c], from, 64) >> slot_i) & 1;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t x = vp[16 * d + 4 * grp + e];
-              if (ok && (x & T::kExp) == T::kExp) O[c][d][e] += T::value(x);
-            }
-        }
-      }
-    }
+    if (dirty || !whole || base < w.inner_lo || base + kBlockKeys > w.inner_hi)
+      compute(base, slot_off, pg, std::true_type{}, dirty);
+    else
+      compute(base, slot_off, pg, std::false_type{}, false);
   }
 
   // ---- out: lane (col, grp) holds dims 16 d + 4 grp .. of its columns
@@ -780,7 +828,12 @@ int launch(const PagedArgs& a, hipStream_t stream) {
   const int64_t cols = (int64_t)a.B * a.Hkv * a.M;
   if (grid > 0x7fffffff || cols > 0x7fffffff) return MRSA_ERR_UNSUPPORTED;
   if (a.tile_cols == 16) {
-    hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a);
+    const size_t lds = kWaves * std::max(kTile * 2 * D, 16 * (D + 4) * 4);
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, D>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+      return MRSA_ERR_LAUNCH;
+    hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves), lds,
+                       stream, a);
   } else {
     const size_t lds = 4 * kBlockKeys * 2 * D + 16;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_block_kernel<T, D>),

@@ -65,7 +65,7 @@ def _paged_append_impl(k, v, k_pages, v_pages, page_table, slots, q, cos, sin, p
     kc, vc = dense_rows(k), dense_rows(v)
     qc = None if q is None else dense_rows(q)
     Hq = 0 if q is None else q.shape[2]
-    q_out = torch.empty((B, L, Hq, D), dtype=k.dtype, device=k.device)
+    q_out = k.new_empty((B, L, Hq, D))
     ct, st = (None, None) if cos is None else (cos.contiguous(), sin.contiguous())
     ps = (0, 0) if positions is None else positions.stride()
     status = _lib.call_on(
@@ -156,12 +156,12 @@ def _paged_attention_impl(q, k_pages, v_pages, page_table, cache_lens, query_sta
         qc = qc.contiguous()
         if qc.data_ptr() % 16:
             qc = qc.clone()
-    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, Lq, Hq), dtype=torch.float32, device=q.device)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((B, Lq, Hq), dtype=torch.float32)
     nbytes, ws = 0, None
     if parts > 1:
         nbytes = _lib.call("mrsa_paged_attention_workspace_bytes", B, Lq, Hq, D, parts)
-        ws = torch.empty(max(nbytes, 0) // 4, dtype=torch.float32, device=q.device)
+        ws = q.new_empty(max(nbytes, 0) // 4, dtype=torch.float32)
     status = _lib.call_on(
         q.device, "mrsa_paged_attention_fwd", qc.data_ptr(), *qc.stride()[:3],
         k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3],

@@ -119,8 +119,7 @@ def _rotary_impl(q, k, cos, sin, positions, interleaved, inverse):
     Hkv = 0 if k is None else k.shape[2]
     qc, kc = dense_rows(q), None if k is None else dense_rows(k)
     ct, st = cos.contiguous(), sin.contiguous()
-    q_out = torch.empty((B, L, Hq, D), dtype=q.dtype, device=q.device)
-    k_out = torch.empty((B, L, Hkv, D), dtype=q.dtype, device=q.device)
+    q_out, k_out = q.new_empty(q.shape), q.new_empty((B, L, Hkv, D))
     ps = (0, 0) if positions is None else positions.stride()
     ks = (0, 0, 0) if kc is None else kc.stride()[:3]
     status = _lib.call_on(
@@ -153,16 +152,14 @@ class _Rotary(torch.autograd.Function):
             grad_q = None
         if not ctx.needs_input_grad[1]:
             grad_k = None
+        turn = _Rotary.apply if torch.is_grad_enabled() else _turn
         args = (cos, sin, positions, ctx.interleaved, not ctx.inverse)
+        dq = dk = None
         if grad_q is not None:
-            dq, dk = _Rotary.apply(grad_q, grad_k, *args)
-            if grad_k is None:
-                dk = None
+            dq, dk = turn(grad_q, grad_k, *args)
         elif grad_k is not None:
-            dq, (dk, _) = None, _Rotary.apply(grad_k, None, *args)
-        else:
-            dq = dk = None
-        return dq, dk, None, None, None, None, None
+            dk, _ = turn(grad_k, None, *args)
+        return dq, None if grad_k is None else dk, None, None, None, None, None
 
 
 def check_heads(t, name: str) -> None:
