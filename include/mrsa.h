@@ -973,7 +973,8 @@ int mrsa_paged_append_fwd(
  *     (mrsa_paged_attention_workspace_bytes; 16-byte aligned; unused for 1)
  *   max_len: bound of cache_lens; sm_scale: finite and > 0
  * Limits: head_dim 64 or 128, page_size a power of two from 16 on, pointers
- * 16-byte aligned and strides multiples of 8 elements, max_len < 2^29.
+ * 16-byte aligned and strides multiples of 8 elements, slot strides below 2^26,
+ * max_len < 2^29.
  */
 int64_t mrsa_paged_attention_workspace_bytes(int64_t batch, int64_t q_len, int64_t q_heads,
                                              int64_t head_dim, int64_t parts);

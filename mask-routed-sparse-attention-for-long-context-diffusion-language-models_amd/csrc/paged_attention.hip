@@ -28,8 +28,7 @@ using namespace mrsa;
 
 namespace {
 
-constexpr int kThreads = 256;              // of the joining kernel
-constexpr int kWaves = 8;                  // of the streaming kernel
+constexpr int kWaves = 4;                  // of the streaming kernel
 constexpr int kTile = 32;                  // keys of a wave's tile
 constexpr int kStep = kWaves * kTile;      // keys of a workgroup's round
 constexpr int kMaxParts = 1024;
@@ -79,6 +78,7 @@ struct PagedArgs {
   int causal, window;         // window < 0: none
   float scale_log2;
   int parts, part_keys, col_tiles, tile_cols;
+  int slots;                  // of the block kernel's ring (a power of two)
   uint16_t* out;
   float* lse;
   float* part_out;            // parts > 1: [B, Hkv, M, parts, D]
@@ -158,12 +158,14 @@ __global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   int64_t id = blockIdx.x;
+  // KV heads next to each other (a row's heads are neighbours in memory), parts last: of
+  // sequences of different lengths the short pieces at their ends then come last.
   const int h = (int)(id % a.Hkv);
   id /= a.Hkv;
-  const int part = (int)(id % a.parts);
-  id /= a.parts;
   const int ct = (int)(id % a.col_tiles);
-  const int b = (int)(id / a.col_tiles);
+  id /= a.col_tiles;
+  const int b = (int)(id % a.B);
+  const int part = (int)(id / a.B);
 
   const int n = length_of(a, b), p0 = start_of(a, b, n);
   const Range r = tile_range(a, n, p0, ct * 16, 16);
@@ -425,6 +427,22 @@ constexpr int kBlockKeys = 64;
 constexpr int kBlockCols = 32;             // of a wave
 constexpr int kBlockWaves = 8;
 
+// A DMA instruction: 1 KB of LDS from `to` on, lane l's 16 bytes from base + at.  As
+// asm, since after the builtin the compiler waits for all DMA in flight before the
+// next LDS read; here the loop's own waits order them.  base and to are
+// wave-uniform; the s_nop covers m0 and a scalar operand that a vector instruction
+// has just written (5 wait states).
+__device__ __forceinline__ void dma_kb(uint32_t to, const uint8_t* base, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at),
+               "s"(base)
+               : "memory", "m0");
+}
+// Swizzle of K's rows: the 16 rows of one operand read meet different banks.
+template <int D>
+__device__ __forceinline__ int swizzle_k(int r) {
+  return D == 128 ? r & 15 : (r >> 1) & 7;
+}
+
 template <class T, int D>
 __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs a) {
   constexpr int KS = D / 32, DT = D / 16, NT = kBlockCols / 16;
@@ -435,19 +453,25 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   constexpr int SLOTB = 2 * TILEB;
   extern __shared__ __align__(256) unsigned char smem[];
   unsigned char* ring = smem;
-  int* flag = reinterpret_cast<int*>(ring + 2 * SLOTB);  // last tile (+ 1) with a value not finite
+  int* flag = reinterpret_cast<int*>(ring + a.slots * SLOTB);  // last tile (+ 1) with a value not finite
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int waves = __builtin_amdgcn_readfirstlane((int)blockDim.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  int64_t id = blockIdx.x;
+  // XCD-aware order: workgroups go to the XCDs in turn, so XCD x takes a contiguous
+  // range, in which the column tiles of one piece of keys meet in its L2.
+  int64_t id;
+  {
+    const int64_t total = gridDim.x, x = blockIdx.x % 8, q8 = total / 8, r8 = total % 8;
+    id = x * q8 + min(x, r8) + blockIdx.x / 8;
+  }
+  const int ct = (int)(id % a.col_tiles);
+  id /= a.col_tiles;
   const int h = (int)(id % a.Hkv);
   id /= a.Hkv;
   const int part = (int)(id % a.parts);
-  id /= a.parts;
-  const int ct = (int)(id % a.col_tiles);
-  const int b = (int)(id / a.col_tiles);
+  const int b = (int)(id / a.parts);
   const int cols = kBlockCols * waves;
   const int n = length_of(a, b), p0 = start_of(a, b, n);
   const Range r = tile_range(a, n, p0, ct * cols, cols);
@@ -494,62 +518,76 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   // fetches the unit that the swizzle puts there.
   const scalar_ints table = scalars(a.table + b * a.table_stride);
   const int page_mask = (1 << a.page_shift) - 1;
-  const int lrow = lane / UNITS, lunit = (lane % UNITS) ^ swizzle<D>(lrow);
-  const int64_t k_lane = 2 * ((int64_t)h * a.k_sh + lrow * a.k_sr);  // bytes
-  const int64_t v_lane = 2 * ((int64_t)h * a.v_sh + lrow * a.v_sr);
-  struct Pages {
-    int p0, p1, p2, p3;                    // of the tile's sixteens of keys
-    __device__ __forceinline__ int at(int i) const {
-      const int lo = i & 1 ? p1 : p0, hi = i & 1 ? p3 : p2;
-      return i & 2 ? hi : lo;
-    }
-  };
-  auto fetch_pages = [&](int base) {
-    return Pages{page_at(a, table, base), page_at(a, table, base + 16), page_at(a, table, base + 32),
-                 page_at(a, table, base + 48)};
-  };
-  auto is_live = [&](int page) { return (uint32_t)page < (uint32_t)a.num_pages; };
-  auto issue = [&](int slot, int base, const Pages& pg) {
-    for (int x = wave; x < 8; x += waves) {
-      const bool is_v = x >= 4;
-      const int page = pg.at(x & 3);
-      const int64_t at = is_live(page) ? page : 0;  // a page that exists; its values are not used
-      const int row = (base + 16 * (x & 3)) & page_mask;
-      const int64_t sr = is_v ? a.v_sr : a.k_sr;
-      const uint8_t* src = (const uint8_t*)(is_v ? a.v : a.k) +
-                           2 * (at * (is_v ? a.v_sp : a.k_sp) + row * sr) + (is_v ? v_lane : k_lane);
-      unsigned char* dst = ring + slot * SLOTB + (is_v ? TILEB : 0) + (x & 3) * 16 * ROWB;
+  constexpr int DMAS = 16 / ROWS;
+  uint32_t k_lane[DMAS], v_lane[DMAS], own_lane[DMAS];  // byte offsets (a piece spans < 2^31 bytes)
 #pragma unroll
-      for (int i = 0; i < 16 / ROWS; ++i) {
-        constexpr int kFlipHi = D == 128 ? 8 : 0;   // row 4's part of the swizzle
-        const int flip = ((i * ROWS) & 4 ? kFlipHi : 0) + ((i * ROWS) >> 3 & 1);
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) uint32_t*)(src + 16 * (lunit ^ flip)),
-            (lds_void_t*)(dst + 1024 * i), 16, 0, 0);
-        src += 2 * ROWS * sr;
-      }
+  for (int i = 0; i < DMAS; ++i) {
+    const int row = i * ROWS + lane / UNITS;
+    k_lane[i] = 2u * (uint32_t)row * (uint32_t)a.k_sr + 16u * ((lane % UNITS) ^ swizzle_k<D>(row));
+    v_lane[i] = 2u * (uint32_t)row * (uint32_t)a.v_sr + 16u * ((lane % UNITS) ^ swizzle<D>(row));
+    own_lane[i] = wave < 4 ? k_lane[i] : v_lane[i];
+  }
+  const uint8_t* const k_pool = (const uint8_t*)(a.k + h * a.k_sh);
+  const uint8_t* const v_pool = (const uint8_t*)(a.v + h * a.v_sh);
+  auto is_live = [&](int page) { return (uint32_t)page < (uint32_t)a.num_pages; };
+  struct Piece {
+    uint32_t to;
+    const uint8_t* src;
+  };
+  auto piece = [&](int x, int slot, int base, int page) {
+    const int64_t at = is_live(page) ? page : 0;   // a page that exists; its values are not used
+    const int64_t row = (base + 16 * (x & 3)) & page_mask;
+    const uint8_t* src = x < 4 ? k_pool + 2 * (at * a.k_sp + row * a.k_sr)
+                               : v_pool + 2 * (at * a.v_sp + row * a.v_sr);
+    return Piece{
+        (uint32_t)__builtin_amdgcn_readfirstlane(lds_addr(ring) + slot * SLOTB + x * 16 * ROWB),
+        (const uint8_t*)uniform_u64((uint64_t)src)};
+  };
+  auto page_for = [&](int base, int x) { return page_at(a, table, base + 16 * (x & 3)); };
+  // The wave's pieces from its second on.
+  auto issue_others = [&](int slot, int base) {
+    for (int x = wave + waves; x < 8; x += waves) {
+      const Piece d = piece(x, slot, base, page_for(base, x));
+#pragma unroll
+      for (int i = 0; i < DMAS; ++i) dma_kb(d.to + 1024 * i, d.src, x < 4 ? k_lane[i] : v_lane[i]);
     }
   };
+  // Whether an entry of this piece of the table is unmapped: then every tile looks.
+  bool holes = false;
+  for (int e = (first >> a.page_shift) + lane; e <= (last - 1) >> a.page_shift; e += 64)
+    holes |= !is_live(a.table[b * a.table_stride + e]);
+  holes = __builtin_amdgcn_ballot_w64(holes) != 0;
+  auto live_at = [&](int base, int i) { return !holes || is_live(page_at(a, table, base + 16 * i)); };
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(Q[t][s]));
   const int tiles = first < last ? (last - first + kBlockKeys - 1) / kBlockKeys : 0;
-  Pages pages = {0, 0, 0, 0}, next = pages;
-  if (tiles > 0) {
-    pages = fetch_pages(first);
-    issue(0, first, pages);
-    next = tiles > 1 ? fetch_pages(first + kBlockKeys) : pages;
+  // Tiles t .. t + slots - 2 are on their way while t - 1 is computed.  A wave waits for its
+  // DMA of tile t only: the newer ones of two further tiles (four instructions a
+  // piece) stay in flight.
+  const int ahead = a.slots - 1;
+  const int ring_mask = a.slots - 1;
+  const bool one_piece = wave + waves >= 8;
+  int next = -1;
+  for (int t = 0; t < min(tiles, ahead); ++t) {
+    const int base = first + t * kBlockKeys;
+    const Piece d = piece(wave, t, base, page_for(base, wave));
+#pragma unroll
+    for (int i = 0; i < DMAS; ++i) dma_kb(d.to + 1024 * i, d.src, own_lane[i]);
+    issue_others(t, base);
   }
+  next = tiles > 0 ? page_for(first + ahead * kBlockKeys, wave) : -1;
   const uint32_t lds0 = lds_addr(ring);
-  const uint32_t arow = lds0 + ROWB * col + 16u * (uint32_t)(grp ^ swizzle<D>(col));
+  const uint32_t arow = lds0 + ROWB * col + 16u * (uint32_t)(grp ^ swizzle_k<D>(col));
   const int rt = 4 * grp + (col >> 2);
   const uint32_t trow = lds0 + TILEB + ROWB * rt +
                         16u * (uint32_t)(((col >> 1) & 1) ^ swizzle<D>(rt)) + 8u * (col & 1);
 
   // One tile's products; MASKED: some column of the wave does not see all of it, DIRTY: and
   // V holds values that are not finite (taken out of LDS: added here).
-  auto compute = [&](int base, uint32_t slot_off, const Pages& pg, auto masked, bool dirty) {
+  auto compute = [&](int base, uint32_t slot_off, bool bring, const Piece& own, auto masked,
+                     bool dirty) {
     constexpr bool MASKED = decltype(masked)::value;
     f32x4_t S[NT][4];
 #pragma unroll
@@ -571,18 +609,20 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
 #pragma unroll
         for (int c = 0; c < NT; ++c) S[c][o & 3] = T::mfma(x[o], Q[c][o >> 2], S[c][o & 3]);
         if (o + AHEAD < 4 * KS) x[o + AHEAD] = operand(o + AHEAD);
+        if (o % 4 == 3 && bring) dma_kb(own.to + 1024 * (o / 4), own.src, own_lane[o / 4]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     uint32_t seen[NT];
     if constexpr (MASKED) {
+      const bool live[4] = {live_at(base, 0), live_at(base, 1), live_at(base, 2), live_at(base, 3)};
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
         seen[c] = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int key = base + 16 * (i >> 2) + 4 * grp + (i & 3);
-          const bool ok = is_live(pg.at(i >> 2)) && key >= lo[c] && key < hi[c];
+          const bool ok = live[i >> 2] && key >= lo[c] && key < hi[c];
           if (ok) seen[c] |= 1u << i;
           S[c][i >> 2][i & 3] = ok ? S[c][i >> 2][i & 3] : neg_inf();
         }
@@ -640,7 +680,7 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
       if (!dirty) return;
       for (int kk = 0; kk < kBlockKeys; ++kk) {
         const int key = base + kk;
-        if (!is_live(pg.at(kk >> 4)) || key < r.lo || key >= r.end) continue;
+        if (!live_at(base, kk >> 4) || key < r.lo || key >= r.end) continue;
         const int from = 16 * ((kk & 15) >> 2) + col, slot_i = 4 * (kk >> 4) + (kk & 3);
         const uint16_t* vp = a.v + h * a.v_sh + page_at(a, table, key) * a.v_sp +
                              (int64_t)(key & page_mask) * a.v_sr;
@@ -661,16 +701,26 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
 
   for (int t = 0; t < tiles; ++t) {
     const int base = first + t * kBlockKeys;
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const Pages pg = pages;
-    if (t + 1 < tiles) {
-      issue((t + 1) & 1, base + kBlockKeys, next);
-      pages = next;
-      if (t + 2 < tiles) next = fetch_pages(base + 2 * kBlockKeys);
+    if (ahead == 3 && t + 2 < tiles) {
+      if (one_piece)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * 16 / ROWS) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 * 16 / ROWS) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    // The wave's first piece of the tile `ahead` goes between the products of S: all waves'
+    // DMA at once would hold them up (32 cycles an instruction).
+    const bool bring = t + ahead < tiles;
+    Piece own = {0, nullptr};
+    if (bring) {
+      own = piece(wave, (t + ahead) & ring_mask, base + ahead * kBlockKeys, next);
+      issue_others((t + ahead) & ring_mask, base + ahead * kBlockKeys);
     }
     asm volatile("" ::: "memory");
-    const uint32_t slot_off = (t & 1) * SLOTB;
-    const bool whole = is_live(pg.p0) && is_live(pg.p1) && is_live(pg.p2) && is_live(pg.p3);
+    const uint32_t slot_off = (t & ring_mask) * SLOTB;
+    const bool whole =
+        !holes || (live_at(base, 0) && live_at(base, 1) && live_at(base, 2) && live_at(base, 3));
     bool dirty = false;
     if (!whole || base < r.inner_lo || base + kBlockKeys > r.inner_hi) {
       // V rows that no column sees become zeros; values that are not finite
@@ -680,7 +730,12 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
       for (int x = tid; x < kBlockKeys * UNITS; x += 64 * waves) {
         const int row = x / UNITS, key = base + row;
         u32x4_t* at = reinterpret_cast<u32x4_t*>(ring + slot_off + TILEB + 16 * x);
-        if (!is_live(pg.at(row >> 4)) || key < r.lo || key >= r.end) {
+        bool lv = true;
+        if (holes) {
+          const int e = key >> a.page_shift;  // (a vector load: rows differ between lanes)
+          lv = e < a.table_width && is_live(a.table[b * a.table_stride + e]);
+        }
+        if (!lv || key < r.lo || key >= r.end) {
           *at = u32x4_t{0, 0, 0, 0};
           continue;
         }
@@ -701,9 +756,11 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
       dirty = *(volatile int*)flag == t + 1;
     }
     if (dirty || !whole || base < w.inner_lo || base + kBlockKeys > w.inner_hi)
-      compute(base, slot_off, pg, std::true_type{}, dirty);
+      compute(base, slot_off, bring, own, std::true_type{}, dirty);
     else
-      compute(base, slot_off, pg, std::false_type{}, false);
+      compute(base, slot_off, bring, own, std::false_type{}, false);
+    // (a scalar load in flight would turn every wait for LDS into a wait for all of it)
+    next = page_for(base + (ahead + 1) * kBlockKeys, wave);
   }
 
   // ---- out: lane (col, grp) holds dims 16 d + 4 grp .. of its columns
@@ -743,16 +800,21 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   }
 }
 
-// One workgroup per column: the parts' maxima and sums, then their outputs.
-template <class T, int D>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(PagedArgs a) {
-  constexpr int TPR = D / 4;                 // threads of a row, four dims each
-  constexpr int LANES = kThreads / TPR;      // parts at a time
-  __shared__ float weight[kMaxParts];
-  __shared__ float red[kThreads / 64];
-  __shared__ f32x4_t acc_l[kThreads];
-  const int tid = threadIdx.x;
-  const int64_t c = blockIdx.x;              // (b Hkv + h) M + m
+// Joining: WAVES waves per column; each reads all of the column's maxima and sums,
+// and the outputs of every WAVES-th part, eight rows in flight.
+template <class T, int D, int WAVES>
+__global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) paged_join_kernel(PagedArgs a) {
+  constexpr int THREADS = WAVES > 4 ? 64 * WAVES : 256;
+  constexpr int COLS = THREADS / 64 / WAVES;    // columns of a workgroup
+  constexpr int VALUES = D / 64;                // dims of a lane
+  typedef float vec_t __attribute__((ext_vector_type(VALUES)));
+  __shared__ vec_t acc_l[THREADS];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t columns = (int64_t)a.B * a.Hkv * a.M;
+  const int64_t c_raw = (int64_t)blockIdx.x * COLS + wave / WAVES;   // (b Hkv + h) M + m
+  const bool there = c_raw < columns;
+  const int64_t c = there ? c_raw : columns - 1;
   const int m = (int)(c % a.M);
   const int64_t bh = c / a.M;
   const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv);
@@ -760,49 +822,51 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(PagedArgs a) {
   const Range r = tile_range(a, n, start_of(a, b, n), m / a.tile_cols * a.tile_cols, a.tile_cols);
   const int np = max(1, (r.end - r.start + a.part_keys - 1) / a.part_keys);
   const float* ml = a.part_ml + 2 * c * a.parts;
+  const vec_t* po = reinterpret_cast<const vec_t*>(a.part_out + c * a.parts * D) + lane;
+  vec_t v[8];
+  float w[8];
+  auto fetch = [&](int p0) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {  // (a part past the last is the last one, and not added)
+      const int p = min(p0 + u * WAVES, np - 1);
+      v[u] = po[(int64_t)p * 64];
+      w[u] = ml[2 * p];
+    }
+  };
+  fetch(wave % WAVES);
   float M = neg_inf();
-  for (int p = tid; p < np; p += kThreads) M = __builtin_fmaxf(M, ml[2 * p]);
+  for (int p = lane; p < np; p += 64) M = __builtin_fmaxf(M, ml[2 * p]);
   M = wave_max(M);
-  if ((tid & 63) == 0) red[tid >> 6] = M;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) M = __builtin_fmaxf(M, red[w]);
-  __syncthreads();
   float total = 0.f;
-  for (int p = tid; p < np; p += kThreads) {
-    const float w = M == neg_inf() ? 1.f : exp2_hw(ml[2 * p] - M);
-    weight[p] = w;
-    total += w * ml[2 * p + 1];
-  }
+  for (int p = lane; p < np; p += 64)
+    total += (M == neg_inf() ? 1.f : exp2_hw(ml[2 * p] - M)) * ml[2 * p + 1];
   total = wave_sum(total);
-  if ((tid & 63) == 0) red[tid >> 6] = total;
-  __syncthreads();
-  total = 0.f;
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) total += red[w];
-  const int d4 = tid % TPR;
-  const f32x4_t* po = reinterpret_cast<const f32x4_t*>(a.part_out + c * a.parts * D) + d4;
-  f32x4_t acc = zero4();
-  // eight rows in flight per thread (a row past the last is the last one, with no part in the sum)
-  for (int p0 = tid / TPR; p0 < np; p0 += 8 * LANES) {
-    f32x4_t v[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = po[(int64_t)min(p0 + u * LANES, np - 1) * TPR];
+  vec_t acc = {};
+  for (int p0 = wave % WAVES;;) {
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (p0 + u * LANES < np) acc += weight[p0 + u * LANES] * v[u];
+      if (p0 + u * WAVES < np) acc += (M == neg_inf() ? 1.f : exp2_hw(w[u] - M)) * v[u];
+    p0 += 8 * WAVES;
+    if (p0 >= np) break;
+    fetch(p0);
   }
-  acc_l[tid] = acc;
-  __syncthreads();
-  if (tid >= TPR) return;
-  for (int l = 1; l < LANES; ++l) acc += acc_l[l * TPR + tid];
+  if constexpr (WAVES > 1) {
+    acc_l[threadIdx.x] = acc;
+    __syncthreads();
+    if (wave % WAVES != 0) return;
+#pragma unroll
+    for (int x = 1; x < WAVES; ++x) acc += acc_l[threadIdx.x + 64 * x];
+  }
+  if (!there) return;
   const int i = m / a.G;
   const int64_t row = ((int64_t)b * a.Lq + i) * a.Hq + h * a.G + (m - i * a.G);
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  u32x2_t o = {0u, 0u};
-  if (total != 0.f) o = u32x2_t{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
-  *reinterpret_cast<u32x2_t*>(a.out + row * D + 4 * d4) = o;
-  if (tid == 0) a.lse[row] = total == 0.f ? neg_inf() : kLn2 * (M + log2_hw(total));
+  uint16_t* out = a.out + row * D + VALUES * lane;
+  if constexpr (VALUES == 2)
+    *reinterpret_cast<uint32_t*>(out) = total == 0.f ? 0u : T::pack(acc[0] * inv, acc[1] * inv);
+  else
+    *out = total == 0.f ? 0 : (uint16_t)T::pack(acc[0] * inv, 0.f);
+  if (lane == 0) a.lse[row] = total == 0.f ? neg_inf() : kLn2 * (M + log2_hw(total));
 }
 
 // Columns of a workgroup: up to 16 the streaming kernel; more, whole waves of the
@@ -835,7 +899,7 @@ int launch(const PagedArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves), lds,
                        stream, a);
   } else {
-    const size_t lds = 4 * kBlockKeys * 2 * D + 16;
+    const size_t lds = (size_t)a.slots * 2 * kBlockKeys * 2 * D + 16;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_block_kernel<T, D>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
       return MRSA_ERR_LAUNCH;
@@ -844,7 +908,15 @@ int launch(const PagedArgs& a, hipStream_t stream) {
   }
   int st = mrsa_launch_status();
   if (st != MRSA_OK || a.parts == 1) return st;
-  hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)cols), dim3(kThreads), 0, stream, a);
+  // As many waves per column as its parts fill with eight rows each, unless there are columns
+  // enough to fill the machine.
+  if (a.parts > 32 && cols <= 1024)
+    hipLaunchKernelGGL((paged_join_kernel<T, D, 16>), dim3((unsigned)cols), dim3(1024), 0, stream, a);
+  else if (a.parts > 8 && cols <= 4096)
+    hipLaunchKernelGGL((paged_join_kernel<T, D, 4>), dim3((unsigned)cols), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_join_kernel<T, D, 1>), dim3((unsigned)((cols + 3) / 4)), dim3(256), 0,
+                       stream, a);
   return mrsa_launch_status();
 }
 
@@ -892,6 +964,9 @@ extern "C" int mrsa_paged_attention_fwd(
       (q_batch_stride | q_row_stride | q_head_stride | k_page_stride | k_slot_stride |
        k_head_stride | v_page_stride | v_slot_stride | v_head_stride) % 8 != 0)
     return MRSA_ERR_UNSUPPORTED;
+  if (k_slot_stride < 0 || k_slot_stride >= (1 << 26) || v_slot_stride < 0 ||
+      v_slot_stride >= (1 << 26))
+    return MRSA_ERR_UNSUPPORTED;
   const int64_t need = mrsa_paged_attention_workspace_bytes(batch, q_len, q_heads, head_dim, parts);
   if (need < 0) return MRSA_ERR_UNSUPPORTED;
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16 != 0))
@@ -920,9 +995,11 @@ extern "C" int mrsa_paged_attention_fwd(
   a.parts = (int)parts;
   a.tile_cols = columns_of(a.M);
   a.col_tiles = (a.M + a.tile_cols - 1) / a.tile_cols;
+  a.slots = a.tile_cols > 4 * kBlockCols ? 4 : 2;
   const int64_t span =
       span_bound(max_len, q_len, a.G, a.tile_cols, a.window, a.causal) + kTile - 1;
-  a.part_keys = (int)(((span + parts - 1) / parts + kStep - 1) / kStep * kStep);
+  const int64_t step = a.tile_cols == 16 ? kStep : kBlockKeys;
+  a.part_keys = (int)(((span + parts - 1) / parts + step - 1) / step * step);
   a.out = (uint16_t*)out;
   a.lse = lse;
   a.part_out = (float*)workspace;

@@ -15,6 +15,7 @@ s % page_size of page table[s // page_size].
 from __future__ import annotations
 
 import ctypes
+import functools
 import heapq
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple
@@ -135,16 +136,29 @@ def paged_cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     return None if q is None else q_out
 
 
+@functools.lru_cache(maxsize=4096)
 def cache_parts(batch: int, q_len: int, q_heads: int, kv_heads: int, span: int) -> int:
-    """Pieces that paged_cached_attention cuts the visible span into."""
+    """Pieces that paged_cached_attention cuts the visible span into: of those that make
+    whole rounds of workgroups over the 256 CUs, the one with the least work for a CU.  A
+    piece costs its keys, about 128 more to start (streaming kernel, up to 16 columns
+    of rows and heads per KV head), the uneven ends of sequences of different lengths,
+    and its part in the join."""
 
     cols = q_len * (q_heads // kv_heads)
-    tiles = batch * kv_heads * -(-cols // (16 if cols <= 16 else 256))
-    if tiles == 0 or span <= 0:
+    stream = cols <= 16
+    units = batch * kv_heads * (1 if stream else -(-cols // 256))
+    if units == 0 or span <= 0:
         return 1
-    keys = max(128, -(-span * tiles // (1536 if cols <= 16 else 512)))
-    keys = -(-keys // 128) * 128
-    return max(1, min(MAX_PARTS, -(-span // keys)))
+    step, start = (128, 128) if stream else (64, 0)
+    most = min(MAX_PARTS, -(-(span + 31) // step))
+    best, least = 1, None
+    for rounds in (1, 2, 3, 4, 6):
+        parts = max(1, min(most, 256 * rounds // units))
+        keys = -(-(span + 31) // (parts * step)) * step
+        cost = -(-units * parts // 256) * (keys + start) + keys // 4 + 4 * parts
+        if least is None or cost < least:
+            best, least = parts, cost
+    return best
 
 
 def _paged_attention_impl(q, k_pages, v_pages, page_table, cache_lens, query_starts, max_len,
@@ -160,8 +174,8 @@ def _paged_attention_impl(q, k_pages, v_pages, page_table, cache_lens, query_sta
     lse = q.new_empty((B, Lq, Hq), dtype=torch.float32)
     nbytes, ws = 0, None
     if parts > 1:
-        nbytes = _lib.call("mrsa_paged_attention_workspace_bytes", B, Lq, Hq, D, parts)
-        ws = q.new_empty(max(nbytes, 0) // 4, dtype=torch.float32)
+        ws = q.new_empty(B * Lq * Hq * parts * (D + 2), dtype=torch.float32)
+        nbytes = ws.numel() * 4
     status = _lib.call_on(
         q.device, "mrsa_paged_attention_fwd", qc.data_ptr(), *qc.stride()[:3],
         k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3],
