@@ -285,10 +285,11 @@ def call(name: str, *args) -> int:
 def call_on(device: torch.device, name: str, *args) -> int:
     """call() with `device` current: a launch needs the device of its stream."""
 
+    fn = getattr(_lib or load(), name)
     if torch._C._cuda_getDevice() == device.index:
-        return getattr(load(), name)(*args)
+        return fn(*args)
     with torch.cuda.device(device):
-        return getattr(load(), name)(*args)
+        return fn(*args)
 
 
 def copy_buffers(dst: list, src: list) -> None:

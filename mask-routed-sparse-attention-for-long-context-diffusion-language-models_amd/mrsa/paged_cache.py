@@ -28,21 +28,30 @@ from .rotary import DTYPES, check_heads, check_tables, check_token_ints, dense_r
 MAX_PARTS = 1024
 
 
-def _check_pool(k_pages, v_pages, heads) -> None:
-    if k_pages.ndim != 4 or v_pages.shape != k_pages.shape:
+def _check_pool(k_pages, v_pages, heads) -> Tuple[int, int]:
+    """(page_size, KV heads) of a layer's pages."""
+
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError(f"k_pages and v_pages must have one shape [pages, page_size, Hkv, D], got "
-                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    P = k_pages.shape[1]
+                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
+    _, P, Hkv, D = shape
     if P < 16 or P & (P - 1):
         raise ValueError(f"page_size must be a power of two from 16 on, got {P}")
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if t.device != heads.device or t.dtype != heads.dtype:
-            raise ValueError(f"{name} must have the device and dtype of the heads")
-        if t.stride(3) != 1 and t.shape[3] > 1:
-            raise ValueError(f"{name} must have a dense last dim")
-    if k_pages.shape[3] != heads.shape[3]:
-        raise ValueError(f"pages of head_dim {k_pages.shape[3]} do not fit heads of "
-                         f"{heads.shape[3]}")
+    device, dtype = heads.device, heads.dtype
+    if (k_pages.device != device or v_pages.device != device or k_pages.dtype != dtype
+            or v_pages.dtype != dtype):
+        raise ValueError("k_pages and v_pages must have the device and dtype of the heads")
+    if (k_pages.stride(3) != 1 or v_pages.stride(3) != 1) and D > 1:
+        raise ValueError("k_pages and v_pages must have a dense last dim")
+    if D != heads.shape[3]:
+        raise ValueError(f"pages of head_dim {D} do not fit heads of {heads.shape[3]}")
+    return P, Hkv
+
+
+def _check_writable(pool, name: str) -> None:
+    if 0 in pool.stride() and any(s == 0 and n > 1 for s, n in zip(pool.stride(), pool.shape)):
+        raise ValueError(f"{name} must not be an expanded tensor")
 
 
 def _check_table(page_table, batch: int, device) -> torch.Tensor:
@@ -56,29 +65,42 @@ def _check_table(page_table, batch: int, device) -> torch.Tensor:
 
 
 def _no_gradient(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
 
 
 def _paged_append_impl(k, v, k_pages, v_pages, page_table, slots, q, cos, sin, positions,
                        interleaved):
     B, L, Hkv, D = k.shape
     kc, vc = dense_rows(k), dense_rows(v)
-    qc = None if q is None else dense_rows(q)
-    Hq = 0 if q is None else q.shape[2]
+    kb, kl, kh, _ = kc.stride()
+    vb, vl, vh, _ = vc.stride()
+    if q is None:
+        Hq, qp, qb, ql, qh = 0, None, 0, 0, 0
+    else:
+        qc = dense_rows(q)
+        Hq, qp = q.shape[2], qc.data_ptr()
+        qb, ql, qh, _ = qc.stride()
     q_out = k.new_empty((B, L, Hq, D))
-    ct, st = (None, None) if cos is None else (cos.contiguous(), sin.contiguous())
-    ps = (0, 0) if positions is None else positions.stride()
+    if cos is None:
+        cp = sp = pp = None
+        rows = half = pb = pl = 0
+    else:
+        ct, st = cos.contiguous(), sin.contiguous()
+        cp, sp, pp = ct.data_ptr(), st.data_ptr(), positions.data_ptr()
+        rows, half = cos.shape
+        pb, pl = positions.stride()
+    sb, sl = slots.stride()
+    kps, kss, khs, _ = k_pages.stride()
+    vps, vss, vhs, _ = v_pages.stride()
+    pages, page_size = k_pages.shape[:2]
     status = _lib.call_on(
-        k.device, "mrsa_paged_append_fwd", _lib.ptr(qc),
-        *((0, 0, 0) if qc is None else qc.stride()[:3]), kc.data_ptr(), *kc.stride()[:3],
-        vc.data_ptr(), *vc.stride()[:3], _lib.ptr(ct), _lib.ptr(st),
-        0 if cos is None else cos.shape[0], _lib.ptr(positions), *ps, slots.data_ptr(),
-        *slots.stride(), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-        k_pages.shape[0], k_pages.shape[1], k_pages.data_ptr(), *k_pages.stride()[:3],
-        v_pages.data_ptr(), *v_pages.stride()[:3], B, L, Hq, Hkv, D,
-        0 if cos is None else 2 * cos.shape[1], DTYPES[k.dtype], int(interleaved),
-        q_out.data_ptr(), _lib.stream_of(k))
+        k.device, "mrsa_paged_append_fwd", qp, qb, ql, qh, kc.data_ptr(), kb, kl, kh,
+        vc.data_ptr(), vb, vl, vh, cp, sp, rows, pp, pb, pl, slots.data_ptr(), sb, sl,
+        page_table.data_ptr(), page_table.stride(0), page_table.shape[1], pages, page_size,
+        k_pages.data_ptr(), kps, kss, khs, v_pages.data_ptr(), vps, vss, vhs, B, L, Hq, Hkv, D,
+        2 * half, DTYPES[k.dtype], interleaved, q_out.data_ptr(), _lib.stream_of(k))
     _lib.check(status, "paged_cache_append")
     return q_out
 
@@ -107,17 +129,16 @@ def paged_cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError(f"k and v must have one shape, dtype and device, got {tuple(k.shape)} "
                          f"{k.dtype} and {tuple(v.shape)} {v.dtype}")
-    _check_pool(k_pages, v_pages, k)
-    if k_pages.shape[2] != Hkv:
-        raise ValueError(f"pages of {k_pages.shape[2]} heads do not fit rows of {Hkv}")
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-            raise ValueError(f"{name} must not be an expanded tensor")
+    _, pool_heads = _check_pool(k_pages, v_pages, k)
+    if pool_heads != Hkv:
+        raise ValueError(f"pages of {pool_heads} heads do not fit rows of {Hkv}")
+    _check_writable(k_pages, "k_pages")
+    _check_writable(v_pages, "v_pages")
     page_table = _check_table(page_table, B, k.device)
     slots = check_token_ints(slots, "slots", B, L, k.device)
     if q is not None:
         check_heads(q, "q")
-        if q.shape[:2] != k.shape[:2] or q.shape[3] != D or q.dtype != k.dtype:
+        if q.shape != (B, L, q.shape[2], D) or q.dtype != k.dtype:
             raise ValueError(f"q and k must agree in batch, length, head_dim and dtype, got "
                              f"{tuple(q.shape)} {q.dtype} and {tuple(k.shape)} {k.dtype}")
         if q.device != k.device:
@@ -130,7 +151,8 @@ def paged_cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
                                                                      k.device)
     elif positions is not None:
         raise ValueError("positions need cos and sin")
-    _no_gradient("paged_cache_append", q, k, v, k_pages, v_pages)
+    if torch.is_grad_enabled():
+        _no_gradient("paged_cache_append", q, k, v, k_pages, v_pages)
     q_out = torch.ops.mrsa.paged_append_.default(k, v, k_pages, v_pages, page_table, slots, q, cos,
                                                  sin, positions, bool(interleaved))
     return None if q is None else q_out
@@ -163,25 +185,27 @@ def cache_parts(batch: int, q_len: int, q_heads: int, kv_heads: int, span: int) 
 
 def _paged_attention_impl(q, k_pages, v_pages, page_table, cache_lens, query_starts, max_len,
                           causal, window, sm_scale, parts):
-    B, Lq, Hq, D = q.shape
-    Hkv = k_pages.shape[2]
+    shape = q.shape
+    B, Lq, Hq, D = shape
     qc = dense_rows(q)
-    if qc.data_ptr() % 16 or any(s % 8 for s in qc.stride()[:3]):
-        qc = qc.contiguous()
-        if qc.data_ptr() % 16:
-            qc = qc.clone()
-    out = q.new_empty(q.shape)
+    qb, ql, qh, _ = qc.stride()
+    if (qb | ql | qh) % 8 or qc.data_ptr() % 16:
+        qc = qc.clone(memory_format=torch.contiguous_format)
+        qb, ql, qh, _ = qc.stride()
+    kps, kss, khs, _ = k_pages.stride()
+    vps, vss, vhs, _ = v_pages.stride()
+    pages, page_size, Hkv, _ = k_pages.shape
+    out = q.new_empty(shape)
     lse = q.new_empty((B, Lq, Hq), dtype=torch.float32)
-    nbytes, ws = 0, None
+    nbytes, wp = 0, None
     if parts > 1:
         ws = q.new_empty(B * Lq * Hq * parts * (D + 2), dtype=torch.float32)
-        nbytes = ws.numel() * 4
+        nbytes, wp = ws.numel() * 4, ws.data_ptr()
     status = _lib.call_on(
-        q.device, "mrsa_paged_attention_fwd", qc.data_ptr(), *qc.stride()[:3],
-        k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3],
-        page_table.data_ptr(), page_table.stride(0), page_table.shape[1], k_pages.shape[0],
-        k_pages.shape[1], cache_lens.data_ptr(), _lib.ptr(query_starts), max_len, B, Lq, Hq, Hkv,
-        D, DTYPES[q.dtype], int(causal), window, sm_scale, parts, _lib.ptr(ws), nbytes,
+        q.device, "mrsa_paged_attention_fwd", qc.data_ptr(), qb, ql, qh, k_pages.data_ptr(), kps,
+        kss, khs, v_pages.data_ptr(), vps, vss, vhs, page_table.data_ptr(), page_table.stride(0),
+        page_table.shape[1], pages, page_size, cache_lens.data_ptr(), _lib.ptr(query_starts),
+        max_len, B, Lq, Hq, Hkv, D, DTYPES[q.dtype], causal, window, sm_scale, parts, wp, nbytes,
         out.data_ptr(), lse.data_ptr(), _lib.stream_of(q))
     _lib.check(status, "paged_cached_attention")
     return out, lse
@@ -223,8 +247,7 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     B, Lq, Hq, D = q.shape
     if D not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {D}")
-    _check_pool(k_pages, v_pages, q)
-    Hkv = k_pages.shape[2]
+    page_size, Hkv = _check_pool(k_pages, v_pages, q)
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError(f"query heads ({Hq}) must be divisible by KV heads ({Hkv})")
     page_table = _check_table(page_table, B, q.device)
@@ -233,7 +256,7 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         query_starts = _check_sequence_ints(query_starts, "query_starts", B, q.device)
     if window is not None and window < 0:
         raise ValueError(f"window must be >= 0, got {window}")
-    rows = page_table.shape[1] * k_pages.shape[1]
+    rows = page_table.shape[1] * page_size
     if max_len is None:
         max_len = rows
     elif max_len < 0:
@@ -241,7 +264,8 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     max_len = min(int(max_len), rows)
     if sm_scale is None:
         sm_scale = D ** -0.5
-    _no_gradient("paged_cached_attention", q, k_pages, v_pages)
+    if torch.is_grad_enabled():
+        _no_gradient("paged_cached_attention", q, k_pages, v_pages)
     window = -1 if window is None else int(window)
     if parts is None:
         span = max_len
@@ -257,15 +281,16 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
 def _copy_pages_impl(k_pages, v_pages, src, dst):
     n = len(src)
     layered = k_pages.ndim == 5
-    k0, v0 = (k_pages, v_pages) if layered else (k_pages[None], v_pages[None])
-    layers, pages = k0.shape[:2]
-    size = k0.element_size()
+    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if not layered:
+        shape, ks, vs = (1, *shape), (0, *ks), (0, *vs)
+    size = k_pages.element_size()
     arrays = (ctypes.c_int64 * max(n, 1))(*src), (ctypes.c_int64 * max(n, 1))(*dst)
     status = _lib.call_on(
-        k_pages.device, "mrsa_copy_pages", k0.data_ptr(), k0.stride(0) * size,
-        k0.stride(1) * size, v0.data_ptr(), v0.stride(0) * size, v0.stride(1) * size, layers,
-        pages, k0[0, 0].numel() * size if layers and pages else 0, n,
-        ctypes.addressof(arrays[0]), ctypes.addressof(arrays[1]), _lib.stream_of(k_pages))
+        k_pages.device, "mrsa_copy_pages", k_pages.data_ptr(), ks[0] * size, ks[1] * size,
+        v_pages.data_ptr(), vs[0] * size, vs[1] * size, shape[0], shape[1],
+        shape[2] * shape[3] * shape[4] * size, n, ctypes.addressof(arrays[0]),
+        ctypes.addressof(arrays[1]), _lib.stream_of(k_pages))
     _lib.check(status, "copy_cache_pages")
 
 
@@ -287,10 +312,9 @@ def copy_cache_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: Sequence
         raise ValueError("k_pages and v_pages must have one dtype")
     lead = k_pages.ndim - 3
     for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if t.numel() and not t[(0,) * lead].is_contiguous():
+        if not t.is_contiguous() and t.numel() and not t[(0,) * lead].is_contiguous():
             raise ValueError(f"the pages of {name} must be dense")
-        if any(s == 0 and n > 1 for s, n in zip(t.stride()[:lead], t.shape)):
-            raise ValueError(f"{name} must not be an expanded tensor")
+        _check_writable(t, name)
     src, dst = [int(i) for i in src], [int(i) for i in dst]
     if len(src) != len(dst):
         raise ValueError(f"{len(src)} sources for {len(dst)} destinations")

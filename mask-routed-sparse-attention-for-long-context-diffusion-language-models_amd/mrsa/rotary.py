@@ -88,15 +88,16 @@ def dense_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def check_tables(cos, sin, head_dim: int, device) -> None:
-    if cos.ndim != 2 or sin.shape != cos.shape:
+    shape = cos.shape
+    if len(shape) != 2 or sin.shape != shape:
         raise ValueError(f"cos and sin must have the same shape [rows, rotary_dim / 2], got "
-                         f"{tuple(cos.shape)} and {tuple(sin.shape)}")
+                         f"{tuple(shape)} and {tuple(sin.shape)}")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError("cos and sin must be fp32")
     if cos.device != device or sin.device != device:
         raise ValueError("cos and sin must be on the device of the heads")
-    if 2 * cos.shape[1] > head_dim:
-        raise ValueError(f"tables for {2 * cos.shape[1]} dims do not fit heads of {head_dim}")
+    if 2 * shape[1] > head_dim:
+        raise ValueError(f"tables for {2 * shape[1]} dims do not fit heads of {head_dim}")
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("cos and sin get no gradient")
 
@@ -106,27 +107,32 @@ def check_token_ints(t, name: str, batch: int, seq_len: int, device) -> torch.Te
 
     if t.dtype != torch.long or t.device != device:
         raise ValueError(f"{name} must be torch.long on the device of the heads")
-    if t.shape == (seq_len,):
-        return t.expand(batch, seq_len)
-    if t.shape != (batch, seq_len):
+    if t.shape == (batch, seq_len):
+        return t
+    if t.shape != (seq_len,):
         raise ValueError(f"{name} must have shape {(batch, seq_len)} or {(seq_len,)}, "
                          f"got {tuple(t.shape)}")
-    return t
+    return t.expand(batch, seq_len)
 
 
 def _rotary_impl(q, k, cos, sin, positions, interleaved, inverse):
-    B, L, Hq, D = q.shape
-    Hkv = 0 if k is None else k.shape[2]
-    qc, kc = dense_rows(q), None if k is None else dense_rows(k)
-    ct, st = cos.contiguous(), sin.contiguous()
-    q_out, k_out = q.new_empty(q.shape), q.new_empty((B, L, Hkv, D))
-    ps = (0, 0) if positions is None else positions.stride()
-    ks = (0, 0, 0) if kc is None else kc.stride()[:3]
+    shape = q.shape
+    B, L, Hq, D = shape
+    qc, ct, st = dense_rows(q), cos.contiguous(), sin.contiguous()
+    qb, ql, qh, _ = qc.stride()
+    if k is None:
+        Hkv, kp, kb, kl, kh = 0, None, 0, 0, 0
+    else:
+        kc = dense_rows(k)
+        Hkv, kp = k.shape[2], kc.data_ptr()
+        kb, kl, kh, _ = kc.stride()
+    pp, pb, pl = (None, 0, 0) if positions is None else (positions.data_ptr(), *positions.stride())
+    q_out, k_out = q.new_empty(shape), q.new_empty((B, L, Hkv, D))
+    rows, half = cos.shape
     status = _lib.call_on(
-        q.device, "mrsa_rotary_fwd", qc.data_ptr(), *qc.stride()[:3], _lib.ptr(kc), *ks,
-        ct.data_ptr(), st.data_ptr(), cos.shape[0], _lib.ptr(positions), *ps, B, L, Hq, Hkv, D,
-        2 * cos.shape[1], DTYPES[q.dtype], int(interleaved), int(inverse), q_out.data_ptr(),
-        k_out.data_ptr(), _lib.stream_of(q))
+        q.device, "mrsa_rotary_fwd", qc.data_ptr(), qb, ql, qh, kp, kb, kl, kh, ct.data_ptr(),
+        st.data_ptr(), rows, pp, pb, pl, B, L, Hq, Hkv, D, 2 * half, DTYPES[q.dtype], interleaved,
+        inverse, q_out.data_ptr(), k_out.data_ptr(), _lib.stream_of(q))
     _lib.check(status, "rotary_qk")
     return q_out, k_out
 
@@ -165,7 +171,7 @@ class _Rotary(torch.autograd.Function):
 def check_heads(t, name: str) -> None:
     if t.ndim != 4:
         raise ValueError(f"{name} must have shape [B, L, heads, head_dim], got {tuple(t.shape)}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in DTYPES:
         raise ValueError(f"{name} must be bf16, fp16 or fp32, got {t.dtype}")
@@ -188,7 +194,7 @@ def rotary_qk(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin
     B, L, _, D = q.shape
     if k is not None:
         check_heads(k, "k")
-        if k.shape[:2] != q.shape[:2] or k.shape[3] != D or k.dtype != q.dtype:
+        if k.shape != (B, L, k.shape[2], D) or k.dtype != q.dtype:
             raise ValueError(f"q and k must agree in batch, length, head_dim and dtype, got "
                              f"{tuple(q.shape)} {q.dtype} and {tuple(k.shape)} {k.dtype}")
         if k.device != q.device:
