@@ -78,7 +78,6 @@ struct PagedArgs {
   int causal, window;         // window < 0: none
   float scale_log2;
   int parts, part_keys, col_tiles, tile_cols;
-  int slots;                  // of the block kernel's ring (a power of two)
   uint16_t* out;
   float* lse;
   float* part_out;            // parts > 1: [B, Hkv, M, parts, D]
@@ -453,7 +452,7 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   constexpr int SLOTB = 2 * TILEB;
   extern __shared__ __align__(256) unsigned char smem[];
   unsigned char* ring = smem;
-  int* flag = reinterpret_cast<int*>(ring + a.slots * SLOTB);  // last tile (+ 1) with a value not finite
+  int* flag = reinterpret_cast<int*>(ring + 2 * SLOTB);  // last tile (+ 1) with a value not finite
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -489,17 +488,10 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   for (int t = 0; t < NT; ++t) {
     const int m = c0 + 16 * t + col;
     const bool cok = m < a.M;
-    const int qi = cok ? m / a.G : 0, qg = cok ? m - qi * a.G : 0;
-    const int pos = p0 + qi;
+    const int pos = p0 + (cok ? m / a.G : 0);
     padding[t] = !cok || pos < 0 || pos >= n;
     lo[t] = hi[t] = 0;
     if (!padding[t]) seen_by(a, n, pos, lo[t], hi[t]);
-    const uint16_t* qp = a.q + b * a.q_sb + qi * a.q_sl + (h * a.G + qg) * a.q_sh + 8 * grp;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      Q[t][s] = u32x4_t{0, 0, 0, 0};
-      if (cok) Q[t][s] = *reinterpret_cast<const u32x4_t*>(qp + 32 * s);
-    }
   }
   f32x4_t O[NT][DT];
   float mx[NT], sum[NT];
@@ -552,184 +544,74 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
       for (int i = 0; i < DMAS; ++i) dma_kb(d.to + 1024 * i, d.src, x < 4 ? k_lane[i] : v_lane[i]);
     }
   };
-  // Whether an entry of this piece of the table is unmapped: then every tile looks.
-  bool holes = false;
+  bool holes = false;  // an entry of this piece of the table is unmapped: then every tile looks
+  auto live_at = [&](int base, int i) { return !holes || is_live(page_at(a, table, base + 16 * i)); };
+  const int tiles = first < last ? (last - first + kBlockKeys - 1) / kBlockKeys : 0;
+  auto issue = [&](int slot, int base, int page) {
+    const Piece d = piece(wave, slot, base, page);
+#pragma unroll
+    for (int i = 0; i < DMAS; ++i) dma_kb(d.to + 1024 * i, d.src, own_lane[i]);
+    issue_others(slot, base);
+  };
+  if (tiles > 0) issue(0, first, page_for(first, wave));
+  int next = tiles > 0 ? page_for(first + kBlockKeys, wave) : -1;
+
+  // (behind the first tile's DMA: the queries, and the look for holes)
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int m = c0 + 16 * t + col;
+    const int qi = m < a.M ? m / a.G : 0, qg = m < a.M ? m - qi * a.G : 0;
+    const uint16_t* qp = a.q + b * a.q_sb + qi * a.q_sl + (h * a.G + qg) * a.q_sh + 8 * grp;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      Q[t][s] = u32x4_t{0, 0, 0, 0};
+      if (m < a.M) Q[t][s] = *reinterpret_cast<const u32x4_t*>(qp + 32 * s);
+    }
+  }
   for (int e = (first >> a.page_shift) + lane; e <= (last - 1) >> a.page_shift; e += 64)
     holes |= !is_live(a.table[b * a.table_stride + e]);
   holes = __builtin_amdgcn_ballot_w64(holes) != 0;
-  auto live_at = [&](int base, int i) { return !holes || is_live(page_at(a, table, base + 16 * i)); };
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(Q[t][s]));
-  const int tiles = first < last ? (last - first + kBlockKeys - 1) / kBlockKeys : 0;
-  // Tiles t .. t + slots - 2 are on their way while t - 1 is computed.  A wave waits for its
-  // DMA of tile t only: the newer ones of two further tiles (four instructions a
-  // piece) stay in flight.
-  const int ahead = a.slots - 1;
-  const int ring_mask = a.slots - 1;
-  const bool one_piece = wave + waves >= 8;
-  int next = -1;
-  for (int t = 0; t < min(tiles, ahead); ++t) {
-    const int base = first + t * kBlockKeys;
-    const Piece d = piece(wave, t, base, page_for(base, wave));
+
+  // LDS addresses, slot 0: K's rows of each reduction step, V's of each dim tile (the slot
+  // and the row tile are instruction offsets: no vector work between the products)
+  uint32_t k_at[KS], v_at[DT];
+  {
+    const uint32_t lds0 = lds_addr(ring);
+    const int rt = 4 * grp + (col >> 2);
 #pragma unroll
-    for (int i = 0; i < DMAS; ++i) dma_kb(d.to + 1024 * i, d.src, own_lane[i]);
-    issue_others(t, base);
+    for (int s = 0; s < KS; ++s)
+      k_at[s] = lds0 + ROWB * col + 16u * (uint32_t)((4 * s + grp) ^ swizzle_k<D>(col));
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      v_at[d] = lds0 + TILEB + ROWB * rt +
+                16u * (uint32_t)((2 * d + ((col >> 1) & 1)) ^ swizzle<D>(rt)) + 8u * (col & 1);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(k_at[s]));
+#pragma unroll
+    for (int d = 0; d < DT; ++d) asm volatile("" : "+v"(v_at[d]));
   }
-  next = tiles > 0 ? page_for(first + ahead * kBlockKeys, wave) : -1;
-  const uint32_t lds0 = lds_addr(ring);
-  const uint32_t arow = lds0 + ROWB * col + 16u * (uint32_t)(grp ^ swizzle_k<D>(col));
-  const int rt = 4 * grp + (col >> 2);
-  const uint32_t trow = lds0 + TILEB + ROWB * rt +
-                        16u * (uint32_t)(((col >> 1) & 1) ^ swizzle<D>(rt)) + 8u * (col & 1);
+  const float scale = a.scale_log2;
 
-  // One tile's products; MASKED: some column of the wave does not see all of it, DIRTY: and
-  // V holds values that are not finite (taken out of LDS: added here).
-  auto compute = [&](int base, uint32_t slot_off, bool bring, const Piece& own, auto masked,
-                     bool dirty) {
-    constexpr bool MASKED = decltype(masked)::value;
-    f32x4_t S[NT][4];
-#pragma unroll
-    for (int c = 0; c < NT; ++c)
-#pragma unroll
-      for (int m = 0; m < 4; ++m) S[c][m] = zero4();
-    {
-      const uint32_t at = arow + slot_off;
-      constexpr int AHEAD = 4;
-      u32x4_t x[4 * KS];
-      auto operand = [&](int o) {  // keys 16 (o & 3) .., dims 32 (o >> 2) ..
-        return lds_read16((at ^ (64u * (o >> 2))) + 16u * ROWB * (o & 3));
-      };
-#pragma unroll
-      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int o = 0; o < 4 * KS; ++o) {
-#pragma unroll
-        for (int c = 0; c < NT; ++c) S[c][o & 3] = T::mfma(x[o], Q[c][o >> 2], S[c][o & 3]);
-        if (o + AHEAD < 4 * KS) x[o + AHEAD] = operand(o + AHEAD);
-        if (o % 4 == 3 && bring) dma_kb(own.to + 1024 * (o / 4), own.src, own_lane[o / 4]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    uint32_t seen[NT];
-    if constexpr (MASKED) {
-      const bool live[4] = {live_at(base, 0), live_at(base, 1), live_at(base, 2), live_at(base, 3)};
-#pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        seen[c] = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = base + 16 * (i >> 2) + 4 * grp + (i & 3);
-          const bool ok = live[i >> 2] && key >= lo[c] && key < hi[c];
-          if (ok) seen[c] |= 1u << i;
-          S[c][i >> 2][i & 3] = ok ? S[c][i >> 2][i & 3] : neg_inf();
-        }
-      }
-    }
-    u32x4_t Pb[NT][2];
-#pragma unroll
-    for (int c = 0; c < NT; ++c) {
-      const float top = across4_max(max16_raw(S[c])) * a.scale_log2;
-      if (__builtin_amdgcn_ballot_w64(top > mx[c] + kSlack) != 0) {
-        const float to = __builtin_fmaxf(mx[c], top);
-        const float f = to == neg_inf() ? 1.f : exp2_hw(mx[c] - to);
-        mx[c] = to;
-        sum[c] *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) O[c][d] *= f;
-      }
-      const float off = mx[c] == neg_inf() ? 0.f : mx[c];
-      float part_sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = exp2_hw(__builtin_fmaf(S[c][i >> 2][i & 3], a.scale_log2, -off));
-        S[c][i >> 2][i & 3] = p;
-        part_sum[i & 3] += p;
-      }
-      sum[c] += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        Pb[c][k] = u32x4_t{T::pack(S[c][2 * k][0], S[c][2 * k][1]), T::pack(S[c][2 * k][2], S[c][2 * k][3]),
-                           T::pack(S[c][2 * k + 1][0], S[c][2 * k + 1][1]),
-                           T::pack(S[c][2 * k + 1][2], S[c][2 * k + 1][3])};
-    }
-    // ---- V^T . P^T
-    {
-      const uint32_t at = trow + slot_off;
-      constexpr int AHEAD = 4;
-      u32x4_t x[2 * DT];
-      auto operand = [&](int o) {  // dims 16 (o >> 1) .., keys 32 (o & 1) ..
-        const uint32_t ad = (at ^ (32u * (o >> 1))) + 32u * ROWB * (o & 1);
-        const u32x2_t y0 = read_transposed(ad), y1 = read_transposed(ad + 16u * ROWB);
-        return u32x4_t{y0[0], y0[1], y1[0], y1[1]};
-      };
-#pragma unroll
-      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int o = 0; o < 2 * DT; ++o) {
-#pragma unroll
-        for (int c = 0; c < NT; ++c) O[c][o >> 1] = T::mfma(x[o], Pb[c][o & 1], O[c][o >> 1]);
-        if (o + AHEAD < 2 * DT) x[o + AHEAD] = operand(o + AHEAD);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    if constexpr (MASKED) {
-      if (!dirty) return;
-      for (int kk = 0; kk < kBlockKeys; ++kk) {
-        const int key = base + kk;
-        if (!live_at(base, kk >> 4) || key < r.lo || key >= r.end) continue;
-        const int from = 16 * ((kk & 15) >> 2) + col, slot_i = 4 * (kk >> 4) + (kk & 3);
-        const uint16_t* vp = a.v + h * a.v_sh + page_at(a, table, key) * a.v_sp +
-                             (int64_t)(key & page_mask) * a.v_sr;
-#pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          const bool ok = (__shfl(seen[c], from, 64) >> slot_i) & 1;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t x = vp[16 * d + 4 * grp + e];
-              if (ok && (x & T::kExp) == T::kExp) O[c][d][e] += T::value(x);
-            }
-        }
-      }
-    }
-  };
-
-  for (int t = 0; t < tiles; ++t) {
+  auto tile = [&](int t, auto slot_c) {
+    constexpr int slot = decltype(slot_c)::value;
     const int base = first + t * kBlockKeys;
-    if (ahead == 3 && t + 2 < tiles) {
-      if (one_piece)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * 16 / ROWS) : "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 * 16 / ROWS) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    }
-    // The wave's first piece of the tile `ahead` goes between the products of S: all waves'
-    // DMA at once would hold them up (32 cycles an instruction).
-    const bool bring = t + ahead < tiles;
-    Piece own = {0, nullptr};
-    if (bring) {
-      own = piece(wave, (t + ahead) & ring_mask, base + ahead * kBlockKeys, next);
-      issue_others((t + ahead) & ring_mask, base + ahead * kBlockKeys);
-    }
-    asm volatile("" ::: "memory");
-    const uint32_t slot_off = (t & ring_mask) * SLOTB;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 1 < tiles) issue(1 - slot, base + kBlockKeys, next);
     const bool whole =
         !holes || (live_at(base, 0) && live_at(base, 1) && live_at(base, 2) && live_at(base, 3));
     bool dirty = false;
     if (!whole || base < r.inner_lo || base + kBlockKeys > r.inner_hi) {
       // V rows that no column sees become zeros; values that are not finite
       // are taken out (a column that does not see them must not get 0 x inf)
-      // and added one by one in compute().
+      // and added one by one below.
       bool odd = false;
       for (int x = tid; x < kBlockKeys * UNITS; x += 64 * waves) {
         const int row = x / UNITS, key = base + row;
-        u32x4_t* at = reinterpret_cast<u32x4_t*>(ring + slot_off + TILEB + 16 * x);
+        u32x4_t* at = reinterpret_cast<u32x4_t*>(ring + slot * SLOTB + TILEB + 16 * x);
         bool lv = true;
         if (holes) {
           const int e = key >> a.page_shift;  // (a vector load: rows differ between lanes)
@@ -755,12 +637,121 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       dirty = *(volatile int*)flag == t + 1;
     }
-    if (dirty || !whole || base < w.inner_lo || base + kBlockKeys > w.inner_hi)
-      compute(base, slot_off, bring, own, std::true_type{}, dirty);
-    else
-      compute(base, slot_off, bring, own, std::false_type{}, false);
+    asm volatile("" ::: "memory");
+    // ---- scores
+    constexpr int AHEAD = 4;                 // operands in flight
+    f32x4_t S[NT][4];
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+      for (int m = 0; m < 4; ++m) S[c][m] = zero4();
+    {
+      u32x4_t x[4 * KS];
+      auto operand = [&](int o) {  // keys 16 (o & 3) .., dims 32 (o >> 2) ..
+        return lds_read16(k_at[o >> 2] + (uint32_t)(slot * SLOTB + 16 * ROWB * (o & 3)));
+      };
+#pragma unroll
+      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int o = 0; o < 4 * KS; ++o) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c) S[c][o & 3] = T::mfma(x[o], Q[c][o >> 2], S[c][o & 3]);
+        if (o + AHEAD < 4 * KS) x[o + AHEAD] = operand(o + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    uint32_t seen[NT];
+    if (!whole || base < w.inner_lo || base + kBlockKeys > w.inner_hi) {
+      const bool live[4] = {live_at(base, 0), live_at(base, 1), live_at(base, 2), live_at(base, 3)};
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        seen[c] = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = base + 16 * (i >> 2) + 4 * grp + (i & 3);
+          const bool ok = live[i >> 2] && key >= lo[c] && key < hi[c];
+          if (ok) seen[c] |= 1u << i;
+          S[c][i >> 2][i & 3] = ok ? S[c][i >> 2][i & 3] : neg_inf();
+        }
+      }
+      asm volatile("");  // (a branch, not selects in every tile)
+    } else {
+#pragma unroll
+      for (int c = 0; c < NT; ++c) seen[c] = 0xffffu;
+    }
+    u32x4_t Pb[NT][2];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+      const float top = across4_max(max16_raw(S[c])) * scale;
+      if (__builtin_amdgcn_ballot_w64(top > mx[c] + kSlack) != 0) {
+        const float to = __builtin_fmaxf(mx[c], top);
+        const float f = to == neg_inf() ? 1.f : exp2_hw(mx[c] - to);
+        mx[c] = to;
+        sum[c] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) O[c][d] *= f;
+      }
+      const float off = mx[c] == neg_inf() ? 0.f : mx[c];
+      float part_sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = exp2_hw(__builtin_fmaf(S[c][i >> 2][i & 3], scale, -off));
+        S[c][i >> 2][i & 3] = p;
+        part_sum[i & 3] += p;
+      }
+      sum[c] += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        Pb[c][k] = u32x4_t{T::pack(S[c][2 * k][0], S[c][2 * k][1]), T::pack(S[c][2 * k][2], S[c][2 * k][3]),
+                           T::pack(S[c][2 * k + 1][0], S[c][2 * k + 1][1]),
+                           T::pack(S[c][2 * k + 1][2], S[c][2 * k + 1][3])};
+    }
+    // ---- V^T . P^T
+    {
+      u32x4_t x[2 * DT];
+      auto operand = [&](int o) {  // dims 16 (o >> 1) .., keys 32 (o & 1) ..
+        const uint32_t ad = v_at[o >> 1] + (uint32_t)(slot * SLOTB + 32 * ROWB * (o & 1));
+        const u32x2_t y0 = read_transposed(ad), y1 = read_transposed(ad + 16u * ROWB);
+        return u32x4_t{y0[0], y0[1], y1[0], y1[1]};
+      };
+#pragma unroll
+      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int o = 0; o < 2 * DT; ++o) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c) O[c][o >> 1] = T::mfma(x[o], Pb[c][o & 1], O[c][o >> 1]);
+        if (o + AHEAD < 2 * DT) x[o + AHEAD] = operand(o + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
     // (a scalar load in flight would turn every wait for LDS into a wait for all of it)
-    next = page_for(base + (ahead + 1) * kBlockKeys, wave);
+    next = page_for(base + 2 * kBlockKeys, wave);
+    if (dirty) {
+      for (int kk = 0; kk < kBlockKeys; ++kk) {
+        const int key = base + kk;
+        if (!live_at(base, kk >> 4) || key < r.lo || key >= r.end) continue;
+        const int from = 16 * ((kk & 15) >> 2) + col, slot_i = 4 * (kk >> 4) + (kk & 3);
+        const uint16_t* vp = a.v + h * a.v_sh + page_at(a, table, key) * a.v_sp +
+                             (int64_t)(key & page_mask) * a.v_sr;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          const bool ok = (__shfl(seen[c], from, 64) >> slot_i) & 1;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x = vp[16 * d + 4 * grp + e];
+              if (ok && (x & T::kExp) == T::kExp) O[c][d][e] += T::value(x);
+            }
+        }
+      }
+    }
+  };
+  for (int t = 0; t < tiles; t += 2) {
+    tile(t, std::integral_constant<int, 0>{});
+    if (t + 1 < tiles) tile(t + 1, std::integral_constant<int, 1>{});
   }
 
   // ---- out: lane (col, grp) holds dims 16 d + 4 grp .. of its columns
@@ -899,7 +890,7 @@ int launch(const PagedArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves), lds,
                        stream, a);
   } else {
-    const size_t lds = (size_t)a.slots * 2 * kBlockKeys * 2 * D + 16;
+    const size_t lds = 4 * kBlockKeys * 2 * D + 16;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_block_kernel<T, D>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
       return MRSA_ERR_LAUNCH;
@@ -995,7 +986,6 @@ extern "C" int mrsa_paged_attention_fwd(
   a.parts = (int)parts;
   a.tile_cols = columns_of(a.M);
   a.col_tiles = (a.M + a.tile_cols - 1) / a.tile_cols;
-  a.slots = a.tile_cols > 4 * kBlockCols ? 4 : 2;
   const int64_t span =
       span_bound(max_len, q_len, a.G, a.tile_cols, a.window, a.causal) + kTile - 1;
   const int64_t step = a.tile_cols == 16 ? kStep : kBlockKeys;
