@@ -156,15 +156,15 @@ __global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedArgs a) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  int64_t id = blockIdx.x;
+  uint32_t id = blockIdx.x;  // (the grid is below 2^31)
   // KV heads next to each other (a row's heads are neighbours in memory), parts last: of
   // sequences of different lengths the short pieces at their ends then come last.
-  const int h = (int)(id % a.Hkv);
-  id /= a.Hkv;
-  const int ct = (int)(id % a.col_tiles);
-  id /= a.col_tiles;
-  const int b = (int)(id % a.B);
-  const int part = (int)(id / a.B);
+  const int h = id % (uint32_t)a.Hkv;
+  id /= (uint32_t)a.Hkv;
+  const int ct = id % (uint32_t)a.col_tiles;
+  id /= (uint32_t)a.col_tiles;
+  const int b = id % (uint32_t)a.B;
+  const int part = id / (uint32_t)a.B;
 
   const int n = length_of(a, b), p0 = start_of(a, b, n);
   const Range r = tile_range(a, n, p0, ct * 16, 16);
@@ -437,6 +437,9 @@ __device__ __forceinline__ void dma_kb(uint32_t to, const uint8_t* base, uint32_
                : "memory", "m0");
 }
 // Swizzle of K's rows: the 16 rows of one operand read meet different banks.
+// Slots of the ring: waves 4 .. are half a tile behind the others and keep a third in use.
+__host__ __device__ constexpr int block_slots(int waves) { return waves > 4 ? 3 : 2; }
+
 template <int D>
 __device__ __forceinline__ int swizzle_k(int r) {
   return D == 128 ? r & 15 : (r >> 1) & 7;
@@ -452,25 +455,25 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   constexpr int SLOTB = 2 * TILEB;
   extern __shared__ __align__(256) unsigned char smem[];
   unsigned char* ring = smem;
-  int* flag = reinterpret_cast<int*>(ring + 2 * SLOTB);  // last tile (+ 1) with a value not finite
-
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int waves = __builtin_amdgcn_readfirstlane((int)blockDim.x >> 6);
+  const uint32_t ring_bytes = block_slots(waves) * SLOTB;
+  int* flag = reinterpret_cast<int*>(ring + ring_bytes);  // last tile (+ 1) with a value not finite
   const int col = lane & 15, grp = lane >> 4;
   // XCD-aware order: workgroups go to the XCDs in turn, so XCD x takes a contiguous
   // range, in which the column tiles of one piece of keys meet in its L2.
-  int64_t id;
+  uint32_t id;  // (the grid is below 2^31)
   {
-    const int64_t total = gridDim.x, x = blockIdx.x % 8, q8 = total / 8, r8 = total % 8;
+    const uint32_t total = gridDim.x, x = blockIdx.x % 8, q8 = total / 8, r8 = total % 8;
     id = x * q8 + min(x, r8) + blockIdx.x / 8;
   }
-  const int ct = (int)(id % a.col_tiles);
-  id /= a.col_tiles;
-  const int h = (int)(id % a.Hkv);
-  id /= a.Hkv;
-  const int part = (int)(id % a.parts);
-  const int b = (int)(id / a.parts);
+  const int ct = id % (uint32_t)a.col_tiles;
+  id /= (uint32_t)a.col_tiles;
+  const int h = id % (uint32_t)a.Hkv;
+  id /= (uint32_t)a.Hkv;
+  const int part = id % (uint32_t)a.parts;
+  const int b = id / (uint32_t)a.parts;
   const int cols = kBlockCols * waves;
   const int n = length_of(a, b), p0 = start_of(a, b, n);
   const Range r = tile_range(a, n, p0, ct * cols, cols);
@@ -478,7 +481,6 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   const int last = min(r.end, first + a.part_keys);
   if (part > 0 && first >= r.end) return;
   const int c0 = ct * cols + kBlockCols * wave;   // this wave's columns
-  const Range w = tile_range(a, n, p0, min(c0, a.M), kBlockCols);
 
   // ---- this lane's columns
   bool padding[NT];
@@ -504,59 +506,66 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   }
   if (tid == 0) *flag = 0;
 
-  // ---- the stream.  A tile is eight pieces of sixteen rows, K's four and V's
-  // four, each inside one page; wave w brings pieces w, w + waves, ...  A DMA
-  // instruction fills ROWS rows (1 KB): lane (row lane / UNITS, unit lane % UNITS)
-  // fetches the unit that the swizzle puts there.
+  // ---- the stream.  A tile is four pieces of sixteen rows of K and of V, each inside one
+  // page.  Waves 0 to 3 bring one each: waves 4 .., which are behind them, have no time to.  A
+  // DMA instruction fills ROWS rows (1 KB): lane (row lane / UNITS, unit
+  // lane % UNITS) fetches the unit that the swizzle puts there.
   const scalar_ints table = scalars(a.table + b * a.table_stride);
   const int page_mask = (1 << a.page_shift) - 1;
   constexpr int DMAS = 16 / ROWS;
-  uint32_t k_lane[DMAS], v_lane[DMAS], own_lane[DMAS];  // byte offsets (a piece spans < 2^31 bytes)
+  const int quarter = wave & 3;
+  const bool late = wave >= 4;
+  uint32_t k_lane[DMAS], v_lane[DMAS];   // byte offsets (a piece spans < 2^31 bytes)
 #pragma unroll
   for (int i = 0; i < DMAS; ++i) {
     const int row = i * ROWS + lane / UNITS;
     k_lane[i] = 2u * (uint32_t)row * (uint32_t)a.k_sr + 16u * ((lane % UNITS) ^ swizzle_k<D>(row));
     v_lane[i] = 2u * (uint32_t)row * (uint32_t)a.v_sr + 16u * ((lane % UNITS) ^ swizzle<D>(row));
-    own_lane[i] = wave < 4 ? k_lane[i] : v_lane[i];
   }
   const uint8_t* const k_pool = (const uint8_t*)(a.k + h * a.k_sh);
   const uint8_t* const v_pool = (const uint8_t*)(a.v + h * a.v_sh);
+  const int64_t k_page_bytes = 2 * a.k_sp, k_row_bytes = 2 * a.k_sr;
+  const int64_t v_page_bytes = 2 * a.v_sp, v_row_bytes = 2 * a.v_sr;
+  const uint32_t lds0 = lds_addr(ring);
+  const uint32_t k_to = lds0 + quarter * 16 * ROWB, v_to = lds0 + TILEB + quarter * 16 * ROWB;
   auto is_live = [&](int page) { return (uint32_t)page < (uint32_t)a.num_pages; };
-  struct Piece {
-    uint32_t to;
-    const uint8_t* src;
+  // The wave's rows in the tile at `base`: K's and V's addresses, of page `page`.
+  struct Source {
+    const uint8_t *k, *v;
   };
-  auto piece = [&](int x, int slot, int base, int page) {
-    const int64_t at = is_live(page) ? page : 0;   // a page that exists; its values are not used
-    const int64_t row = (base + 16 * (x & 3)) & page_mask;
-    const uint8_t* src = x < 4 ? k_pool + 2 * (at * a.k_sp + row * a.k_sr)
-                               : v_pool + 2 * (at * a.v_sp + row * a.v_sr);
-    return Piece{
-        (uint32_t)__builtin_amdgcn_readfirstlane(lds_addr(ring) + slot * SLOTB + x * 16 * ROWB),
-        (const uint8_t*)uniform_u64((uint64_t)src)};
+  auto source = [&](int base, int page) {
+    const uint32_t at = is_live(page) ? page : 0;  // a page that exists; its values are not used
+    const uint32_t row = (base + 16 * quarter) & page_mask;
+    return Source{k_pool + (at * k_page_bytes + row * k_row_bytes),
+                  v_pool + (at * v_page_bytes + row * v_row_bytes)};
   };
-  auto page_for = [&](int base, int x) { return page_at(a, table, base + 16 * (x & 3)); };
-  // The wave's pieces from its second on.
-  auto issue_others = [&](int slot, int base) {
-    for (int x = wave + waves; x < 8; x += waves) {
-      const Piece d = piece(x, slot, base, page_for(base, x));
+  auto bring = [&](const Source& s, uint32_t slot_off) {
 #pragma unroll
-      for (int i = 0; i < DMAS; ++i) dma_kb(d.to + 1024 * i, d.src, x < 4 ? k_lane[i] : v_lane[i]);
+    for (int i = 0; i < DMAS; ++i) {
+      dma_kb(k_to + slot_off + 1024 * i, s.k, k_lane[i]);
+      dma_kb(v_to + slot_off + 1024 * i, s.v, v_lane[i]);
     }
   };
-  bool holes = false;  // an entry of this piece of the table is unmapped: then every tile looks
-  auto live_at = [&](int base, int i) { return !holes || is_live(page_at(a, table, base + 16 * i)); };
-  const int tiles = first < last ? (last - first + kBlockKeys - 1) / kBlockKeys : 0;
-  auto issue = [&](int slot, int base, int page) {
-    const Piece d = piece(wave, slot, base, page);
-#pragma unroll
-    for (int i = 0; i < DMAS; ++i) dma_kb(d.to + 1024 * i, d.src, own_lane[i]);
-    issue_others(slot, base);
+  // The table entry of the wave's rows, read a tile ahead.  (A vector load: a scalar one in
+  // flight would turn every wait for LDS into a wait for all of it.)
+  const int32_t* const entries = a.table + b * a.table_stride;
+  auto entry_for = [&](int base) {
+    return entries[max(0, min((base + 16 * quarter) >> a.page_shift, a.table_width - 1))];
   };
-  if (tiles > 0) issue(0, first, page_for(first, wave));
-  int next = tiles > 0 ? page_for(first + kBlockKeys, wave) : -1;
+  auto page_from = [&](int base, int32_t entry) {
+    return (base + 16 * quarter) >> a.page_shift < a.table_width
+               ? __builtin_amdgcn_readfirstlane(entry) : -1;
+  };
 
-  // (behind the first tile's DMA: the queries, and the look for holes)
+  const int tiles = first < last ? (last - first + kBlockKeys - 1) / kBlockKeys : 0;
+  int32_t entry = 0;
+  if (tiles > 0 && !late) {
+    bring(source(first, page_from(first, entry_for(first))), 0);
+    entry = entry_for(first + kBlockKeys);
+  }
+  // (behind the first tile's DMA: the queries, and whether an entry of this piece of the table
+  // is unmapped, in which case every tile looks)
+  bool holes = false;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int m = c0 + 16 * t + col;
@@ -569,7 +578,7 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
     }
   }
   for (int e = (first >> a.page_shift) + lane; e <= (last - 1) >> a.page_shift; e += 64)
-    holes |= !is_live(a.table[b * a.table_stride + e]);
+    holes |= !is_live(entries[e]);
   holes = __builtin_amdgcn_ballot_w64(holes) != 0;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -580,7 +589,6 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   // and the row tile are instruction offsets: no vector work between the products)
   uint32_t k_at[KS], v_at[DT];
   {
-    const uint32_t lds0 = lds_addr(ring);
     const int rt = 4 * grp + (col >> 2);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -595,163 +603,200 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
     for (int d = 0; d < DT; ++d) asm volatile("" : "+v"(v_at[d]));
   }
   const float scale = a.scale_log2;
+  const bool active = c0 < a.M;            // the wave has columns
 
-  auto tile = [&](int t, auto slot_c) {
-    constexpr int slot = decltype(slot_c)::value;
-    const int base = first + t * kBlockKeys;
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + 1 < tiles) issue(1 - slot, base + kBlockKeys, next);
-    const bool whole =
-        !holes || (live_at(base, 0) && live_at(base, 1) && live_at(base, 2) && live_at(base, 3));
-    bool dirty = false;
-    if (!whole || base < r.inner_lo || base + kBlockKeys > r.inner_hi) {
-      // V rows that no column sees become zeros; values that are not finite
-      // are taken out (a column that does not see them must not get 0 x inf)
-      // and added one by one below.
-      bool odd = false;
-      for (int x = tid; x < kBlockKeys * UNITS; x += 64 * waves) {
-        const int row = x / UNITS, key = base + row;
-        u32x4_t* at = reinterpret_cast<u32x4_t*>(ring + slot * SLOTB + TILEB + 16 * x);
-        bool lv = true;
-        if (holes) {
-          const int e = key >> a.page_shift;  // (a vector load: rows differ between lanes)
-          lv = e < a.table_width && is_live(a.table[b * a.table_stride + e]);
-        }
-        if (!lv || key < r.lo || key >= r.end) {
-          *at = u32x4_t{0, 0, 0, 0};
-          continue;
-        }
-        u32x4_t v = *at;
-        bool bad = false;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool b0 = (v[e] & T::kExp) == T::kExp, b1 = ((v[e] >> 16) & T::kExp) == T::kExp;
-          bad |= b0 || b1;
-          if (b0) v[e] &= 0xffff0000u;
-          if (b1) v[e] &= 0x0000ffffu;
-        }
-        if (bad) *at = v;
-        odd |= bad;
-      }
-      if (odd) *flag = t + 1;
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      dirty = *(volatile int*)flag == t + 1;
-    }
-    asm volatile("" ::: "memory");
-    // ---- scores
-    constexpr int AHEAD = 4;                 // operands in flight
-    f32x4_t S[NT][4];
+  // The pieces of one tile's work; `off`: the slot's offset.
+  constexpr int AHEAD = 4;                 // operands in flight
+  f32x4_t S[NT][4];
+  u32x4_t Pb[NT][2];
+  auto scores = [&](uint32_t off) {
 #pragma unroll
     for (int c = 0; c < NT; ++c)
 #pragma unroll
       for (int m = 0; m < 4; ++m) S[c][m] = zero4();
-    {
-      u32x4_t x[4 * KS];
-      auto operand = [&](int o) {  // keys 16 (o & 3) .., dims 32 (o >> 2) ..
-        return lds_read16(k_at[o >> 2] + (uint32_t)(slot * SLOTB + 16 * ROWB * (o & 3)));
-      };
+    u32x4_t x[4 * KS];
+    auto operand = [&](int o) {  // keys 16 (o & 3) .., dims 32 (o >> 2) ..
+      return lds_read16(k_at[o >> 2] + (off + 16 * ROWB * (o & 3)));
+    };
 #pragma unroll
-      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
+    for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int o = 0; o < 4 * KS; ++o) {
+#pragma unroll
+      for (int c = 0; c < NT; ++c) S[c][o & 3] = T::mfma(x[o], Q[c][o >> 2], S[c][o & 3]);
+      if (o + AHEAD < 4 * KS) x[o + AHEAD] = operand(o + AHEAD);
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int o = 0; o < 4 * KS; ++o) {
-#pragma unroll
-        for (int c = 0; c < NT; ++c) S[c][o & 3] = T::mfma(x[o], Q[c][o >> 2], S[c][o & 3]);
-        if (o + AHEAD < 4 * KS) x[o + AHEAD] = operand(o + AHEAD);
-        __builtin_amdgcn_sched_barrier(0);
-      }
     }
+  };
+  auto softmax = [&](int c) {
+    const float top = across4_max(max16_raw(S[c])) * scale;
+    if (__builtin_amdgcn_ballot_w64(top > mx[c] + kSlack) != 0) {
+      const float to = __builtin_fmaxf(mx[c], top);
+      const float f = to == neg_inf() ? 1.f : exp2_hw(mx[c] - to);
+      mx[c] = to;
+      sum[c] *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) O[c][d] *= f;
+    }
+    const float off = mx[c] == neg_inf() ? 0.f : mx[c];
+    float part_sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float p = exp2_hw(__builtin_fmaf(S[c][i >> 2][i & 3], scale, -off));
+      S[c][i >> 2][i & 3] = p;
+      part_sum[i & 3] += p;
+    }
+    sum[c] += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      Pb[c][k] = u32x4_t{T::pack(S[c][2 * k][0], S[c][2 * k][1]), T::pack(S[c][2 * k][2], S[c][2 * k][3]),
+                         T::pack(S[c][2 * k + 1][0], S[c][2 * k + 1][1]),
+                         T::pack(S[c][2 * k + 1][2], S[c][2 * k + 1][3])};
+  };
+  auto outputs = [&](uint32_t off) {
+    u32x4_t x[2 * DT];
+    auto operand = [&](int o) {  // dims 16 (o >> 1) .., keys 32 (o & 1) ..
+      const uint32_t ad = v_at[o >> 1] + (off + 32 * ROWB * (o & 1));
+      const u32x2_t y0 = read_transposed(ad), y1 = read_transposed(ad + 16u * ROWB);
+      return u32x4_t{y0[0], y0[1], y1[0], y1[1]};
+    };
+#pragma unroll
+    for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int o = 0; o < 2 * DT; ++o) {
+#pragma unroll
+      for (int c = 0; c < NT; ++c) O[c][o >> 1] = T::mfma(x[o], Pb[c][o & 1], O[c][o >> 1]);
+      if (o + AHEAD < 2 * DT) x[o + AHEAD] = operand(o + AHEAD);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // The ring: the slot of the current tile, and of the one whose rows are on their way.
+  uint32_t now = 0;
+  auto behind = [&](uint32_t off) { return off + SLOTB == ring_bytes ? 0 : off + SLOTB; };
+  auto before = [&](uint32_t off) { return off == 0 ? ring_bytes - SLOTB : off - SLOTB; };
+
+  // Any tile: masks, rows nobody sees, unmapped pages, the last.
+  auto live_at = [&](int base, int i) { return !holes || is_live(page_at(a, table, base + 16 * i)); };
+  auto edge_tile = [&](int t) {
+    const uint32_t off = now;
+    const int base = first + t * kBlockKeys;
+    now = behind(now);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 1 < tiles && !late) {
+      bring(source(base + kBlockKeys, page_from(base + kBlockKeys, entry)), now);
+      entry = entry_for(base + 2 * kBlockKeys);
+    }
+    // V rows that no column sees become zeros; values that are not finite
+    // are taken out (a column that does not see them must not get 0 x inf) and
+    // added one by one below.
+    bool odd = false;
+    for (int x = tid; x < kBlockKeys * UNITS; x += 64 * waves) {
+      const int key = base + x / UNITS;
+      u32x4_t* at = reinterpret_cast<u32x4_t*>(ring + off + TILEB + 16 * x);
+      bool lv = true;
+      if (holes) {
+        const int e = key >> a.page_shift;  // (a vector load: rows differ between lanes)
+        lv = e < a.table_width && is_live(entries[e]);
+      }
+      if (!lv || key < r.lo || key >= r.end) {
+        *at = u32x4_t{0, 0, 0, 0};
+        continue;
+      }
+      u32x4_t v = *at;
+      bool bad = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool b0 = (v[e] & T::kExp) == T::kExp, b1 = ((v[e] >> 16) & T::kExp) == T::kExp;
+        bad |= b0 || b1;
+        if (b0) v[e] &= 0xffff0000u;
+        if (b1) v[e] &= 0x0000ffffu;
+      }
+      if (bad) *at = v;
+      odd |= bad;
+    }
+    if (odd) *flag = t + 1;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const bool dirty = *(volatile int*)flag == t + 1;
+    if (!active) return;
+    scores(off);
+    const bool live[4] = {live_at(base, 0), live_at(base, 1), live_at(base, 2), live_at(base, 3)};
     uint32_t seen[NT];
-    if (!whole || base < w.inner_lo || base + kBlockKeys > w.inner_hi) {
-      const bool live[4] = {live_at(base, 0), live_at(base, 1), live_at(base, 2), live_at(base, 3)};
-#pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        seen[c] = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = base + 16 * (i >> 2) + 4 * grp + (i & 3);
-          const bool ok = live[i >> 2] && key >= lo[c] && key < hi[c];
-          if (ok) seen[c] |= 1u << i;
-          S[c][i >> 2][i & 3] = ok ? S[c][i >> 2][i & 3] : neg_inf();
-        }
-      }
-      asm volatile("");  // (a branch, not selects in every tile)
-    } else {
-#pragma unroll
-      for (int c = 0; c < NT; ++c) seen[c] = 0xffffu;
-    }
-    u32x4_t Pb[NT][2];
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
-      const float top = across4_max(max16_raw(S[c])) * scale;
-      if (__builtin_amdgcn_ballot_w64(top > mx[c] + kSlack) != 0) {
-        const float to = __builtin_fmaxf(mx[c], top);
-        const float f = to == neg_inf() ? 1.f : exp2_hw(mx[c] - to);
-        mx[c] = to;
-        sum[c] *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) O[c][d] *= f;
-      }
-      const float off = mx[c] == neg_inf() ? 0.f : mx[c];
-      float part_sum[4] = {0.f, 0.f, 0.f, 0.f};
+      seen[c] = 0;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float p = exp2_hw(__builtin_fmaf(S[c][i >> 2][i & 3], scale, -off));
-        S[c][i >> 2][i & 3] = p;
-        part_sum[i & 3] += p;
+        const int key = base + 16 * (i >> 2) + 4 * grp + (i & 3);
+        const bool ok = live[i >> 2] && key >= lo[c] && key < hi[c];
+        if (ok) seen[c] |= 1u << i;
+        S[c][i >> 2][i & 3] = ok ? S[c][i >> 2][i & 3] : neg_inf();
       }
-      sum[c] += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        Pb[c][k] = u32x4_t{T::pack(S[c][2 * k][0], S[c][2 * k][1]), T::pack(S[c][2 * k][2], S[c][2 * k][3]),
-                           T::pack(S[c][2 * k + 1][0], S[c][2 * k + 1][1]),
-                           T::pack(S[c][2 * k + 1][2], S[c][2 * k + 1][3])};
+      softmax(c);
     }
-    // ---- V^T . P^T
-    {
-      u32x4_t x[2 * DT];
-      auto operand = [&](int o) {  // dims 16 (o >> 1) .., keys 32 (o & 1) ..
-        const uint32_t ad = v_at[o >> 1] + (uint32_t)(slot * SLOTB + 32 * ROWB * (o & 1));
-        const u32x2_t y0 = read_transposed(ad), y1 = read_transposed(ad + 16u * ROWB);
-        return u32x4_t{y0[0], y0[1], y1[0], y1[1]};
-      };
+    outputs(off);
+    if (!dirty) return;
+    for (int kk = 0; kk < kBlockKeys; ++kk) {
+      const int key = base + kk;
+      if (!live_at(base, kk >> 4) || key < r.lo || key >= r.end) continue;
+      const int from = 16 * ((kk & 15) >> 2) + col, slot_i = 4 * (kk >> 4) + (kk & 3);
+      const uint16_t* vp = a.v + h * a.v_sh + page_at(a, table, key) * a.v_sp +
+                           (int64_t)(key & page_mask) * a.v_sr;
 #pragma unroll
-      for (int o = 0; o < AHEAD; ++o) x[o] = operand(o);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int c = 0; c < NT; ++c) {
+        const bool ok = (__shfl(seen[c], from, 64) >> slot_i) & 1;
 #pragma unroll
-      for (int o = 0; o < 2 * DT; ++o) {
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int c = 0; c < NT; ++c) O[c][o >> 1] = T::mfma(x[o], Pb[c][o & 1], O[c][o >> 1]);
-        if (o + AHEAD < 2 * DT) x[o + AHEAD] = operand(o + AHEAD);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    // (a scalar load in flight would turn every wait for LDS into a wait for all of it)
-    next = page_for(base + 2 * kBlockKeys, wave);
-    if (dirty) {
-      for (int kk = 0; kk < kBlockKeys; ++kk) {
-        const int key = base + kk;
-        if (!live_at(base, kk >> 4) || key < r.lo || key >= r.end) continue;
-        const int from = 16 * ((kk & 15) >> 2) + col, slot_i = 4 * (kk >> 4) + (kk & 3);
-        const uint16_t* vp = a.v + h * a.v_sh + page_at(a, table, key) * a.v_sp +
-                             (int64_t)(key & page_mask) * a.v_sr;
-#pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          const bool ok = (__shfl(seen[c], from, 64) >> slot_i) & 1;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t x = vp[16 * d + 4 * grp + e];
-              if (ok && (x & T::kExp) == T::kExp) O[c][d][e] += T::value(x);
-            }
-        }
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = vp[16 * d + 4 * grp + e];
+            if (ok && (x & T::kExp) == T::kExp) O[c][d][e] += T::value(x);
+          }
       }
     }
   };
-  for (int t = 0; t < tiles; t += 2) {
-    tile(t, std::integral_constant<int, 0>{});
-    if (t + 1 < tiles) tile(t + 1, std::integral_constant<int, 1>{});
+  // Edge tiles, then the plain ones (every column sees all of the tile), then edge
+  // tiles: two passes of a loop, so that the edge code is there once.
+  // Waves 4 .. share their SIMDs with waves 0 .. and go half a tile behind them: their
+  // softmax runs while the others' products do.
+  int plain = 0, plain_end = 0;
+  if (!holes && tiles > 0) {
+    plain = max(0, r.inner_lo - first + kBlockKeys - 1) / kBlockKeys;
+    plain_end = max(0, min(last, r.inner_hi) - first) / kBlockKeys;
+  }
+  auto arrive = [&](int t) {  // tile t is there, and its successor, if any, on its way
+    const int base = first + t * kBlockKeys;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    now = behind(now);
+    if (late || t + 1 >= tiles) return;
+    bring(source(base + kBlockKeys, page_from(base + kBlockKeys, entry)), now);
+    entry = entry_for(base + 2 * kBlockKeys);
+  };
+  int t = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (const int to = pass == 0 && plain < plain_end ? plain : tiles; t < to; ++t) edge_tile(t);
+    if (t >= plain_end) continue;
+    uint32_t off = now;
+    arrive(t);
+    for (;; off = behind(off)) {
+      const bool more = t + 1 < plain_end;
+      if (active) scores(off);
+      if (late && more) arrive(t + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (active) {
+        __builtin_amdgcn_s_setprio(1);  // vector work first: the matrix unit is fed a tile at a time
+        softmax(0);
+        softmax(1);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        outputs(off);
+      }
+      ++t;
+      if (!more) break;
+      if (!late) arrive(t);
+    }
   }
 
   // ---- out: lane (col, grp) holds dims 16 d + 4 grp .. of its columns
@@ -794,21 +839,20 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
 // Joining: WAVES waves per column; each reads all of the column's maxima and sums,
 // and the outputs of every WAVES-th part, eight rows in flight.
 template <class T, int D, int WAVES>
-__global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) paged_join_kernel(PagedArgs a) {
-  constexpr int THREADS = WAVES > 4 ? 64 * WAVES : 256;
-  constexpr int COLS = THREADS / 64 / WAVES;    // columns of a workgroup
+__global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a) {
+  constexpr int COLS = 4 / WAVES;               // columns of a workgroup
   constexpr int VALUES = D / 64;                // dims of a lane
   typedef float vec_t __attribute__((ext_vector_type(VALUES)));
-  __shared__ vec_t acc_l[THREADS];
+  __shared__ vec_t acc_l[256];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t columns = (int64_t)a.B * a.Hkv * a.M;
-  const int64_t c_raw = (int64_t)blockIdx.x * COLS + wave / WAVES;   // (b Hkv + h) M + m
+  const uint32_t columns = (uint32_t)a.B * a.Hkv * a.M;       // (at most 2^31 - 1)
+  const uint32_t c_raw = blockIdx.x * COLS + wave / WAVES;    // (b Hkv + h) M + m
   const bool there = c_raw < columns;
   const int64_t c = there ? c_raw : columns - 1;
-  const int m = (int)(c % a.M);
-  const int64_t bh = c / a.M;
-  const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv);
+  const uint32_t bh = (uint32_t)c / (uint32_t)a.M;
+  const int m = (uint32_t)c - bh * a.M;
+  const int b = bh / (uint32_t)a.Hkv, h = bh % (uint32_t)a.Hkv;
   const int n = length_of(a, b);
   const Range r = tile_range(a, n, start_of(a, b, n), m / a.tile_cols * a.tile_cols, a.tile_cols);
   const int np = max(1, (r.end - r.start + a.part_keys - 1) / a.part_keys);
@@ -861,20 +905,22 @@ __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) paged_join_kerne
 }
 
 // Columns of a workgroup: up to 16 the streaming kernel; more, whole waves of the
-// block kernel, as even as they come.
+// block kernel, four at least (each brings its share of the rows), as even as they come.
 int columns_of(int64_t M) {
   if (M <= 16) return 16;
   const int64_t groups = (M + kBlockCols - 1) / kBlockCols;
   const int64_t tiles = (groups + kBlockWaves - 1) / kBlockWaves;
-  return (int)((groups + tiles - 1) / tiles * kBlockCols);
+  return (int)std::max<int64_t>(4, (groups + tiles - 1) / tiles) * kBlockCols;
 }
 
-// Most keys that the columns of one workgroup can see.
+// Most keys that the columns of one workgroup can see.  (Rows at the end of their
+// sequence have at most the other rows behind them.)
 int64_t span_bound(int64_t max_len, int64_t q_len, int64_t group, int64_t cols, int64_t window,
-                   int causal) {
+                   int causal, bool at_end) {
   if (window < 0) return max_len;
   const int64_t rows = std::min<int64_t>(q_len, cols / group + 2);
-  return std::min(max_len, rows + (causal ? 1 : 2) * window + 1);
+  const int64_t right = causal ? 0 : at_end ? std::min(window, q_len) : window;
+  return std::min(max_len, rows + window + right + 1);
 }
 
 template <class T, int D>
@@ -890,20 +936,21 @@ int launch(const PagedArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves), lds,
                        stream, a);
   } else {
-    const size_t lds = 4 * kBlockKeys * 2 * D + 16;
+    const size_t slot = 2 * kBlockKeys * 2 * D;
+    const size_t lds = block_slots(a.tile_cols / kBlockCols) * slot + 16;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_block_kernel<T, D>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+                            hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (int)(3 * slot + 16)) != hipSuccess)
       return MRSA_ERR_LAUNCH;
     hipLaunchKernelGGL((paged_block_kernel<T, D>), dim3((unsigned)grid),
                        dim3(64 * a.tile_cols / kBlockCols), lds, stream, a);
   }
   int st = mrsa_launch_status();
   if (st != MRSA_OK || a.parts == 1) return st;
-  // As many waves per column as its parts fill with eight rows each, unless there are columns
-  // enough to fill the machine.
-  if (a.parts > 32 && cols <= 1024)
-    hipLaunchKernelGGL((paged_join_kernel<T, D, 16>), dim3((unsigned)cols), dim3(1024), 0, stream, a);
-  else if (a.parts > 8 && cols <= 4096)
+  // Four waves per column where there are many parts and few columns (896 columns of 64 parts:
+  // 7.7 us, 9.2 by one wave; 28 of 256: 5.4 and 8.1), otherwise one (1792 columns of 6:
+  // 5.0 us, 7.4 by four; 7168 of 11: 7.8 and 19.7).
+  if (a.parts > 8 && cols <= 4096)
     hipLaunchKernelGGL((paged_join_kernel<T, D, 4>), dim3((unsigned)cols), dim3(256), 0, stream, a);
   else
     hipLaunchKernelGGL((paged_join_kernel<T, D, 1>), dim3((unsigned)((cols + 3) / 4)), dim3(256), 0,
@@ -987,7 +1034,8 @@ extern "C" int mrsa_paged_attention_fwd(
   a.tile_cols = columns_of(a.M);
   a.col_tiles = (a.M + a.tile_cols - 1) / a.tile_cols;
   const int64_t span =
-      span_bound(max_len, q_len, a.G, a.tile_cols, a.window, a.causal) + kTile - 1;
+      span_bound(max_len, q_len, a.G, a.tile_cols, a.window, a.causal, !query_starts) +
+      kTile - 1;
   const int64_t step = a.tile_cols == 16 ? kStep : kBlockKeys;
   a.part_keys = (int)(((span + parts - 1) / parts + step - 1) / step * step);
   a.out = (uint16_t*)out;

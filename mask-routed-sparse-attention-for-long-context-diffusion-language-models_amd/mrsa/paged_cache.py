@@ -270,8 +270,8 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if parts is None:
         span = max_len
         if window >= 0:
-            span = min(span, Lq, 256) + (1 if causal else 2) * window
-            span = min(span, max_len)
+            right = 0 if causal else window if query_starts is not None else min(window, Lq)
+            span = min(max_len, min(Lq, 256) + window + right)
         parts = cache_parts(B, Lq, Hq, Hkv, span)
     return torch.ops.mrsa.paged_attention.default(q, k_pages, v_pages, page_table, cache_lens,
                                                   query_starts, max_len, bool(causal), window,
