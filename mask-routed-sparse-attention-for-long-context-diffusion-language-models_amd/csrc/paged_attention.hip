@@ -927,7 +927,10 @@ template <class T, int D>
 int launch(const PagedArgs& a, hipStream_t stream) {
   const int64_t grid = (int64_t)a.B * a.Hkv * a.col_tiles * a.parts;
   const int64_t cols = (int64_t)a.B * a.Hkv * a.M;
-  if (grid > 0x7fffffff || cols > 0x7fffffff) return MRSA_ERR_UNSUPPORTED;
+  const int64_t threads = a.tile_cols == 16 ? 64 * kWaves : 64 * a.tile_cols / kBlockCols;
+  // (a launch holds fewer than 2^32 threads; the join has at most 64 a column)
+  if (grid > 0xffffffffll / threads || (a.parts > 1 && cols > (1 << 26) - 4) || cols > 0x7fffffff)
+    return MRSA_ERR_UNSUPPORTED;
   if (a.tile_cols == 16) {
     const size_t lds = kWaves * std::max(kTile * 2 * D, 16 * (D + 4) * 4);
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, D>),
@@ -985,7 +988,7 @@ extern "C" int mrsa_paged_attention_fwd(
       max_len < 0 || table_pages < 0 || num_pages < 0 || page_size <= 0 || parts < 1 ||
       parts > kMaxParts)
     return MRSA_ERR_INVALID_ARGUMENT;
-  if (!(sm_scale > 0.f) || !(sm_scale < __builtin_inff())) return MRSA_ERR_INVALID_ARGUMENT;
+  if (!(sm_scale > 0.f) || !(sm_scale * kLog2e < __builtin_inff())) return MRSA_ERR_INVALID_ARGUMENT;
   if (dtype != MRSA_DTYPE_BF16 && dtype != MRSA_DTYPE_FP16) return MRSA_ERR_UNSUPPORTED;
   if (head_dim != 64 && head_dim != 128) return MRSA_ERR_UNSUPPORTED;
   if ((page_size & (page_size - 1)) != 0 || page_size < 16 || page_size > (1 << 20))

@@ -331,7 +331,8 @@ int launch(RotaryArgs a, bool interleaved, hipStream_t stream) {
       if (whole >= kThreads && idle < waste) waste = idle, a.tokens_per_block = t, threads = whole;
     }
   }
-  const unsigned blocks = (unsigned)((a.tokens + a.tokens_per_block - 1) / a.tokens_per_block);
+  const int64_t blocks = ((int64_t)a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
+  if (blocks > 0xffffffffll / threads) return MRSA_ERR_UNSUPPORTED;  // (threads of a launch)
   void (*kern)(RotaryArgs);
   if (!vec)
     kern = interleaved ? rotary_scalar_kernel<T, true, PAGED> : rotary_scalar_kernel<T, false, PAGED>;
@@ -340,7 +341,7 @@ int launch(RotaryArgs a, bool interleaved, hipStream_t stream) {
   else
     kern = interleaved ? rotary_kernel<T, true, PAGED, kHeadsPerThread>
                        : rotary_kernel<T, false, PAGED, kHeadsPerThread>;
-  hipLaunchKernelGGL(kern, dim3(blocks), dim3(threads), 0, stream, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(threads), 0, stream, a);
   return mrsa_launch_status();
 }
 

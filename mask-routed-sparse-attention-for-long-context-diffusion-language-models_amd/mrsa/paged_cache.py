@@ -117,7 +117,7 @@ def paged_cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     row of its sequence that each new row becomes.  A negative slot (a padded token),
     one past the table and one whose page is outside the pool are skipped.  Two rows
     of a call must not name the same cache row, as one of them would be left (also
-    through a page that two sequences share).
+    through a page that two sequences share), and q, k and v must not lie in the pages.
     With cos, sin (``rotary_tables``) k rows are turned as by ``rotary_qk`` at
     ``positions`` (torch.long [B, L] or [L]; None: the slots), the same bits; q
     [B, L, Hq, D], if given, is turned too, skipped rows as well, and returned (without

@@ -109,6 +109,32 @@ def test_attention_matches_the_oracle(shape, dtype):
         _check(_run(*args, window=40, parts=parts, max_len=max(lens)), *args, window=40)
 
 
+# Columns of two to ten waves, over tiles that fill the ring more than once: rows of one KV
+# head, whole tiles and one key more or less.
+@pytest.mark.parametrize("Lq", [17, 40, 128, 129, 160, 225, 256, 257, 300])
+@pytest.mark.parametrize("D", [64, 128])
+def test_blocks_over_many_tiles(Lq, D):
+    for lens, page in (([64, 65], 64), ([191, 0, 192], 16), ([321, 449], 32), ([1000, 703], 128)):
+        args = _case(len(lens), Lq, lens, 2, 2, D, page, torch.bfloat16, seed=Lq + D)
+        starts = torch.tensor([n // 2 for n in lens], dtype=torch.int32)
+        for kw in (dict(parts=1), dict(parts=2, causal=True), dict(window=200, parts=1),
+                   dict(query_starts=starts, window=130, parts=3),
+                   dict(query_starts=starts, causal=True)):
+            _check(_run(*args, **kw), *args, **kw)
+
+
+def test_holes_and_values_not_finite_among_many_tiles():
+    args = _case(1, 200, [900], 2, 1, 128, 32, torch.bfloat16, seed=3, unmap=[(0, 9, -1), (0, 20, 3)])
+    for kw in (dict(parts=1), dict(parts=2, causal=True)):
+        _check(_run(*args, **kw), *args, **kw)
+    q, k, v, table, lens = _case(1, 200, [900], 2, 1, 128, 32, torch.bfloat16, seed=4)
+    v[P.place(table, 0, 850, 32, k.shape[0])] = float("inf")
+    out, lse = (t.cpu() for t in _run(q, k, v, table, lens, causal=True))
+    want, wlse, _, _ = P.attention(q, k, v, table, lens, causal=True)
+    assert torch.equal(torch.isposinf(out), torch.isposinf(want)) and not torch.isnan(out).any()
+    assert bool(torch.isposinf(out[0, 150:]).all()) and bool(torch.isfinite(out[0, :150]).all())
+
+
 @pytest.mark.parametrize("window", [0, 1, 5, 31, 64, 100000])
 @pytest.mark.parametrize("causal", [False, True])
 def test_windows_and_blocks_inside_a_sequence(window, causal):

@@ -388,3 +388,15 @@ def test_c_rotary_and_append_refusals():
                    dict(L=-1), dict(R=3), dict(width=-1)):
         assert append(**change) == _lib.MRSA_ERR_INVALID_ARGUMENT, change
     assert append(P=24) == _lib.MRSA_ERR_UNSUPPORTED
+
+
+def test_c_refusals_of_sizes_past_a_launch():
+    # strides of rows that the DMA's 32-bit offsets do not span, scales that leave fp32
+    assert _c_attend(sr=1 << 26) == _lib.MRSA_ERR_UNSUPPORTED
+    assert _c_attend(scale=3e38) == _lib.MRSA_ERR_INVALID_ARGUMENT
+    # more threads than a launch holds
+    for B in (1 << 26, 1 << 30):
+        assert _c_attend(B=B) == _lib.MRSA_ERR_UNSUPPORTED
+    big = 1 << 24
+    assert _lib.call("mrsa_rotary_fwd", 4096, 512, 512, 33, None, 0, 0, 0, 4096, 4096, 4, None, 0,
+                     0, big, 1, 64, 0, 33, 32, 0, 0, 0, 8192, None, None) == _lib.MRSA_ERR_UNSUPPORTED
