@@ -159,25 +159,46 @@ def paged_cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
 
 
 @functools.lru_cache(maxsize=4096)
-def cache_parts(batch: int, q_len: int, q_heads: int, kv_heads: int, span: int) -> int:
+def cache_parts(batch: int, q_len: int, q_heads: int, kv_heads: int, span: int, live: int) -> int:
     """Pieces that paged_cached_attention cuts the visible span into: of those that make
-    whole rounds of workgroups over the 256 CUs, the one with the least work for a CU.  A
-    piece costs its keys, about 128 more to start (streaming kernel, up to 16 columns
-    of rows and heads per KV head), the uneven ends of sequences of different lengths,
-    and its part in the join."""
+    whole rounds of workgroups over the 256 CUs, the one with the least work for a CU.
+    ``live``: the keys of the span that there are if the rows stand at their sequence's end.
+
+    Up to 16 columns (rows and heads of a KV head; streaming kernel) a piece costs its
+    keys, about 128 more to start, the uneven ends of sequences of different lengths, and
+    its part in the join.  More columns (block kernel; in keys of 28 ns): a round costs 230
+    to start and its keys, the join 140 and its bytes, 1 KB a column and piece, written and
+    read.  64 sequences of 32 rows of 2048 keys: 1 piece 91 us, 3 147; 8 of 4096: 8 pieces
+    43 us, 24 66; 1 of 8192: 48 pieces 29 us, 8 47."""
 
     cols = q_len * (q_heads // kv_heads)
-    stream = cols <= 16
-    units = batch * kv_heads * (1 if stream else -(-cols // 256))
-    if units == 0 or span <= 0:
+    if cols == 0 or batch == 0 or span <= 0:
         return 1
-    step, start = (128, 128) if stream else (64, 0)
-    most = min(MAX_PARTS, -(-(span + 31) // step))
     best, least = 1, None
-    for rounds in (1, 2, 3, 4, 6):
-        parts = max(1, min(most, 256 * rounds // units))
-        keys = -(-(span + 31) // (parts * step)) * step
-        cost = -(-units * parts // 256) * (keys + start) + keys // 4 + 4 * parts
+    if cols <= 16:
+        units = batch * kv_heads
+        most = min(MAX_PARTS, -(-(span + 31) // 128))
+        for rounds in (1, 2, 3, 4, 6):
+            parts = max(1, min(most, 256 * rounds // units))
+            keys = -(-(span + 31) // (parts * 128)) * 128
+            cost = -(-units * parts // 256) * (keys + 128) + keys // 4 + 4 * parts
+            if least is None or cost < least:
+                best, least = parts, cost
+        return best
+    groups = -(-cols // 32)
+    tiles = -(-groups // 8)
+    units = batch * kv_heads * tiles
+    slots = 256 if -(-groups // tiles) > 4 else 512   # workgroups at a time
+    most = min(MAX_PARTS, -(-(span + 31) // 64))
+    for quarters in (0, 2, 3, 4, 8, 12, 16, 24):
+        parts = max(1, min(most, slots * quarters * span // (4 * units * live)))
+        keys = -(-(span + 31) // (parts * 64)) * 64
+        there = min(parts, -(-(live + 31) // keys))
+        cost = -(-units * there // slots) * (230 + keys)
+        if slots == 512 and units * there > 256:   # two on a CU slow each other
+            cost = cost * 13 // 10
+        if parts > 1:
+            cost += 140 + batch * kv_heads * cols * there // 120
         if least is None or cost < least:
             best, least = parts, cost
     return best
@@ -195,6 +216,13 @@ def _paged_attention_impl(q, k_pages, v_pages, page_table, cache_lens, query_sta
     kps, kss, khs, _ = k_pages.stride()
     vps, vss, vhs, _ = v_pages.stride()
     pages, page_size, Hkv, _ = k_pages.shape
+    if parts == 0:  # (here, not in the caller, which a compiler traces)
+        span = live = max_len
+        if window >= 0:
+            right = 0 if causal else window if query_starts is not None else min(window, Lq)
+            span = min(max_len, min(Lq, 256) + window + right)
+            live = min(span, min(Lq, 256) + window)
+        parts = cache_parts(B, Lq, Hq, Hkv, span, live)
     out = q.new_empty(shape)
     lse = q.new_empty((B, Lq, Hq), dtype=torch.float32)
     nbytes, wp = 0, None
@@ -267,15 +295,11 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if torch.is_grad_enabled():
         _no_gradient("paged_cached_attention", q, k_pages, v_pages)
     window = -1 if window is None else int(window)
-    if parts is None:
-        span = max_len
-        if window >= 0:
-            right = 0 if causal else window if query_starts is not None else min(window, Lq)
-            span = min(max_len, min(Lq, 256) + window + right)
-        parts = cache_parts(B, Lq, Hq, Hkv, span)
+    if parts is not None and not 1 <= parts <= MAX_PARTS:
+        raise ValueError(f"parts must be in [1, {MAX_PARTS}], got {parts}")
     return torch.ops.mrsa.paged_attention.default(q, k_pages, v_pages, page_table, cache_lens,
                                                   query_starts, max_len, bool(causal), window,
-                                                  float(sm_scale), int(parts))
+                                                  float(sm_scale), int(parts or 0))
 
 
 def _copy_pages_impl(k_pages, v_pages, src, dst):

@@ -400,3 +400,12 @@ def test_c_refusals_of_sizes_past_a_launch():
     big = 1 << 24
     assert _lib.call("mrsa_rotary_fwd", 4096, 512, 512, 33, None, 0, 0, 0, 4096, 4096, 4, None, 0,
                      0, big, 1, 64, 0, 33, 32, 0, 0, 0, 8192, None, None) == _lib.MRSA_ERR_UNSUPPORTED
+
+
+def test_parts_are_refused_outside_their_range():
+    with FakeTensorMode():
+        a = _paged_args()
+        for parts in (0, -1, 1025):
+            with pytest.raises(ValueError):
+                mrsa.paged_cached_attention(**a, parts=parts)
+        mrsa.paged_cached_attention(**a, parts=1024)
