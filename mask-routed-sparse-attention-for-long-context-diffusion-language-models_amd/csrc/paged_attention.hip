@@ -34,6 +34,7 @@ constexpr int kStep = kWaves * kTile;      // keys of a workgroup's round
 constexpr int kMaxParts = 1024;
 constexpr int kFar = 1 << 29;              // bound of positions and windows: their sums fit 32 bits
 constexpr float kSlack = 8.f;              // base-2 growth before the maximum moves
+constexpr float kMostSum = 1024.f;         // sum of sixteen weights before it moves (block kernel)
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
@@ -629,30 +630,48 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto softmax = [&](int c) {
-    const float top = across4_max(max16_raw(S[c])) * scale;
-    if (__builtin_amdgcn_ballot_w64(top > mx[c] + kSlack) != 0) {
-      const float to = __builtin_fmaxf(mx[c], top);
-      const float f = to == neg_inf() ? 1.f : exp2_hw(mx[c] - to);
-      mx[c] = to;
-      sum[c] *= f;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) O[c][d] *= f;
-    }
-    const float off = mx[c] == neg_inf() ? 0.f : mx[c];
+  // Weights of column tile c's scores over the maximum `off`, and their sum in this lane.
+  auto weigh = [&](int c, float off) {
     float part_sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float p = exp2_hw(__builtin_fmaf(S[c][i >> 2][i & 3], scale, -off));
-      S[c][i >> 2][i & 3] = p;
-      part_sum[i & 3] += p;
-    }
-    sum[c] += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+    for (int k = 0; k < 2; ++k) {
+      float w[8];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      Pb[c][k] = u32x4_t{T::pack(S[c][2 * k][0], S[c][2 * k][1]), T::pack(S[c][2 * k][2], S[c][2 * k][3]),
-                         T::pack(S[c][2 * k + 1][0], S[c][2 * k + 1][1]),
-                         T::pack(S[c][2 * k + 1][2], S[c][2 * k + 1][3])};
+      for (int i = 0; i < 8; ++i) {
+        w[i] = exp2_hw(__builtin_fmaf(S[c][2 * k + (i >> 2)][i & 3], scale, -off));
+        part_sum[i & 3] += w[i];
+      }
+      Pb[c][k] = u32x4_t{T::pack(w[0], w[1]), T::pack(w[2], w[3]), T::pack(w[4], w[5]),
+                         T::pack(w[6], w[7])};
+    }
+    return (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+  };
+  // The weights are taken over the maximum so far, which need not be the tile's: it moves
+  // only when a lane's sixteen weights sum past kMostSum, or are not finite (in a
+  // part's first tile the maximum is -inf), and then they are taken again.  A maximum per tile
+  // would cost a tenth of the vector work.
+  auto softmax = [&] {
+    float add[NT];
+    bool fits = true;
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+      add[c] = weigh(c, mx[c]);
+      fits &= add[c] < kMostSum;
+    }
+    if (__builtin_amdgcn_ballot_w64(!fits) != 0) {
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        const float to = __builtin_fmaxf(mx[c], across4_max(max16_raw(S[c])) * scale);
+        const float f = to == neg_inf() ? 1.f : exp2_hw(mx[c] - to);
+        mx[c] = to;
+        sum[c] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) O[c][d] *= f;
+        add[c] = weigh(c, to == neg_inf() ? 0.f : to);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NT; ++c) sum[c] += add[c];
   };
   auto outputs = [&](uint32_t off) {
     u32x4_t x[2 * DT];
@@ -719,7 +738,7 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
     }
     if (odd) *flag = t + 1;
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const bool dirty = *(volatile int*)flag == t + 1;
+    const bool dirty = *(const volatile __attribute__((address_space(3))) int*)flag == t + 1;
     if (!active) return;
     scores(off);
     const bool live[4] = {live_at(base, 0), live_at(base, 1), live_at(base, 2), live_at(base, 3)};
@@ -734,8 +753,8 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
         if (ok) seen[c] |= 1u << i;
         S[c][i >> 2][i & 3] = ok ? S[c][i >> 2][i & 3] : neg_inf();
       }
-      softmax(c);
     }
+    softmax();
     outputs(off);
     if (!dirty) return;
     for (int kk = 0; kk < kBlockKeys; ++kk) {
@@ -787,8 +806,7 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
       __builtin_amdgcn_sched_barrier(0);
       if (active) {
         __builtin_amdgcn_s_setprio(1);  // vector work first: the matrix unit is fed a tile at a time
-        softmax(0);
-        softmax(1);
+        softmax();
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
         outputs(off);
