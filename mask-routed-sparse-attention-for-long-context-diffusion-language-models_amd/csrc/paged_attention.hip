@@ -92,6 +92,14 @@ typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
 __device__ __forceinline__ scalar_ints scalars(const int32_t* p) {
   return (scalar_ints)(uintptr_t)p;
 }
+// The kernel's arguments, to be read again: what only a kernel's end or a rare path needs would
+// otherwise hold scalar registers through its loop.
+typedef const __attribute__((address_space(4))) PagedArgs* args_again_t;
+__device__ __forceinline__ args_again_t args_again() {
+  args_again_t p = (args_again_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
 // The page of sixteen keys from `key` on (wave-uniform); -1 past the table.
 __device__ __forceinline__ int page_at(const PagedArgs& a, scalar_ints table, int key) {
   const int e = key >> a.page_shift;
@@ -438,29 +446,28 @@ __device__ __forceinline__ void dma_kb(uint32_t to, const uint8_t* base, uint32_
                : "memory", "m0");
 }
 // Swizzle of K's rows: the 16 rows of one operand read meet different banks.
-// Slots of the ring: waves 4 .. are half a tile behind the others and keep a third in use.
-__host__ __device__ constexpr int block_slots(int waves) { return waves > 4 ? 3 : 2; }
 
 template <int D>
 __device__ __forceinline__ int swizzle_k(int r) {
   return D == 128 ? r & 15 : (r >> 1) & 7;
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs a) {
+// SLOTS of the ring: 2, or 3 for more than four waves: waves 4 .. are half a tile behind the
+// others and keep a third in use.
+template <class T, int D, int SLOTS>
+__global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256) paged_block_kernel(PagedArgs a) {
   constexpr int KS = D / 32, DT = D / 16, NT = kBlockCols / 16;
   constexpr int ROWB = 2 * D;
   constexpr int UNITS = D / 8;
   constexpr int ROWS = 64 / UNITS;         // of one DMA instruction (1 KB)
   constexpr int TILEB = kBlockKeys * ROWB;
-  constexpr int SLOTB = 2 * TILEB;
+  constexpr int V_AT = SLOTS * TILEB;      // K's slots, then V's
   extern __shared__ __align__(256) unsigned char smem[];
   unsigned char* ring = smem;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int waves = __builtin_amdgcn_readfirstlane((int)blockDim.x >> 6);
-  const uint32_t ring_bytes = block_slots(waves) * SLOTB;
-  int* flag = reinterpret_cast<int*>(ring + ring_bytes);  // last tile (+ 1) with a value not finite
+  int* flag = reinterpret_cast<int*>(ring + 2 * V_AT);  // last tile (+ 1) with a value not finite
   const int col = lane & 15, grp = lane >> 4;
   // XCD-aware order: workgroups go to the XCDs in turn, so XCD x takes a contiguous
   // range, in which the column tiles of one piece of keys meet in its L2.
@@ -515,7 +522,7 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   const int page_mask = (1 << a.page_shift) - 1;
   constexpr int DMAS = 16 / ROWS;
   const int quarter = wave & 3;
-  const bool late = wave >= 4;
+  const bool late = SLOTS == 3 && wave >= 4;
   uint32_t k_lane[DMAS], v_lane[DMAS];   // byte offsets (a piece spans < 2^31 bytes)
 #pragma unroll
   for (int i = 0; i < DMAS; ++i) {
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   const int64_t k_page_bytes = 2 * a.k_sp, k_row_bytes = 2 * a.k_sr;
   const int64_t v_page_bytes = 2 * a.v_sp, v_row_bytes = 2 * a.v_sr;
   const uint32_t lds0 = lds_addr(ring);
-  const uint32_t k_to = lds0 + quarter * 16 * ROWB, v_to = lds0 + TILEB + quarter * 16 * ROWB;
+  const uint32_t k_to = lds0 + quarter * 16 * ROWB, v_to = lds0 + V_AT + quarter * 16 * ROWB;
   auto is_live = [&](int page) { return (uint32_t)page < (uint32_t)a.num_pages; };
   // The wave's rows in the tile at `base`: K's and V's addresses, of page `page`.
   struct Source {
@@ -558,10 +565,17 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
                ? __builtin_amdgcn_readfirstlane(entry) : -1;
   };
 
+  // Tiles; those from `plain` on up to plain_end are seen whole by every column.  Tile t is
+  // in slot (t - plain) mod SLOTS.
   const int tiles = first < last ? (last - first + kBlockKeys - 1) / kBlockKeys : 0;
+  const int plain = max(0, r.inner_lo - first + kBlockKeys - 1) / kBlockKeys;
+  int plain_end = max(0, min(last, r.inner_hi) - first) / kBlockKeys;
+  auto slot_of = [&](int t) {
+    return (uint32_t)(t + SLOTS - plain % SLOTS) % (uint32_t)SLOTS * (uint32_t)TILEB;
+  };
   int32_t entry = 0;
   if (tiles > 0 && !late) {
-    bring(source(first, page_from(first, entry_for(first))), 0);
+    bring(source(first, page_from(first, entry_for(first))), slot_of(0));
     entry = entry_for(first + kBlockKeys);
   }
   // (behind the first tile's DMA: the queries, and whether an entry of this piece of the table
@@ -596,7 +610,7 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
       k_at[s] = lds0 + ROWB * col + 16u * (uint32_t)((4 * s + grp) ^ swizzle_k<D>(col));
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      v_at[d] = lds0 + TILEB + ROWB * rt +
+      v_at[d] = lds0 + V_AT + ROWB * rt +
                 16u * (uint32_t)((2 * d + ((col >> 1) & 1)) ^ swizzle<D>(rt)) + 8u * (col & 1);
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(k_at[s]));
@@ -692,29 +706,28 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
     }
   };
 
-  // The ring: the slot of the current tile, and of the one whose rows are on their way.
-  uint32_t now = 0;
-  auto behind = [&](uint32_t off) { return off + SLOTB == ring_bytes ? 0 : off + SLOTB; };
-  auto before = [&](uint32_t off) { return off == 0 ? ring_bytes - SLOTB : off - SLOTB; };
+  // Tile t is there, and its successor, if any, on its way to slot `to`.
+  auto arrive = [&](int t, uint32_t to) {
+    const int base = first + t * kBlockKeys;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (late || t + 1 >= tiles) return;
+    bring(source(base + kBlockKeys, page_from(base + kBlockKeys, entry)), to);
+    entry = entry_for(base + 2 * kBlockKeys);
+  };
 
   // Any tile: masks, rows nobody sees, unmapped pages, the last.
   auto live_at = [&](int base, int i) { return !holes || is_live(page_at(a, table, base + 16 * i)); };
   auto edge_tile = [&](int t) {
-    const uint32_t off = now;
+    const uint32_t off = slot_of(t);
     const int base = first + t * kBlockKeys;
-    now = behind(now);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + 1 < tiles && !late) {
-      bring(source(base + kBlockKeys, page_from(base + kBlockKeys, entry)), now);
-      entry = entry_for(base + 2 * kBlockKeys);
-    }
+    arrive(t, slot_of(t + 1));
     // V rows that no column sees become zeros; values that are not finite
     // are taken out (a column that does not see them must not get 0 x inf) and
     // added one by one below.
     bool odd = false;
     for (int x = tid; x < kBlockKeys * UNITS; x += 64 * waves) {
       const int key = base + x / UNITS;
-      u32x4_t* at = reinterpret_cast<u32x4_t*>(ring + off + TILEB + 16 * x);
+      u32x4_t* at = reinterpret_cast<u32x4_t*>(ring + V_AT + off + 16 * x);
       bool lv = true;
       if (holes) {
         const int e = key >> a.page_shift;  // (a vector load: rows differ between lanes)
@@ -757,12 +770,13 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
     softmax();
     outputs(off);
     if (!dirty) return;
+    const args_again_t z = args_again();
     for (int kk = 0; kk < kBlockKeys; ++kk) {
       const int key = base + kk;
       if (!live_at(base, kk >> 4) || key < r.lo || key >= r.end) continue;
       const int from = 16 * ((kk & 15) >> 2) + col, slot_i = 4 * (kk >> 4) + (kk & 3);
-      const uint16_t* vp = a.v + h * a.v_sh + page_at(a, table, key) * a.v_sp +
-                           (int64_t)(key & page_mask) * a.v_sr;
+      const uint16_t* vp = z->v + h * z->v_sh + page_at(a, table, key) * z->v_sp +
+                           (int64_t)(key & page_mask) * z->v_sr;
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
         const bool ok = (__shfl(seen[c], from, 64) >> slot_i) & 1;
@@ -780,44 +794,41 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
   // tiles: two passes of a loop, so that the edge code is there once.
   // Waves 4 .. share their SIMDs with waves 0 .. and go half a tile behind them: their
   // softmax runs while the others' products do.
-  int plain = 0, plain_end = 0;
-  if (!holes && tiles > 0) {
-    plain = max(0, r.inner_lo - first + kBlockKeys - 1) / kBlockKeys;
-    plain_end = max(0, min(last, r.inner_hi) - first) / kBlockKeys;
-  }
-  auto arrive = [&](int t) {  // tile t is there, and its successor, if any, on its way
-    const int base = first + t * kBlockKeys;
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    now = behind(now);
-    if (late || t + 1 >= tiles) return;
-    bring(source(base + kBlockKeys, page_from(base + kBlockKeys, entry)), now);
-    entry = entry_for(base + 2 * kBlockKeys);
-  };
+  if (holes) plain_end = 0;
   int t = 0;
+  // A plain tile in slot SLOT (constants, so that no address is computed); false: the last.
+  auto plain_tile = [&](auto slot) {
+    constexpr uint32_t off = decltype(slot)::value * TILEB;
+    constexpr uint32_t after = (decltype(slot)::value + 2) % SLOTS * TILEB;
+    const bool more = t + 1 < plain_end;
+    if (active) scores(off);
+    if (late && more) arrive(t + 1, after);
+    __builtin_amdgcn_sched_barrier(0);
+    if (active) {
+      __builtin_amdgcn_s_setprio(1);  // vector work first: the matrix unit is fed a tile at a time
+      softmax();
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      outputs(off);
+    }
+    ++t;
+    if (!late && more) arrive(t, after);
+    return more;
+  };
   for (int pass = 0; pass < 2; ++pass) {
     for (const int to = pass == 0 && plain < plain_end ? plain : tiles; t < to; ++t) edge_tile(t);
     if (t >= plain_end) continue;
-    uint32_t off = now;
-    arrive(t);
-    for (;; off = behind(off)) {
-      const bool more = t + 1 < plain_end;
-      if (active) scores(off);
-      if (late && more) arrive(t + 1);
-      __builtin_amdgcn_sched_barrier(0);
-      if (active) {
-        __builtin_amdgcn_s_setprio(1);  // vector work first: the matrix unit is fed a tile at a time
-        softmax();
-        __builtin_amdgcn_s_setprio(0);
-        __builtin_amdgcn_sched_barrier(0);
-        outputs(off);
-      }
-      ++t;
-      if (!more) break;
-      if (!late) arrive(t);
+    arrive(t, TILEB);
+    for (;;) {
+      if (!plain_tile(std::integral_constant<int, 0>{})) break;
+      if (!plain_tile(std::integral_constant<int, 1>{})) break;
+      if constexpr (SLOTS == 3)
+        if (!plain_tile(std::integral_constant<int, 2>{})) break;
     }
   }
 
   // ---- out: lane (col, grp) holds dims 16 d + 4 grp .. of its columns
+  const args_again_t z = args_again();
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int m = c0 + 16 * t + col;
@@ -828,29 +839,29 @@ __global__ void __launch_bounds__(64 * kBlockWaves) paged_block_kernel(PagedArgs
 #pragma unroll
       for (int d = 0; d < DT; ++d) O[t][d] = zero4();
     }
-    if (m >= a.M) continue;
-    if (a.parts > 1) {
-      const int64_t at = (((int64_t)b * a.Hkv + h) * a.M + m) * a.parts + part;
+    if (m >= z->M) continue;
+    if (z->parts > 1) {
+      const int64_t at = (((int64_t)b * z->Hkv + h) * z->M + m) * z->parts + part;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
-        *reinterpret_cast<f32x4_t*>(a.part_out + at * D + 16 * d + 4 * grp) = O[t][d];
+        *reinterpret_cast<f32x4_t*>(z->part_out + at * D + 16 * d + 4 * grp) = O[t][d];
       if (grp == 0) {
-        a.part_ml[2 * at] = mx[t];
-        a.part_ml[2 * at + 1] = total;
+        z->part_ml[2 * at] = mx[t];
+        z->part_ml[2 * at + 1] = total;
       }
       continue;
     }
-    const int qi = m / a.G;
-    const int64_t row = ((int64_t)b * a.Lq + qi) * a.Hq + h * a.G + (m - qi * a.G);
+    const int qi = m / z->G;
+    const int64_t row = ((int64_t)b * z->Lq + qi) * z->Hq + h * z->G + (m - qi * z->G);
     const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       u32x2_t o = {0u, 0u};
       if (total != 0.f)
         o = u32x2_t{T::pack(O[t][d][0] * inv, O[t][d][1] * inv), T::pack(O[t][d][2] * inv, O[t][d][3] * inv)};
-      *reinterpret_cast<u32x2_t*>(a.out + row * D + 16 * d + 4 * grp) = o;
+      *reinterpret_cast<u32x2_t*>(z->out + row * D + 16 * d + 4 * grp) = o;
     }
-    if (grp == 0) a.lse[row] = total == 0.f ? neg_inf() : kLn2 * (mx[t] + log2_hw(total));
+    if (grp == 0) z->lse[row] = total == 0.f ? neg_inf() : kLn2 * (mx[t] + log2_hw(total));
   }
 }
 
@@ -957,14 +968,13 @@ int launch(const PagedArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves), lds,
                        stream, a);
   } else {
-    const size_t slot = 2 * kBlockKeys * 2 * D;
-    const size_t lds = block_slots(a.tile_cols / kBlockCols) * slot + 16;
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_block_kernel<T, D>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize,
-                            (int)(3 * slot + 16)) != hipSuccess)
+    const int waves = a.tile_cols / kBlockCols;
+    auto kern = waves > 4 ? paged_block_kernel<T, D, 3> : paged_block_kernel<T, D, 2>;
+    const size_t lds = (waves > 4 ? 3 : 2) * 2 * kBlockKeys * 2 * D + 16;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
       return MRSA_ERR_LAUNCH;
-    hipLaunchKernelGGL((paged_block_kernel<T, D>), dim3((unsigned)grid),
-                       dim3(64 * a.tile_cols / kBlockCols), lds, stream, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * waves), lds, stream, a);
   }
   int st = mrsa_launch_status();
   if (st != MRSA_OK || a.parts == 1) return st;
