@@ -10,17 +10,23 @@
 // and out = 0, lse = -inf for a row that sees none.
 //
 // The G query heads of a KV head and the q_len rows are matrix columns
-// (column m: row m / G, head m % G), 16 to a tile.  A wave streams tiles of 32
-// keys with a running maximum and sum per column:
-//   S^T = K . Q^T    K rows straight from HBM to registers (operand A)
-//   O^T += V^T . P^T P^T is S^T's own register layout (operand B); V goes
-//                    through the wave's own piece of LDS and comes back
-//                    transposed (gfx950's transposing reads).
+// (column m: row m / G, head m % G).  Tiles of keys are passed once, with a running
+// maximum and sum per column:
+//   S^T = K . Q^T    K rows as operand A
+//   O^T += V^T . P^T P^T is S^T's own register layout (operand B); V comes
+//                    transposed from LDS (gfx950's transposing reads).
 // Products of 16-bit inputs are exact, sums fp32; P is rounded to the inputs'
 // type as a matrix operand (the sum uses the unrounded values), which is half
-// a step of that type per term.  The maximum moves only when a score passes it
-// by more than 8 (base 2), so that P stays below 2^8 and the accumulators are
-// rarely rescaled.
+// a step of that type per term.  The maximum moves only when scores have passed it
+// by some powers of two, so that the accumulators are rarely rescaled.
+//
+// Up to 16 columns (a token's heads) the work is the cache's bytes: `paged_attn_kernel`
+// streams them.  With more columns every key is multiplied often enough to be
+// brought to LDS once for all: `paged_block_kernel`.  8 sequences of 8191 keys of 4 KV
+// heads: 14 columns 30 us by the former, 21 columns 32 by the latter, 48 by two tiles
+// of the former.  `parts` cuts the keys of a sequence into pieces for workgroups of
+// their own, where there are few; fp32 partial results go through a workspace to
+// `paged_join_kernel`.
 #include "chunk_tile.h"
 #include "mrsa_device.h"
 
@@ -150,6 +156,11 @@ __device__ __forceinline__ int swizzle(int r) {
   return D == 128 ? 2 * (r & 7) + ((r >> 3) & 1) : 2 * ((r >> 1) & 3) + ((r >> 3) & 1);
 }
 
+// Up to 16 columns.  A workgroup's four waves take tiles of 32 keys in turn: K rows straight
+// from HBM to registers, V rows through the wave's own piece of LDS, a tile's loads
+// in flight while the one before is worked on.  Bound by HBM: 131072 keys of 4 KV heads,
+// 256 MB, in 51.6 us, 5.2 TB/s (a large copy: 5.3); 64 sequences of up to 8192 keys, 584 MB, in
+// 121 us, 5.0 TB/s; 1000 keys in 7.4 us, the launch and three dependent reads.
 template <class T, int D>
 __global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedArgs a) {
   constexpr int KS = D / 32;             // reduction steps of S
@@ -429,8 +440,18 @@ __global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedArgs a) {
 
 // Many columns: a workgroup of up to eight waves, 32 columns each, over tiles of
 // 64 keys that all its waves read from LDS.  K and V rows come by global->LDS
-// DMA into a two-slot ring, one barrier per tile; K is read along the row
+// DMA into a ring, a tile ahead, one barrier per tile; K is read along the row
 // (operand A of S^T), V by transposing reads (operand A of O^T).
+//
+// Bound by vector issue: a wave's tile is 64 matrix instructions and about 200 vector ones
+// (16 exponentials a lane and column tile, the sums, the packing), and two waves share a
+// SIMD.  So the two go half a tile apart (the softmax of one runs beside the products of the
+// other), tiles that every column sees whole have a loop of their own without masks, with
+// the ring's slots as constants, and the maximum is not taken per tile.  28 heads in 4 groups,
+// 32 rows, 65503 keys (30 GFLOP, 134 MB; 64 pieces): 45.6 us, 660 TFLOP/s; of them 5 until the
+// first rows are there, 30 for sixteen tiles (1.6 us a tile with few workgroups, 2.0 with 256)
+// and 8 for the partial results' way out.  The same with waves in step 49.7 us; masks in
+// the one loop 54.
 constexpr int kBlockKeys = 64;
 constexpr int kBlockCols = 32;             // of a wave
 constexpr int kBlockWaves = 8;
@@ -446,14 +467,14 @@ __device__ __forceinline__ void dma_kb(uint32_t to, const uint8_t* base, uint32_
                : "memory", "m0");
 }
 // Swizzle of K's rows: the 16 rows of one operand read meet different banks.
-
 template <int D>
 __device__ __forceinline__ int swizzle_k(int r) {
   return D == 128 ? r & 15 : (r >> 1) & 7;
 }
 
 // SLOTS of the ring: 2, or 3 for more than four waves: waves 4 .. are half a tile behind the
-// others and keep a third in use.
+// others and keep a third in use.  (Four waves or fewer: two workgroups fit a CU, 16 sequences
+// of 8 rows 58 us, 67 where they do not.)
 template <class T, int D, int SLOTS>
 __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256) paged_block_kernel(PagedArgs a) {
   constexpr int KS = D / 32, DT = D / 16, NT = kBlockCols / 16;
