@@ -983,9 +983,7 @@ int launch(const PagedArgs& a, hipStream_t stream) {
     return MRSA_ERR_UNSUPPORTED;
   if (a.tile_cols == 16) {
     const size_t lds = kWaves * std::max(kTile * 2 * D, 16 * (D + 4) * 4);
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, D>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
-      return MRSA_ERR_LAUNCH;
+    static_assert(kWaves * std::max(kTile * 2 * D, 16 * (D + 4) * 4) <= 65536);  // (needs no attribute)
     hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves), lds,
                        stream, a);
   } else {
