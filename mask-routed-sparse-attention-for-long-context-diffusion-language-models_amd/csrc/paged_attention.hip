@@ -473,10 +473,11 @@ __device__ __forceinline__ int swizzle_k(int r) {
 }
 
 // SLOTS of the ring: 2, or 3 for more than four waves: waves 4 .. are half a tile behind the
-// others and keep a third in use.  (Four waves or fewer: two workgroups fit a CU, 16 sequences
-// of 8 rows 58 us, 67 where they do not.)
+// others and keep a third in use.  Two workgroups of four waves fit a CU (hence the bound on
+// registers).
 template <class T, int D, int SLOTS>
-__global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256) paged_block_kernel(PagedArgs a) {
+__global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256, 2)
+    paged_block_kernel(PagedArgs a) {
   constexpr int KS = D / 32, DT = D / 16, NT = kBlockCols / 16;
   constexpr int ROWB = 2 * D;
   constexpr int UNITS = D / 8;
@@ -599,8 +600,8 @@ __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256) paged_blo
     bring(source(first, page_from(first, entry_for(first))), slot_of(0));
     entry = entry_for(first + kBlockKeys);
   }
-  // (behind the first tile's DMA: the queries, and whether an entry of this piece of the table
-  // is unmapped, in which case every tile looks)
+  // (behind the first tile's DMA: the queries, none for padding, whose values may be anything;
+  // and whether an entry of this piece of the table is unmapped, in which case every tile looks)
   bool holes = false;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256) paged_blo
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       Q[t][s] = u32x4_t{0, 0, 0, 0};
-      if (m < a.M) Q[t][s] = *reinterpret_cast<const u32x4_t*>(qp + 32 * s);
+      if (!padding[t]) Q[t][s] = *reinterpret_cast<const u32x4_t*>(qp + 32 * s);
     }
   }
   for (int e = (first >> a.page_shift) + lane; e <= (last - 1) >> a.page_shift; e += 64)

@@ -168,8 +168,8 @@ def cache_parts(batch: int, q_len: int, q_heads: int, kv_heads: int, span: int, 
     keys, about 128 more to start, the uneven ends of sequences of different lengths, and
     its part in the join.  More columns (block kernel; in keys of 28 ns): a round costs 230
     to start and its keys, the join 140 and its bytes, 1 KB a column and piece, written and
-    read.  64 sequences of 32 rows of 2048 keys: 1 piece 91 us, 3 147; 8 of 4096: 8 pieces
-    43 us, 24 66; 1 of 8192: 48 pieces 29 us, 8 47."""
+    read.  64 sequences of 32 rows of 2048 keys: 1 piece 78 us, 3 140; 8 of 4096: 8 pieces
+    39 us, 24 64; 1 of 8192: 48 pieces 29 us, 8 42."""
 
     cols = q_len * (q_heads // kv_heads)
     if cols == 0 or batch == 0 or span <= 0:
