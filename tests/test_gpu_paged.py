@@ -552,6 +552,46 @@ def test_graphs_of_a_decode_step_replay_with_new_inputs():
                 assert torch.equal(vp[at[0], at[1]], v[b, 0])
 
 
+def test_padding_queries_may_hold_anything():
+    for Lq, n in ((2, 70), (40, 300), (200, 500)):
+        q, k, v, table, lens = _case(2, Lq, [n, n - 30], 14, 2, 128, 16, torch.bfloat16, seed=Lq)
+        for starts in (lens - Lq + 1, torch.full_like(lens, -(Lq // 2))):  # past the end, before 0
+            pos = starts[:, None] + torch.arange(Lq)
+            pad = (pos < 0) | (pos >= lens[:, None])
+            assert pad.any() and not pad.all()
+            bad = q.clone()
+            bad[pad] = torch.tensor([float("nan"), float("inf")]).repeat(64).to(q.dtype)
+            clean = torch.where(pad[..., None, None], 0, q)
+            for kw in (dict(), dict(causal=True), dict(window=50, parts=3)):
+                got = _run(bad, k, v, table, lens, query_starts=starts, **kw)
+                _check(got, clean, k, v, table, lens, query_starts=starts, **kw)
+
+
+def test_graphs_that_share_a_pool_replay_in_turn():
+    # blocks (more than 16 columns) and tokens, in pieces, whose workspaces may be the same memory
+    cases = [_case(2, Lq, lens, 14, 2, 128, 32, torch.bfloat16, seed=20 + Lq)
+             for Lq, lens in ((1, [500, 90]), (32, [700, 333]), (90, [640, 90]))]
+    dev = [[t.to(DEV) for t in c] for c in cases]
+    calls = [lambda c=c, parts=parts: mrsa.paged_cached_attention(*c, parts=parts)
+             for c, parts in zip(dev, (4, 5, 9))]
+    for call in calls:
+        call()
+    graphs, pool = [], None
+    for call in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            out = call()
+        pool = graph.pool()
+        graphs.append((graph, out))
+    for i in (0, 1, 2, 1, 0, 2, 2, 0):
+        dev[i][0].mul_(-1)
+        graphs[i][0].replay()
+        got = [t.clone() for t in graphs[i][1]]
+        want = calls[i]()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_the_operators_trace_without_a_graph_break():
     args = [t.to(DEV) for t in _case(2, 4, [50, 20], 8, 2, 64, 16, torch.bfloat16, seed=12)]
     cos, sin = mrsa.rotary_tables(90, mrsa.rotary_frequencies(64)[0], device=DEV)

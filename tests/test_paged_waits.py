@@ -14,7 +14,7 @@ from test_dma_waits import HIPCC, device_assembly
 def test_paged_block_tiles_wait_for_their_rows_before_the_barrier(tmp_path):
     text = device_assembly("paged_attention", tmp_path / "paged.s")
     kernels = re.findall(r"^(_ZN\S*paged_block_kernel\S*):(.*?)^\.Lfunc_end", text, re.S | re.M)
-    assert len(kernels) == 4  # type x head dim
+    assert len(kernels) == 8  # type x head dim x slots
     for name, body in kernels:
         assert "global_load_lds_dwordx4" in body, name
         waits = re.findall(r"s_waitcnt (vmcnt\(0\) )?lgkmcnt\(0\)\n\s*s_barrier", body)
