@@ -188,6 +188,8 @@ def rotary_qk(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin
     others are copied.  positions: torch.long [B, L] or [L]; None: row i is at
     position i.  A position outside the tables makes its rows' turned dims NaN.
     Returns new dense (q', k'); fp32 arithmetic with one rounding.
+    To capture a backward pass, take it by torch.autograd.grad inside the capture, with no
+    eager graph of the same leaves alive.
     """
 
     check_heads(q, "q")

@@ -216,3 +216,29 @@ def test_other_streams_and_replayed_graphs():
         want = mrsa.rotary_qk(q, k, cos, sin, pos)
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_a_captured_backward_pass():
+    g = torch.Generator().manual_seed(9)
+    cos, sin = (t.to(DEV) for t in _tables(64, 64))
+    q, k, gq, gk = (torch.randn(2, 9, h, 64, generator=g).half().to(DEV) for h in (6, 2, 6, 2))
+    q.requires_grad_(), k.requires_grad_()
+
+    def step():
+        out = mrsa.rotary_qk(q, k, cos, sin)
+        return torch.autograd.grad(out, (q, k), (gq, gk))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        gq.copy_(torch.randn(gq.shape, generator=g)), gk.mul_(-2)
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
