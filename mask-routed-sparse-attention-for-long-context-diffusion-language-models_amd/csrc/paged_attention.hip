@@ -998,10 +998,10 @@ int launch(const PagedArgs& a, hipStream_t stream) {
   }
   int st = mrsa_launch_status();
   if (st != MRSA_OK || a.parts == 1) return st;
-  // Four waves per column where there are many parts and few columns (896 columns of 64 parts:
-  // 7.7 us, 9.2 by one wave; 28 of 256: 5.4 and 8.1), otherwise one (1792 columns of 6:
-  // 5.0 us, 7.4 by four; 7168 of 11: 7.8 and 19.7).
-  if (a.parts > 8 && cols <= 4096)
+  // Four waves per column where there are many parts and few columns, otherwise one. Both
+  // kernels' time by four and by one: 28 columns of 64 parts 11.0 and 12.7 us, 448 of 64 20.3 and
+  // 22.4, 896 of 32 23.2 and 24.2, of 12 20.6 and 19.3, 2688 of 12 27.4 and 23.7.
+  if (a.parts > 16 && cols <= 1024)
     hipLaunchKernelGGL((paged_join_kernel<T, D, 4>), dim3((unsigned)cols), dim3(256), 0, stream, a);
   else
     hipLaunchKernelGGL((paged_join_kernel<T, D, 1>), dim3((unsigned)((cols + 3) / 4)), dim3(256), 0,
