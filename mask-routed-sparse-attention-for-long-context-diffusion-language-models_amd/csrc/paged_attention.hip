@@ -1086,7 +1086,7 @@ extern "C" int mrsa_paged_attention_fwd(
   a.col_tiles = (a.M + a.tile_cols - 1) / a.tile_cols;
   const int64_t span =
       span_bound(max_len, q_len, a.G, a.tile_cols, a.window, a.causal, !query_starts) +
-      kTile - 1;
+      (a.window >= 0 ? kTile - 1 : 0);  // (a window's first tile may start before it)
   const int64_t step = a.tile_cols == 16 ? kStep : kBlockKeys;
   a.part_keys = (int)(((span + parts - 1) / parts + step - 1) / step * step);
   a.out = (uint16_t*)out;

@@ -166,10 +166,12 @@ def cache_parts(batch: int, q_len: int, q_heads: int, kv_heads: int, span: int, 
 
     Up to 16 columns (rows and heads of a KV head; streaming kernel) a piece costs its
     keys, about 128 more to start, the uneven ends of sequences of different lengths, and
-    its part in the join.  More columns (block kernel; in keys of 28 ns): a round costs 230
-    to start and its keys, the join 140 and its bytes, 1 KB a column and piece, written and
-    read.  64 sequences of 32 rows of 2048 keys: 1 piece 78 us, 3 140; 8 of 4096: 8 pieces
-    39 us, 24 64; 1 of 8192: 48 pieces 29 us, 8 42."""
+    its part in the join, which itself costs 512.  32 sequences of 500 keys: 1 piece 13.4 us,
+    2 16.6; 1 of 500: 1 piece 11.0, 5 10.9; 1 of 1000: 1 piece 15.3, 8 11.0; 64 of 1024 to
+    8192: 3 pieces 128, 1 143.  More columns (block kernel; in keys of 28 ns): a round costs
+    230 to start and its keys, the join 140 and its bytes, 1 KB a column and piece, written
+    and read.  64 sequences of 32 rows of 2048 keys: 1 piece 78 us, 3 140; 8 of 4096: 8
+    pieces 39 us, 24 64; 1 of 8192: 48 pieces 29 us, 8 42."""
 
     cols = q_len * (q_heads // kv_heads)
     if cols == 0 or batch == 0 or span <= 0:
@@ -177,11 +179,13 @@ def cache_parts(batch: int, q_len: int, q_heads: int, kv_heads: int, span: int, 
     best, least = 1, None
     if cols <= 16:
         units = batch * kv_heads
-        most = min(MAX_PARTS, -(-(span + 31) // 128))
-        for rounds in (1, 2, 3, 4, 6):
+        most = min(MAX_PARTS, -(-span // 128))
+        for rounds in (0, 1, 2, 3, 4, 6):
             parts = max(1, min(most, 256 * rounds // units))
-            keys = -(-(span + 31) // (parts * 128)) * 128
+            keys = -(-(span + 31) // (parts * 128)) * 128   # (with room: lengths grow)
             cost = -(-units * parts // 256) * (keys + 128) + keys // 4 + 4 * parts
+            if parts > 1:
+                cost += 512
             if least is None or cost < least:
                 best, least = parts, cost
         return best
@@ -189,11 +193,11 @@ def cache_parts(batch: int, q_len: int, q_heads: int, kv_heads: int, span: int, 
     tiles = -(-groups // 8)
     units = batch * kv_heads * tiles
     slots = 256 if -(-groups // tiles) > 4 else 512   # workgroups at a time
-    most = min(MAX_PARTS, -(-(span + 31) // 64))
+    most = min(MAX_PARTS, -(-span // 64))
     for quarters in (0, 2, 3, 4, 8, 12, 16, 24):
         parts = max(1, min(most, slots * quarters * span // (4 * units * live)))
-        keys = -(-(span + 31) // (parts * 64)) * 64
-        there = min(parts, -(-(live + 31) // keys))
+        keys = -(-span // (parts * 64)) * 64
+        there = min(parts, -(-live // keys))
         cost = -(-units * there // slots) * (230 + keys)
         if slots == 512 and units * there > 256:   # two on a CU slow each other
             cost = cost * 13 // 10
@@ -221,7 +225,8 @@ def _paged_attention_impl(q, k_pages, v_pages, page_table, cache_lens, query_sta
         if window >= 0:
             right = 0 if causal else window if query_starts is not None else min(window, Lq)
             span = min(max_len, min(Lq, 256) + window + right)
-            live = min(span, min(Lq, 256) + window)
+            live = min(span, min(Lq, 256) + window) + 31
+            span += 31   # (a window's first tile may start before it)
         parts = cache_parts(B, Lq, Hq, Hkv, span, live)
     out = q.new_empty(shape)
     lse = q.new_empty((B, Lq, Hq), dtype=torch.float32)
