@@ -149,6 +149,11 @@ __device__ __forceinline__ Range tile_range(const PagedArgs& a, int n, int p0, i
   return r;
 }
 
+// Whether some column, not every one, sees a key of [base, base + keys).
+__device__ __forceinline__ bool is_uneven(const Range& r, int base, int keys) {
+  return max(base, r.lo) < r.inner_lo || min(base + keys, r.end) > r.inner_hi;
+}
+
 // Swizzle of V's LDS rows in 16-byte units: the transposing read's rows of one
 // lane group meet different banks.
 template <int D>
@@ -271,15 +276,20 @@ __global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedArgs a) {
     const bool edge = !whole || base < r.lo || base + kTile > r.end;           // V rows nobody sees
     const bool mixed = !whole || base < r.inner_lo || base + kTile > r.inner_hi;  // masked scores
     uint64_t dirty = 0;
-    if (mixed) {
-      // Keys that some columns see and others do not: a non-finite value
-      // must not reach the others as 0 x inf, so it is taken out here and its
-      // terms are added one by one below.  Rows nobody sees become zeros.
+    if (edge) {  // rows nobody sees become zeros
 #pragma unroll
       for (int i = 0; i < VL; ++i) {
         const int key = base + i * VROWS + vrow;
         const bool there = live[i / (VL / 2)] && key >= r.lo && key < r.end;
-        if (edge && !there) V[i] = u32x4_t{0, 0, 0, 0};
+        if (!there) V[i] = u32x4_t{0, 0, 0, 0};
+      }
+    }
+    if (is_uneven(r, base, kTile)) {
+      // Keys that some columns see and others do not: a non-finite value
+      // must not reach the others as 0 x inf, so it is taken out here and its
+      // terms are added one by one below.
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
         bool odd = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -744,8 +754,9 @@ __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256, 2)
     const int base = first + t * kBlockKeys;
     arrive(t, slot_of(t + 1));
     // V rows that no column sees become zeros; values that are not finite
-    // are taken out (a column that does not see them must not get 0 x inf) and
-    // added one by one below.
+    // are taken out where some columns see them and others do not (which must not get
+    // 0 x inf) and added one by one below.
+    const bool uneven = is_uneven(r, base, kBlockKeys);
     bool odd = false;
     for (int x = tid; x < kBlockKeys * UNITS; x += 64 * waves) {
       const int key = base + x / UNITS;
@@ -759,6 +770,7 @@ __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256, 2)
         *at = u32x4_t{0, 0, 0, 0};
         continue;
       }
+      if (!uneven) continue;
       u32x4_t v = *at;
       bool bad = false;
 #pragma unroll
