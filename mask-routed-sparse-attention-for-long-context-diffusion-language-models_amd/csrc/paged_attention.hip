@@ -37,6 +37,10 @@ namespace {
 constexpr int kWaves = 4;                  // of the streaming kernel
 constexpr int kTile = 32;                  // keys of a wave's tile
 constexpr int kStep = kWaves * kTile;      // keys of a workgroup's round
+// LDS of a streaming workgroup: more than it needs, so that two are on a CU and not three: 64
+// sequences of 1024 to 8192 keys in three pieces then take 128 us, 155 with three on a CU, and
+// the other lengths and numbers of pieces differ by less.
+constexpr int kStreamLds = 56 * 1024;
 constexpr int kMaxParts = 1024;
 constexpr int kFar = 1 << 29;              // bound of positions and windows: their sums fit 32 bits
 constexpr float kSlack = 8.f;              // base-2 growth before the maximum moves
@@ -167,7 +171,7 @@ __device__ __forceinline__ int swizzle(int r) {
 // 256 MB, in 51.6 us, 5.2 TB/s (a large copy: 5.3); 64 sequences of up to 8192 keys, 584 MB, in
 // 121 us, 5.0 TB/s; 1000 keys in 7.4 us, the launch and three dependent reads.
 template <class T, int D>
-__global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedArgs a) {
+__global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedArgs a) {
   constexpr int KS = D / 32;             // reduction steps of S
   constexpr int DT = D / 16;             // output tiles
   constexpr int UNITS = D / 8;           // 16-byte units of a row
@@ -995,10 +999,9 @@ int launch(const PagedArgs& a, hipStream_t stream) {
   if (grid > 0xffffffffll / threads || (a.parts > 1 && cols > (1 << 26) - 4) || cols > 0x7fffffff)
     return MRSA_ERR_UNSUPPORTED;
   if (a.tile_cols == 16) {
-    const size_t lds = kWaves * std::max(kTile * 2 * D, 16 * (D + 4) * 4);
-    static_assert(kWaves * std::max(kTile * 2 * D, 16 * (D + 4) * 4) <= 65536);  // (needs no attribute)
-    hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves), lds,
-                       stream, a);
+    static_assert(kStreamLds >= kWaves * std::max(kTile * 2 * D, 16 * (D + 4) * 4));
+    hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)grid), dim3(64 * kWaves),
+                       kStreamLds, stream, a);
   } else {
     const int waves = a.tile_cols / kBlockCols;
     auto kern = waves > 4 ? paged_block_kernel<T, D, 3> : paged_block_kernel<T, D, 2>;
