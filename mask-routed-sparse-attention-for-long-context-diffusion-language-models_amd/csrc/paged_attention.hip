@@ -168,8 +168,10 @@ __device__ __forceinline__ int swizzle(int r) {
 // Up to 16 columns.  A workgroup's four waves take tiles of 32 keys in turn: K rows straight
 // from HBM to registers, V rows through the wave's own piece of LDS, a tile's loads
 // in flight while the one before is worked on.  Bound by HBM: 131072 keys of 4 KV heads,
-// 256 MB, in 51.6 us, 5.2 TB/s (a large copy: 5.3); 64 sequences of up to 8192 keys, 584 MB, in
-// 121 us, 5.0 TB/s; 1000 keys in 7.4 us, the launch and three dependent reads.
+// 256 MB, in 50.4 us, 5.3 TB/s, a large copy's rate; 64 sequences of 1024 to 8192 keys, 584 MB, in
+// 122 us, 5.0 TB/s; 1000 keys in 5.8 us, the launch and three dependent reads.  (Without the
+// bound on registers the compiler moves the accumulators between register files every
+// tile: 0.8 us more for a token.)
 template <class T, int D>
 __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedArgs a) {
   constexpr int KS = D / 32;             // reduction steps of S
