@@ -916,7 +916,8 @@ int mrsa_candidate_token_scores_fwd(const void* q, const void* kv_frags, const i
  *     at position i); a position outside [0, table_rows) makes its rows'
  *     rotated dims NaN
  *   q_out, k_out: dense, not overlapping the inputs
- * Limits: batch * seq_len < 2^31, head_dim <= 4096.
+ * Limits: batch * seq_len < 2^31, head_dim <= 4096, one launch (fewer than 2^32
+ * threads, 16 bytes or a pair each).
  */
 int mrsa_rotary_fwd(const void* q, int64_t q_batch_stride, int64_t q_row_stride,
                     int64_t q_head_stride, const void* k, int64_t k_batch_stride,
@@ -940,7 +941,7 @@ int mrsa_rotary_fwd(const void* q, int64_t q_batch_stride, int64_t q_row_stride,
  *   page_table: int32 [batch, table_pages], row stride page_table_stride
  *   k_pages, v_pages (in/out): [num_pages, page_size, kv_heads, head_dim] in
  *     any order given by page, slot and head strides, dense last dim
- * Limits: page_size a power of two, as mrsa_rotary_fwd otherwise.
+ * Limits: page_size a power of two up to 2^20, as mrsa_rotary_fwd otherwise.
  */
 int mrsa_paged_append_fwd(
     const void* q, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride,
@@ -971,10 +972,11 @@ int mrsa_paged_append_fwd(
  *   parts (1..1024): pieces that the visible span is cut into, joined by a
  *     second kernel over fp32 partials in `workspace`
  *     (mrsa_paged_attention_workspace_bytes; 16-byte aligned; unused for 1)
- *   max_len: bound of cache_lens; sm_scale: finite and > 0
+ *   max_len: bound of cache_lens; sm_scale: > 0 and finite, also times log2 e
  * Limits: head_dim 64 or 128, page_size a power of two from 16 on, pointers
  * 16-byte aligned and strides multiples of 8 elements, slot strides below 2^26,
- * max_len < 2^29.
+ * max_len and q_len * q_heads / kv_heads < 2^29, one launch (fewer than 2^32
+ * threads).
  */
 int64_t mrsa_paged_attention_workspace_bytes(int64_t batch, int64_t q_len, int64_t q_heads,
                                              int64_t head_dim, int64_t parts);
