@@ -744,12 +744,16 @@ __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256, 2)
     }
   };
 
-  // Tile t is there, and its successor, if any, on its way to slot `to`.
+  // Tile t is there, and its successor, if any, on its way to slot `to`.  (Where that comes from
+  // is computed before the barrier, which waves 0 .. mostly wait at.)
   auto arrive = [&](int t, uint32_t to) {
     const int base = first + t * kBlockKeys;
+    const bool brings = !late && t + 1 < tiles;
+    Source s = {nullptr, nullptr};
+    if (brings) s = source(base + kBlockKeys, page_from(base + kBlockKeys, entry));
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (late || t + 1 >= tiles) return;
-    bring(source(base + kBlockKeys, page_from(base + kBlockKeys, entry)), to);
+    if (!brings) return;
+    bring(s, to);
     entry = entry_for(base + 2 * kBlockKeys);
   };
 
