@@ -472,15 +472,28 @@ constexpr int kBlockKeys = 64;
 constexpr int kBlockCols = 32;             // of a wave
 constexpr int kBlockWaves = 8;
 
-// A DMA instruction: 1 KB of LDS from `to` on, lane l's 16 bytes from base + at.  As
-// asm, since after the builtin the compiler waits for all DMA in flight before the
-// next LDS read; here the loop's own waits order them.  base and to are
-// wave-uniform; the s_nop covers m0 and a scalar operand that a vector instruction
-// has just written (5 wait states).
-__device__ __forceinline__ void dma_kb(uint32_t to, const uint8_t* base, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at),
-               "s"(base)
-               : "memory", "m0");
+// A piece by DMA: N instructions, each 1 KB of LDS from `to` on, lane l's 16 bytes from
+// base + at[i].  As asm, since after the builtin the compiler waits for all DMA in flight before
+// the next LDS read; here the loop's own waits order them.  base and to are
+// wave-uniform; the first s_nop covers a scalar operand that a vector instruction
+// has just written (5 wait states), the others m0.
+template <int N>
+__device__ __forceinline__ void dma_piece(uint32_t to, const uint8_t* base, const uint32_t (&at)[N]) {
+  static_assert(N == 2 || N == 4);
+  if constexpr (N == 4)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %1\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %1\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %1\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %1" ::"s"(to),
+        "s"(base), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[N - 1])
+        : "memory", "m0", "scc");
+  else
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %1\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %1" ::"s"(to),
+        "s"(base), "v"(at[0]), "v"(at[1])
+        : "memory", "m0", "scc");
 }
 // Swizzle of K's rows: the 16 rows of one operand read meet different banks.
 template <int D>
@@ -586,11 +599,8 @@ __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256, 2)
                   v_pool + (at * v_page_bytes + row * v_row_bytes)};
   };
   auto bring = [&](const Source& s, uint32_t slot_off) {
-#pragma unroll
-    for (int i = 0; i < DMAS; ++i) {
-      dma_kb(k_to + slot_off + 1024 * i, s.k, k_lane[i]);
-      dma_kb(v_to + slot_off + 1024 * i, s.v, v_lane[i]);
-    }
+    dma_piece(k_to + slot_off, s.k, k_lane);
+    dma_piece(v_to + slot_off, s.v, v_lane);
   };
   // The table entry of the wave's rows, read a tile ahead.  (A vector load: a scalar one in
   // flight would turn every wait for LDS into a wait for all of it.)
