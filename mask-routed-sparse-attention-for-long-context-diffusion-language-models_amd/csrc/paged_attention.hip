@@ -463,11 +463,13 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedArgs a)
 // (16 exponentials a lane and column tile, the sums, the packing), and two waves share a
 // SIMD.  So the two go half a tile apart (the softmax of one runs beside the products of the
 // other), tiles that every column sees whole have a loop of their own without masks, with
-// the ring's slots as constants, and the maximum is not taken per tile.  28 heads in 4 groups,
-// 32 rows, 65503 keys (30 GFLOP, 134 MB; 64 pieces): 45.6 us, 660 TFLOP/s; of them 5 until the
-// first rows are there, 30 for sixteen tiles (1.6 us a tile with few workgroups, 2.0 with 256)
-// and 8 for the partial results' way out.  The same with waves in step 49.7 us; masks in
-// the one loop 54.
+// the ring's slots as constants, the maximum is not taken per tile, and the next rows'
+// addresses are computed before the barrier.  28 heads in 4 groups, 32 rows, 65503 keys (30
+// GFLOP, 134 MB; 64 pieces): 43.4 us, 690 TFLOP/s; of them 5 until the first rows are there, 28
+// for sixteen tiles (1.45 us a tile with few workgroups, more with 256, which stream 3.7 TB/s)
+// and 8 for the partial results' way out.  Without the one after the other: addresses
+// behind the barrier 45.2, slots as variables 47.8, a maximum per tile 49.7, masks and waves
+// in step 54.
 constexpr int kBlockKeys = 64;
 constexpr int kBlockCols = 32;             // of a wave
 constexpr int kBlockWaves = 8;
@@ -859,9 +861,7 @@ __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256, 2)
     if (late && more) arrive(t + 1, after);
     __builtin_amdgcn_sched_barrier(0);
     if (active) {
-      __builtin_amdgcn_s_setprio(1);  // vector work first: the matrix unit is fed a tile at a time
       softmax();
-      __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
       outputs(off);
     }
