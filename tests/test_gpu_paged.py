@@ -552,6 +552,28 @@ def test_graphs_of_a_decode_step_replay_with_new_inputs():
                 assert torch.equal(vp[at[0], at[1]], v[b, 0])
 
 
+def test_long_tables_with_a_hole_past_their_first_entries():
+    # 130 pages of 16: a hole among the first 64 entries, past them, and none
+    for unmap in ([(0, 20, -1)], [(0, 100, -1)], [(0, 129, 7)], []):
+        for Lq in (1, 40):
+            args = _case(1, Lq, [2075], 8, 2, 128, 16, torch.bfloat16, seed=Lq, unmap=unmap)
+            for kw in (dict(parts=1), dict(parts=3, causal=True)):
+                _check(_run(*args, **kw), *args, **kw)
+
+
+def test_blocks_at_offsets_past_32_bits():
+    # 70 000 pages of 32768 values, as above, by more columns than a tile of tokens has
+    N, page, Hkv, D = 70000, 64, 4, 128
+    kp = torch.empty(N, page, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    vp = torch.empty(N, page, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    q, k, v, table, lens = _case(2, 40, [330, 190], 28, Hkv, D, page, torch.bfloat16, seed=9)
+    far = torch.where(table >= 0, N - 1 - table * 13, -1).int()
+    where = N - 1 - torch.arange(k.shape[0], device=DEV) * 13
+    kp[where], vp[where] = k.to(DEV), v.to(DEV)
+    for kw in (dict(), dict(causal=True, parts=2)):
+        _check(_run(q, kp, vp, far, lens, **kw), q, k, v, table, lens, **kw)
+
+
 def test_padding_queries_may_hold_anything():
     for Lq, n in ((2, 70), (40, 300), (200, 500)):
         q, k, v, table, lens = _case(2, Lq, [n, n - 30], 14, 2, 128, 16, torch.bfloat16, seed=Lq)
