@@ -26,6 +26,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMostThreads = 512;
 constexpr int kHeadsPerThread = 4;
+constexpr int kScalarHeads = 8;
 // Head units from which a thread takes that many.  Half as many units (512 rows of 32 heads):
 // 4.35 us, 3.86 by a head each; as many: 4.99 and 5.17; twice: 7.03 and 7.81.
 constexpr int64_t kManyUnits = 256 * 1024;
@@ -252,48 +253,59 @@ __global__ void __launch_bounds__(kMostThreads) rotary_kernel(RotaryArgs a) {
   }
 }
 
-// The same one value (a tail dim or a v dim) or pair at a time, for head parts
-// that 16-byte units do not divide and for unaligned tensors: units = half
-// pairs and D - 2 half tail dims.
+// The same one value (a tail dim) or pair at a time, for head parts that 16-byte
+// units do not divide and for unaligned tensors: units = half pairs and D - 2 half
+// tail dims, of kScalarHeads heads a thread.  Bound by the number of its loads and stores:
+// 16384 rows of 28 + 4 heads 63 us, 49 by 16-byte units (161 with a head a thread); 32 rows 4.7
+// and 4.1.
 template <class T, bool INTERLEAVED, bool PAGED>
 __global__ void __launch_bounds__(kThreads) rotary_scalar_kernel(RotaryArgs a) {
-  const int per_token = a.units * a.head_slots;  // head_slots = every head
+  const int per_token = a.units * a.head_slots;
+  const int total_heads = a.q.heads + a.k.heads + (PAGED ? a.v.heads : 0);
   for (int lid = threadIdx.x; lid < a.tokens_per_block * per_token; lid += kThreads) {
     const int ti = lid / per_token;
     const int64_t tok = (int64_t)blockIdx.x * a.tokens_per_block + ti;
     if (tok >= a.tokens) return;
     const int rem = lid - ti * per_token;
-    const int h = rem / a.units;
-    const int u = rem - h * a.units;
+    const int hs = rem / a.units;
+    const int u = rem - hs * a.units;
     const int b = (int)tok / a.L, l = (int)tok - b * a.L;
     const Rows<T, PAGED> rows(a, b, l);
-    const T* in;
-    T* out;
-    bool turned, there;
-    rows.head(a, h, in, out, turned, there);
-    if (!there) continue;
-    if (u >= a.half) {
-      const int at = u + a.half;
-      out[at] = in[at];
-      continue;
+    const bool pair = u < a.half;
+    const int i1 = !pair ? u + a.half : INTERLEAVED ? 2 * u : u;
+    const int i2 = !pair ? i1 : INTERLEAVED ? 2 * u + 1 : u + a.half;
+    T x1[kScalarHeads], x2[kScalarHeads];
+    T* out[kScalarHeads];
+    bool turned[kScalarHeads], there[kScalarHeads];
+#pragma unroll
+    for (int i = 0; i < kScalarHeads; ++i) {
+      const int h = hs + i * a.head_slots;
+      const T* in;
+      rows.head(a, min(h, total_heads - 1), in, out[i], turned[i], there[i]);
+      there[i] &= h < total_heads;
+      x1[i] = in[i1];
+      x2[i] = in[i2];
     }
-    const int i1 = INTERLEAVED ? 2 * u : u, i2 = INTERLEAVED ? 2 * u + 1 : u + a.half;
-    const T x1 = in[i1], x2 = in[i2];
-    if (!turned) {
-      out[i1] = x1;
-      out[i2] = x2;
-      continue;
-    }
-    const int64_t pos = a.positions ? a.positions[b * a.ps_b + l * a.ps_l] : l;
     float c = __builtin_nanf(""), s = c;
-    if (pos >= 0 && pos < a.table_rows) {
-      c = a.cos_t[pos * a.half + u];
-      s = a.sign * a.sin_t[pos * a.half + u];
+    if (pair) {
+      const int64_t pos = a.positions ? a.positions[b * a.ps_b + l * a.ps_l] : l;
+      if (pos >= 0 && pos < a.table_rows) {
+        c = a.cos_t[pos * a.half + u];
+        s = a.sign * a.sin_t[pos * a.half + u];
+      }
     }
-    float f1 = (float)x1, f2 = (float)x2;
-    turn_pair(f1, f2, c, s);
-    out[i1] = (T)f1;
-    out[i2] = (T)f2;
+#pragma unroll
+    for (int i = 0; i < kScalarHeads; ++i) {
+      if (!there[i]) continue;
+      if (pair && turned[i]) {
+        float f1 = (float)x1[i], f2 = (float)x2[i];
+        turn_pair(f1, f2, c, s);
+        x1[i] = (T)f1;
+        x2[i] = (T)f2;
+      }
+      out[i][i1] = x1[i];
+      if (pair) out[i][i2] = x2[i];
+    }
   }
 }
 
@@ -321,7 +333,7 @@ int launch(RotaryArgs a, bool interleaved, hipStream_t stream) {
     a.head_slots = (heads + heads_each - 1) / heads_each;
   } else {
     a.units = a.D - a.half;
-    a.head_slots = heads;
+    a.head_slots = (heads + kScalarHeads - 1) / kScalarHeads;
   }
   const int per_token = a.units * a.head_slots;
   a.tokens_per_block = std::max(1, kThreads / per_token);
