@@ -347,6 +347,10 @@ int launch(RotaryArgs a, bool interleaved, hipStream_t stream) {
       const int idle = 64 * (whole - t * per_token) / whole;
       if (whole >= kThreads && idle < waste) waste = idle, a.tokens_per_block = t, threads = whole;
     }
+    if (per_token > kMostThreads) {  // a token takes several even rounds
+      const int rounds = (per_token + kMostThreads - 1) / kMostThreads;
+      threads = ((per_token + rounds - 1) / rounds + 63) / 64 * 64;
+    }
   }
   const int64_t blocks = ((int64_t)a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
   if (blocks > 0xffffffffll / threads) return MRSA_ERR_UNSUPPORTED;  // (threads of a launch)
