@@ -459,9 +459,9 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedArgs a)
 // DMA into a ring, a tile ahead, one barrier per tile; K is read along the row
 // (operand A of S^T), V by transposing reads (operand A of O^T).
 //
-// Bound by vector issue: a wave's tile is 64 matrix instructions and about 200 vector ones
-// (16 exponentials a lane and column tile, the sums, the packing), and two waves share a
-// SIMD.  So the two go half a tile apart (the softmax of one runs beside the products of the
+// Bound by issue and, with all CUs at work, by HBM: a wave's tile is 64 matrix instructions and
+// about 130 vector ones (32 exponentials, their arguments, the sums, the packing), and two
+// waves share a SIMD.  So the two go half a tile apart (the softmax of one runs beside the products of the
 // other), tiles that every column sees whole have a loop of their own without masks, with
 // the ring's slots as constants, the maximum is not taken per tile, and the next rows'
 // addresses are computed before the barrier.  28 heads in 4 groups, 32 rows, 65503 keys (30
