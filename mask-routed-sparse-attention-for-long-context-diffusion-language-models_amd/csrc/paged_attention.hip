@@ -1119,7 +1119,8 @@ extern "C" int mrsa_paged_attention_fwd(
       span_bound(max_len, q_len, a.G, a.tile_cols, a.window, a.causal, !query_starts) +
       (a.window >= 0 ? kTile - 1 : 0);  // (a window's first tile may start before it)
   const int64_t step = a.tile_cols == 16 ? kStep : kBlockKeys;
-  a.part_keys = (int)(((span + parts - 1) / parts + step - 1) / step * step);
+  // (at least one step: without keys, max_len 0, the join still divides by it)
+  a.part_keys = (int)((std::max<int64_t>(1, (span + parts - 1) / parts) + step - 1) / step * step);
   a.out = (uint16_t*)out;
   a.lse = lse;
   a.part_out = (float*)workspace;
