@@ -938,7 +938,8 @@ int mrsa_rotary_fwd(const void* q, int64_t q_batch_stride, int64_t q_row_stride,
  *   q, k, v, tables, positions: as in mrsa_rotary_fwd
  *   slots: int64 [batch, seq_len] with strides; two rows of one call must not
  *     name the same cache row (either's units remain)
- *   page_table: int32 [batch, table_pages], row stride page_table_stride
+ *   page_table: int32 [batch, table_pages], row stride page_table_stride (read for every
+ *     row, also with 0 KV heads; NULL only if table_pages or num_pages is 0)
  *   k_pages, v_pages (in/out): [num_pages, page_size, kv_heads, head_dim] in
  *     any order given by page, slot and head strides, dense last dim
  * Limits: page_size a power of two up to 2^20, as mrsa_rotary_fwd otherwise.

@@ -451,8 +451,9 @@ extern "C" int mrsa_paged_append_fwd(
   if (batch * seq_len == 0 || q_heads + kv_heads == 0) return MRSA_OK;
   if ((q_heads && (!q || !q_out)) || !slots) return MRSA_ERR_INVALID_ARGUMENT;
   if (kv_heads && (!k || !v)) return MRSA_ERR_INVALID_ARGUMENT;
-  if (kv_heads && table_pages && num_pages &&
-      (!page_table || !k_pages || !v_pages || k_pages == v_pages))
+  // (the table is read for every row, also where there are no KV heads to place)
+  if (table_pages && num_pages &&
+      (!page_table || (kv_heads && (!k_pages || !v_pages || k_pages == v_pages))))
     return MRSA_ERR_INVALID_ARGUMENT;
   if (rotary_dim && table_rows && (!cos_table || !sin_table)) return MRSA_ERR_INVALID_ARGUMENT;
   RotaryArgs a = {};
