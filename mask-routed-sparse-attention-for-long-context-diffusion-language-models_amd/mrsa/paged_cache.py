@@ -70,6 +70,16 @@ def _no_gradient(name: str, *tensors) -> None:
             raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
 
 
+def _written(*pools) -> None:
+    """Raise the version counters of pools that a kernel has written, as torch's own in-place
+    operators do: backward passes that saved them and ``kv_fragments_cached`` go by it.
+    (Tensors made in inference mode have none.)"""
+
+    for t in pools:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _paged_append_impl(k, v, k_pages, v_pages, page_table, slots, q, cos, sin, positions,
                        interleaved):
     B, L, Hkv, D = k.shape
@@ -102,6 +112,7 @@ def _paged_append_impl(k, v, k_pages, v_pages, page_table, slots, q, cos, sin, p
         k_pages.data_ptr(), kps, kss, khs, v_pages.data_ptr(), vps, vss, vhs, B, L, Hq, Hkv, D,
         2 * half, DTYPES[k.dtype], interleaved, q_out.data_ptr(), _lib.stream_of(k))
     _lib.check(status, "paged_cache_append")
+    _written(k_pages, v_pages)
     return q_out
 
 
@@ -321,6 +332,7 @@ def _copy_pages_impl(k_pages, v_pages, src, dst):
         shape[2] * shape[3] * shape[4] * size, n, ctypes.addressof(arrays[0]),
         ctypes.addressof(arrays[1]), _lib.stream_of(k_pages))
     _lib.check(status, "copy_cache_pages")
+    _written(k_pages, v_pages)
 
 
 def copy_cache_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: Sequence[int],

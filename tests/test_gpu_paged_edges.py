@@ -20,3 +20,27 @@ def test_no_keys_in_several_parts():
             for parts in (1, 2, 7, 1024):
                 out, lse = _run(q, pool, v[:pool.shape[0]], t, n, parts=parts, **kw)
                 assert not out.any() and bool((lse == float("-inf")).all())
+
+
+def test_a_view_of_the_pool_is_laid_out_again_after_a_write():
+    # a sequence whose pages follow each other, read by a dense operator through a view
+    g = torch.Generator().manual_seed(30)
+    kp, vp = torch.randn(2, 6, 32, 2, 128, generator=g).bfloat16().to(DEV)
+    k, v = kp[:4].view(1, 128, 2, 128), vp[:4].view(1, 128, 2, 128)
+    q = torch.randn(1, 128, 4, 128, generator=g).bfloat16().to(DEV)
+    table = torch.arange(4, dtype=torch.int32, device=DEV)[None]
+    valid = torch.ones(1, 128, dtype=torch.bool, device=DEV)
+
+    def check():
+        got = mrsa.bidir_local_attention(q, k, v, valid, 64, 64)
+        want = mrsa.bidir_local_attention(q, k.clone(), v.clone(), valid, 64, 64)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        return got[0]
+
+    first = check()
+    new = torch.randn(2, 1, 50, 2, 128, generator=g).bfloat16().to(DEV)
+    mrsa.paged_cache_append(new[0], new[1], kp, vp, table, torch.arange(60, 110, device=DEV)[None])
+    second = check()
+    mrsa.copy_cache_pages(kp, vp, [0, 5], [3, 1])
+    third = check()
+    assert not torch.equal(first, second) and not torch.equal(second, third)
