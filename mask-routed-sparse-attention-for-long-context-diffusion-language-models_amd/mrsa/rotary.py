@@ -11,6 +11,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -158,14 +159,51 @@ class _Rotary(torch.autograd.Function):
             grad_q = None
         if not ctx.needs_input_grad[1]:
             grad_k = None
-        turn = _Rotary.apply if torch.is_grad_enabled() else _turn
         args = (cos, sin, positions, ctx.interleaved, not ctx.inverse)
         dq = dk = None
         if grad_q is not None:
-            dq, dk = turn(grad_q, grad_k, *args)
+            dq, dk = _rotate(grad_q, grad_k, *args)
         elif grad_k is not None:
-            dk, _ = turn(grad_k, None, *args)
+            dk, _ = _rotate(grad_k, None, *args)
         return dq, None if grad_k is None else dk, None, None, None, None, None
+
+
+class _RotaryTransformed(_Rotary):
+    # The form for forward-mode derivatives and torch.func's transforms (a call of it takes
+    # longer, hence two forms): the derivative along a tangent is the tangent, turned.
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(q, k, cos, sin, positions, interleaved, inverse):
+        return _turn(q, k, cos, sin, positions, interleaved, inverse)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        q, k, cos, sin, positions, ctx.interleaved, ctx.inverse = inputs
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.save_for_forward(cos, sin, positions)
+        ctx.q_shape, ctx.k_shape = q.shape, output[1].shape
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def jvp(ctx, q_tangent, k_tangent, *_):
+        args = (*ctx.saved_tensors, ctx.interleaved, ctx.inverse)
+        if q_tangent is None:
+            return k_tangent.new_zeros(ctx.q_shape), _rotate(k_tangent, None, *args)[0]
+        dq, dk = _rotate(q_tangent, k_tangent, *args)
+        return dq, dk if k_tangent is not None else dk.new_zeros(ctx.k_shape)
+
+
+def _rotate(q, k, *args):
+    """The operator, recorded where a derivative of it may be asked for."""
+
+    if forward_ad._current_level >= 0:   # (of dual tensors and of torch.func.jvp)
+        return _RotaryTransformed.apply(q, k, *args)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if torch._C._are_functorch_transforms_active():
+            return _RotaryTransformed.apply(q, k, *args)
+        return _Rotary.apply(q, k, *args)
+    return _turn(q, k, *args)
 
 
 def check_heads(t, name: str) -> None:
@@ -180,7 +218,9 @@ def check_heads(t, name: str) -> None:
 def rotary_qk(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
               positions: Optional[torch.Tensor] = None, *, interleaved: bool = False
               ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """Query and key heads turned by their positions; differentiable in q and k.
+    """Query and key heads turned by their positions; differentiable in q and k (reverse and
+    forward mode, and under torch.func's transforms; what torch.compile has traced knows
+    only reverse mode).
 
     q [B, L, Hq, D] and k [B, L, Hkv, D] (or None) in bf16, fp16 or fp32, any
     strides; cos, sin fp32 [rows, R / 2] (``rotary_tables``), R <= D: the first R dims
@@ -206,8 +246,5 @@ def rotary_qk(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin
         positions = check_token_ints(positions, "positions", B, L, q.device)
     elif L > cos.shape[0]:
         raise ValueError(f"tables of {cos.shape[0]} rows do not reach {L} positions")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        q_out, k_out = _Rotary.apply(q, k, cos, sin, positions, bool(interleaved), False)
-    else:
-        q_out, k_out = _turn(q, k, cos, sin, positions, bool(interleaved), False)
+    q_out, k_out = _rotate(q, k, cos, sin, positions, bool(interleaved), False)
     return q_out, None if k is None else k_out

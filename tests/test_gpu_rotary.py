@@ -242,3 +242,22 @@ def test_a_captured_backward_pass():
         want = step()
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_forward_mode(dtype):
+    from torch.autograd import forward_ad
+
+    g = torch.Generator().manual_seed(10)
+    cos, sin = (t.to(DEV) for t in _tables(16, 32))
+    q, tq = torch.randn(2, 2, 9, 6, 64, generator=g).to(dtype).to(DEV)
+    k, tk = torch.randn(2, 2, 9, 2, 64, generator=g).to(dtype).to(DEV)
+    want = mrsa.rotary_qk(tq, tk, cos, sin, interleaved=True)
+    with forward_ad.dual_level():
+        out = mrsa.rotary_qk(forward_ad.make_dual(q, tq), forward_ad.make_dual(k, tk), cos, sin,
+                             interleaved=True)
+        got = [forward_ad.unpack_dual(t).tangent for t in out]
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    _, got = torch.func.jvp(lambda a, b: mrsa.rotary_qk(a, b, cos, sin, interleaved=True), (q, k),
+                            (tq, tk))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -1,8 +1,12 @@
 """The paged operators and rotary_qk at their edges, without a GPU: what the C entry points
 refuse, and what the operators' own Python code does around a kernel (a stand-in here)."""
 
+import ctypes
+
+import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import mrsa
 from mrsa import _lib, paged_cache, rotary
@@ -16,15 +20,39 @@ def test_c_append_without_kv_heads_still_needs_its_table():
     assert status == _lib.MRSA_ERR_INVALID_ARGUMENT
 
 
+def _plain_rotary(q, qb, ql, qh, k, kb, kl, kh, cos, sin, rows, pos, pb, pl, B, L, Hq, Hkv, D, R,
+                  dtype, interleaved, inverse, q_out, k_out, stream):
+    """mrsa_rotary_fwd of fp32 host memory (half layout, every position given by its row)."""
+
+    def array(at, shape, strides):
+        size = 1 + sum((n - 1) * s for n, s in zip(shape, strides))
+        flat = np.ctypeslib.as_array((ctypes.c_float * size).from_address(at))
+        return np.lib.stride_tricks.as_strided(flat, shape, [4 * s for s in strides])
+
+    assert dtype == 2 and not interleaved and pos is None
+    h = R // 2
+    c = array(cos, (L, h), (h, 1))[:, None]
+    s = array(sin, (L, h), (h, 1))[:, None] * (-1 if inverse else 1)
+    for x, sb, sl, sh, H, y in ((q, qb, ql, qh, Hq, q_out), (k, kb, kl, kh, Hkv, k_out)):
+        if H:
+            x = array(x, (B, L, H, D), (sb, sl, sh, 1))
+            y = array(y, (B, L, H, D), (L * H * D, H * D, D, 1))
+            y[:] = x
+            y[..., :h] = x[..., :h] * c - x[..., h:R] * s
+            y[..., h:R] = x[..., h:R] * c + x[..., :h] * s
+
+
 @pytest.fixture
 def cpu_ops(monkeypatch):
     """The operators' own code on CPU tensors, with a stand-in for the library: what it was
-    called with is kept, nothing is computed."""
+    called with is kept, and of the kernels only the rotation is computed."""
 
     calls = []
 
     def call_on(device, name, *args):
         calls.append(name)
+        if name == "mrsa_rotary_fwd":
+            _plain_rotary(*args)
         return _lib.MRSA_OK
 
     monkeypatch.setattr(_lib, "call_on", call_on)
@@ -32,6 +60,7 @@ def cpu_ops(monkeypatch):
     monkeypatch.setattr(paged_cache, "check_heads", lambda t, name: None)
     monkeypatch.setattr(rotary, "check_heads", lambda t, name: None)
     lib = torch.library.Library("mrsa", "IMPL")
+    lib.impl("rotary", rotary._rotary_impl, "CPU")
     lib.impl("paged_append_", paged_cache._paged_append_impl, "CPU")
     lib.impl("paged_attention", paged_cache._paged_attention_impl, "CPU")
     lib.impl("copy_pages_", paged_cache._copy_pages_impl, "CPU")
@@ -71,3 +100,77 @@ def test_in_place_operators_raise_the_pools_version_counters(cpu_ops):
     torch.ops.mrsa.copy_pages_(kp, vp, [0], [1])
     assert cpu_ops == ["mrsa_paged_append_fwd", "mrsa_copy_pages",
                        "mrsa_paged_append_fwd", "mrsa_paged_append_fwd", "mrsa_copy_pages"]
+
+
+def _rope(seed=0):
+    g = torch.Generator().manual_seed(seed)
+    q, tq, gq = torch.randn(3, 2, 5, 3, 8, generator=g)
+    k, tk, gk = torch.randn(3, 2, 5, 1, 8, generator=g)
+    cos, sin = mrsa.rotary_tables(9, mrsa.rotary_frequencies(6)[0], device="cpu")
+    return q, k, tq, tk, gq, gk, lambda q, k: mrsa.rotary_qk(q, k, cos, sin)
+
+
+def test_rotary_forward_mode(cpu_ops):
+    # the rotation is linear: its derivative along a tangent is the tangent, turned
+    q, k, tq, tk, gq, gk, f = _rope()
+    want_q, want_k = f(tq, tk)
+    assert not torch.equal(want_q, tq)
+
+    def tangents(a, b):
+        with forward_ad.dual_level():
+            return [forward_ad.unpack_dual(t).tangent
+                    for t in f(*(forward_ad.make_dual(x, t) if t is not None else x
+                                 for x, t in ((q, a), (k, b))))]
+
+    for grads in (False, True):          # (no_grad leaves forward mode on)
+        with torch.set_grad_enabled(grads):
+            got = tangents(tq, tk)
+            assert torch.equal(got[0], want_q) and torch.equal(got[1], want_k)
+            got = tangents(tq, None)
+            assert torch.equal(got[0], want_q) and not got[1].any()
+            got = tangents(None, tk)
+            assert not got[0].any() and torch.equal(got[1], want_k)
+            with forward_ad.dual_level():
+                out = f(forward_ad.make_dual(q, tq), None)[0]
+                assert torch.equal(forward_ad.unpack_dual(out).tangent, want_q)
+                out = f(q, k)            # nothing dual in a dual level
+                assert torch.equal(out[0], f(q, k)[0])
+    # forward over reverse: the gradient of sum(f(q)^2) / 2 is f'(f(q)), its derivative along t
+    # f'(f(t)) = t, off by two rotations, each by at most 3 x 2^-24 (|x1| + |x2|), of values up to 4
+    x = q.clone().requires_grad_()
+    with forward_ad.dual_level():
+        y = f(forward_ad.make_dual(x, tq), None)[0]
+        dx, = torch.autograd.grad((y * y).sum() / 2, x)
+        assert (forward_ad.unpack_dual(dx).tangent - tq).abs().max() <= 2 * 3 * 8 * 2.0 ** -24
+
+
+@pytest.mark.filterwarnings("ignore:There is a performance drop")
+def test_rotary_under_function_transforms(cpu_ops):
+    q, k, tq, tk, gq, gk, f = _rope(1)
+    want = f(tq, tk)
+    out, got = torch.func.jvp(f, (q, k), (tq, tk))
+    assert all(torch.equal(a, b) for a, b in zip((*out, *got), (*f(q, k), *want)))
+    x, y = q.clone().requires_grad_(), k.clone().requires_grad_()
+    grads = torch.autograd.grad(f(x, y), (x, y), (gq, gk))
+    got = torch.func.grad(lambda a, b: sum((o * w).sum() for o, w in zip(f(a, b), (gq, gk))),
+                          argnums=(0, 1))(q, k)
+    assert all(torch.equal(a, b) for a, b in zip(got, grads))
+    got = torch.func.vjp(f, q, k)[1]((gq, gk))
+    assert all(torch.equal(a, b) for a, b in zip(got, grads))
+    two, tangents = torch.stack((q, gq)), torch.stack((tq, q))
+    one = lambda a, t: torch.func.jvp(lambda x: f(x, None)[0], (a,), (t,))[1]  # noqa: E731
+    got = torch.func.vmap(one)(two, tangents)
+    assert torch.equal(got, torch.stack([f(t, None)[0] for t in tangents]))
+    got = torch.func.vmap(torch.func.grad(lambda a: f(a, None)[0].square().sum() / 2))(two)
+    assert (got - two).abs().max() <= 2 * 3 * 8 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_rotary_and_its_gradient_trace_without_a_graph_break(cpu_ops, backend):
+    q, k, tq, tk, gq, gk, f = _rope(2)
+    compiled = torch.compile(f, backend=backend, fullgraph=True)
+    assert all(torch.equal(a, b) for a, b in zip(compiled(q, k), f(q, k)))
+    x, y = q.clone().requires_grad_(), k.clone().requires_grad_()
+    want = torch.autograd.grad(f(x, y), (x, y), (gq, gk))
+    got = torch.autograd.grad(compiled(x, y), (x, y), (gq, gk))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
