@@ -10,6 +10,8 @@ s % page_size of page table[s // page_size].
     copy_cache_pages        pages copied inside the pool, all layers at once
     PagedKVCache            the host's book-keeping: add, extend, fork (pages shared until
                             written), truncate, free, compact
+
+The operators have no derivative and refuse tensors that ask for one.
 """
 
 from __future__ import annotations
@@ -21,6 +23,7 @@ from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .rotary import DTYPES, check_heads, check_tables, check_token_ints, dense_rows
@@ -65,9 +68,17 @@ def _check_table(page_table, batch: int, device) -> torch.Tensor:
 
 
 def _no_gradient(name: str, *tensors) -> None:
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
+    """Refuse tensors whose derivative a caller would wait for in vain, in either mode."""
+
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:   # (of dual tensors and of torch.func.jvp)
+        wrapped = torch._C._functorch.is_functorch_wrapped_tensor
+        for t in tensors:
+            if t is not None and (wrapped(t) or forward_ad.unpack_dual(t).tangent is not None):
+                raise ValueError(f"{name} has no forward-mode derivative")
 
 
 def _written(*pools) -> None:
@@ -162,8 +173,7 @@ def paged_cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
                                                                      k.device)
     elif positions is not None:
         raise ValueError("positions need cos and sin")
-    if torch.is_grad_enabled():
-        _no_gradient("paged_cache_append", q, k, v, k_pages, v_pages)
+    _no_gradient("paged_cache_append", q, k, v, k_pages, v_pages)
     q_out = torch.ops.mrsa.paged_append_.default(k, v, k_pages, v_pages, page_table, slots, q, cos,
                                                  sin, positions, bool(interleaved))
     return None if q is None else q_out
@@ -308,8 +318,7 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     max_len = min(int(max_len), rows)
     if sm_scale is None:
         sm_scale = D ** -0.5
-    if torch.is_grad_enabled():
-        _no_gradient("paged_cached_attention", q, k_pages, v_pages)
+    _no_gradient("paged_cached_attention", q, k_pages, v_pages)
     window = -1 if window is None else int(window)
     if parts is not None and not 1 <= parts <= MAX_PARTS:
         raise ValueError(f"parts must be in [1, {MAX_PARTS}], got {parts}")
@@ -359,6 +368,7 @@ def copy_cache_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: Sequence
     src, dst = [int(i) for i in src], [int(i) for i in dst]
     if len(src) != len(dst):
         raise ValueError(f"{len(src)} sources for {len(dst)} destinations")
+    _no_gradient("copy_cache_pages", k_pages, v_pages)
     torch.ops.mrsa.copy_pages_.default(k_pages, v_pages, src, dst)
 
 

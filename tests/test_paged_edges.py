@@ -6,6 +6,7 @@ import ctypes
 import numpy as np
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
 
 import mrsa
@@ -100,6 +101,61 @@ def test_in_place_operators_raise_the_pools_version_counters(cpu_ops):
     torch.ops.mrsa.copy_pages_(kp, vp, [0], [1])
     assert cpu_ops == ["mrsa_paged_append_fwd", "mrsa_copy_pages",
                        "mrsa_paged_append_fwd", "mrsa_paged_append_fwd", "mrsa_copy_pages"]
+
+
+def _paged_calls():
+    """Append and attention as functions of one of their float tensors, and that tensor."""
+
+    kp, vp = _pools(dtype=torch.bfloat16)
+    k = torch.zeros(1, 3, 2, 64, dtype=torch.bfloat16)
+    table, slots = torch.zeros(1, 5, dtype=torch.int32), torch.arange(3)[None]
+    lens = torch.tensor([3], dtype=torch.int32)
+    append = lambda **kw: mrsa.paged_cache_append(  # noqa: E731
+        **{**dict(k=k, v=k, k_pages=kp[0], v_pages=vp[0], page_table=table, slots=slots, q=k), **kw})
+    attend = lambda **kw: mrsa.paged_cached_attention(  # noqa: E731
+        **{**dict(q=k, k_pages=kp[0], v_pages=vp[0], page_table=table, cache_lens=lens), **kw})
+    for name in ("q", "k", "v"):
+        yield (lambda t, name=name: append(**{name: t})), k
+    for name in ("k_pages", "v_pages"):
+        yield (lambda t, name=name: append(**{name: t})), kp[0]
+        yield (lambda t, name=name: attend(**{name: t})), kp[0]
+    yield (lambda t: attend(q=t)), k
+
+
+@pytest.mark.parametrize("i", range(8))
+def test_paged_operators_refuse_what_they_have_no_derivative_of(cpu_ops, i):
+    call, t = list(_paged_calls())[i]
+    call(t)
+    with pytest.raises(ValueError, match="no gradient"):
+        call(t.clone().requires_grad_())
+    with torch.no_grad():
+        call(t.clone().requires_grad_())
+    n = len(cpu_ops)
+    for grads in (False, True):          # (no_grad leaves forward mode on)
+        with torch.set_grad_enabled(grads):
+            with forward_ad.dual_level():
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call(forward_ad.make_dual(t, torch.ones_like(t)))
+            with pytest.raises(ValueError, match="forward-mode"):
+                torch.func.jvp(call, (t,), (torch.ones_like(t),))
+            assert len(cpu_ops) == n
+            with forward_ad.dual_level():
+                call(t)              # nothing dual
+            n = len(cpu_ops)
+
+
+def test_page_copies_refuse_what_they_have_no_derivative_of():
+    with FakeTensorMode():
+        kp, vp = _pools(device="cuda")
+        for call, t in ((lambda t: mrsa.copy_cache_pages(t, vp, [0], [1]), kp),
+                        (lambda t: mrsa.copy_cache_pages(kp, t, [0], [1]), vp)):
+            call(t)
+            with pytest.raises(ValueError, match="no gradient"):
+                call(t.clone().requires_grad_())
+            with torch.no_grad():
+                call(t.clone().requires_grad_())
+            with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+                call(forward_ad.make_dual(t, torch.ones_like(t)))
 
 
 def _rope(seed=0):
