@@ -44,3 +44,32 @@ def test_a_view_of_the_pool_is_laid_out_again_after_a_write():
     mrsa.copy_cache_pages(kp, vp, [0, 5], [3, 1])
     third = check()
     assert not torch.equal(first, second) and not torch.equal(second, third)
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_a_traced_step_writes_the_pools_it_was_given(backend):
+    g = torch.Generator().manual_seed(31)
+    args = [t.to(DEV) for t in _case(2, 3, [50, 20], 8, 2, 64, 16, torch.bfloat16, seed=12,
+                                     poison=False)]
+    k, v = torch.randn(2, 2, 3, 2, 64, generator=g).bfloat16().to(DEV)
+    slots = torch.tensor([[47, 48, 49], [17, 18, 19]], device=DEV)
+    cos, sin = mrsa.rotary_tables(90, mrsa.rotary_frequencies(64)[0], device=DEV)
+    table = args[3]
+    src, dst = [int(table[0, 0])], [int(table[1, 0])]
+
+    def step(q, kp, vp, table, lens):
+        before = mrsa.paged_cached_attention(q, kp, vp, table, lens)
+        rq = mrsa.paged_cache_append(k, v, kp, vp, table, slots, q=q, cos=cos, sin=sin)
+        mid = mrsa.paged_cached_attention(rq, kp, vp, table, lens)
+        mrsa.copy_cache_pages(kp, vp, src, dst)
+        return *before, rq, *mid, *mrsa.paged_cached_attention(rq, kp, vp, table, lens)
+
+    mine, theirs = ([t.clone() for t in args] for _ in range(2))
+    want = step(*mine)
+    traced = torch.compile(step, backend=backend, fullgraph=True)
+    versions = theirs[1]._version, theirs[2]._version
+    got = traced(*theirs)
+    for a, b in zip((*got, *theirs), (*want, *mine)):
+        assert torch.equal(a, b)
+    assert not torch.equal(theirs[1], args[1]) and not torch.equal(want[0], want[3])
+    assert theirs[1]._version > versions[0] and theirs[2]._version > versions[1]
