@@ -291,7 +291,7 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     Padding, and a row that sees no key, give out = 0 and lse = -inf.
 
     max_len: a bound of cache_lens that the caller knows (None: the table's rows; lengths
-    past it are cut to it); it sizes the launch.  parts: pieces the span is cut into,
+    past it are cut to it); it sizes the launch, and a captured call keeps it.  parts: pieces the span is cut into,
     None picks them.  Returns out [B, Lq, Hq, D] in q's dtype and lse fp32 [B, Lq, Hq].
     """
 
@@ -571,10 +571,15 @@ class PagedKVCache:
         return live
 
     # ---- the operators
-    def batch(self, seqs: Sequence[int], rows=1) -> PagedBatch:
+    def batch(self, seqs: Sequence[int], rows=1, *, max_len: Optional[int] = None) -> PagedBatch:
         """What the operators need of some sequences, in one upload.  ``rows``: how many of
         each sequence's newest rows the call brings, one number or one per sequence; rows
-        of shorter ones are padding behind theirs."""
+        of shorter ones are padding behind theirs.
+
+        ``max_len``: a length that no sequence passes while this batch is in use (None: the
+        longest one's now).  It is the table's width and attention's bound, both of which a
+        captured graph keeps: capture with a max_len that covers every replay, then copy the
+        tensors of ``batch(seqs, rows, max_len=...)`` into the captured batch's before each."""
 
         seqs = tuple(int(s) for s in seqs)
         if len(set(seqs)) != len(seqs):
@@ -587,7 +592,12 @@ class PagedKVCache:
             if not 0 <= r <= s.length:
                 raise ValueError(f"rows must be in [0, {s.length}], got {r}")
         B, L = len(held), max(counts, default=0)
-        width = max((len(s.pages) for s in held), default=0)
+        longest = max((s.length for s in held), default=0)
+        if max_len is None:
+            max_len = longest
+        elif max_len < longest:
+            raise ValueError(f"max_len must be at least {longest}, got {max_len}")
+        width = -(-max_len // self.page_size)
         starts = [s.length - r for s, r in zip(held, counts)]
         row = torch.arange(L)
         positions = torch.tensor(starts, dtype=torch.long).view(B, 1) + row
@@ -607,7 +617,7 @@ class PagedKVCache:
             cache_lens=ints[B * width:B * width + B], query_starts=ints[B * width + B:],
             slots=dev[:8 * B * L].view(torch.long).view(B, L),
             positions=dev[8 * B * L:16 * B * L].view(torch.long).view(B, L),
-            max_len=max((s.length for s in held), default=0), version=self.version)
+            max_len=int(max_len), version=self.version)
 
     def _current(self, batch: PagedBatch) -> None:
         if batch.version != self.version:
@@ -629,12 +639,17 @@ class PagedKVCache:
         return paged_cache_append(k, v, self.k_pages[layer], self.v_pages[layer],
                                   batch.page_table, batch.slots, **rotary)
 
-    def attend(self, layer: int, batch: PagedBatch, q: torch.Tensor, **options):
+    def attend(self, layer: int, batch: PagedBatch, q: torch.Tensor, *,
+               max_len: Optional[int] = None, **options):
         """``paged_cached_attention`` of the batch's newest rows against a layer's pages;
-        keywords causal, window, sm_scale and parts as there."""
+        keywords causal, window, sm_scale and parts as there.  max_len: a larger bound of the
+        lengths than the batch's (a captured call keeps its bound, parts and table width)."""
 
         self._current(batch)
+        if max_len is None:
+            max_len = batch.max_len
+        elif max_len < batch.max_len:
+            raise ValueError(f"max_len must be at least the batch's, {batch.max_len}, got {max_len}")
         return paged_cached_attention(q, self.k_pages[layer], self.v_pages[layer],
                                       batch.page_table, batch.cache_lens,
-                                      query_starts=batch.query_starts, max_len=batch.max_len,
-                                      **options)
+                                      query_starts=batch.query_starts, max_len=max_len, **options)

@@ -73,3 +73,49 @@ def test_a_traced_step_writes_the_pools_it_was_given(backend):
         assert torch.equal(a, b)
     assert not torch.equal(theirs[1], args[1]) and not torch.equal(want[0], want[3])
     assert theirs[1]._version > versions[0] and theirs[2]._version > versions[1]
+
+
+def test_a_captured_step_of_the_cache_serves_sequences_that_grow():
+    # captured at 20 and 7 rows, replayed up to 170 and 157: the bound and the table's width
+    # are the capture's, everything else is read anew
+    Hq, Hkv, D, page, L, most = 14, 2, 128, 16, 5, 200
+    g = torch.Generator().manual_seed(32)
+    c = mrsa.PagedKVCache(1, 30, page, Hkv, D, device=DEV)
+    c.k_pages.fill_(float("nan")), c.v_pages.fill_(float("nan"))
+    cos, sin = mrsa.rotary_tables(most, mrsa.rotary_frequencies(D)[0], device=DEV)
+    seqs = [c.add(20), c.add(7)]
+    rows = torch.randn(2, 2, 20, Hkv, D, generator=g).bfloat16().to(DEV)
+    c.append(0, c.batch(seqs, rows=[20, 7]), rows[0], rows[1], cos=cos, sin=sin)
+    q = torch.zeros(2, L, Hq, D, dtype=torch.bfloat16, device=DEV)
+    k, v = torch.zeros(2, 2, L, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    held = c.batch(seqs, rows=L, max_len=most)
+
+    def step():
+        rq = c.append(0, held, k, v, q=q, cos=cos, sin=sin)
+        return (rq, *c.attend(0, held, rq, causal=True))
+
+    saved = c.k_pages.clone(), c.v_pages.clone()
+    step()                                             # (once outside, as torch asks)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    c.k_pages.copy_(saved[0]), c.v_pages.copy_(saved[1])
+    for i in range(30):
+        for s in seqs:
+            c.extend(s, L)
+        now = c.batch(seqs, rows=L, max_len=most)
+        for name in ("page_table", "cache_lens", "query_starts", "slots", "positions"):
+            getattr(held, name).copy_(getattr(now, name))
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=g))
+        graph.replay()
+        got = [t.clone() for t in out]
+        exact = c.batch(seqs, rows=L)                  # no wider than needed
+        rq = c.append(0, exact, k, v, q=q, cos=cos, sin=sin)
+        torch.cuda.synchronize()
+        assert torch.equal(rq, got[0])
+        if i % 7 == 0 or i > 27:
+            _check(got[1:], rq.cpu(), c.k_pages[0].cpu(), c.v_pages[0].cpu(),
+                   now.page_table.cpu(), now.cache_lens.cpu(), causal=True)
+        assert bool(torch.isfinite(got[2]).all())
+    assert c.length(seqs[0]) == 170

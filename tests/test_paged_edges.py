@@ -103,6 +103,33 @@ def test_in_place_operators_raise_the_pools_version_counters(cpu_ops):
                        "mrsa_paged_append_fwd", "mrsa_paged_append_fwd", "mrsa_copy_pages"]
 
 
+def test_batches_and_attention_with_room_to_grow(cpu_ops, monkeypatch):
+    c = mrsa.PagedKVCache(1, 12, 16, 2, 64, device="cpu")
+    a, b = c.add(20), c.add(3)
+    now, room = c.batch([a, b]), c.batch([a, b], max_len=70)
+    assert now.max_len == 20 and now.page_table.shape == (2, 2)
+    assert room.max_len == 70 and room.page_table.shape == (2, 5)
+    assert room.page_table.tolist() == [c.pages(a) + [-1] * 3, c.pages(b) + [-1] * 4]
+    for x, y in ((room.slots, now.slots), (room.cache_lens, now.cache_lens),
+                 (room.positions, now.positions), (room.query_starts, now.query_starts)):
+        assert torch.equal(x, y)
+    c.batch([a, b], max_len=20)
+    c.batch([], max_len=0)
+    for bad in (19, 0, -1):
+        with pytest.raises(ValueError, match="max_len"):
+            c.batch([a, b], max_len=bad)
+    seen = []
+    monkeypatch.setattr(paged_cache, "paged_cached_attention",
+                        lambda *args, **kw: seen.append(kw["max_len"]))
+    q = torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16)
+    c.attend(0, now, q)
+    c.attend(0, room, q, causal=True)
+    c.attend(0, now, q, max_len=500, parts=2)
+    assert seen == [20, 70, 500]
+    with pytest.raises(ValueError, match="max_len"):
+        c.attend(0, room, q, max_len=69)
+
+
 def _paged_calls():
     """Append and attention as functions of one of their float tensors, and that tensor."""
 
