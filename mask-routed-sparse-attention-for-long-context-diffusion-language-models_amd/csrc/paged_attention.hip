@@ -1050,7 +1050,7 @@ extern "C" int64_t mrsa_paged_attention_workspace_bytes(int64_t batch, int64_t q
       q_len > most || q_heads > 65536 || head_dim > 4096 || parts > kMaxParts)
     return -1;
   if (parts == 1 || batch == 0 || q_len == 0) return 0;
-  if (q_len > (1ll << 40) / batch / q_heads) return -1;
+  if (q_len > (1ll << 38) / batch / q_heads) return -1;   // (so that the product fits 63 bits)
   return batch * q_len * q_heads * parts * (head_dim + 2) * (int64_t)sizeof(float);
 }
 

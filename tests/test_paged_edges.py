@@ -21,6 +21,20 @@ def test_c_append_without_kv_heads_still_needs_its_table():
     assert status == _lib.MRSA_ERR_INVALID_ARGUMENT
 
 
+def test_c_workspace_sizes_do_not_wrap():
+    def size(*args):
+        return _lib.call("mrsa_paged_attention_workspace_bytes", *args)
+
+    for batch, q_len, heads in ((1 << 9, 1 << 31, 1), (1 << 24, 1, 1 << 16), (1 << 7, 1 << 31, 1),
+                                (1 << 6, 1 << 31, 2), (3, 1000003, 7)):
+        for head_dim in (64, 128, 4096):
+            for parts in (2, 1024):
+                want = batch * q_len * heads * parts * (head_dim + 2) * 4
+                assert size(batch, q_len, heads, head_dim, parts) in (
+                    (want, -1) if want < 1 << 63 else (-1,))
+    assert size(3, 1000003, 7, 128, 1024) == 3 * 1000003 * 7 * 1024 * 130 * 4
+
+
 def _plain_rotary(q, qb, ql, qh, k, kb, kl, kh, cos, sin, rows, pos, pb, pl, B, L, Hq, Hkv, D, R,
                   dtype, interleaved, inverse, q_out, k_out, stream):
     """mrsa_rotary_fwd of fp32 host memory (half layout, every position given by its row)."""
