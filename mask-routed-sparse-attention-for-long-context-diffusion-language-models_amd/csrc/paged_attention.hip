@@ -19,6 +19,11 @@
 // type as a matrix operand (the sum uses the unrounded values), which is half
 // a step of that type per term.  The maximum moves only when scores have passed it
 // by some powers of two, so that the accumulators are rarely rescaled.
+// fp16 reaches down to 2^-24 only, and many weights below that can be much of a row's sum: they
+// are taken times 2^lift (the running maximum is held that much lower; sums and outputs have
+// the same factor), which the room up to the moving maximum and fp16's largest value leave.
+// What a weight then loses is below 2^-25 / 2^lift of the largest: 20000 keys of 2^-25.2 gave
+// 0 of the output's 5.0e-4 before.
 //
 // Up to 16 columns (a token's heads) the work is the cache's bytes: `paged_attn_kernel`
 // streams them.  With more columns every key is multiplied often enough to be
@@ -56,6 +61,7 @@ struct Bf16 {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
   static __device__ __forceinline__ float value(uint32_t bits) { return bf16_to_f32(bits); }
   static constexpr uint32_t kExp = 0x7f80u;
+  static constexpr float kStreamLift = 0.f, kBlockLift = 0.f;   // (exponents as fp32's)
 };
 struct Fp16 {
   static __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
@@ -70,6 +76,8 @@ struct Fp16 {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
   }
   static constexpr uint32_t kExp = 0x7c00u;
+  // weights below 2^(kSlack + 7) and kMostSum 2^5: 2^15
+  static constexpr float kStreamLift = 7.f, kBlockLift = 5.f;
 };
 
 struct PagedArgs {
@@ -342,8 +350,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedArgs a)
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, S[i >> 2][i & 3]);
     top = across4_max(top) * a.scale_log2;   // (-inf stays: the scale is positive)
-    if (__builtin_amdgcn_ballot_w64(top > mx + kSlack) != 0) {
-      const float to = __builtin_fmaxf(mx, top);
+    if (__builtin_amdgcn_ballot_w64(top > mx + (kSlack + T::kStreamLift)) != 0) {
+      const float to = __builtin_fmaxf(mx, top - T::kStreamLift);
       const float f = to == neg_inf() ? 1.f : exp2_hw(mx - to);
       mx = to;
       sum *= f;
@@ -711,21 +719,23 @@ __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256, 2)
     return (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
   };
   // The weights are taken over the maximum so far, which need not be the tile's: it moves
-  // only when a lane's sixteen weights sum past kMostSum, or are not finite (in a
+  // only when a lane's sixteen weights sum past most_sum, or are not finite (in a
   // part's first tile the maximum is -inf), and then they are taken again.  A maximum per tile
   // would cost a tenth of the vector work.
+  constexpr float most_sum = kMostSum * (1 << (int)T::kBlockLift);
   auto softmax = [&] {
     float add[NT];
     bool fits = true;
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
       add[c] = weigh(c, mx[c]);
-      fits &= add[c] < kMostSum;
+      fits &= add[c] < most_sum;
     }
     if (__builtin_amdgcn_ballot_w64(!fits) != 0) {
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
-        const float to = __builtin_fmaxf(mx[c], across4_max(max16_raw(S[c])) * scale);
+        const float to =
+            __builtin_fmaxf(mx[c], across4_max(max16_raw(S[c])) * scale - T::kBlockLift);
         const float f = to == neg_inf() ? 1.f : exp2_hw(mx[c] - to);
         mx[c] = to;
         sum[c] *= f;

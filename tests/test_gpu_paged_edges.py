@@ -119,3 +119,34 @@ def test_a_captured_step_of_the_cache_serves_sequences_that_grow():
                    now.page_table.cpu(), now.cache_lens.cpu(), causal=True)
         assert bool(torch.isfinite(got[2]).all())
     assert c.length(seqs[0]) == 170
+
+
+@pytest.mark.parametrize("Lq,Hq", [(1, 8), (20, 2), (150, 2)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_weights_far_below_the_largest_still_count(Lq, Hq, D):
+    # One key of score 17.5 with value 0 and n keys of score 0 with value 1: weights of
+    # 2^-25.2, below half of fp16's smallest, are together n w / (1 + n w) of the output.
+    # As operands they are multiplied by 2^5 at least, so each is off by 2^-25 / 2^5 at most.
+    n, page = 20000, 64
+    pages = -(-n // page)
+    k = torch.zeros(pages, page, 1, D, dtype=torch.float16)
+    v = torch.ones_like(k)
+    q = torch.zeros(1, Lq, Hq, D, dtype=torch.float16)
+    q[..., 0] = 1
+    table = torch.arange(pages, dtype=torch.int32)[None]
+    lens = torch.tensor([n], dtype=torch.int32)
+    w = (n - 1) * torch.tensor(-17.5, dtype=torch.float64).exp()
+    want, wlse = w / (1 + w), 17.5 + torch.log1p(w)
+    e_p = (D + 2) * F24 * 17.5 + (4 * 17.5 + 4) * F24
+    sums = (n + 64) * F24
+    for first in (0, 130, n - 1):           # where the large one is
+        kk, vv = k.clone(), v.clone()
+        kk[first // page, first % page, 0, 0] = 17.5
+        vv[first // page, first % page] = 0
+        for parts in (1, 2):
+            out, lse = (t.cpu().double() for t in _run(q, kk, vv, table, lens, sm_scale=1.0,
+                                                       parts=parts))
+            tol = want * (2.0 ** -11 + 2 * e_p + 2 * sums) + n * 2.0 ** -30
+            assert bool(((out - want).abs() <= tol).all()), (first, parts, float(out.min()),
+                                                             float(out.max()), float(want))
+            assert bool(((lse - wlse).abs() <= e_p + sums + 2.0 ** -22 * (1 + wlse)).all())
