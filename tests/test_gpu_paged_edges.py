@@ -121,6 +121,55 @@ def test_a_captured_step_of_the_cache_serves_sequences_that_grow():
     assert c.length(seqs[0]) == 170
 
 
+# Columns of four waves (a ring of two slots), of five and of eight (three slots).
+BLOCKS = [(20, 2, 1), (150, 2, 1), (64, 4, 1)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Lq,Hq,Hkv", BLOCKS)
+@pytest.mark.parametrize("rise", [4.0, 5.0, 6.5, 9.0, 30.0, -9.0])
+def test_the_maximum_of_a_block_moves(Lq, Hq, Hkv, dtype, rise):
+    # Scores of row i are c_i (j // 96) rise, c_i in 0, 1/4, 1/2, 1, -1: of a wave's columns some
+    # rise past what a running maximum allows, some just below it, some fall and some stay.
+    D, n = 64, 430
+    q, k, v, table, lens = _case(1, Lq, [n], Hq, Hkv, D, 32, dtype, seed=Lq)
+    c = torch.tensor([0.0, 0.25, 0.5, 1.0, -1.0])[torch.arange(Lq) * 7 % 5]
+    q.mul_(0.125)
+    q[..., 0] = c[None, :, None].to(dtype)
+    at = torch.arange(n)
+    page = table[0].long()[at // 32]
+    k[page, at % 32, :, 0] = ((at // 96) * rise)[:, None].to(dtype)
+    for kw in (dict(parts=1), dict(parts=3), dict(parts=1, causal=True), dict(window=130, parts=2)):
+        _check(_run(q, k, v, table, lens, sm_scale=1.0, **kw), q, k, v, table, lens, sm_scale=1.0,
+               **{x: y for x, y in kw.items() if x != "parts"})
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Lq,Hq,Hkv", BLOCKS)
+def test_one_key_of_a_block_just_past_the_others(Lq, Hq, Hkv, dtype):
+    # one weight of e^d over a tile's others: below 1024 (d < 6.93) the maximum stays, and the
+    # operand holds up to that
+    for d in (6.0, 6.9, 6.95, 7.5, 11.0):
+        q, k, v, table, lens = _case(1, Lq, [300], Hq, Hkv, 128, 64, dtype, seed=int(d))
+        q.zero_()
+        q[..., 5] = 1
+        k[table[0, :5].long(), :, :, 5] = 0
+        k[table[0, 3].long(), 11, :, 5] = d     # key 203
+        k[table[0, 4].long(), 40:, :, 5] = d    # keys 296 ..
+        for kw in (dict(parts=1), dict(parts=1, causal=True)):
+            _check(_run(q, k, v, table, lens, sm_scale=1.0, **kw), q, k, v, table, lens,
+                   sm_scale=1.0, causal=kw.get("causal", False))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scales_of_blocks(dtype):
+    for Lq, Hq, Hkv in BLOCKS:
+        q, k, v, table, lens = _case(1, Lq, [250], Hq, Hkv, 128, 16, dtype, seed=Lq)
+        for scale in (0.01, 1.0, 3.0):
+            _check(_run(q, k, v, table, lens, sm_scale=scale), q, k, v, table, lens,
+                   sm_scale=scale)
+
+
 @pytest.mark.parametrize("Lq,Hq", [(1, 8), (20, 2), (150, 2)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_fp16_weights_far_below_the_largest_still_count(Lq, Hq, D):
