@@ -33,6 +33,7 @@ whose landmark slot the block holds, and runs mrsa.cached_route_attention.
 from __future__ import annotations
 
 import argparse
+import gc
 import json
 import math
 import os
@@ -120,6 +121,15 @@ def cpu_baseline(budget_s: float = 30.0):
     }
 
 
+def set_garbage_aside() -> None:
+    """Python's full collection walks the modules' objects for 40-80 ms (200 ms on a busy
+    host), which is as long as all the timed steps, and its turn comes anywhere among them:
+    take it now, and leave those objects out of later ones."""
+
+    gc.collect()
+    gc.freeze()
+
+
 def main() -> int:
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
@@ -158,6 +168,7 @@ def main() -> int:
 
     import mrsa
 
+    set_garbage_aside()
     dev = torch.device("cuda:0")
     if args.workload == "decode":
         return decode_main(args, torch, mrsa, dev)
