@@ -986,8 +986,9 @@ int mrsa_paged_attention_fwd(
     const void* k_pages, int64_t k_page_stride, int64_t k_slot_stride, int64_t k_head_stride,
     const void* v_pages, int64_t v_page_stride, int64_t v_slot_stride, int64_t v_head_stride,
     const int32_t* page_table, int64_t page_table_stride, int64_t table_pages, int64_t num_pages,
-    int64_t page_size, const int32_t* cache_lens, const int32_t* query_starts, int64_t max_len, int64_t batch, int64_t q_len,
-    int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t dtype, int32_t causal,
+    int64_t page_size, const int32_t* cache_lens, const int32_t* query_starts, int64_t max_len,
+    int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+    int32_t dtype, int32_t causal,
     int64_t window, float sm_scale, int64_t parts, void* workspace, int64_t workspace_bytes,
     void* out, float* lse, void* stream);
 

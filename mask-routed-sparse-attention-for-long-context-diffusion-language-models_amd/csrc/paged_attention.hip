@@ -58,7 +58,9 @@ struct Bf16 {
   static __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
     return mfma_bf16_16x16x32(a, b, c);
   }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    return pack_bf16x2(lo, hi);
+  }
   static __device__ __forceinline__ float value(uint32_t bits) { return bf16_to_f32(bits); }
   static constexpr uint32_t kExp = 0x7f80u;
   static constexpr float kStreamLift = 0.f, kBlockLift = 0.f;   // (exponents as fp32's)
@@ -242,7 +244,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedArgs a)
   const uint32_t vbase = lds_addr(vl);
   // transposing reads: row 4 grp + (col >> 2), piece col & 3 of its 32 bytes
   const int tr = 4 * grp + (col >> 2);
-  const uint32_t tr0 = vbase + tr * ROWB + ((((col & 3) >> 1) ^ swizzle<D>(tr)) << 4) + (col & 1) * 8;
+  const uint32_t tr0 =
+      vbase + tr * ROWB + ((((col & 3) >> 1) ^ swizzle<D>(tr)) << 4) + (col & 1) * 8;
 
   // Every load is issued a tile ahead: V's as soon as the registers have gone
   // to LDS, K's after the products, page indices one tile before those.
@@ -396,7 +399,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedArgs a)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t w = vp[16 * t + 4 * grp + e];
-            if (ok && (w & T::kExp) == T::kExp) O[t][e] += T::value(w);  // (p > 0: its size is no matter)
+            // (p > 0: its size is no matter)
+            if (ok && (w & T::kExp) == T::kExp) O[t][e] += T::value(w);
           }
       }
     }
@@ -467,12 +471,15 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_attn_kernel(PagedArgs a)
 // DMA into a ring, a tile ahead, one barrier per tile; K is read along the row
 // (operand A of S^T), V by transposing reads (operand A of O^T).
 //
-// Bound by issue and, with all CUs at work, by HBM: a wave's tile is 64 matrix instructions and
-// about 130 vector ones (32 exponentials, their arguments, the sums, the packing), and two
-// waves share a SIMD.  So the two go half a tile apart (the softmax of one runs beside the products of the
-// other), tiles that every column sees whole have a loop of their own without masks, with
-// the ring's slots as constants, the maximum is not taken per tile, and the next rows'
-// addresses are computed before the barrier.  28 heads in 4 groups, 32 rows, 65503 keys (30
+// Bound by what lies between its units: a wave's tile is 64 matrix instructions and about 130
+// vector ones (32 exponentials, their arguments, the sums, the packing), two waves share a
+// SIMD, and in a long loop (8192 rows of 8192 keys) the matrix cores and the vector unit are at
+// work for 45 and 43% of the cycles, with waves waiting a fifth of theirs at the tile's barrier and
+// for operands; with few rows and all CUs at work HBM comes near, too.  So the two go half a
+// tile apart (the softmax of one runs beside the products of the other), tiles that every
+// column sees whole have a loop of their own without masks, with the ring's slots as
+// constants, the maximum is not taken per tile, and the next rows' addresses are computed
+// before the barrier.  28 heads in 4 groups, 32 rows, 65503 keys (30
 // GFLOP, 134 MB; 64 pieces): 43.4 us, 690 TFLOP/s; of them 5 until the first rows are there, 28
 // for sixteen tiles (1.45 us a tile with few workgroups, more with 256, which stream 3.7 TB/s)
 // and 8 for the partial results' way out.  Without the one after the other: addresses
@@ -488,7 +495,8 @@ constexpr int kBlockWaves = 8;
 // wave-uniform; the first s_nop covers a scalar operand that a vector instruction
 // has just written (5 wait states), the others m0.
 template <int N>
-__device__ __forceinline__ void dma_piece(uint32_t to, const uint8_t* base, const uint32_t (&at)[N]) {
+__device__ __forceinline__ void dma_piece(uint32_t to, const uint8_t* base,
+                                          const uint32_t (&at)[N]) {
   static_assert(N == 2 || N == 4);
   if constexpr (N == 4)
     asm volatile(
@@ -780,7 +788,9 @@ __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256, 2)
   };
 
   // Any tile: masks, rows nobody sees, unmapped pages, the last.
-  auto live_at = [&](int base, int i) { return !holes || is_live(page_at(a, table, base + 16 * i)); };
+  auto live_at = [&](int base, int i) {
+    return !holes || is_live(page_at(a, table, base + 16 * i));
+  };
   auto edge_tile = [&](int t) {
     const uint32_t off = slot_of(t);
     const int base = first + t * kBlockKeys;
@@ -922,7 +932,8 @@ __global__ void __launch_bounds__(SLOTS == 3 ? 64 * kBlockWaves : 256, 2)
     for (int d = 0; d < DT; ++d) {
       u32x2_t o = {0u, 0u};
       if (total != 0.f)
-        o = u32x2_t{T::pack(O[t][d][0] * inv, O[t][d][1] * inv), T::pack(O[t][d][2] * inv, O[t][d][3] * inv)};
+        o = u32x2_t{T::pack(O[t][d][0] * inv, O[t][d][1] * inv),
+                    T::pack(O[t][d][2] * inv, O[t][d][3] * inv)};
       *reinterpret_cast<u32x2_t*>(z->out + row * D + 16 * d + 4 * grp) = o;
     }
     if (grp == 0) z->lse[row] = total == 0.f ? neg_inf() : kLn2 * (mx[t] + log2_hw(total));
@@ -1021,7 +1032,7 @@ int launch(const PagedArgs& a, hipStream_t stream) {
   const int64_t grid = (int64_t)a.B * a.Hkv * a.col_tiles * a.parts;
   const int64_t cols = (int64_t)a.B * a.Hkv * a.M;
   const int64_t threads = a.tile_cols == 16 ? 64 * kWaves : 64 * a.tile_cols / kBlockCols;
-  // (a launch holds fewer than 2^32 threads; the join has at most 64 a column)
+  // (a launch holds fewer than 2^32 threads; the join has 64 a column, or 256 of at most 1024)
   if (grid > 0xffffffffll / threads || (a.parts > 1 && cols > (1 << 26) - 4) || cols > 0x7fffffff)
     return MRSA_ERR_UNSUPPORTED;
   if (a.tile_cols == 16) {
@@ -1069,15 +1080,17 @@ extern "C" int mrsa_paged_attention_fwd(
     const void* k_pages, int64_t k_page_stride, int64_t k_slot_stride, int64_t k_head_stride,
     const void* v_pages, int64_t v_page_stride, int64_t v_slot_stride, int64_t v_head_stride,
     const int32_t* page_table, int64_t page_table_stride, int64_t table_pages, int64_t num_pages,
-    int64_t page_size, const int32_t* cache_lens, const int32_t* query_starts, int64_t max_len, int64_t batch, int64_t q_len,
-    int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t dtype, int32_t causal,
+    int64_t page_size, const int32_t* cache_lens, const int32_t* query_starts, int64_t max_len,
+    int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+    int32_t dtype, int32_t causal,
     int64_t window, float sm_scale, int64_t parts, void* workspace, int64_t workspace_bytes,
     void* out, float* lse, void* stream) {
   if (batch < 0 || q_len < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 ||
       max_len < 0 || table_pages < 0 || num_pages < 0 || page_size <= 0 || parts < 1 ||
       parts > kMaxParts)
     return MRSA_ERR_INVALID_ARGUMENT;
-  if (!(sm_scale > 0.f) || !(sm_scale * kLog2e < __builtin_inff())) return MRSA_ERR_INVALID_ARGUMENT;
+  if (!(sm_scale > 0.f) || !(sm_scale * kLog2e < __builtin_inff()))
+    return MRSA_ERR_INVALID_ARGUMENT;
   if (dtype != MRSA_DTYPE_BF16 && dtype != MRSA_DTYPE_FP16) return MRSA_ERR_UNSUPPORTED;
   if (head_dim != 64 && head_dim != 128) return MRSA_ERR_UNSUPPORTED;
   if ((page_size & (page_size - 1)) != 0 || page_size < 16 || page_size > (1 << 20))

@@ -3,9 +3,9 @@
 //
 // A copy reads and writes each byte once: bound by HBM, or for few pages by the
 // launch.  300 pages of 64 rows of 4 heads in 28 layers (2.2 GB read and written) 418 us,
-// 5.3 TB/s, a large copy's rate; 8 pages (59 MB) 10.6 us.  The page pairs travel in the kernel's arguments (4 KB hold
-// kPairs of them), so that no index tensor is uploaded and the call neither
-// allocates nor waits; longer lists are further launches.  Sources and
+// 5.3 TB/s, a large copy's rate; 8 pages (59 MB) 10.6 us.  The page pairs travel in the
+// kernel's arguments (4 KB hold kPairs of them), so that no index tensor is uploaded and the
+// call neither allocates nor waits; longer lists are further launches.  Sources and
 // destinations are disjoint and destinations distinct (checked on the host), so
 // the pairs are independent and need no order.
 #include "mrsa_device.h"

@@ -15,8 +15,8 @@
 // kHeadsPerThread heads of one token, so that a token's table row is read once
 // per thread and not once per head, and all its loads are in flight together.
 // 28 + 4 heads of 128 dims, bf16: 16384 rows (273 MB) 47-54 us, 5.0-5.8 TB/s (a large
-// copy: 5.3); 32 rows 3.5 us, a launch.  Append of 16002 rows of 28 + 4 + 4 heads (292 MB)
-// 52 us; of 16 rows 4.2 us.
+// copy, whose results do not fit the caches: 5.3); 32 rows 3.5 us, a launch.  Append of 16002
+// rows of 28 + 4 + 4 heads (292 MB) 53 us; of 16 rows 4.2 us.
 #include "mrsa_device.h"
 
 using namespace mrsa;
@@ -171,8 +171,8 @@ struct Rows {
 };
 
 // Appended rows are stored past the caches (evicted first): 16002 rows of 28 + 4 + 4
-// heads take 58 us so and 64 without; the dense rotation of 16384 rows takes
-// 49 us without and 53 so.
+// heads take 53 us so and 58 without.  The dense rotation, whose result the next kernel reads,
+// leaves it there: 16384 rows 54 us, 51 past the caches; short ones alike.
 template <bool PAST, class T>
 __device__ __forceinline__ void store(T* to, const Vec<T>& v) {
   u32x4_t* at = reinterpret_cast<u32x4_t*>(to);
@@ -356,7 +356,8 @@ int launch(RotaryArgs a, bool interleaved, hipStream_t stream) {
   if (blocks > 0xffffffffll / threads) return MRSA_ERR_UNSUPPORTED;  // (threads of a launch)
   void (*kern)(RotaryArgs);
   if (!vec)
-    kern = interleaved ? rotary_scalar_kernel<T, true, PAGED> : rotary_scalar_kernel<T, false, PAGED>;
+    kern = interleaved ? rotary_scalar_kernel<T, true, PAGED>
+                       : rotary_scalar_kernel<T, false, PAGED>;
   else if (heads_each == 1)
     kern = interleaved ? rotary_kernel<T, true, PAGED, 1> : rotary_kernel<T, false, PAGED, 1>;
   else

@@ -291,8 +291,9 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     Padding, and a row that sees no key, give out = 0 and lse = -inf.
 
     max_len: a bound of cache_lens that the caller knows (None: the table's rows; lengths
-    past it are cut to it); it sizes the launch, and a captured call keeps it.  parts: pieces the span is cut into,
-    None picks them.  Returns out [B, Lq, Hq, D] in q's dtype and lse fp32 [B, Lq, Hq].
+    past it are cut to it); it sizes the launch, and a captured call keeps it.  parts: pieces
+    the span is cut into, None picks them.  sm_scale: above 0, D^-0.5 if None.  Returns out
+    [B, Lq, Hq, D] in q's dtype and lse fp32 [B, Lq, Hq].
     """
 
     check_heads(q, "q")
@@ -405,8 +406,9 @@ class PagedKVCache:
     ``batch`` uploads what the operators need, ``append`` and ``attend`` run them on a
     layer.  Forked sequences share pages; a shared page is copied before one of
     them writes to it (``extend`` for the rows it adds, ``make_writable`` for rows
-    rewritten).  Not for use from several threads at once; page copies go to the
-    current stream, where the operators have to follow."""
+    rewritten).  fp32 pools can be written and copied, but not attended.  Not for use from
+    several threads at once; page copies go to the current stream, where the operators have
+    to follow."""
 
     def __init__(self, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
                  *, dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -448,7 +450,8 @@ class PagedKVCache:
 
     def _need(self, count: int) -> None:
         if count > len(self._free):
-            raise PagesExhausted(f"{count} pages wanted, {len(self._free)} of {self.num_pages} free")
+            raise PagesExhausted(f"{count} pages wanted, {len(self._free)} of {self.num_pages} "
+                                 "free")
 
     def _take(self) -> int:
         page = heapq.heappop(self._free)
@@ -613,7 +616,8 @@ class PagedKVCache:
         dev = host.to(self.k_pages.device, non_blocking=True)
         ints = dev[16 * B * L:].view(torch.int32)
         return PagedBatch(
-            seqs=seqs, lens=tuple(s.length for s in held), rows=tuple(counts), page_table=ints[:B * width].view(B, width),
+            seqs=seqs, lens=tuple(s.length for s in held), rows=tuple(counts),
+            page_table=ints[:B * width].view(B, width),
             cache_lens=ints[B * width:B * width + B], query_starts=ints[B * width + B:],
             slots=dev[:8 * B * L].view(torch.long).view(B, L),
             positions=dev[8 * B * L:16 * B * L].view(torch.long).view(B, L),
@@ -633,7 +637,8 @@ class PagedKVCache:
             start, stop = batch.lens[i] - batch.rows[i], batch.lens[i]
             held = self._get(seq).pages[start // P:-(-stop // P)] if start < stop else ()
             if any(self._refs[p] > 1 for p in held):
-                raise ValueError(f"rows of sequence {seq} lie in a shared page: make_writable first")
+                raise ValueError(f"rows of sequence {seq} lie in a shared page: make_writable "
+                                 "first")
         if rotary.get("cos") is not None and rotary.get("positions") is None:
             rotary["positions"] = batch.positions
         return paged_cache_append(k, v, self.k_pages[layer], self.v_pages[layer],
@@ -649,7 +654,7 @@ class PagedKVCache:
         if max_len is None:
             max_len = batch.max_len
         elif max_len < batch.max_len:
-            raise ValueError(f"max_len must be at least the batch's, {batch.max_len}, got {max_len}")
+            raise ValueError(f"max_len must be at least the batch's {batch.max_len}, got {max_len}")
         return paged_cached_attention(q, self.k_pages[layer], self.v_pages[layer],
                                       batch.page_table, batch.cache_lens,
                                       query_starts=batch.query_starts, max_len=max_len, **options)

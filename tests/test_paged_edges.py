@@ -15,8 +15,8 @@ from mrsa import _lib, paged_cache, rotary
 
 def test_c_append_without_kv_heads_still_needs_its_table():
     s = (512, 512, 128)
-    status = _lib.call("mrsa_paged_append_fwd", 4096, *s, None, 0, 0, 0, None, 0, 0, 0, None, None, 0,
-                       None, 0, 0, 4096, 1, 1, None, 4, 4, 7, 16, None, *s, None, *s, 1, 1, 4, 0,
+    status = _lib.call("mrsa_paged_append_fwd", 4096, *s, None, 0, 0, 0, None, 0, 0, 0, None, None,
+                       0, None, 0, 0, 4096, 1, 1, None, 4, 4, 7, 16, None, *s, None, *s, 1, 1, 4, 0,
                        128, 0, 0, 0, 4096, None)
     assert status == _lib.MRSA_ERR_INVALID_ARGUMENT
 
@@ -152,7 +152,8 @@ def _paged_calls():
     table, slots = torch.zeros(1, 5, dtype=torch.int32), torch.arange(3)[None]
     lens = torch.tensor([3], dtype=torch.int32)
     append = lambda **kw: mrsa.paged_cache_append(  # noqa: E731
-        **{**dict(k=k, v=k, k_pages=kp[0], v_pages=vp[0], page_table=table, slots=slots, q=k), **kw})
+        **{**dict(k=k, v=k, q=k, k_pages=kp[0], v_pages=vp[0], page_table=table, slots=slots),
+           **kw})
     attend = lambda **kw: mrsa.paged_cached_attention(  # noqa: E731
         **{**dict(q=k, k_pages=kp[0], v_pages=vp[0], page_table=table, cache_lens=lens), **kw})
     for name in ("q", "k", "v"):
