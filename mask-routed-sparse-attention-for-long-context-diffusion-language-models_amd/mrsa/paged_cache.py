@@ -86,9 +86,9 @@ def _written(*pools) -> None:
     operators do: backward passes that saved them and ``kv_fragments_cached`` go by it.
     (Tensors made in inference mode have none.)"""
 
-    for t in pools:
-        if not t.is_inference():
-            torch.autograd.graph.increment_version(t)
+    if pools[0].is_inference() or pools[1].is_inference():
+        pools = [t for t in pools if not t.is_inference()]
+    torch.autograd.graph.increment_version(pools)
 
 
 def _paged_append_impl(k, v, k_pages, v_pages, page_table, slots, q, cos, sin, positions,

@@ -113,8 +113,11 @@ def test_in_place_operators_raise_the_pools_version_counters(cpu_ops):
         kp, vp = _pools()
     _append(kp[0], vp[0])
     torch.ops.mrsa.copy_pages_(kp, vp, [0], [1])
-    assert cpu_ops == ["mrsa_paged_append_fwd", "mrsa_copy_pages",
-                       "mrsa_paged_append_fwd", "mrsa_paged_append_fwd", "mrsa_copy_pages"]
+    mixed, _ = _pools()
+    _append(kp[0], mixed[0]), _append(mixed[0], vp[0])
+    assert mixed._version == 2
+    assert cpu_ops[:5] == ["mrsa_paged_append_fwd", "mrsa_copy_pages",
+                            "mrsa_paged_append_fwd", "mrsa_paged_append_fwd", "mrsa_copy_pages"]
 
 
 def test_batches_and_attention_with_room_to_grow(cpu_ops, monkeypatch):
