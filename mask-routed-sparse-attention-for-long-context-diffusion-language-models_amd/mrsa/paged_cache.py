@@ -26,7 +26,8 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
-from .rotary import DTYPES, check_heads, check_tables, check_token_ints, dense_rows
+from .rotary import (DTYPES, check_heads, check_tables, check_token_ints, dense_rows,
+                     refuse_tangents)
 
 MAX_PARTS = 1024
 
@@ -93,6 +94,7 @@ def _written(*pools) -> None:
 
 def _paged_append_impl(k, v, k_pages, v_pages, page_table, slots, q, cos, sin, positions,
                        interleaved):
+    refuse_tangents("mrsa::paged_append_", q, k, v, k_pages, v_pages)
     B, L, Hkv, D = k.shape
     kc, vc = dense_rows(k), dense_rows(v)
     kb, kl, kh, _ = kc.stride()
@@ -231,6 +233,7 @@ def cache_parts(batch: int, q_len: int, q_heads: int, kv_heads: int, span: int, 
 
 def _paged_attention_impl(q, k_pages, v_pages, page_table, cache_lens, query_starts, max_len,
                           causal, window, sm_scale, parts):
+    refuse_tangents("mrsa::paged_attention", q, k_pages, v_pages)
     shape = q.shape
     B, Lq, Hq, D = shape
     qc = dense_rows(q)
@@ -329,6 +332,7 @@ def paged_cached_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
 
 
 def _copy_pages_impl(k_pages, v_pages, src, dst):
+    refuse_tangents("mrsa::copy_pages_", k_pages, v_pages)
     n = len(src)
     layered = k_pages.ndim == 5
     shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()

@@ -116,7 +116,18 @@ def check_token_ints(t, name: str, batch: int, seq_len: int, device) -> torch.Te
     return t.expand(batch, seq_len)
 
 
+def refuse_tangents(name: str, *tensors) -> None:
+    """For the operators themselves, which have no forward-mode derivative: what a compiler has
+    traced, or calls them directly, reaches them past the checks of the public functions."""
+
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no forward-mode derivative here")
+
+
 def _rotary_impl(q, k, cos, sin, positions, interleaved, inverse):
+    refuse_tangents("mrsa::rotary", q, k)
     shape = q.shape
     B, L, Hq, D = shape
     qc, ct, st = dense_rows(q), cos.contiguous(), sin.contiguous()
@@ -219,8 +230,8 @@ def rotary_qk(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin
               positions: Optional[torch.Tensor] = None, *, interleaved: bool = False
               ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Query and key heads turned by their positions; differentiable in q and k (reverse and
-    forward mode, and under torch.func's transforms; what torch.compile has traced knows
-    only reverse mode).
+    forward mode, and under torch.func's transforms; what torch.compile has traced refuses
+    dual tensors).
 
     q [B, L, Hq, D] and k [B, L, Hkv, D] (or None) in bf16, fp16 or fp32, any
     strides; cos, sin fp32 [rows, R / 2] (``rotary_tables``), R <= D: the first R dims

@@ -275,3 +275,30 @@ def test_rotary_and_its_gradient_trace_without_a_graph_break(cpu_ops, backend):
     want = torch.autograd.grad(f(x, y), (x, y), (gq, gk))
     got = torch.autograd.grad(compiled(x, y), (x, y), (gq, gk))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("backend", [None, "eager", "aot_eager"])
+def test_traced_and_direct_calls_refuse_tangents(cpu_ops, backend):
+    q, _, tq, _, _, _, _ = _rope(3)
+    cos, sin = torch.zeros(5, 3), torch.zeros(5, 3)
+    kp, vp = _pools()
+    k = torch.zeros(1, 3, 2, 64)
+    table, slots = torch.zeros(1, 5, dtype=torch.int32), torch.arange(3)[None]
+    lens = torch.tensor([3], dtype=torch.int32)
+    ops, rest = torch.ops.mrsa, (None, None, None, None, False)
+    calls = [
+        (lambda t: ops.rotary(t, None, cos, sin, None, False, False), q),
+        (lambda t: ops.paged_append_(t, k, kp[0], vp[0], table, slots, *rest), k),
+        (lambda t: ops.paged_append_(k, k, t, vp[0], table, slots, *rest), kp[0]),
+        (lambda t: ops.paged_attention(t, kp[0], vp[0], table, lens, None, 3, False, -1, 0.1, 1),
+         k),
+        (lambda t: ops.copy_pages_(kp, t, [0], [1]), vp),
+    ]
+    for call, t in calls:
+        torch._dynamo.reset()
+        f = call if backend is None else torch.compile(call, backend=backend)
+        f(t)
+        n = len(cpu_ops)
+        with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+            f(forward_ad.make_dual(t, torch.ones_like(t)))
+        assert len(cpu_ops) == n
