@@ -1005,6 +1005,62 @@ int mrsa_copy_pages(void* k_pages, int64_t k_layer_stride, int64_t k_page_stride
                     const int64_t* dst, void* stream);
 
 /*
+ * Linear layers in 8-bit integers.  A row y of `dim` values is held as int8
+ * values v and one fp32 scale: with a = max |y_k|,
+ *   scale = a / 127,  v_k = rint(y_k 127 / a)  (ties to even, |v_k| <= 127);
+ * a = 0: scale and values 0; a not finite: scale NaN and values 0.
+ *   values (out): [rows, dim] dense; scales (out): [rows]
+ *   x, gate_up, ..: `dtype` (MRSA_DTYPE_*), rows at strides in elements (0 and
+ *     overlapping rows allowed), dense in the last dim, aligned to an element
+ * Outputs must not overlap inputs.  Limits: 1 <= dim <= 2^31, rows <= 2^40, row
+ * sizes and strides times rows < 2^56.
+ */
+
+/* y = x. */
+int mrsa_quantize_rows_fwd(const void* x, int64_t x_row_stride, int64_t rows, int64_t dim,
+                           int32_t dtype, int8_t* values, float* scales, void* stream);
+
+/* out [rows, dim] of `dtype` = values * scale (values' rows at a stride in bytes). */
+int mrsa_dequantize_rows_fwd(const int8_t* values, int64_t row_stride, const float* scales,
+                             int64_t rows, int64_t dim, int32_t dtype, void* out, void* stream);
+
+/*
+ * t = x + residual rounded to `dtype` (written to total, dense; residual and
+ * total are both given or both NULL, then t = x),
+ * y = t / sqrt(mean(t^2) + eps) * weight, in fp32 with no rounding before the 8
+ * bits.  1e-24 <= eps <= 1e24.
+ */
+int mrsa_add_rms_norm_int8_fwd(const void* x, int64_t x_row_stride, const void* residual,
+                               int64_t residual_row_stride, const void* weight, int64_t rows,
+                               int64_t dim, float eps, int32_t dtype, void* total, int8_t* values,
+                               float* scales, void* stream);
+
+/*
+ * y = silu(gate) * up; gate_up: rows of 2 * dim (gate columns first).  fp32, no
+ * rounding before the 8 bits; a product past fp32 counts as an infinity.
+ */
+int mrsa_swiglu_int8_fwd(const void* gate_up, int64_t row_stride, int64_t rows, int64_t dim,
+                         int32_t dtype, int8_t* values, float* scales, void* stream);
+
+/*
+ * out[m, n] = x_scales[m] weight_scales[n] sum_k x[m, k] weight[n, k] + bias[n],
+ * the sum exact in int32, the rest in fp32, rounded once to `dtype`.
+ *   x: int8 [rows, dim], weight: int8 [out_dim, dim], rows at strides in bytes
+ *   bias: optional [out_dim] of `dtype`; out: [rows, out_dim] of `dtype`, dense
+ *   workspace: mrsa_int8_linear_workspace_bytes (16-byte aligned; may be NULL
+ *     for 0 bytes), held by one call at a time
+ * Rows at multiples of 16 bytes with dim a multiple of 16 are fastest.  Limits:
+ * dim <= 131071, rows, out_dim and strides < 2^31, fewer than 2^23 workgroups
+ * (tiles of 128 x 128 or more results, 16 columns for up to 64 rows).
+ */
+int64_t mrsa_int8_linear_workspace_bytes(int64_t rows, int64_t out_dim, int64_t dim);
+int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const float* x_scales,
+                         const int8_t* weight, int64_t weight_row_stride,
+                         const float* weight_scales, const void* bias, int64_t rows,
+                         int64_t out_dim, int64_t dim, int32_t dtype, void* workspace,
+                         int64_t workspace_bytes, void* out, void* stream);
+
+/*
  * Self-test of the matrix-core lane layout every kernel above relies on:
  * c = a @ b for a = bf16 [16, 32], b = bf16 [32, 16], c = fp32 [16, 16],
  * computed with one v_mfma_f32_16x16x32_bf16.  No reference counterpart.

@@ -1,0 +1,637 @@
+// Rows in 8 bits times a matrix in 8 bits, with a scale for each token and
+// each output channel:
+//     out[m, n] = sx[m] sw[n] sum_k x[m, k] w[n, k] + bias[n].
+// The sum is exact: products of at most 2^14 in int32, K <= 131071.  The
+// scales, the bias and the rounding to the output's type are one fp32 step at
+// the end, so the result does not depend on how the sum is cut.
+#include "mrsa_device.h"
+
+using namespace mrsa;
+
+namespace {
+
+typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
+typedef int32_t i32x16_t __attribute__((ext_vector_type(16)));
+
+template <class E, int N>
+struct __attribute__((packed, aligned(1))) Pack {
+  E e[N];
+};
+__device__ __forceinline__ u32x4_t load16(const int8_t* p) {  // any alignment
+  const Pack<uint32_t, 4> v = *reinterpret_cast<const Pack<uint32_t, 4>*>(p);
+  return u32x4_t{v.e[0], v.e[1], v.e[2], v.e[3]};
+}
+
+struct LinearArgs {
+  const int8_t* x;
+  const int8_t* w;
+  const float* sx;
+  const float* sw;
+  const void* bias;      // optional, of the output's type
+  void* out;             // dense [M, N]
+  int32_t* partial;      // parts > 1
+  int64_t M, N, K, x_stride, w_stride;
+  int32_t dtype, parts, tiles_m, tiles_n;
+};
+
+__device__ __forceinline__ float widen(const void* p, int64_t at, int dtype) {
+  if (dtype == MRSA_DTYPE_FP32) return ((const float*)p)[at];
+  const uint16_t e = ((const uint16_t*)p)[at];
+  return dtype == MRSA_DTYPE_BF16 ? bf16_to_f32(e) : (float)__builtin_bit_cast(_Float16, e);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, int dtype) {
+  if (dtype == MRSA_DTYPE_BF16) return pack_bf16x2(lo, hi);
+  const uint32_t a = __builtin_bit_cast(uint16_t, (_Float16)lo);
+  const uint32_t b = __builtin_bit_cast(uint16_t, (_Float16)hi);
+  return a | b << 16;
+}
+__device__ __forceinline__ float scaled(int32_t sum, float sx, float sw, float bias) {
+  return fmaf((float)sum * sx, sw, bias);
+}
+
+// Bytes of a row's chunk [k, k + 16): read at min(k, K - 16), and those before k (part of the
+// chunk before, or all of a chunk past K) made zero in one of the two operands.
+__device__ __forceinline__ u32x4_t without_first(u32x4_t v, int64_t bytes) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const int n = (int)min(max(bytes - 4 * d, (int64_t)0), (int64_t)4);
+    v[d] = n == 4 ? 0u : v[d] >> (8 * n) << (8 * n);
+  }
+  return v;
+}
+
+// ---- many rows: tiles through LDS -------------------------------------------------------
+
+template <int TM_, int TN_, int WM_, int WN_, int BK_, int STAGES_>
+struct Tile {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, BK = BK_, STAGES = STAGES_;
+  static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int MT = TM / WM / 32, NT = TN / WN / 32;   // 32 x 32 products of a wave
+  static constexpr int KS = BK / 32;
+  static constexpr int CH = BK / 16;                           // chunks of a row
+  static constexpr int STAGE = (TM + TN) * BK;                 // bytes
+  static constexpr int PIECES = STAGE / 1024 / WAVES;          // 1 KB each, of a wave
+  static constexpr int W_PIECES = TN * BK / 1024;
+  // epilogue: a wave's scales and bias, then 32 rows of its columns
+  static constexpr int COLS = 32 * NT;
+  static constexpr int ROWB = COLS * 4 + 16;
+  static constexpr int OUT = 2 * COLS * 4 + 32 * ROWB;
+  static constexpr int LDS = STAGES * STAGE > WAVES * OUT ? STAGES * STAGE : WAVES * OUT;
+  static_assert(STAGE % (1024 * WAVES) == 0 && (TN * BK) % 1024 == 0 && LDS <= 160 * 1024);
+};
+
+// Chunk c of row r lies in slot c ^ swizzle(r) of the row: sixteen rows' reads of one chunk meet
+// all banks.
+template <int BK>
+__device__ __forceinline__ int swizzle(int r) {
+  return BK == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
+}
+
+__device__ __forceinline__ u32x4_t lds16(uint32_t at) {
+  return *(const __attribute__((address_space(3))) u32x4_t*)(uintptr_t)at;
+}
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+__device__ __forceinline__ i32x16_t mfma(u32x4_t a, u32x4_t b, i32x16_t c) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a),
+                                               __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
+}
+
+// 1 KB of LDS from `to` on, lane l's 16 bytes from base + at.  As asm, since after the builtin
+// the compiler waits for all DMA in flight before the next LDS read; the loop's own waits order
+// them.  (s_nop: m0 and scalars that a vector instruction has just written.)
+__device__ __forceinline__ void dma(uint32_t to, const int8_t* base, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %1" ::"s"(to),
+               "s"(base), "v"(at)
+               : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_dma() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+
+// Tiles in an order that gives each XCD (workgroups go round them) a contiguous range of bands of
+// 8 tile rows, walked column by column: its concurrent tiles share operands in its L2.
+__device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int tiles = tiles_m * tiles_n, each = tiles / 8, more = tiles % 8;
+  const int xcd = b % 8, i = b / 8;
+  const int t = xcd * each + min(xcd, more) + i;
+  const int band = t / (8 * tiles_n), rest = t - band * 8 * tiles_n;
+  const int rows = min(8, tiles_m - 8 * band);
+  tn = rest / rows;
+  tm = 8 * band + rest - tn * rows;
+}
+
+template <class T>
+struct Position {
+  int lane, wave, wm, wn;
+  int64_t m0, n0;  // of the tile
+  __device__ __forceinline__ Position(const LinearArgs& a, int tile) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wm = wave / T::WN;
+    wn = wave % T::WN;
+    int tm, tn;
+    tile_of(tile, a.tiles_m, a.tiles_n, tm, tn);
+    m0 = (int64_t)tm * T::TM;
+    n0 = (int64_t)tn * T::TN;
+  }
+};
+
+// Sums to results.  A product's result has row 8 (i / 4) + 4 (lane / 32) + i % 4 (a column n of
+// the output, W being the first operand) in register i and column lane % 32 (a row m).  Each wave
+// turns 32 rows of its columns at a time in LDS of its own, so that rows leave as 16-byte pieces.
+template <class T>
+__device__ __forceinline__ void finish(const LinearArgs& a, const Position<T>& p, uint8_t* lds,
+                                       const i32x16_t (&acc)[T::MT][T::NT]) {
+  uint8_t* const mine = lds + p.wave * T::OUT;
+  float* const scale = (float*)mine;
+  float* const bias = scale + T::COLS;
+  uint8_t* const rows = mine + 2 * T::COLS * 4;
+  const int64_t n0 = p.n0 + p.wn * T::COLS;
+  const int64_t m0 = p.m0 + p.wm * 32 * T::MT;
+  if (n0 >= a.N || m0 >= a.M) return;
+  const int cols = (int)min((int64_t)T::COLS, a.N - n0);
+  for (int c = p.lane; c < T::COLS; c += 64) {
+    const int64_t n = n0 + min(c, cols - 1);
+    scale[c] = a.sw[n];
+    bias[c] = a.bias ? widen(a.bias, n, a.dtype) : 0.f;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int half = p.lane >> 5, col = p.lane & 31;
+  const bool wide = a.dtype == MRSA_DTYPE_FP32;
+#pragma unroll
+  for (int mt = 0; mt < T::MT; ++mt) {
+    const int64_t m1 = m0 + 32 * mt;
+    if (m1 >= a.M) break;
+    const float sx = a.sx[min(m1 + col, a.M - 1)];
+#pragma unroll
+    for (int nt = 0; nt < T::NT; ++nt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * nt + 8 * g + 4 * half;
+        const f32x4_t s = *(const f32x4_t*)(scale + c), b = *(const f32x4_t*)(bias + c);
+        f32x4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = scaled(acc[mt][nt][4 * g + i], sx, s[i], b[i]);
+        if (wide) {
+          *(f32x4_t*)(rows + col * T::ROWB + 4 * c) = v;
+        } else {
+          *(u32x2_t*)(rows + col * T::ROWB + 2 * c) =
+              u32x2_t{pack2(v[0], v[1], a.dtype), pack2(v[2], v[3], a.dtype)};
+        }
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int size = wide ? 4 : 2;
+    const int per_row = T::COLS * size / 16;      // 16-byte pieces
+    const int there = (int)min((int64_t)32, a.M - m1);
+    for (int at = p.lane; at < 32 * per_row; at += 64) {
+      const int r = at / per_row, piece = at - r * per_row, c = piece * (16 / size);
+      if (r >= there || c >= cols) continue;
+      const uint8_t* const from = rows + r * T::ROWB + 16 * piece;
+      uint8_t* const to = (uint8_t*)a.out + ((m1 + r) * a.N + n0 + c) * size;
+      if (c + 16 / size <= cols) {
+        const u32x4_t v = *(const u32x4_t*)from;
+        *reinterpret_cast<Pack<uint32_t, 4>*>(to) = Pack<uint32_t, 4>{{v[0], v[1], v[2], v[3]}};
+      } else if (wide) {
+        for (int i = 0; i < cols - c; ++i) ((float*)to)[i] = ((const float*)from)[i];
+      } else {
+        for (int i = 0; i < cols - c; ++i) ((uint16_t*)to)[i] = ((const uint16_t*)from)[i];
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// DMA: rows 16-byte aligned and K a multiple of 16.  Otherwise rows go through registers.
+template <class T, bool DMA>
+__global__ void __launch_bounds__(T::THREADS)
+    int8_tile_kernel(LinearArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
+  constexpr int BK = T::BK, RP = 1024 / BK, P = T::PIECES;
+  const int tiles = a.tiles_m * a.tiles_n;
+  const int part = blockIdx.x / tiles, tile = blockIdx.x - part * tiles;
+  const Position<T> p(a, tile);
+  const int lane = p.lane, wave = p.wave;
+  const int steps = (int)((a.K + BK - 1) / BK);
+  const int t0 = (int)((int64_t)steps * part / a.parts);
+  const int t1 = (int)((int64_t)steps * (part + 1) / a.parts);
+
+  // ---- where this wave's pieces come from: rows past the end repeat the last one
+  const int8_t* base[P];
+  uint32_t off[P];
+  int chunk[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int piece = wave * P + i;
+    const bool is_w = piece < T::W_PIECES;
+    const int r = (piece - (is_w ? 0 : T::W_PIECES)) * RP + lane / T::CH;
+    const int64_t first = is_w ? p.n0 : p.m0, rows = is_w ? a.N : a.M;
+    const int64_t stride = is_w ? a.w_stride : a.x_stride;
+    base[i] = (is_w ? a.w : a.x) + first * stride;
+    chunk[i] = (lane % T::CH) ^ swizzle<BK>(r);
+    off[i] = (uint32_t)(min((int64_t)r, rows - 1 - first) * stride) + 16u * chunk[i];
+  }
+  const uint32_t lds0 = lds_at(lds);
+  const uint32_t to = lds0 + wave * P * 1024;
+
+  // ---- fragments
+  i32x16_t acc[T::MT][T::NT];
+#pragma unroll
+  for (int m = 0; m < T::MT; ++m)
+#pragma unroll
+    for (int n = 0; n < T::NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[m][n][i] = 0;
+  uint32_t w_at[T::KS], x_at[T::KS];
+  {
+    const int r = lane & 31;
+#pragma unroll
+    for (int s = 0; s < T::KS; ++s) {
+      const uint32_t c = 16u * ((2 * s + (lane >> 5)) ^ swizzle<BK>(r));
+      w_at[s] = lds0 + (p.wn * T::COLS + r) * BK + c;
+      x_at[s] = lds0 + T::TN * BK + (p.wm * 32 * T::MT + r) * BK + c;
+    }
+  }
+  struct Frags {
+    u32x4_t w[T::NT], x[T::MT];
+  };
+  auto read = [&](Frags& f, int s, uint32_t slot) {
+#pragma unroll
+    for (int n = 0; n < T::NT; ++n) f.w[n] = lds16(w_at[s] + slot + 32 * BK * n);
+#pragma unroll
+    for (int m = 0; m < T::MT; ++m) f.x[m] = lds16(x_at[s] + slot + 32 * BK * m);
+  };
+  auto products = [&](const Frags& f) {
+#pragma unroll
+    for (int m = 0; m < T::MT; ++m)
+#pragma unroll
+      for (int n = 0; n < T::NT; ++n) acc[m][n] = mfma(f.w[n], f.x[m], acc[m][n]);
+  };
+
+  if constexpr (DMA) {
+    static_assert(T::STAGES >= 3);
+    // Stage t is K's bytes BK t ..; chunks past K repeat the stage's first one and are made zero
+    // in W's fragments.
+    auto issue = [&](int t, uint32_t slot) {
+      const int64_t k = (int64_t)t * BK;
+      const int left = (int)min((int64_t)BK, a.K - k);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        uint32_t at = off[i];
+        if (left < BK) at = 16 * chunk[i] < left ? at : at - 16u * chunk[i];
+        dma(to + slot + 1024 * i, base[i] + k, at);
+      }
+    };
+    auto slot_of = [&](int t) { return (uint32_t)((t - t0) % T::STAGES) * (uint32_t)T::STAGE; };
+    for (int t = t0; t < min(t0 + T::STAGES - 1, t1); ++t) issue(t, slot_of(t));
+    const int tail = (int)(a.K - (int64_t)(steps - 1) * BK);  // bytes of the last stage
+    Frags f[2];
+    if (t0 < t1) {
+      if (t0 + T::STAGES - 1 <= t1) wait_dma<(T::STAGES - 2) * P>();
+      else wait_dma<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      read(f[0], 0, 0);
+    }
+    uint32_t slot = 0;
+    for (int t = t0; t < t1; ++t) {
+      // stage t + 1 is there for every wave, and every wave is done with stage t - 1
+      if (t + T::STAGES - 2 < t1) wait_dma<(T::STAGES - 3) * P>();
+      else wait_dma<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (t + T::STAGES - 1 < t1) issue(t + T::STAGES - 1, slot_of(t + T::STAGES - 1));
+      uint32_t next = slot + T::STAGE;
+      if (next == (uint32_t)(T::STAGES * T::STAGE)) next = 0;
+      const bool partial = t == steps - 1 && tail < BK;
+#pragma unroll
+      for (int s = 0; s < T::KS; ++s) {
+        Frags& now = f[s & 1];
+        if (s + 1 < T::KS) read(f[(s + 1) & 1], s + 1, slot);
+        else read(f[(s + 1) & 1], 0, next);   // (behind the last stage: read, not used)
+        if (partial) {
+          const bool in = 32 * s + 16 * (lane >> 5) < tail;
+#pragma unroll
+          for (int n = 0; n < T::NT; ++n)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) now.w[n][d] = in ? now.w[n][d] : 0u;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        products(now);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      slot = next;
+    }
+    static_assert(T::KS % 2 == 0);
+  } else {
+    // Through registers, two slots; rows at any address, K from 16 on.
+    u32x4_t held[P];
+    const int8_t* row[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int piece = wave * P + i;
+      const bool is_w = piece < T::W_PIECES;
+      const int r = (piece - (is_w ? 0 : T::W_PIECES)) * RP + lane / T::CH;
+      const int64_t first = is_w ? p.n0 : p.m0, rows = is_w ? a.N : a.M;
+      row[i] = (is_w ? a.w : a.x) +
+               min(first + r, rows - 1) * (is_w ? a.w_stride : a.x_stride);
+    }
+    auto load = [&](int t) {
+      const int64_t k0 = (int64_t)t * BK;
+      if (k0 + BK <= a.K) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) held[i] = load16(row[i] + k0 + 16 * chunk[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const int64_t k = k0 + 16 * chunk[i], at = min(k, a.K - 16);
+          held[i] = load16(row[i] + at);
+          if (wave * P + i < T::W_PIECES) held[i] = without_first(held[i], k - at);
+        }
+      }
+    };
+    auto store = [&](uint32_t slot) {
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        *(__attribute__((address_space(3))) u32x4_t*)(uintptr_t)(to + slot + 1024 * i + 16 * lane) =
+            held[i];
+      __syncthreads();
+    };
+    if (t0 < t1) {
+      load(t0);
+      store(0);
+    }
+    uint32_t slot = 0;
+    for (int t = t0; t < t1; ++t) {
+      if (t + 1 < t1) load(t + 1);
+      Frags f;
+#pragma unroll
+      for (int s = 0; s < T::KS; ++s) {
+        read(f, s, slot);
+        products(f);
+      }
+      slot ^= (uint32_t)T::STAGE;
+      if (t + 1 < t1) store(slot);
+    }
+  }
+
+  if (a.parts > 1) {
+    // the registers as they are, 16 bytes a lane
+    i32x4_t* const to_part = (i32x4_t*)a.partial +
+        ((int64_t)tile * a.parts + part) * (T::MT * T::NT * 4 * T::THREADS) + threadIdx.x;
+#pragma unroll
+    for (int m = 0; m < T::MT; ++m)
+#pragma unroll
+      for (int n = 0; n < T::NT; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          to_part[((m * T::NT + n) * 4 + g) * T::THREADS] =
+              i32x4_t{acc[m][n][4 * g], acc[m][n][4 * g + 1], acc[m][n][4 * g + 2],
+                      acc[m][n][4 * g + 3]};
+    return;
+  }
+  __syncthreads();  // (all fragments have been read)
+  finish<T>(a, p, lds, acc);
+}
+
+// The sums of a tile's parts, then its results.
+template <class T>
+__global__ void __launch_bounds__(T::THREADS) int8_join_kernel(LinearArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[T::WAVES * T::OUT];
+  const int tile = blockIdx.x;
+  const Position<T> p(a, tile);
+  i32x16_t acc[T::MT][T::NT];
+  const i32x4_t* from = (const i32x4_t*)a.partial +
+      (int64_t)tile * a.parts * (T::MT * T::NT * 4 * T::THREADS) + threadIdx.x;
+#pragma unroll
+  for (int m = 0; m < T::MT; ++m)
+#pragma unroll
+    for (int n = 0; n < T::NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[m][n][i] = 0;
+  for (int part = 0; part < a.parts; ++part, from += T::MT * T::NT * 4 * T::THREADS)
+#pragma unroll
+    for (int m = 0; m < T::MT; ++m)
+#pragma unroll
+      for (int n = 0; n < T::NT; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const i32x4_t v = from[((m * T::NT + n) * 4 + g) * T::THREADS];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][n][4 * g + i] += v[i];
+        }
+  finish<T>(a, p, lds, acc);
+}
+
+// ---- few rows: the weights' bytes through registers --------------------------------------
+
+__device__ __forceinline__ i32x4_t mfma16(u32x4_t a, u32x4_t b, i32x4_t c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a),
+                                               __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
+}
+
+// A workgroup has 16 columns and up to 16 MT rows; its waves take K's steps of 64 in turn, U at a
+// time, and add their sums in LDS.  W and X go from memory to the operands' registers.
+template <int MT, int WAVES, int U>
+__global__ void __launch_bounds__(64 * WAVES) int8_few_rows_kernel(LinearArgs a) {
+  __shared__ i32x4_t sums[WAVES][MT][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int r = lane & 15, grp = lane >> 4;
+  const int8_t* const w = a.w + min(n0 + r, a.N - 1) * a.w_stride + 16 * grp;
+  const int8_t* x[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    x[m] = a.x + min((int64_t)(16 * m + r), a.M - 1) * a.x_stride + 16 * grp;
+  // scales of the results that this thread will write: row m, columns n ..
+  const int64_t m = 16 * wave + r, n = n0 + 4 * grp;
+  float sx = 0.f, sw[4], bias[4];
+  if (wave < MT) {
+    sx = a.sx[min(m, a.M - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sw[i] = a.sw[min(n + i, a.N - 1)];
+      bias[i] = a.bias ? widen(a.bias, min(n + i, a.N - 1), a.dtype) : 0.f;
+    }
+  }
+  i32x4_t acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = i32x4_t{0, 0, 0, 0};
+  const int full = (int)(a.K / 64);
+  int t = wave;
+  for (; t + (U - 1) * WAVES < full; t += U * WAVES) {
+    u32x4_t wf[U], xf[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = 64 * (int64_t)(t + u * WAVES);
+      wf[u] = load16(w + k);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xf[u][i] = load16(x[i] + k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i] = mfma16(wf[u], xf[u][i], acc[i]);
+  }
+  for (; 64 * (int64_t)t < a.K; t += WAVES) {
+    const int64_t k0 = 64 * (int64_t)t, k = k0 + 16 * grp, at = min(k, a.K - 16);
+    u32x4_t wf = load16(w - 16 * grp + at);
+    if (k0 + 64 > a.K) wf = without_first(wf, k - at);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      acc[i] = mfma16(wf, load16(x[i] - 16 * grp + at), acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) sums[wave][i][lane] = acc[i];
+  __syncthreads();
+  if (wave >= MT) return;
+  i32x4_t s = sums[0][wave][lane];
+#pragma unroll
+  for (int v = 1; v < WAVES; ++v) s += sums[v][wave][lane];
+  if (m >= a.M) return;
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = scaled(s[i], sx, sw[i], bias[i]);
+  if (a.dtype == MRSA_DTYPE_FP32) {
+    float* const to = (float*)a.out + m * a.N + n;
+    if (n + 4 <= a.N) *reinterpret_cast<Pack<float, 4>*>(to) = Pack<float, 4>{{y[0], y[1], y[2], y[3]}};
+    else
+      for (int i = 0; i < 4; ++i)
+        if (n + i < a.N) to[i] = y[i];
+  } else {
+    uint16_t* const to = (uint16_t*)a.out + m * a.N + n;
+    const uint32_t v[2] = {pack2(y[0], y[1], a.dtype), pack2(y[2], y[3], a.dtype)};
+    if (n + 4 <= a.N) *reinterpret_cast<Pack<uint32_t, 2>*>(to) = Pack<uint32_t, 2>{{v[0], v[1]}};
+    else
+      for (int i = 0; i < 4; ++i)
+        if (n + i < a.N) to[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+  }
+}
+
+// A row of fewer than 16 values: one result a thread.
+__global__ void __launch_bounds__(256) int8_short_rows_kernel(LinearArgs a) {
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < a.M * a.N;
+       e += (int64_t)gridDim.x * 256) {
+    const int64_t m = e / a.N, n = e - m * a.N;
+    int32_t sum = 0;
+    for (int k = 0; k < a.K; ++k)
+      sum += (int32_t)a.x[m * a.x_stride + k] * a.w[n * a.w_stride + k];
+    const float y = scaled(sum, a.sx[m], a.sw[n], a.bias ? widen(a.bias, n, a.dtype) : 0.f);
+    if (a.dtype == MRSA_DTYPE_FP32) ((float*)a.out)[e] = y;
+    else ((uint16_t*)a.out)[e] = (uint16_t)pack2(y, 0.f, a.dtype);
+  }
+}
+
+typedef Tile<128, 128, 2, 2, 64, 4> Small;
+typedef Tile<256, 256, 2, 4, 64, 4> Large;
+
+// How a product is cut: by rows, size and alignment alone.
+struct Plan {
+  enum { kShort, kFew, kSmall, kLarge } kind;
+  bool dma;
+  int64_t tiles_m, tiles_n, parts, bytes;
+};
+Plan plan_of(int64_t M, int64_t N, int64_t K, bool aligned) {
+  Plan p = {Plan::kSmall, aligned, 1, 1, 1, 0};
+  if (K < 16) {
+    p.kind = Plan::kShort;
+    return p;
+  }
+  if (M <= 64) {
+    p.kind = Plan::kFew;
+    return p;
+  }
+  auto tiles = [&](int64_t tm, int64_t tn) {
+    p.tiles_m = (M + tm - 1) / tm;
+    p.tiles_n = (N + tn - 1) / tn;
+  };
+  tiles(256, 256);
+  if (aligned && p.tiles_m * p.tiles_n >= 256) {
+    p.kind = Plan::kLarge;
+    return p;
+  }
+  tiles(128, 128);
+  const int64_t steps = (K + 63) / 64, want = 512 / std::max<int64_t>(1, p.tiles_m * p.tiles_n);
+  p.parts = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 16), steps / 16));
+  if (p.parts > 1) p.bytes = p.tiles_m * p.tiles_n * p.parts * 128 * 128 * 4;
+  return p;
+}
+bool aligned_rows(const void* p, int64_t stride, int64_t rows) {
+  return (uintptr_t)p % 16 == 0 && (rows == 1 || (stride % 16 == 0 && stride < (1 << 22)));
+}
+
+template <class T>
+void launch_tiles(const LinearArgs& a, bool dma, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)a.tiles_m * a.tiles_n * a.parts)), block(T::THREADS);
+  if (dma) hipLaunchKernelGGL((int8_tile_kernel<T, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((int8_tile_kernel<T, false>), grid, block, 0, stream, a);
+  if (a.parts > 1)
+    hipLaunchKernelGGL((int8_join_kernel<T>), dim3((unsigned)(a.tiles_m * a.tiles_n)), block, 0,
+                       stream, a);
+}
+
+}  // namespace
+
+extern "C" int64_t mrsa_int8_linear_workspace_bytes(int64_t rows, int64_t out_dim, int64_t dim) {
+  if (rows < 0 || out_dim < 0 || dim < 0 || rows >= (int64_t)1 << 31 ||
+      out_dim >= (int64_t)1 << 31 || dim > 131071)
+    return -1;
+  return std::max(plan_of(rows, out_dim, dim, true).bytes,
+                  plan_of(rows, out_dim, dim, false).bytes);
+}
+
+extern "C" int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const float* x_scales,
+                                    const int8_t* weight, int64_t weight_row_stride,
+                                    const float* weight_scales, const void* bias, int64_t rows,
+                                    int64_t out_dim, int64_t dim, int32_t dtype, void* workspace,
+                                    int64_t workspace_bytes, void* out, void* stream) {
+  if (rows < 0 || out_dim < 0 || dim < 0 || x_row_stride < 0 || weight_row_stride < 0)
+    return MRSA_ERR_INVALID_ARGUMENT;
+  if (dtype != MRSA_DTYPE_BF16 && dtype != MRSA_DTYPE_FP16 && dtype != MRSA_DTYPE_FP32)
+    return MRSA_ERR_UNSUPPORTED;
+  if (dim > 131071 || rows >= (int64_t)1 << 31 || out_dim >= (int64_t)1 << 31 ||
+      x_row_stride >= (int64_t)1 << 31 || weight_row_stride >= (int64_t)1 << 31)
+    return MRSA_ERR_UNSUPPORTED;
+  if (rows == 0 || out_dim == 0) return MRSA_OK;
+  const int size = dtype == MRSA_DTYPE_FP32 ? 4 : 2;
+  if (!x_scales || !weight_scales || !out || (dim > 0 && (!x || !weight)))
+    return MRSA_ERR_INVALID_ARGUMENT;
+  if (((uintptr_t)x_scales | (uintptr_t)weight_scales) % 4 != 0 ||
+      ((uintptr_t)bias | (uintptr_t)out) % size != 0)
+    return MRSA_ERR_INVALID_ARGUMENT;
+  const bool aligned = dim % 16 == 0 && aligned_rows(x, x_row_stride, rows) &&
+                       aligned_rows(weight, weight_row_stride, out_dim);
+  const Plan p = plan_of(rows, out_dim, dim, aligned);
+  const int64_t groups = p.kind == Plan::kFew ? (out_dim + 15) / 16
+                                              : p.tiles_m * p.tiles_n * p.parts;
+  if (groups >= (int64_t)1 << 23) return MRSA_ERR_UNSUPPORTED;
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16 != 0))
+    return MRSA_ERR_INVALID_ARGUMENT;
+  const LinearArgs a = {x, weight, x_scales, weight_scales, bias, out, (int32_t*)workspace, rows,
+                        out_dim, dim, x_row_stride, weight_row_stride, dtype, (int32_t)p.parts,
+                        (int32_t)p.tiles_m, (int32_t)p.tiles_n};
+  const hipStream_t st = (hipStream_t)stream;
+  switch (p.kind) {
+    case Plan::kShort: {
+      const int64_t blocks = std::min<int64_t>((rows * out_dim + 255) / 256, 1 << 20);
+      hipLaunchKernelGGL(int8_short_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
+      break;
+    }
+    case Plan::kFew: {
+      auto kern = rows <= 16   ? int8_few_rows_kernel<1, 8, 8>
+                  : rows <= 32 ? int8_few_rows_kernel<2, 8, 4>
+                               : int8_few_rows_kernel<4, 8, 2>;
+      hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(512), 0, st, a);
+      break;
+    }
+    case Plan::kSmall: launch_tiles<Small>(a, p.dma, st); break;
+    case Plan::kLarge: launch_tiles<Large>(a, p.dma, st); break;
+  }
+  return mrsa_launch_status();
+}

@@ -215,6 +215,17 @@ SIGNATURES = {
     "mrsa_copy_pages": (
         _I, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P],
     ),
+    "mrsa_quantize_rows_fwd": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "mrsa_dequantize_rows_fwd": (_I, [_P, _I64, _P, _I64, _I64, _I, _P, _P]),
+    "mrsa_add_rms_norm_int8_fwd": (
+        _I, [_P, _I64, _P, _I64, _P, _I64, _I64, _F, _I, _P, _P, _P, _P],
+    ),
+    "mrsa_swiglu_int8_fwd": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "mrsa_int8_linear_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "mrsa_int8_linear_fwd": (
+        _I,
+        [_P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I, _P, _I64, _P, _P],
+    ),
     "mrsa_selftest_mfma_layout": (_I, [_P, _P, _P, _P]),
 }
 

@@ -21,6 +21,8 @@ import torch
 from torch import Tensor
 
 from .fusion import _fuse_bwd_impl, _fuse_impl
+from .int8_linear import (_add_rms_norm_int8_impl, _dequantize_rows_impl, _int8_linear_impl,
+                          _quantize_rows_impl, _swiglu_int8_impl)
 from .kernel_utils import _drop_mask_impl, _drop_mask_rows_impl
 from .local_attention import _local_attention_impl
 from .paged_cache import _copy_pages_impl, _paged_append_impl, _paged_attention_impl
@@ -414,6 +416,41 @@ def _(k_pages, v_pages, src, dst):
     return None
 
 
+# -- linear layers in 8 bits ------------------------------------------------
+def _rows_fake(x, dim):
+    return x.new_empty((*x.shape[:-1], dim), dtype=torch.int8), x.new_empty(x.shape[:-1],
+                                                                            dtype=torch.float32)
+
+
+@_define("quantize_rows(Tensor x) -> (Tensor, Tensor)", _quantize_rows_impl)
+def _(x):
+    return _rows_fake(x, x.shape[-1])
+
+
+@_define("dequantize_rows(Tensor values, Tensor scales, ScalarType dtype) -> Tensor",
+         _dequantize_rows_impl)
+def _(values, scales, dtype):
+    return values.new_empty(values.shape, dtype=dtype)
+
+
+@_define("add_rms_norm_int8(Tensor x, Tensor? residual, Tensor weight, float eps) "
+         "-> (Tensor, Tensor, Tensor)", _add_rms_norm_int8_impl)
+def _(x, residual, weight, eps):
+    total = x.new_empty(0 if residual is None else x.shape)
+    return (total, *_rows_fake(x, x.shape[-1]))
+
+
+@_define("swiglu_int8(Tensor gate_up) -> (Tensor, Tensor)", _swiglu_int8_impl)
+def _(gate_up):
+    return _rows_fake(gate_up, gate_up.shape[-1] // 2)
+
+
+@_define("int8_linear(Tensor x, Tensor x_scales, Tensor weight, Tensor weight_scales, "
+         "Tensor? bias, ScalarType dtype) -> Tensor", _int8_linear_impl)
+def _(x, x_scales, weight, weight_scales, bias, dtype):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=dtype)
+
+
 OPERATORS = (
     "kv_fragments", "kv_fragments_rows_", "q_fragments", "local_attention",
     "local_attention_qf", "chunk_attn_pool", "kv_fragments_pool",
@@ -422,4 +459,5 @@ OPERATORS = (
     "remote_drop_mask",
     "remote_drop_mask_rows", "candidate_token_scores", "token_keep", "token_keep_entropy",
     "gather_selected_chunk_entropy", "rotary", "paged_append_", "paged_attention", "copy_pages_",
+    "quantize_rows", "dequantize_rows", "add_rms_norm_int8", "swiglu_int8", "int8_linear",
 )
