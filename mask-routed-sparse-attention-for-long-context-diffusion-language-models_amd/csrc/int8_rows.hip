@@ -83,6 +83,22 @@ __device__ __forceinline__ void store8(typename T::elem* p, int64_t K, const flo
   }
 }
 
+// g / (1 + exp(-g)): the quotient by the hardware's reciprocal and one correction, which rounds it
+// as a division does (the divisor, from 1 to 2^127, needs no scaling).
+__device__ __forceinline__ float silu(float g) {
+  const float d = 1.f + fminf(expf(-g), 0x1p126f), r = rcp_hw(d);
+  const float q = g * r;
+  return fmaf(fmaf(-q, d, g), r, q);
+}
+
+// f + 1.5 2^23, whose low byte is the whole number nearest to f, ties to even.  (The product
+// that f is stays a number of its own: an exact half, as bf16 rows have them, is a tie.)
+__device__ __forceinline__ float whole(float f) {
+#pragma clang fp contract(off)
+  asm("" : "+v"(f));
+  return f + 12582912.f;
+}
+
 constexpr uint32_t kInfBits = 0x7f800000u;
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
@@ -195,7 +211,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) int8_rows_kernel(RowArg
       if constexpr (OP == kSwiglu) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          y[j] = y[j] * rcp_hw(1.f + exp2_hw(-kLog2e * y[j])) * T::widen(n.other.e[j]);
+          y[j] = silu(y[j]) * T::widen(n.other.e[j]);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = max(top, magnitude(y[j]));
@@ -242,20 +258,19 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) int8_rows_kernel(RowArg
     const float most = __uint_as_float(top);
     // (rows below 2^-100, whose 127 / a could pass fp32, are lifted first)
     const float lift = most < 0x1p-100f ? 0x1p100f : 1.f;
-    const float up = bad || top == 0 ? 0.f : 127.f / (most * lift);
+    const float up = bad || top == 0 ? 0.f : 1.f / (most * lift) * 127.f;
     auto put = [&](int64_t s, float (&f)[8]) {
       uint32_t v[2];
       if (lift != 1.f) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] *= lift;
       }
-      // 1.5 2^23 added: the sum's low byte is the whole number, rounded once, ties to even.
-      // |f up| <= 127 (1 + 2^-23), so it is at most 127.
+      // |f up| <= 127 (1 + 2^-22), so the whole number is at most 127.
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t q[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = __float_as_uint(fmaf(f[4 * h + j], up, 12582912.f));
+        for (int j = 0; j < 4; ++j) q[j] = __float_as_uint(whole(f[4 * h + j] * up));
         const uint32_t lo = __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400u);
         const uint32_t hi = __builtin_amdgcn_perm(q[3], q[2], 0x04000c0cu);
         v[h] = bad ? 0u : lo | hi;
