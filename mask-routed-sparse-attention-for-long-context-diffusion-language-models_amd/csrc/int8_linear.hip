@@ -11,7 +11,6 @@ using namespace mrsa;
 namespace {
 
 typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
-typedef int32_t i32x16_t __attribute__((ext_vector_type(16)));
 
 template <class E, int N>
 struct __attribute__((packed, aligned(1))) Pack {
@@ -62,30 +61,28 @@ __device__ __forceinline__ u32x4_t without_first(u32x4_t v, int64_t bytes) {
 
 // ---- many rows: tiles through LDS -------------------------------------------------------
 
-template <int TM_, int TN_, int WM_, int WN_, int BK_, int STAGES_>
+// A step is 128 bytes of K: whole cache lines.
+constexpr int kStep = 128;
+
+template <int TM_, int TN_, int WM_, int WN_>
 struct Tile {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, BK = BK_, STAGES = STAGES_;
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
-  static constexpr int MT = TM / WM / 32, NT = TN / WN / 32;   // 32 x 32 products of a wave
-  static constexpr int KS = BK / 32;
-  static constexpr int CH = BK / 16;                           // chunks of a row
-  static constexpr int STAGE = (TM + TN) * BK;                 // bytes
-  static constexpr int PIECES = STAGE / 1024 / WAVES;          // 1 KB each, of a wave
-  static constexpr int W_PIECES = TN * BK / 1024;
+  static constexpr int MT = TM / WM / 16, NT = TN / WN / 16;   // 16 x 16 products of a wave
+  static constexpr int SLOT = (TM + TN) * kStep;               // bytes of a step: W's rows, X's
+  static constexpr int PIECES = SLOT / 1024 / WAVES;           // 1 KB each, of a wave
+  static constexpr int W_PIECES = TN * kStep / 1024;
   // epilogue: a wave's scales and bias, then 32 rows of its columns
-  static constexpr int COLS = 32 * NT;
+  static constexpr int COLS = 16 * NT;
   static constexpr int ROWB = COLS * 4 + 16;
   static constexpr int OUT = 2 * COLS * 4 + 32 * ROWB;
-  static constexpr int LDS = STAGES * STAGE > WAVES * OUT ? STAGES * STAGE : WAVES * OUT;
-  static_assert(STAGE % (1024 * WAVES) == 0 && (TN * BK) % 1024 == 0 && LDS <= 160 * 1024);
+  static constexpr int LDS = 2 * SLOT > WAVES * OUT ? 2 * SLOT : WAVES * OUT;
+  static_assert(SLOT % (1024 * WAVES) == 0 && MT % 4 == 0 && NT <= MT && LDS <= 160 * 1024);
 };
 
-// Chunk c of row r lies in slot c ^ swizzle(r) of the row: sixteen rows' reads of one chunk meet
-// all banks.
-template <int BK>
-__device__ __forceinline__ int swizzle(int r) {
-  return BK == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
-}
+// Chunk c (16 bytes) of row r lies in place c ^ swizzle(r) of the row: sixteen rows' reads of one
+// chunk meet all banks.
+__device__ __forceinline__ int swizzle(int r) { return (r >> 1) & 7; }
 
 __device__ __forceinline__ u32x4_t lds16(uint32_t at) {
   return *(const __attribute__((address_space(3))) u32x4_t*)(uintptr_t)at;
@@ -93,8 +90,8 @@ __device__ __forceinline__ u32x4_t lds16(uint32_t at) {
 __device__ __forceinline__ uint32_t lds_at(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
-__device__ __forceinline__ i32x16_t mfma(u32x4_t a, u32x4_t b, i32x16_t c) {
-  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a),
+__device__ __forceinline__ i32x4_t mfma(u32x4_t a, u32x4_t b, i32x4_t c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a),
                                                __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
 }
 
@@ -105,10 +102,6 @@ __device__ __forceinline__ void dma(uint32_t to, const int8_t* base, uint32_t at
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %1" ::"s"(to),
                "s"(base), "v"(at)
                : "memory", "m0");
-}
-template <int N>
-__device__ __forceinline__ void wait_dma() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
 }
 
 // Tiles in an order that gives each XCD (workgroups go round them) a contiguous range of bands of
@@ -139,18 +132,26 @@ struct Position {
   }
 };
 
-// Sums to results.  A product's result has row 8 (i / 4) + 4 (lane / 32) + i % 4 (a column n of
-// the output, W being the first operand) in register i and column lane % 32 (a row m).  Each wave
-// turns 32 rows of its columns at a time in LDS of its own, so that rows leave as 16-byte pieces.
+template <class T>
+__device__ __forceinline__ void clear(i32x4_t (&acc)[T::MT][T::NT]) {
+#pragma unroll
+  for (int m = 0; m < T::MT; ++m)
+#pragma unroll
+    for (int n = 0; n < T::NT; ++n) acc[m][n] = i32x4_t{0, 0, 0, 0};
+}
+
+// Sums to results.  W is the products' first operand: lane l holds columns 4 (l / 16) .. + 3 of
+// row l % 16.  Each wave turns 32 rows of its columns at a time in LDS of its own, so that rows
+// leave as 16-byte pieces of whole lines.
 template <class T>
 __device__ __forceinline__ void finish(const LinearArgs& a, const Position<T>& p, uint8_t* lds,
-                                       const i32x16_t (&acc)[T::MT][T::NT]) {
+                                       const i32x4_t (&acc)[T::MT][T::NT]) {
   uint8_t* const mine = lds + p.wave * T::OUT;
   float* const scale = (float*)mine;
   float* const bias = scale + T::COLS;
   uint8_t* const rows = mine + 2 * T::COLS * 4;
   const int64_t n0 = p.n0 + p.wn * T::COLS;
-  const int64_t m0 = p.m0 + p.wm * 32 * T::MT;
+  const int64_t m0 = p.m0 + p.wm * 16 * T::MT;
   if (n0 >= a.N || m0 >= a.M) return;
   const int cols = (int)min((int64_t)T::COLS, a.N - n0);
   for (int c = p.lane; c < T::COLS; c += 64) {
@@ -160,29 +161,31 @@ __device__ __forceinline__ void finish(const LinearArgs& a, const Position<T>& p
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  const int half = p.lane >> 5, col = p.lane & 31;
+  const int quad = p.lane >> 4, col = p.lane & 15;
   const bool wide = a.dtype == MRSA_DTYPE_FP32;
 #pragma unroll
-  for (int mt = 0; mt < T::MT; ++mt) {
-    const int64_t m1 = m0 + 32 * mt;
+  for (int mt = 0; mt < T::MT; mt += 2) {
+    const int64_t m1 = m0 + 16 * mt;
     if (m1 >= a.M) break;
-    const float sx = a.sx[min(m1 + col, a.M - 1)];
 #pragma unroll
-    for (int nt = 0; nt < T::NT; ++nt)
+    for (int h = 0; h < 2; ++h) {
+      const int row = 16 * h + col;
+      const float sx = a.sx[min(m1 + row, a.M - 1)];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int c = 32 * nt + 8 * g + 4 * half;
+      for (int nt = 0; nt < T::NT; ++nt) {
+        const int c = 16 * nt + 4 * quad;
         const f32x4_t s = *(const f32x4_t*)(scale + c), b = *(const f32x4_t*)(bias + c);
         f32x4_t v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = scaled(acc[mt][nt][4 * g + i], sx, s[i], b[i]);
+        for (int i = 0; i < 4; ++i) v[i] = scaled(acc[mt + h][nt][i], sx, s[i], b[i]);
         if (wide) {
-          *(f32x4_t*)(rows + col * T::ROWB + 4 * c) = v;
+          *(f32x4_t*)(rows + row * T::ROWB + 4 * c) = v;
         } else {
-          *(u32x2_t*)(rows + col * T::ROWB + 2 * c) =
+          *(u32x2_t*)(rows + row * T::ROWB + 2 * c) =
               u32x2_t{pack2(v[0], v[1], a.dtype), pack2(v[2], v[3], a.dtype)};
         }
       }
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     const int size = wide ? 4 : 2;
@@ -209,141 +212,144 @@ __device__ __forceinline__ void finish(const LinearArgs& a, const Position<T>& p
 
 // DMA: rows 16-byte aligned and K a multiple of 16.  Otherwise rows go through registers.
 template <class T, bool DMA>
-__global__ void __launch_bounds__(T::THREADS)
+__global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 : 2))
     int8_tile_kernel(LinearArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
-  constexpr int BK = T::BK, RP = 1024 / BK, P = T::PIECES;
+  constexpr int P = T::PIECES, MT = T::MT, NT = T::NT;
   const int tiles = a.tiles_m * a.tiles_n;
   const int part = blockIdx.x / tiles, tile = blockIdx.x - part * tiles;
   const Position<T> p(a, tile);
   const int lane = p.lane, wave = p.wave;
-  const int steps = (int)((a.K + BK - 1) / BK);
+  const int steps = (int)((a.K + kStep - 1) / kStep);
   const int t0 = (int)((int64_t)steps * part / a.parts);
   const int t1 = (int)((int64_t)steps * (part + 1) / a.parts);
+  const int tail = (int)(a.K - (int64_t)(steps - 1) * kStep);  // bytes of the last step
 
-  // ---- where this wave's pieces come from: rows past the end repeat the last one
-  const int8_t* base[P];
-  uint32_t off[P];
-  int chunk[P];
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const int piece = wave * P + i;
-    const bool is_w = piece < T::W_PIECES;
-    const int r = (piece - (is_w ? 0 : T::W_PIECES)) * RP + lane / T::CH;
-    const int64_t first = is_w ? p.n0 : p.m0, rows = is_w ? a.N : a.M;
-    const int64_t stride = is_w ? a.w_stride : a.x_stride;
-    base[i] = (is_w ? a.w : a.x) + first * stride;
-    chunk[i] = (lane % T::CH) ^ swizzle<BK>(r);
-    off[i] = (uint32_t)(min((int64_t)r, rows - 1 - first) * stride) + 16u * chunk[i];
-  }
+  // ---- operands in LDS: row lane % 16 of a product, chunk lane / 16 of its 64 bytes
   const uint32_t lds0 = lds_at(lds);
+  uint32_t w_at[2], x_at[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int r = lane & 15;
+    const uint32_t c = 16u * ((4 * s + (lane >> 4)) ^ swizzle(r));
+    w_at[s] = lds0 + (p.wn * T::COLS + r) * kStep + c;
+    x_at[s] = lds0 + T::TN * kStep + (p.wm * 16 * MT + r) * kStep + c;
+  }
+  i32x4_t acc[MT][NT];
+  clear<T>(acc);
+  u32x4_t w[2][NT], x[MT];
+  // W's operands of a half step past K's end are made zero.
+  auto cut = [&](u32x4_t (&f)[NT], int s) {
+    const bool in = 64 * s + 16 * (lane >> 4) < tail;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) f[n][d] = in ? f[n][d] : 0u;
+  };
   const uint32_t to = lds0 + wave * P * 1024;
 
-  // ---- fragments
-  i32x16_t acc[T::MT][T::NT];
-#pragma unroll
-  for (int m = 0; m < T::MT; ++m)
-#pragma unroll
-    for (int n = 0; n < T::NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[m][n][i] = 0;
-  uint32_t w_at[T::KS], x_at[T::KS];
-  {
-    const int r = lane & 31;
-#pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
-      const uint32_t c = 16u * ((2 * s + (lane >> 5)) ^ swizzle<BK>(r));
-      w_at[s] = lds0 + (p.wn * T::COLS + r) * BK + c;
-      x_at[s] = lds0 + T::TN * BK + (p.wm * 32 * T::MT + r) * BK + c;
-    }
-  }
-  struct Frags {
-    u32x4_t w[T::NT], x[T::MT];
-  };
-  auto read = [&](Frags& f, int s, uint32_t slot) {
-#pragma unroll
-    for (int n = 0; n < T::NT; ++n) f.w[n] = lds16(w_at[s] + slot + 32 * BK * n);
-#pragma unroll
-    for (int m = 0; m < T::MT; ++m) f.x[m] = lds16(x_at[s] + slot + 32 * BK * m);
-  };
-  auto products = [&](const Frags& f) {
-#pragma unroll
-    for (int m = 0; m < T::MT; ++m)
-#pragma unroll
-      for (int n = 0; n < T::NT; ++n) acc[m][n] = mfma(f.w[n], f.x[m], acc[m][n]);
-  };
-
   if constexpr (DMA) {
-    static_assert(T::STAGES >= 3);
-    // Stage t is K's bytes BK t ..; chunks past K repeat the stage's first one and are made zero
-    // in W's fragments.
-    auto issue = [&](int t, uint32_t slot) {
-      const int64_t k = (int64_t)t * BK;
-      const int left = (int)min((int64_t)BK, a.K - k);
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        uint32_t at = off[i];
-        if (left < BK) at = 16 * chunk[i] < left ? at : at - 16u * chunk[i];
-        dma(to + slot + 1024 * i, base[i] + k, at);
-      }
-    };
-    auto slot_of = [&](int t) { return (uint32_t)((t - t0) % T::STAGES) * (uint32_t)T::STAGE; };
-    for (int t = t0; t < min(t0 + T::STAGES - 1, t1); ++t) issue(t, slot_of(t));
-    const int tail = (int)(a.K - (int64_t)(steps - 1) * BK);  // bytes of the last stage
-    Frags f[2];
-    if (t0 < t1) {
-      if (t0 + T::STAGES - 1 <= t1) wait_dma<(T::STAGES - 2) * P>();
-      else wait_dma<0>();
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      read(f[0], 0, 0);
-    }
-    uint32_t slot = 0;
-    for (int t = t0; t < t1; ++t) {
-      // stage t + 1 is there for every wave, and every wave is done with stage t - 1
-      if (t + T::STAGES - 2 < t1) wait_dma<(T::STAGES - 3) * P>();
-      else wait_dma<0>();
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (t + T::STAGES - 1 < t1) issue(t + T::STAGES - 1, slot_of(t + T::STAGES - 1));
-      uint32_t next = slot + T::STAGE;
-      if (next == (uint32_t)(T::STAGES * T::STAGE)) next = 0;
-      const bool partial = t == steps - 1 && tail < BK;
-#pragma unroll
-      for (int s = 0; s < T::KS; ++s) {
-        Frags& now = f[s & 1];
-        if (s + 1 < T::KS) read(f[(s + 1) & 1], s + 1, slot);
-        else read(f[(s + 1) & 1], 0, next);   // (behind the last stage: read, not used)
-        if (partial) {
-          const bool in = 32 * s + 16 * (lane >> 5) < tail;
-#pragma unroll
-          for (int n = 0; n < T::NT; ++n)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) now.w[n][d] = in ? now.w[n][d] : 0u;
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        products(now);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      slot = next;
-    }
-    static_assert(T::KS % 2 == 0);
-  } else {
-    // Through registers, two slots; rows at any address, K from 16 on.
-    u32x4_t held[P];
-    const int8_t* row[P];
+    // Where this wave's pieces come from: rows past the end repeat the last one.
+    const int8_t* base[P];
+    uint32_t off[P];
+    int chunk[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const int piece = wave * P + i;
       const bool is_w = piece < T::W_PIECES;
-      const int r = (piece - (is_w ? 0 : T::W_PIECES)) * RP + lane / T::CH;
+      const int r = (piece - (is_w ? 0 : T::W_PIECES)) * 8 + (lane >> 3);
+      const int64_t first = is_w ? p.n0 : p.m0, rows = is_w ? a.N : a.M;
+      const int64_t stride = is_w ? a.w_stride : a.x_stride;
+      base[i] = (is_w ? a.w : a.x) + first * stride;
+      chunk[i] = (lane & 7) ^ swizzle(r);
+      off[i] = (uint32_t)(min((int64_t)r, rows - 1 - first) * stride) + 16u * chunk[i];
+    }
+    // Chunks past K repeat the step's first one.
+    auto issue = [&](int t, int i, uint32_t slot) {
+      uint32_t at = off[i];
+      if (t == steps - 1 && tail < kStep) at = 16 * chunk[i] < tail ? at : at - 16u * chunk[i];
+      dma(to + slot + 1024 * i, base[i] + (int64_t)t * kStep, at);
+    };
+    auto arrived = [&] {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    uint32_t slot = 0;
+    if (t0 < t1) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) issue(t0, i, 0);
+      arrived();
+#pragma unroll
+      for (int n = 0; n < NT; ++n) w[0][n] = lds16(w_at[0] + 16 * kStep * n);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[m] = lds16(x_at[0] + 16 * kStep * m);
+      if (t0 + 1 < t1) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) issue(t0 + 1, i, T::SLOT);
+      }
+    }
+    for (int t = t0; t < t1; ++t) {
+      const bool partial = t == steps - 1 && tail < kStep;
+      const uint32_t next = slot ^ (uint32_t)T::SLOT;
+      // first half: its products, each row tile's operand replaced by the second half's
+      if (partial) cut(w[0], 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[0][n], x[m], acc[m][n]);
+        if (m < NT) w[1][m] = lds16(w_at[1] + slot + 16 * kStep * m);
+        x[m] = lds16(x_at[1] + slot + 16 * kStep * m);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (partial) cut(w[1], 1);
+      // second half: in its middle the next step has arrived for every wave, and every wave
+      // has read all of this one, whose slot the step after the next then fills
+#pragma unroll
+      for (int m = 0; m < MT / 2; ++m) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[1][n], x[m], acc[m][n]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      arrived();
+      const bool more = t + 2 < t1;
+#pragma unroll
+      for (int m = MT / 2; m < MT; ++m) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[1][n], x[m], acc[m][n]);
+        // (behind the last step: read, not used)
+        constexpr int WR = NT / (MT / 2) + (NT % (MT / 2) != 0);
+        const int j = m - MT / 2;
+#pragma unroll
+        for (int n = j * WR; n < (j + 1) * WR && n < NT; ++n)
+          w[0][n] = lds16(w_at[0] + next + 16 * kStep * n);
+        x[j] = lds16(x_at[0] + next + 16 * kStep * j);
+        x[m] = lds16(x_at[0] + next + 16 * kStep * m);
+        if (more) {
+          constexpr int EACH = (P + MT / 2 - 1) / (MT / 2);
+#pragma unroll
+          for (int i = j * EACH; i < (j + 1) * EACH && i < P; ++i) issue(t + 2, i, slot);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      slot = next;
+    }
+  } else {
+    // Through registers; rows at any address, K from 16 on.
+    u32x4_t held[P];
+    const int8_t* row[P];
+    int chunk[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int piece = wave * P + i;
+      const bool is_w = piece < T::W_PIECES;
+      const int r = (piece - (is_w ? 0 : T::W_PIECES)) * 8 + (lane >> 3);
       const int64_t first = is_w ? p.n0 : p.m0, rows = is_w ? a.N : a.M;
       row[i] = (is_w ? a.w : a.x) +
                min(first + r, rows - 1) * (is_w ? a.w_stride : a.x_stride);
+      chunk[i] = (lane & 7) ^ swizzle(r);
     }
     auto load = [&](int t) {
-      const int64_t k0 = (int64_t)t * BK;
-      if (k0 + BK <= a.K) {
+      const int64_t k0 = (int64_t)t * kStep;
+      if (k0 + kStep <= a.K) {
 #pragma unroll
         for (int i = 0; i < P; ++i) held[i] = load16(row[i] + k0 + 16 * chunk[i]);
       } else {
@@ -369,13 +375,18 @@ __global__ void __launch_bounds__(T::THREADS)
     uint32_t slot = 0;
     for (int t = t0; t < t1; ++t) {
       if (t + 1 < t1) load(t + 1);
-      Frags f;
 #pragma unroll
-      for (int s = 0; s < T::KS; ++s) {
-        read(f, s, slot);
-        products(f);
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) w[0][n] = lds16(w_at[s] + slot + 16 * kStep * n);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          x[m] = lds16(x_at[s] + slot + 16 * kStep * m);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[0][n], x[m], acc[m][n]);
+        }
       }
-      slot ^= (uint32_t)T::STAGE;
+      slot ^= (uint32_t)T::SLOT;
       if (t + 1 < t1) store(slot);
     }
   }
@@ -383,19 +394,14 @@ __global__ void __launch_bounds__(T::THREADS)
   if (a.parts > 1) {
     // the registers as they are, 16 bytes a lane
     i32x4_t* const to_part = (i32x4_t*)a.partial +
-        ((int64_t)tile * a.parts + part) * (T::MT * T::NT * 4 * T::THREADS) + threadIdx.x;
+        ((int64_t)tile * a.parts + part) * (MT * NT * T::THREADS) + threadIdx.x;
 #pragma unroll
-    for (int m = 0; m < T::MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int n = 0; n < T::NT; ++n)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          to_part[((m * T::NT + n) * 4 + g) * T::THREADS] =
-              i32x4_t{acc[m][n][4 * g], acc[m][n][4 * g + 1], acc[m][n][4 * g + 2],
-                      acc[m][n][4 * g + 3]};
+      for (int n = 0; n < NT; ++n) to_part[(m * NT + n) * T::THREADS] = acc[m][n];
     return;
   }
-  __syncthreads();  // (all fragments have been read)
+  __syncthreads();  // (all operands have been read)
   finish<T>(a, p, lds, acc);
 }
 
@@ -405,35 +411,19 @@ __global__ void __launch_bounds__(T::THREADS) int8_join_kernel(LinearArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[T::WAVES * T::OUT];
   const int tile = blockIdx.x;
   const Position<T> p(a, tile);
-  i32x16_t acc[T::MT][T::NT];
+  i32x4_t acc[T::MT][T::NT];
   const i32x4_t* from = (const i32x4_t*)a.partial +
-      (int64_t)tile * a.parts * (T::MT * T::NT * 4 * T::THREADS) + threadIdx.x;
-#pragma unroll
-  for (int m = 0; m < T::MT; ++m)
-#pragma unroll
-    for (int n = 0; n < T::NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[m][n][i] = 0;
-  for (int part = 0; part < a.parts; ++part, from += T::MT * T::NT * 4 * T::THREADS)
+      (int64_t)tile * a.parts * (T::MT * T::NT * T::THREADS) + threadIdx.x;
+  clear<T>(acc);
+  for (int part = 0; part < a.parts; ++part, from += T::MT * T::NT * T::THREADS)
 #pragma unroll
     for (int m = 0; m < T::MT; ++m)
 #pragma unroll
-      for (int n = 0; n < T::NT; ++n)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const i32x4_t v = from[((m * T::NT + n) * 4 + g) * T::THREADS];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][n][4 * g + i] += v[i];
-        }
+      for (int n = 0; n < T::NT; ++n) acc[m][n] += from[(m * T::NT + n) * T::THREADS];
   finish<T>(a, p, lds, acc);
 }
 
 // ---- few rows: the weights' bytes through registers --------------------------------------
-
-__device__ __forceinline__ i32x4_t mfma16(u32x4_t a, u32x4_t b, i32x4_t c) {
-  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a),
-                                               __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
-}
 
 // A workgroup has 16 columns and up to 16 MT rows; its waves take K's steps of 64 in turn, U at a
 // time, and add their sums in LDS.  W and X go from memory to the operands' registers.
@@ -477,7 +467,7 @@ __global__ void __launch_bounds__(64 * WAVES) int8_few_rows_kernel(LinearArgs a)
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i] = mfma16(wf[u], xf[u][i], acc[i]);
+      for (int i = 0; i < MT; ++i) acc[i] = mfma(wf[u], xf[u][i], acc[i]);
   }
   for (; 64 * (int64_t)t < a.K; t += WAVES) {
     const int64_t k0 = 64 * (int64_t)t, k = k0 + 16 * grp, at = min(k, a.K - 16);
@@ -485,7 +475,7 @@ __global__ void __launch_bounds__(64 * WAVES) int8_few_rows_kernel(LinearArgs a)
     if (k0 + 64 > a.K) wf = without_first(wf, k - at);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
-      acc[i] = mfma16(wf, load16(x[i] - 16 * grp + at), acc[i]);
+      acc[i] = mfma(wf, load16(x[i] - 16 * grp + at), acc[i]);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) sums[wave][i][lane] = acc[i];
@@ -528,8 +518,8 @@ __global__ void __launch_bounds__(256) int8_short_rows_kernel(LinearArgs a) {
   }
 }
 
-typedef Tile<128, 128, 2, 2, 64, 4> Small;
-typedef Tile<256, 256, 2, 4, 64, 4> Large;
+typedef Tile<128, 128, 2, 2> Small;
+typedef Tile<256, 256, 2, 4> Large;
 
 // How a product is cut: by rows, size and alignment alone.
 struct Plan {
@@ -551,14 +541,14 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, bool aligned) {
     p.tiles_m = (M + tm - 1) / tm;
     p.tiles_n = (N + tn - 1) / tn;
   };
-  tiles(256, 256);
+  tiles(Large::TM, Large::TN);
   if (aligned && p.tiles_m * p.tiles_n >= 256) {
     p.kind = Plan::kLarge;
     return p;
   }
   tiles(128, 128);
-  const int64_t steps = (K + 63) / 64, want = 512 / std::max<int64_t>(1, p.tiles_m * p.tiles_n);
-  p.parts = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 16), steps / 16));
+  const int64_t steps = (K + kStep - 1) / kStep, want = 512 / std::max<int64_t>(1, p.tiles_m * p.tiles_n);
+  p.parts = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 16), steps / 8));
   if (p.parts > 1) p.bytes = p.tiles_m * p.tiles_n * p.parts * 128 * 128 * 4;
   return p;
 }

@@ -23,14 +23,13 @@ hand-written HIP kernels in ../csrc (C ABI: include/mrsa.h).  Module map:
     rotary.py           rotary_qk (with its gradient), rotary_tables, rotary_frequencies
     paged_cache.py      PagedKVCache, paged_cache_append, paged_cached_attention,
                         copy_cache_pages: several sequences' K/V in shared pages
-    int8_linear.py      quantize_rows, add_rms_norm_int8, swiglu_int8, int8_linear,
+    int8.py             quantize_rows, add_rms_norm_int8, swiglu_int8, int8_linear,
                         dequantize_rows: linear layers in 8-bit integers
     ops.py              torch.ops.mrsa.* custom operators (schemas, CUDA and fake kernels)
 """
 
 from .fusion import fuse_hils_outputs
-from .int8_linear import (add_rms_norm_int8, dequantize_rows, int8_linear, quantize_rows,
-                          swiglu_int8)
+from .int8 import (add_rms_norm_int8, dequantize_rows, int8_linear, quantize_rows, swiglu_int8)
 from .kernel_utils import (
     chunk_aligned_local_bounds,
     group_pad_to,

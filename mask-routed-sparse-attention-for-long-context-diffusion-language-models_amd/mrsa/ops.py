@@ -21,8 +21,8 @@ import torch
 from torch import Tensor
 
 from .fusion import _fuse_bwd_impl, _fuse_impl
-from .int8_linear import (_add_rms_norm_int8_impl, _dequantize_rows_impl, _int8_linear_impl,
-                          _quantize_rows_impl, _swiglu_int8_impl)
+from .int8 import (_add_rms_norm_int8_impl, _dequantize_rows_impl, _int8_linear_impl,
+                   _quantize_rows_impl, _swiglu_int8_impl)
 from .kernel_utils import _drop_mask_impl, _drop_mask_rows_impl
 from .local_attention import _local_attention_impl
 from .paged_cache import _copy_pages_impl, _paged_append_impl, _paged_attention_impl
