@@ -72,17 +72,22 @@ struct Tile {
   static constexpr int SLOT = (TM + TN) * kStep;               // bytes of a step: W's rows, X's
   static constexpr int PIECES = SLOT / 1024 / WAVES;           // 1 KB each, of a wave
   static constexpr int W_PIECES = TN * kStep / 1024;
-  // epilogue: a wave's scales and bias, then 32 rows of its columns
   static constexpr int COLS = 16 * NT;
-  static constexpr int ROWB = COLS * 4 + 16;
-  static constexpr int OUT = 2 * COLS * 4 + 32 * ROWB;
-  static constexpr int LDS = 2 * SLOT > WAVES * OUT ? 2 * SLOT : WAVES * OUT;
-  static_assert(SLOT % (1024 * WAVES) == 0 && MT % 4 == 0 && NT <= MT && LDS <= 160 * 1024);
+  static constexpr int SCALES = 2 * COLS + 16 * MT;            // floats, of a wave
+  static constexpr int LDS = 2 * SLOT + 4 * WAVES * SCALES;
+  static_assert(SLOT % (1024 * WAVES) == 0 && MT % 4 == 0 && NT <= MT && NT == 4 &&
+                LDS <= 160 * 1024);
 };
 
-// Chunk c (16 bytes) of row r lies in place c ^ swizzle(r) of the row: sixteen rows' reads of one
-// chunk meet all banks.
+// Chunk c (16 bytes) of row r lies in place c ^ swizzle(r) of the row: the sixteen rows of a
+// product's operand meet all banks.  X's are 16 consecutive ones; W's are those of column_of, so
+// that a lane's results of two products are eight consecutive columns.
 __device__ __forceinline__ int swizzle(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ int swizzle_w(int r) { return ((r >> 1) & 1) | ((r >> 3) & 3) << 1; }
+// The column of W's product nt that its operand's row r is.
+__device__ __forceinline__ int column_of(int nt, int r) {
+  return 32 * (nt >> 1) + 8 * (r >> 2) + 4 * (nt & 1) + (r & 3);
+}
 
 __device__ __forceinline__ u32x4_t lds16(uint32_t at) {
   return *(const __attribute__((address_space(3))) u32x4_t*)(uintptr_t)at;
@@ -95,12 +100,20 @@ __device__ __forceinline__ i32x4_t mfma(u32x4_t a, u32x4_t b, i32x4_t c) {
                                                __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
 }
 
+__device__ __forceinline__ const int8_t* uniform(const int8_t* p) {
+  const uint64_t v = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (const int8_t*)(uintptr_t)((uint64_t)hi << 32 | lo);
+}
+
 // 1 KB of LDS from `to` on, lane l's 16 bytes from base + at.  As asm, since after the builtin
 // the compiler waits for all DMA in flight before the next LDS read; the loop's own waits order
 // them.  (s_nop: m0 and scalars that a vector instruction has just written.)
 __device__ __forceinline__ void dma(uint32_t to, const int8_t* base, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %1" ::"s"(to),
-               "s"(base), "v"(at)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %1" ::"s"(
+                   __builtin_amdgcn_readfirstlane(to)),
+               "s"(uniform(base)), "v"(at)
                : "memory", "m0");
 }
 
@@ -112,8 +125,8 @@ __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int& tm
   const int t = xcd * each + min(xcd, more) + i;
   const int band = t / (8 * tiles_n), rest = t - band * 8 * tiles_n;
   const int rows = min(8, tiles_m - 8 * band);
-  tn = rest / rows;
-  tm = 8 * band + rest - tn * rows;
+  tn = __builtin_amdgcn_readfirstlane(rest / rows);
+  tm = __builtin_amdgcn_readfirstlane(8 * band + rest - tn * rows);
 }
 
 template <class T>
@@ -132,6 +145,14 @@ struct Position {
   }
 };
 
+// Four bytes a lane.
+__device__ __forceinline__ void dma4(uint32_t to, const int8_t* base, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %2, %1" ::"s"(
+                   __builtin_amdgcn_readfirstlane(to)),
+               "s"(uniform(base)), "v"(at)
+               : "memory", "m0");
+}
+
 template <class T>
 __device__ __forceinline__ void clear(i32x4_t (&acc)[T::MT][T::NT]) {
 #pragma unroll
@@ -140,77 +161,92 @@ __device__ __forceinline__ void clear(i32x4_t (&acc)[T::MT][T::NT]) {
     for (int n = 0; n < T::NT; ++n) acc[m][n] = i32x4_t{0, 0, 0, 0};
 }
 
-// Sums to results.  W is the products' first operand: lane l holds columns 4 (l / 16) .. + 3 of
-// row l % 16.  Each wave turns 32 rows of its columns at a time in LDS of its own, so that rows
-// leave as 16-byte pieces of whole lines.
+// The scales (and the bias) of the wave's columns and rows, to LDS of its own: [columns], [bias],
+// [rows].  By DMA, behind which the first operands are waited for anyway; a bias is loaded where
+// there is one, so that nothing else depends on its type.
 template <class T>
-__device__ __forceinline__ void finish(const LinearArgs& a, const Position<T>& p, uint8_t* lds,
-                                       const i32x4_t (&acc)[T::MT][T::NT]) {
-  uint8_t* const mine = lds + p.wave * T::OUT;
-  float* const scale = (float*)mine;
-  float* const bias = scale + T::COLS;
-  uint8_t* const rows = mine + 2 * T::COLS * 4;
-  const int64_t n0 = p.n0 + p.wn * T::COLS;
-  const int64_t m0 = p.m0 + p.wm * 16 * T::MT;
-  if (n0 >= a.N || m0 >= a.M) return;
-  const int cols = (int)min((int64_t)T::COLS, a.N - n0);
-  for (int c = p.lane; c < T::COLS; c += 64) {
-    const int64_t n = n0 + min(c, cols - 1);
-    scale[c] = a.sw[n];
-    bias[c] = a.bias ? widen(a.bias, n, a.dtype) : 0.f;
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  const int quad = p.lane >> 4, col = p.lane & 15;
-  const bool wide = a.dtype == MRSA_DTYPE_FP32;
+__device__ __forceinline__ void fetch_scales(const LinearArgs& a, const Position<T>& p,
+                                             float* scales) {
+  const int64_t n0 = min(p.n0 + p.wn * T::COLS, a.N - 1);
+  const int64_t m0 = min(p.m0 + p.wm * 16 * T::MT, a.M - 1);
+  const uint32_t to = lds_at(scales);
+  static_assert(T::COLS == 64);
+  const int64_t n = min(n0 + p.lane, a.N - 1);
+  dma4(to, (const int8_t*)(a.sw + n0), 4u * (uint32_t)(n - n0));
 #pragma unroll
-  for (int mt = 0; mt < T::MT; mt += 2) {
-    const int64_t m1 = m0 + 16 * mt;
-    if (m1 >= a.M) break;
+  for (int i = 0; i < T::MT / 4; ++i)
+    dma4(to + 4 * (2 * T::COLS + 64 * i), (const int8_t*)(a.sx + m0),
+         4u * (uint32_t)(min(m0 + 64 * i + p.lane, a.M - 1) - m0));
+  scales[T::COLS + p.lane] = a.bias ? widen(a.bias, n, a.dtype) : 0.f;
+}
+
+// Sums to results.  W is the products' first operand: lane l holds, of row l % 16, columns
+// 8 (l / 16) .. + 7 of two products: 16 bytes (or 32) to write, 64 bytes of a row by one
+// instruction.
+template <class T>
+__device__ __forceinline__ void finish(const LinearArgs& a, const Position<T>& p,
+                                       const float* scales, const i32x4_t (&acc)[T::MT][T::NT]) {
+  constexpr int PAIRS = T::NT / 2;
+  const int c0 = 8 * (p.lane >> 4);
+  const int64_t n0 = p.n0 + p.wn * T::COLS + c0;
+  const int64_t m0 = p.m0 + p.wm * 16 * T::MT + (p.lane & 15);
+  const bool wide = a.dtype == MRSA_DTYPE_FP32;
+  float scale[PAIRS][8], bias[PAIRS][8];
+#pragma unroll
+  for (int q = 0; q < PAIRS; ++q)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = 16 * h + col;
-      const float sx = a.sx[min(m1 + row, a.M - 1)];
+      const f32x4_t s = *(const f32x4_t*)(scales + 32 * q + c0 + 4 * h);
+      const f32x4_t b = *(const f32x4_t*)(scales + T::COLS + 32 * q + c0 + 4 * h);
 #pragma unroll
-      for (int nt = 0; nt < T::NT; ++nt) {
-        const int c = 16 * nt + 4 * quad;
-        const f32x4_t s = *(const f32x4_t*)(scale + c), b = *(const f32x4_t*)(bias + c);
-        f32x4_t v;
+      for (int i = 0; i < 4; ++i) {
+        scale[q][4 * h + i] = s[i];
+        bias[q][4 * h + i] = b[i];
+      }
+    }
+  float sx[T::MT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = scaled(acc[mt + h][nt][i], sx, s[i], b[i]);
-        if (wide) {
-          *(f32x4_t*)(rows + row * T::ROWB + 4 * c) = v;
+  for (int mt = 0; mt < T::MT; ++mt) sx[mt] = scales[2 * T::COLS + 16 * mt + (p.lane & 15)];
+#pragma unroll
+  for (int mt = 0; mt < T::MT; ++mt) {
+    const int64_t m = m0 + 16 * mt;
+    if (m >= a.M) break;
+#pragma unroll
+    for (int q = 0; q < PAIRS; ++q) {
+      const int64_t n = n0 + 32 * q;
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        y[i] = scaled(acc[mt][2 * q + (i >> 2)][i & 3], sx[mt], scale[q][i], bias[q][i]);
+      if (wide) {
+        float* const to = (float*)a.out + m * a.N + n;
+        if (n + 8 <= a.N) {
+          *reinterpret_cast<Pack<float, 4>*>(to) = Pack<float, 4>{{y[0], y[1], y[2], y[3]}};
+          *reinterpret_cast<Pack<float, 4>*>(to + 4) = Pack<float, 4>{{y[4], y[5], y[6], y[7]}};
         } else {
-          *(u32x2_t*)(rows + row * T::ROWB + 2 * c) =
-              u32x2_t{pack2(v[0], v[1], a.dtype), pack2(v[2], v[3], a.dtype)};
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (n + i < a.N) to[i] = y[i];
+        }
+      } else {
+        uint16_t* const to = (uint16_t*)a.out + m * a.N + n;
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = pack2(y[2 * i], y[2 * i + 1], a.dtype);
+        if (n + 8 <= a.N) {
+          *reinterpret_cast<Pack<uint32_t, 4>*>(to) = Pack<uint32_t, 4>{{v[0], v[1], v[2], v[3]}};
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (n + i < a.N) to[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
         }
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int size = wide ? 4 : 2;
-    const int per_row = T::COLS * size / 16;      // 16-byte pieces
-    const int there = (int)min((int64_t)32, a.M - m1);
-    for (int at = p.lane; at < 32 * per_row; at += 64) {
-      const int r = at / per_row, piece = at - r * per_row, c = piece * (16 / size);
-      if (r >= there || c >= cols) continue;
-      const uint8_t* const from = rows + r * T::ROWB + 16 * piece;
-      uint8_t* const to = (uint8_t*)a.out + ((m1 + r) * a.N + n0 + c) * size;
-      if (c + 16 / size <= cols) {
-        const u32x4_t v = *(const u32x4_t*)from;
-        *reinterpret_cast<Pack<uint32_t, 4>*>(to) = Pack<uint32_t, 4>{{v[0], v[1], v[2], v[3]}};
-      } else if (wide) {
-        for (int i = 0; i < cols - c; ++i) ((float*)to)[i] = ((const float*)from)[i];
-      } else {
-        for (int i = 0; i < cols - c; ++i) ((uint16_t*)to)[i] = ((const uint16_t*)from)[i];
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
-// DMA: rows 16-byte aligned and K a multiple of 16.  Otherwise rows go through registers.
+// A workgroup computes one part of K of a tile.  DMA: rows 16-byte aligned and K a multiple of 16.
+// Otherwise rows go through registers.
 template <class T, bool DMA>
 __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 : 2))
     int8_tile_kernel(LinearArgs a) {
@@ -218,23 +254,31 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
   constexpr int P = T::PIECES, MT = T::MT, NT = T::NT;
   const int tiles = a.tiles_m * a.tiles_n;
   const int part = blockIdx.x / tiles, tile = blockIdx.x - part * tiles;
-  const Position<T> p(a, tile);
-  const int lane = p.lane, wave = p.wave;
   const int steps = (int)((a.K + kStep - 1) / kStep);
+  const int tail = (int)(a.K - (int64_t)(steps - 1) * kStep);  // bytes of the last step
   const int t0 = (int)((int64_t)steps * part / a.parts);
   const int t1 = (int)((int64_t)steps * (part + 1) / a.parts);
-  const int tail = (int)(a.K - (int64_t)(steps - 1) * kStep);  // bytes of the last step
+  const Position<T> p(a, tile);
+  float* const scales = (float*)(lds + 2 * T::SLOT) + p.wave * T::SCALES;
+  if (a.parts == 1) fetch_scales<T>(a, p, scales);
+  const int lane = p.lane, wave = p.wave;
 
-  // ---- operands in LDS: row lane % 16 of a product, chunk lane / 16 of its 64 bytes
+  // ---- operands in LDS: row lane % 16 of a product, chunk lane / 16 of its 64 bytes.  (Products
+  // 2 i and 2 i + 1 of W: rows 32 i .., the second's four further on.)
   const uint32_t lds0 = lds_at(lds);
   uint32_t w_at[2], x_at[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const int r = lane & 15;
-    const uint32_t c = 16u * ((4 * s + (lane >> 4)) ^ swizzle(r));
-    w_at[s] = lds0 + (p.wn * T::COLS + r) * kStep + c;
-    x_at[s] = lds0 + T::TN * kStep + (p.wm * 16 * MT + r) * kStep + c;
+    const int r = lane & 15, c = 4 * s + (lane >> 4), rw = column_of(0, r);
+    w_at[s] = lds0 + (p.wn * T::COLS + rw) * kStep + 16u * (c ^ swizzle_w(rw));
+    x_at[s] = lds0 + T::TN * kStep + (p.wm * 16 * MT + r) * kStep + 16u * (c ^ swizzle(r));
   }
+  auto w_read = [&](int s, int n, uint32_t slot) {
+    return lds16(w_at[s] + slot + kStep * column_of(n, 0));
+  };
+  auto x_read = [&](int s, int m, uint32_t slot) {
+    return lds16(x_at[s] + slot + 16 * kStep * m);
+  };
   i32x4_t acc[MT][NT];
   clear<T>(acc);
   u32x4_t w[2][NT], x[MT];
@@ -247,46 +291,59 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
       for (int d = 0; d < 4; ++d) f[n][d] = in ? f[n][d] : 0u;
   };
   const uint32_t to = lds0 + wave * P * 1024;
+  auto row_of = [&](int i, int l) {  // piece i of the wave: rows 8 at a time of W, then of X
+    const int piece = wave * P + i;
+    return (piece - (piece < T::W_PIECES ? 0 : T::W_PIECES)) * 8 + (l >> 3);
+  };
+  auto chunk_of = [&](int i, int l) {
+    const int r = row_of(i, l);
+    return (l & 7) ^ (wave * P + i < T::W_PIECES ? swizzle_w(r) : swizzle(r));
+  };
 
   if constexpr (DMA) {
     // Where this wave's pieces come from: rows past the end repeat the last one.
-    const int8_t* base[P];
+    const int8_t* const w_from = uniform(a.w + p.n0 * a.w_stride);
+    const int8_t* const x_from = uniform(a.x + p.m0 * a.x_stride);
     uint32_t off[P];
-    int chunk[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const int piece = wave * P + i;
-      const bool is_w = piece < T::W_PIECES;
-      const int r = (piece - (is_w ? 0 : T::W_PIECES)) * 8 + (lane >> 3);
-      const int64_t first = is_w ? p.n0 : p.m0, rows = is_w ? a.N : a.M;
-      const int64_t stride = is_w ? a.w_stride : a.x_stride;
-      base[i] = (is_w ? a.w : a.x) + first * stride;
-      chunk[i] = (lane & 7) ^ swizzle(r);
-      off[i] = (uint32_t)(min((int64_t)r, rows - 1 - first) * stride) + 16u * chunk[i];
+      const bool is_w = wave * P + i < T::W_PIECES;
+      const int64_t last = is_w ? a.N - 1 - p.n0 : a.M - 1 - p.m0;
+      off[i] = (uint32_t)(min((int64_t)row_of(i, lane), last) * (is_w ? a.w_stride : a.x_stride)) +
+               16u * chunk_of(i, lane);
     }
-    // Chunks past K repeat the step's first one.
+    // Before the step that K ends in: its chunks past K repeat the step's first one.
+    auto trim = [&](int t) {
+      if (t != steps - 1 || tail == kStep) return;
+      int l = lane;
+      asm volatile("" : "+v"(l));  // (a branch, which hardly any step takes)
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int c = 16 * chunk_of(i, l);
+        if (c >= tail) off[i] -= c;
+      }
+    };
     auto issue = [&](int t, int i, uint32_t slot) {
-      uint32_t at = off[i];
-      if (t == steps - 1 && tail < kStep) at = 16 * chunk[i] < tail ? at : at - 16u * chunk[i];
-      dma(to + slot + 1024 * i, base[i] + (int64_t)t * kStep, at);
+      dma(to + slot + 1024 * i,
+          (wave * P + i < T::W_PIECES ? w_from : x_from) + (int64_t)t * kStep, off[i]);
     };
     auto arrived = [&] {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
-    uint32_t slot = 0;
-    if (t0 < t1) {
+    trim(t0);
 #pragma unroll
-      for (int i = 0; i < P; ++i) issue(t0, i, 0);
-      arrived();
+    for (int i = 0; i < P; ++i) issue(t0, i, 0);
+    arrived();
 #pragma unroll
-      for (int n = 0; n < NT; ++n) w[0][n] = lds16(w_at[0] + 16 * kStep * n);
+    for (int n = 0; n < NT; ++n) w[0][n] = w_read(0, n, 0);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) x[m] = lds16(x_at[0] + 16 * kStep * m);
-      if (t0 + 1 < t1) {
+    for (int m = 0; m < MT; ++m) x[m] = x_read(0, m, 0);
+    if (t0 + 1 < t1) {
+      trim(t0 + 1);
 #pragma unroll
-        for (int i = 0; i < P; ++i) issue(t0 + 1, i, T::SLOT);
-      }
+      for (int i = 0; i < P; ++i) issue(t0 + 1, i, T::SLOT);
     }
+    uint32_t slot = 0;
     for (int t = t0; t < t1; ++t) {
       const bool partial = t == steps - 1 && tail < kStep;
       const uint32_t next = slot ^ (uint32_t)T::SLOT;
@@ -296,8 +353,8 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
       for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[0][n], x[m], acc[m][n]);
-        if (m < NT) w[1][m] = lds16(w_at[1] + slot + 16 * kStep * m);
-        x[m] = lds16(x_at[1] + slot + 16 * kStep * m);
+        if (m < NT) w[1][m] = w_read(1, m, slot);
+        x[m] = x_read(1, m, slot);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (partial) cut(w[1], 1);
@@ -311,18 +368,18 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
       }
       arrived();
       const bool more = t + 2 < t1;
+      if (more) trim(t + 2);
 #pragma unroll
       for (int m = MT / 2; m < MT; ++m) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[1][n], x[m], acc[m][n]);
         // (behind the last step: read, not used)
-        constexpr int WR = NT / (MT / 2) + (NT % (MT / 2) != 0);
+        constexpr int WR = (NT + MT / 2 - 1) / (MT / 2);
         const int j = m - MT / 2;
 #pragma unroll
-        for (int n = j * WR; n < (j + 1) * WR && n < NT; ++n)
-          w[0][n] = lds16(w_at[0] + next + 16 * kStep * n);
-        x[j] = lds16(x_at[0] + next + 16 * kStep * j);
-        x[m] = lds16(x_at[0] + next + 16 * kStep * m);
+        for (int n = j * WR; n < (j + 1) * WR && n < NT; ++n) w[0][n] = w_read(0, n, next);
+        x[j] = x_read(0, j, next);
+        x[m] = x_read(0, m, next);
         if (more) {
           constexpr int EACH = (P + MT / 2 - 1) / (MT / 2);
 #pragma unroll
@@ -336,26 +393,22 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
     // Through registers; rows at any address, K from 16 on.
     u32x4_t held[P];
     const int8_t* row[P];
-    int chunk[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const int piece = wave * P + i;
-      const bool is_w = piece < T::W_PIECES;
-      const int r = (piece - (is_w ? 0 : T::W_PIECES)) * 8 + (lane >> 3);
-      const int64_t first = is_w ? p.n0 : p.m0, rows = is_w ? a.N : a.M;
+      const bool is_w = wave * P + i < T::W_PIECES;
       row[i] = (is_w ? a.w : a.x) +
-               min(first + r, rows - 1) * (is_w ? a.w_stride : a.x_stride);
-      chunk[i] = (lane & 7) ^ swizzle(r);
+               min((is_w ? p.n0 : p.m0) + row_of(i, lane), (is_w ? a.N : a.M) - 1) *
+                   (is_w ? a.w_stride : a.x_stride);
     }
     auto load = [&](int t) {
       const int64_t k0 = (int64_t)t * kStep;
       if (k0 + kStep <= a.K) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) held[i] = load16(row[i] + k0 + 16 * chunk[i]);
+        for (int i = 0; i < P; ++i) held[i] = load16(row[i] + k0 + 16 * chunk_of(i, lane));
       } else {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const int64_t k = k0 + 16 * chunk[i], at = min(k, a.K - 16);
+          const int64_t k = k0 + 16 * chunk_of(i, lane), at = min(k, a.K - 16);
           held[i] = load16(row[i] + at);
           if (wave * P + i < T::W_PIECES) held[i] = without_first(held[i], k - at);
         }
@@ -368,20 +421,18 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
             held[i];
       __syncthreads();
     };
-    if (t0 < t1) {
-      load(t0);
-      store(0);
-    }
+    load(t0);
+    store(0);
     uint32_t slot = 0;
     for (int t = t0; t < t1; ++t) {
       if (t + 1 < t1) load(t + 1);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) w[0][n] = lds16(w_at[s] + slot + 16 * kStep * n);
+        for (int n = 0; n < NT; ++n) w[0][n] = w_read(s, n, slot);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          x[m] = lds16(x_at[s] + slot + 16 * kStep * m);
+          x[m] = x_read(s, m, slot);
 #pragma unroll
           for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[0][n], x[m], acc[m][n]);
         }
@@ -389,8 +440,8 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
       slot ^= (uint32_t)T::SLOT;
       if (t + 1 < t1) store(slot);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the scales)
   }
-
   if (a.parts > 1) {
     // the registers as they are, 16 bytes a lane
     i32x4_t* const to_part = (i32x4_t*)a.partial +
@@ -401,16 +452,17 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
       for (int n = 0; n < NT; ++n) to_part[(m * NT + n) * T::THREADS] = acc[m][n];
     return;
   }
-  __syncthreads();  // (all operands have been read)
-  finish<T>(a, p, lds, acc);
+  finish<T>(a, p, scales, acc);
 }
 
 // The sums of a tile's parts, then its results.
 template <class T>
 __global__ void __launch_bounds__(T::THREADS) int8_join_kernel(LinearArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[T::WAVES * T::OUT];
+  __shared__ __attribute__((aligned(16))) float scales_of[T::WAVES][T::SCALES];
   const int tile = blockIdx.x;
   const Position<T> p(a, tile);
+  float* const scales = scales_of[p.wave];
+  fetch_scales<T>(a, p, scales);
   i32x4_t acc[T::MT][T::NT];
   const i32x4_t* from = (const i32x4_t*)a.partial +
       (int64_t)tile * a.parts * (T::MT * T::NT * T::THREADS) + threadIdx.x;
@@ -420,87 +472,193 @@ __global__ void __launch_bounds__(T::THREADS) int8_join_kernel(LinearArgs a) {
     for (int m = 0; m < T::MT; ++m)
 #pragma unroll
       for (int n = 0; n < T::NT; ++n) acc[m][n] += from[(m * T::NT + n) * T::THREADS];
-  finish<T>(a, p, lds, acc);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the scales)
+  finish<T>(a, p, scales, acc);
 }
 
-// ---- few rows: the weights' bytes through registers --------------------------------------
+// ---- few rows: the weights' bytes ---------------------------------------------------------
 
-// A workgroup has 16 columns and up to 16 MT rows; its waves take K's steps of 64 in turn, U at a
-// time, and add their sums in LDS.  W and X go from memory to the operands' registers.
+// Four results of row m from column n on.
+__device__ __forceinline__ void put4(const LinearArgs& a, int64_t m, int64_t n, i32x4_t sum) {
+  if (m >= a.M) return;
+  const float sx = a.sx[m];
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t c = min(n + i, a.N - 1);
+    y[i] = scaled(sum[i], sx, a.sw[c], a.bias ? widen(a.bias, c, a.dtype) : 0.f);
+  }
+  if (a.dtype == MRSA_DTYPE_FP32) {
+    float* const to = (float*)a.out + m * a.N + n;
+    if (n + 4 <= a.N) {
+      *reinterpret_cast<Pack<float, 4>*>(to) = Pack<float, 4>{{y[0], y[1], y[2], y[3]}};
+    } else {
+      for (int i = 0; i < 4; ++i)
+        if (n + i < a.N) to[i] = y[i];
+    }
+  } else {
+    uint16_t* const to = (uint16_t*)a.out + m * a.N + n;
+    const uint32_t v[2] = {pack2(y[0], y[1], a.dtype), pack2(y[2], y[3], a.dtype)};
+    if (n + 4 <= a.N) {
+      *reinterpret_cast<Pack<uint32_t, 2>*>(to) = Pack<uint32_t, 2>{{v[0], v[1]}};
+    } else {
+      for (int i = 0; i < 4; ++i)
+        if (n + i < a.N) to[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// Aligned rows, by DMA: consecutive lanes fetch consecutive bytes of a row, which operands loaded
+// straight from memory (16 rows side by side) do not.  A workgroup has 16 NT columns and up to 16 MT
+// rows; its waves take K's steps of 128 in turn, each through a ring of its own in LDS, RING steps
+// deep, without barriers, and add their sums in the end.
+template <int MT, int NT, int WAVES, int RING>
+__global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
+  constexpr int P = 2 * NT + 2 * MT, SLOT = P * 1024, Q = MT * NT;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * RING * SLOT];
+  static_assert(Q * 1024 <= RING * SLOT && RING >= 2 && RING <= 4);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
+  const int r = lane & 15, grp = lane >> 4;
+  const int K = (int)a.K, steps = (K + kStep - 1) / kStep, tail = K - (steps - 1) * kStep;
+  const int mine = steps > wave ? (steps - wave - 1) / WAVES + 1 : 0;
+  const uint32_t ring = lds_at(lds) + wave * RING * SLOT;
+  // piece i: rows 8 i .. of W, then of X
+  uint32_t off[P];
+  int chunk[2];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const bool is_w = i < 2 * NT;
+    const int row = (is_w ? i : i - 2 * NT) * 8 + (lane >> 3);
+    chunk[i & 1] = (lane & 7) ^ swizzle(row & 15);
+    const int64_t last = is_w ? a.N - 1 - n0 : a.M - 1;
+    off[i] = (uint32_t)(min((int64_t)row, last) * (is_w ? a.w_stride : a.x_stride)) +
+             16u * chunk[i & 1];
+  }
+  const int8_t* const w_base = a.w + n0 * a.w_stride;
+  auto issue = [&](int i, uint32_t slot) {
+    const int t = wave + i * WAVES;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      uint32_t at = off[j];
+      if (t == steps - 1 && tail < kStep)
+        at = 16 * chunk[j & 1] < tail ? at : at - 16u * chunk[j & 1];
+      dma(ring + slot + 1024 * j, (j < 2 * NT ? w_base : a.x) + (int64_t)t * kStep, at);
+    }
+  };
+  uint32_t at[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) at[s] = ring + r * kStep + 16u * ((4 * s + grp) ^ swizzle(r));
+  i32x4_t acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < RING; ++i)
+    if (i < mine) issue(i, i * SLOT);
+  uint32_t slot = 0;
+  for (int i = 0; i < mine; ++i) {
+    const int later = min(RING - 1, mine - 1 - i);   // steps still on their way
+    if (later == 3) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(3 * P) : "memory");
+    else if (later == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * P) : "memory");
+    else if (later == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(P) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    u32x4_t w[2][NT], x[2][MT];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) w[s][n] = lds16(at[s] + slot + 16 * kStep * n);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[s][m] = lds16(at[s] + slot + 16 * kStep * (NT + m));
+    }
+    if (wave + i * WAVES == steps - 1 && tail < kStep) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const bool in = 64 * s + 16 * grp < tail;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) w[s][n][d] = in ? w[s][n][d] : 0u;
+      }
+    }
+    // (read before the slot is filled again)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (i + RING < mine) issue(i + RING, slot);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[s][n], x[s][m], acc[m][n]);
+    slot = slot + SLOT == RING * SLOT ? 0 : slot + SLOT;
+  }
+  i32x4_t* const sums = (i32x4_t*)lds;   // [WAVES][Q][64], once no ring is in use
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) sums[(wave * Q + m * NT + n) * 64 + lane] = acc[m][n];
+  __syncthreads();
+  for (int q = wave; q < Q; q += WAVES) {
+    const int64_t m = 16 * (q / NT) + r, n = n0 + 16 * (q % NT) + 4 * grp;
+    i32x4_t s = sums[q * 64 + lane];
+#pragma unroll
+    for (int v = 1; v < WAVES; ++v) s += sums[(v * Q + q) * 64 + lane];
+    put4(a, m, n, s);
+  }
+}
+
+// Rows at any address: a workgroup has 16 columns and up to 16 MT rows; its waves take K's steps of 64
+// in turn, U at a time, and add their sums in LDS.  W and X go from memory to the operands'
+// registers.
 template <int MT, int WAVES, int U>
 __global__ void __launch_bounds__(64 * WAVES) int8_few_rows_kernel(LinearArgs a) {
-  __shared__ i32x4_t sums[WAVES][MT][64];
+  constexpr int Q = MT;
+  __shared__ i32x4_t sums[WAVES][Q][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int r = lane & 15, grp = lane >> 4;
-  const int8_t* const w = a.w + min(n0 + r, a.N - 1) * a.w_stride + 16 * grp;
   const int8_t* x[MT];
+  const int8_t* const w = a.w + min(n0 + r, a.N - 1) * a.w_stride;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
-    x[m] = a.x + min((int64_t)(16 * m + r), a.M - 1) * a.x_stride + 16 * grp;
-  // scales of the results that this thread will write: row m, columns n ..
-  const int64_t m = 16 * wave + r, n = n0 + 4 * grp;
-  float sx = 0.f, sw[4], bias[4];
-  if (wave < MT) {
-    sx = a.sx[min(m, a.M - 1)];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sw[i] = a.sw[min(n + i, a.N - 1)];
-      bias[i] = a.bias ? widen(a.bias, min(n + i, a.N - 1), a.dtype) : 0.f;
-    }
-  }
+    x[m] = a.x + min((int64_t)(16 * m + r), a.M - 1) * a.x_stride;
   i32x4_t acc[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = i32x4_t{0, 0, 0, 0};
-  const int full = (int)(a.K / 64);
-  int t = wave;
-  for (; t + (U - 1) * WAVES < full; t += U * WAVES) {
+  for (int m = 0; m < MT; ++m) acc[m] = i32x4_t{0, 0, 0, 0};
+  const int K = (int)a.K, steps = (K + 63) / 64;
+  for (int t = wave; t < steps; t += U * WAVES) {
     u32x4_t wf[U], xf[U][MT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t k = 64 * (int64_t)(t + u * WAVES);
+      const int k = min(64 * (t + u * WAVES) + 16 * grp, K - 16);
       wf[u] = load16(w + k);
 #pragma unroll
       for (int i = 0; i < MT; ++i) xf[u][i] = load16(x[i] + k);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      const int k0 = 64 * (t + u * WAVES);
+      if (k0 + 64 > K) {
+        const int k = k0 + 16 * grp;
+        wf[u] = without_first(wf[u], k - min(k, K - 16));
+      }
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[i] = mfma(wf[u], xf[u][i], acc[i]);
-  }
-  for (; 64 * (int64_t)t < a.K; t += WAVES) {
-    const int64_t k0 = 64 * (int64_t)t, k = k0 + 16 * grp, at = min(k, a.K - 16);
-    u32x4_t wf = load16(w - 16 * grp + at);
-    if (k0 + 64 > a.K) wf = without_first(wf, k - at);
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-      acc[i] = mfma(wf, load16(x[i] - 16 * grp + at), acc[i]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) sums[wave][i][lane] = acc[i];
   __syncthreads();
-  if (wave >= MT) return;
-  i32x4_t s = sums[0][wave][lane];
+  for (int q = wave; q < Q; q += WAVES) {
+    const int64_t m = 16 * q + r, n = n0 + 4 * grp;
+    i32x4_t s = sums[0][q][lane];
 #pragma unroll
-  for (int v = 1; v < WAVES; ++v) s += sums[v][wave][lane];
-  if (m >= a.M) return;
-  float y[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = scaled(s[i], sx, sw[i], bias[i]);
-  if (a.dtype == MRSA_DTYPE_FP32) {
-    float* const to = (float*)a.out + m * a.N + n;
-    if (n + 4 <= a.N) *reinterpret_cast<Pack<float, 4>*>(to) = Pack<float, 4>{{y[0], y[1], y[2], y[3]}};
-    else
-      for (int i = 0; i < 4; ++i)
-        if (n + i < a.N) to[i] = y[i];
-  } else {
-    uint16_t* const to = (uint16_t*)a.out + m * a.N + n;
-    const uint32_t v[2] = {pack2(y[0], y[1], a.dtype), pack2(y[2], y[3], a.dtype)};
-    if (n + 4 <= a.N) *reinterpret_cast<Pack<uint32_t, 2>*>(to) = Pack<uint32_t, 2>{{v[0], v[1]}};
-    else
-      for (int i = 0; i < 4; ++i)
-        if (n + i < a.N) to[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+    for (int v = 1; v < WAVES; ++v) s += sums[v][q][lane];
+    put4(a, m, n, s);
   }
 }
 
@@ -525,16 +683,20 @@ typedef Tile<256, 256, 2, 4> Large;
 struct Plan {
   enum { kShort, kFew, kSmall, kLarge } kind;
   bool dma;
-  int64_t tiles_m, tiles_n, parts, bytes;
+  int64_t tiles_m, tiles_n, parts, bytes, cols;
 };
 Plan plan_of(int64_t M, int64_t N, int64_t K, bool aligned) {
-  Plan p = {Plan::kSmall, aligned, 1, 1, 1, 0};
+  Plan p = {Plan::kSmall, aligned, 1, 1, 1, 0, 0};
   if (K < 16) {
     p.kind = Plan::kShort;
     return p;
   }
-  if (M <= 64) {
+  // Up to 64 rows the weights' bytes count.  Columns of a workgroup: 32 while that leaves enough
+  // workgroups (rows are then fetched half as often), else 16.
+  if (M <= 64 && !(aligned && M > 32 && N > 16384)) {
     p.kind = Plan::kFew;
+    p.cols = aligned && N >= 32 * 144 ? 32 : 16;
+    p.tiles_n = (N + p.cols - 1) / p.cols;
     return p;
   }
   auto tiles = [&](int64_t tm, int64_t tn) {
@@ -564,6 +726,24 @@ void launch_tiles(const LinearArgs& a, bool dma, hipStream_t stream) {
   if (a.parts > 1)
     hipLaunchKernelGGL((int8_join_kernel<T>), dim3((unsigned)(a.tiles_m * a.tiles_n)), block, 0,
                        stream, a);
+}
+
+void launch_few(const LinearArgs& a, const Plan& p, hipStream_t stream) {
+  const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+  void (*kern)(LinearArgs);
+  if (!p.dma)
+    kern = mt == 1   ? int8_few_rows_kernel<1, 8, 4>
+           : mt == 2 ? int8_few_rows_kernel<2, 8, 4>
+                     : int8_few_rows_kernel<4, 8, 2>;
+  else if (p.cols == 16)
+    kern = mt == 1   ? int8_stream_kernel<1, 1, 4, 4>
+           : mt == 2 ? int8_stream_kernel<2, 1, 4, 3>
+                     : int8_stream_kernel<4, 1, 4, 2>;
+  else
+    kern = mt == 1   ? int8_stream_kernel<1, 2, 4, 2>
+           : mt == 2 ? int8_stream_kernel<2, 2, 4, 2>
+                     : int8_stream_kernel<4, 2, 4, 2>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)p.tiles_n), dim3(p.dma ? 256 : 512), 0, stream, a);
 }
 
 }  // namespace
@@ -598,8 +778,7 @@ extern "C" int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const
   const bool aligned = dim % 16 == 0 && aligned_rows(x, x_row_stride, rows) &&
                        aligned_rows(weight, weight_row_stride, out_dim);
   const Plan p = plan_of(rows, out_dim, dim, aligned);
-  const int64_t groups = p.kind == Plan::kFew ? (out_dim + 15) / 16
-                                              : p.tiles_m * p.tiles_n * p.parts;
+  const int64_t groups = p.kind == Plan::kFew ? p.tiles_n : p.tiles_m * p.tiles_n * p.parts;
   if (groups >= (int64_t)1 << 23) return MRSA_ERR_UNSUPPORTED;
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16 != 0))
     return MRSA_ERR_INVALID_ARGUMENT;
@@ -614,10 +793,7 @@ extern "C" int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const
       break;
     }
     case Plan::kFew: {
-      auto kern = rows <= 16   ? int8_few_rows_kernel<1, 8, 8>
-                  : rows <= 32 ? int8_few_rows_kernel<2, 8, 4>
-                               : int8_few_rows_kernel<4, 8, 2>;
-      hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(512), 0, st, a);
+      launch_few(a, p, st);
       break;
     }
     case Plan::kSmall: launch_tiles<Small>(a, p.dma, st); break;
