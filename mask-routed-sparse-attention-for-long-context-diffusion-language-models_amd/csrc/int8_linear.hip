@@ -64,18 +64,19 @@ __device__ __forceinline__ u32x4_t without_first(u32x4_t v, int64_t bytes) {
 // A step is 128 bytes of K: whole cache lines.
 constexpr int kStep = 128;
 
-template <int TM_, int TN_, int WM_, int WN_>
+template <int TM_, int TN_, int WM_, int WN_, int SLOTS_>
 struct Tile {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, SLOTS = SLOTS_;
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int MT = TM / WM / 16, NT = TN / WN / 16;   // 16 x 16 products of a wave
   static constexpr int SLOT = (TM + TN) * kStep;               // bytes of a step: W's rows, X's
   static constexpr int PIECES = SLOT / 1024 / WAVES;           // 1 KB each, of a wave
   static constexpr int W_PIECES = TN * kStep / 1024;
   static constexpr int COLS = 16 * NT;
-  static constexpr int SCALES = 2 * COLS + 16 * MT;            // floats, of a wave
-  static constexpr int LDS = 2 * SLOT + 4 * WAVES * SCALES;
-  static_assert(SLOT % (1024 * WAVES) == 0 && MT % 4 == 0 && NT <= MT && NT == 4 &&
+  static constexpr int ROWS = (16 * MT + 63) / 64;             // loads of a wave's rows' scales
+  static constexpr int SCALES = 2 * COLS + 64 * ROWS;           // floats, of a wave
+  static constexpr int LDS = SLOTS * SLOT + 4 * WAVES * SCALES;
+  static_assert(SLOT % (1024 * WAVES) == 0 && MT % 2 == 0 && NT == 4 &&
                 LDS <= 160 * 1024);
 };
 
@@ -174,10 +175,43 @@ __device__ __forceinline__ void fetch_scales(const LinearArgs& a, const Position
   const int64_t n = min(n0 + p.lane, a.N - 1);
   dma4(to, (const int8_t*)(a.sw + n0), 4u * (uint32_t)(n - n0));
 #pragma unroll
-  for (int i = 0; i < T::MT / 4; ++i)
+  for (int i = 0; i < T::ROWS; ++i)
     dma4(to + 4 * (2 * T::COLS + 64 * i), (const int8_t*)(a.sx + m0),
          4u * (uint32_t)(min(m0 + 64 * i + p.lane, a.M - 1) - m0));
   scales[T::COLS + p.lane] = a.bias ? widen(a.bias, n, a.dtype) : 0.f;
+}
+
+// Eight results of row m from column n < N on.
+__device__ __forceinline__ void put8(const LinearArgs& a, int64_t m, int64_t n, i32x4_t lo,
+                                     i32x4_t hi, float sx, const float (&scale)[8],
+                                     const float (&bias)[8]) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    y[i] = scaled(i < 4 ? lo[i & 3] : hi[i & 3], sx, scale[i], bias[i]);
+  if (a.dtype == MRSA_DTYPE_FP32) {
+    float* const to = (float*)a.out + m * a.N + n;
+    if (n + 8 <= a.N) {
+      *reinterpret_cast<Pack<float, 4>*>(to) = Pack<float, 4>{{y[0], y[1], y[2], y[3]}};
+      *reinterpret_cast<Pack<float, 4>*>(to + 4) = Pack<float, 4>{{y[4], y[5], y[6], y[7]}};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < a.N) to[i] = y[i];
+    }
+  } else {
+    uint16_t* const to = (uint16_t*)a.out + m * a.N + n;
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pack2(y[2 * i], y[2 * i + 1], a.dtype);
+    if (n + 8 <= a.N) {
+      *reinterpret_cast<Pack<uint32_t, 4>*>(to) = Pack<uint32_t, 4>{{v[0], v[1], v[2], v[3]}};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < a.N) to[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+    }
+  }
 }
 
 // Sums to results.  W is the products' first operand: lane l holds, of row l % 16, columns
@@ -190,7 +224,6 @@ __device__ __forceinline__ void finish(const LinearArgs& a, const Position<T>& p
   const int c0 = 8 * (p.lane >> 4);
   const int64_t n0 = p.n0 + p.wn * T::COLS + c0;
   const int64_t m0 = p.m0 + p.wm * 16 * T::MT + (p.lane & 15);
-  const bool wide = a.dtype == MRSA_DTYPE_FP32;
   float scale[PAIRS][8], bias[PAIRS][8];
 #pragma unroll
   for (int q = 0; q < PAIRS; ++q)
@@ -214,39 +247,14 @@ __device__ __forceinline__ void finish(const LinearArgs& a, const Position<T>& p
 #pragma unroll
     for (int q = 0; q < PAIRS; ++q) {
       const int64_t n = n0 + 32 * q;
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        y[i] = scaled(acc[mt][2 * q + (i >> 2)][i & 3], sx[mt], scale[q][i], bias[q][i]);
-      if (wide) {
-        float* const to = (float*)a.out + m * a.N + n;
-        if (n + 8 <= a.N) {
-          *reinterpret_cast<Pack<float, 4>*>(to) = Pack<float, 4>{{y[0], y[1], y[2], y[3]}};
-          *reinterpret_cast<Pack<float, 4>*>(to + 4) = Pack<float, 4>{{y[4], y[5], y[6], y[7]}};
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (n + i < a.N) to[i] = y[i];
-        }
-      } else {
-        uint16_t* const to = (uint16_t*)a.out + m * a.N + n;
-        uint32_t v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = pack2(y[2 * i], y[2 * i + 1], a.dtype);
-        if (n + 8 <= a.N) {
-          *reinterpret_cast<Pack<uint32_t, 4>*>(to) = Pack<uint32_t, 4>{{v[0], v[1], v[2], v[3]}};
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (n + i < a.N) to[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
-        }
-      }
+      if (n < a.N)
+        put8(a, m, n, acc[mt][2 * q], acc[mt][2 * q + 1], sx[mt], scale[q], bias[q]);
     }
   }
 }
 
-// A workgroup computes one part of K of a tile.  DMA: rows 16-byte aligned and K a multiple of 16.
-// Otherwise rows go through registers.
+// A workgroup computes one part of K of a tile.  DMA: rows 16-byte aligned and K a multiple of 16,
+// from 128 on.  Otherwise rows go through registers.
 template <class T, bool DMA>
 __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 : 2))
     int8_tile_kernel(LinearArgs a) {
@@ -259,7 +267,7 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
   const int t0 = (int)((int64_t)steps * part / a.parts);
   const int t1 = (int)((int64_t)steps * (part + 1) / a.parts);
   const Position<T> p(a, tile);
-  float* const scales = (float*)(lds + 2 * T::SLOT) + p.wave * T::SCALES;
+  float* const scales = (float*)(lds + T::SLOTS * T::SLOT) + p.wave * T::SCALES;
   if (a.parts == 1) fetch_scales<T>(a, p, scales);
   const int lane = p.lane, wave = p.wave;
 
@@ -282,22 +290,22 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
   i32x4_t acc[MT][NT];
   clear<T>(acc);
   u32x4_t w[2][NT], x[MT];
-  // W's operands of a half step past K's end are made zero.
+  // The last step is the last 128 bytes of K: what the step before has, too, is made zero in W.
   auto cut = [&](u32x4_t (&f)[NT], int s) {
-    const bool in = 64 * s + 16 * (lane >> 4) < tail;
+    const bool in = 64 * s + 16 * (lane >> 4) >= kStep - tail;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int d = 0; d < 4; ++d) f[n][d] = in ? f[n][d] : 0u;
   };
   const uint32_t to = lds0 + wave * P * 1024;
-  auto row_of = [&](int i, int l) {  // piece i of the wave: rows 8 at a time of W, then of X
+  auto row_of = [&](int i) {  // piece i of the wave: rows 8 at a time of W, then of X
     const int piece = wave * P + i;
-    return (piece - (piece < T::W_PIECES ? 0 : T::W_PIECES)) * 8 + (l >> 3);
+    return (piece - (piece < T::W_PIECES ? 0 : T::W_PIECES)) * 8 + (lane >> 3);
   };
-  auto chunk_of = [&](int i, int l) {
-    const int r = row_of(i, l);
-    return (l & 7) ^ (wave * P + i < T::W_PIECES ? swizzle_w(r) : swizzle(r));
+  auto chunk_of = [&](int i) {
+    const int r = row_of(i);
+    return (lane & 7) ^ (wave * P + i < T::W_PIECES ? swizzle_w(r) : swizzle(r));
   };
 
   if constexpr (DMA) {
@@ -309,66 +317,71 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
     for (int i = 0; i < P; ++i) {
       const bool is_w = wave * P + i < T::W_PIECES;
       const int64_t last = is_w ? a.N - 1 - p.n0 : a.M - 1 - p.m0;
-      off[i] = (uint32_t)(min((int64_t)row_of(i, lane), last) * (is_w ? a.w_stride : a.x_stride)) +
-               16u * chunk_of(i, lane);
+      off[i] = (uint32_t)(min((int64_t)row_of(i), last) * (is_w ? a.w_stride : a.x_stride)) +
+               16u * chunk_of(i);
     }
-    // Before the step that K ends in: its chunks past K repeat the step's first one.
-    auto trim = [&](int t) {
-      if (t != steps - 1 || tail == kStep) return;
-      int l = lane;
-      asm volatile("" : "+v"(l));  // (a branch, which hardly any step takes)
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const int c = 16 * chunk_of(i, l);
-        if (c >= tail) off[i] -= c;
-      }
-    };
     auto issue = [&](int t, int i, uint32_t slot) {
       dma(to + slot + 1024 * i,
-          (wave * P + i < T::W_PIECES ? w_from : x_from) + (int64_t)t * kStep, off[i]);
+          (wave * P + i < T::W_PIECES ? w_from : x_from) + min((int64_t)t * kStep, a.K - kStep),
+          off[i]);
     };
-    auto arrived = [&] {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // The wave's own pieces of a step have landed (those of the LATER steps behind it may be on
+    // their way), its reads are done, and so for every wave.
+    auto arrived = [&](auto later) {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(P * later()) : "memory");
     };
-    trim(t0);
+    constexpr int SLOTS = T::SLOTS;
+    auto none = [] { return 0; };
+    auto most = [] { return SLOTS - 2; };
 #pragma unroll
-    for (int i = 0; i < P; ++i) issue(t0, i, 0);
-    arrived();
+    for (int j = 0; j < SLOTS - 1; ++j) {
+      if (t0 + j >= t1) break;
+#pragma unroll
+      for (int i = 0; i < P; ++i) issue(t0 + j, i, j * T::SLOT);
+    }
+    if (t0 + SLOTS - 2 < t1) arrived(most);
+    else arrived(none);
 #pragma unroll
     for (int n = 0; n < NT; ++n) w[0][n] = w_read(0, n, 0);
 #pragma unroll
     for (int m = 0; m < MT; ++m) x[m] = x_read(0, m, 0);
-    if (t0 + 1 < t1) {
-      trim(t0 + 1);
+    if (t0 + SLOTS - 1 < t1) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) issue(t0 + 1, i, T::SLOT);
+      for (int i = 0; i < P; ++i) issue(t0 + SLOTS - 1, i, (SLOTS - 1) * T::SLOT);
     }
     uint32_t slot = 0;
     for (int t = t0; t < t1; ++t) {
+      // (in registers that the products need no copies of)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) asm volatile("" : "+v"(acc[m][n]));
       const bool partial = t == steps - 1 && tail < kStep;
-      const uint32_t next = slot ^ (uint32_t)T::SLOT;
+      const uint32_t next = slot == (SLOTS - 1) * T::SLOT ? 0 : slot + (uint32_t)T::SLOT;
       // first half: its products, each row tile's operand replaced by the second half's
       if (partial) cut(w[0], 0);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[0][n], x[m], acc[m][n]);
-        if (m < NT) w[1][m] = w_read(1, m, slot);
+        constexpr int WR = (NT + MT - 1) / MT;
+#pragma unroll
+        for (int n = m * WR; n < (m + 1) * WR && n < NT; ++n) w[1][n] = w_read(1, n, slot);
         x[m] = x_read(1, m, slot);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (partial) cut(w[1], 1);
       // second half: in its middle the next step has arrived for every wave, and every wave
-      // has read all of this one, whose slot the step after the next then fills
+      // has read all of this one, whose slot the step SLOTS further on then fills
 #pragma unroll
       for (int m = 0; m < MT / 2; ++m) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[1][n], x[m], acc[m][n]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      arrived();
-      const bool more = t + 2 < t1;
-      if (more) trim(t + 2);
+      if (t + SLOTS - 1 < t1) arrived(most);
+      else arrived(none);
+      const bool more = t + SLOTS < t1;
 #pragma unroll
       for (int m = MT / 2; m < MT; ++m) {
 #pragma unroll
@@ -383,7 +396,7 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
         if (more) {
           constexpr int EACH = (P + MT / 2 - 1) / (MT / 2);
 #pragma unroll
-          for (int i = j * EACH; i < (j + 1) * EACH && i < P; ++i) issue(t + 2, i, slot);
+          for (int i = j * EACH; i < (j + 1) * EACH && i < P; ++i) issue(t + SLOTS, i, slot);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -397,18 +410,18 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
     for (int i = 0; i < P; ++i) {
       const bool is_w = wave * P + i < T::W_PIECES;
       row[i] = (is_w ? a.w : a.x) +
-               min((is_w ? p.n0 : p.m0) + row_of(i, lane), (is_w ? a.N : a.M) - 1) *
+               min((is_w ? p.n0 : p.m0) + row_of(i), (is_w ? a.N : a.M) - 1) *
                    (is_w ? a.w_stride : a.x_stride);
     }
     auto load = [&](int t) {
       const int64_t k0 = (int64_t)t * kStep;
       if (k0 + kStep <= a.K) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) held[i] = load16(row[i] + k0 + 16 * chunk_of(i, lane));
+        for (int i = 0; i < P; ++i) held[i] = load16(row[i] + k0 + 16 * chunk_of(i));
       } else {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const int64_t k = k0 + 16 * chunk_of(i, lane), at = min(k, a.K - 16);
+          const int64_t k = k0 + 16 * chunk_of(i), at = min(k, a.K - 16);
           held[i] = load16(row[i] + at);
           if (wave * P + i < T::W_PIECES) held[i] = without_first(held[i], k - at);
         }
@@ -455,25 +468,31 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
   finish<T>(a, p, scales, acc);
 }
 
-// The sums of a tile's parts, then its results.
+// Sums of a tile's parts and its results, for eight columns of a row a thread: two of the
+// registers that int8_tile_kernel kept, of one of its lanes.
 template <class T>
 __global__ void __launch_bounds__(T::THREADS) int8_join_kernel(LinearArgs a) {
-  __shared__ __attribute__((aligned(16))) float scales_of[T::WAVES][T::SCALES];
-  const int tile = blockIdx.x;
+  constexpr int PAIRS = T::MT * T::NT / 2, EACH = 2 * PAIRS * T::THREADS;
+  const int tile = blockIdx.x / PAIRS, pair = blockIdx.x - tile * PAIRS;
   const Position<T> p(a, tile);
-  float* const scales = scales_of[p.wave];
-  fetch_scales<T>(a, p, scales);
-  i32x4_t acc[T::MT][T::NT];
-  const i32x4_t* from = (const i32x4_t*)a.partial +
-      (int64_t)tile * a.parts * (T::MT * T::NT * T::THREADS) + threadIdx.x;
-  clear<T>(acc);
-  for (int part = 0; part < a.parts; ++part, from += T::MT * T::NT * T::THREADS)
+  const i32x4_t* from = (const i32x4_t*)a.partial + (int64_t)tile * a.parts * EACH +
+                        2 * pair * T::THREADS + threadIdx.x;
+  i32x4_t lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+  for (int part = 0; part < a.parts; ++part, from += EACH) {
+    lo += from[0];
+    hi += from[T::THREADS];
+  }
+  const int64_t m = p.m0 + (p.wm * T::MT + pair / (T::NT / 2)) * 16 + (p.lane & 15);
+  const int64_t n = p.n0 + p.wn * T::COLS + 32 * (pair % (T::NT / 2)) + 8 * (p.lane >> 4);
+  if (m >= a.M || n >= a.N) return;
+  float scale[8], bias[8];
 #pragma unroll
-    for (int m = 0; m < T::MT; ++m)
-#pragma unroll
-      for (int n = 0; n < T::NT; ++n) acc[m][n] += from[(m * T::NT + n) * T::THREADS];
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the scales)
-  finish<T>(a, p, scales, acc);
+  for (int i = 0; i < 8; ++i) {
+    const int64_t c = min(n + i, a.N - 1);
+    scale[i] = a.sw[c];
+    bias[i] = a.bias ? widen(a.bias, c, a.dtype) : 0.f;
+  }
+  put8(a, m, n, lo, hi, a.sx[m], scale, bias);
 }
 
 // ---- few rows: the weights' bytes ---------------------------------------------------------
@@ -526,26 +545,20 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
   const uint32_t ring = lds_at(lds) + wave * RING * SLOT;
   // piece i: rows 8 i .. of W, then of X
   uint32_t off[P];
-  int chunk[2];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const bool is_w = i < 2 * NT;
     const int row = (is_w ? i : i - 2 * NT) * 8 + (lane >> 3);
-    chunk[i & 1] = (lane & 7) ^ swizzle(row & 15);
     const int64_t last = is_w ? a.N - 1 - n0 : a.M - 1;
     off[i] = (uint32_t)(min((int64_t)row, last) * (is_w ? a.w_stride : a.x_stride)) +
-             16u * chunk[i & 1];
+             16u * ((lane & 7) ^ swizzle(row));
   }
   const int8_t* const w_base = a.w + n0 * a.w_stride;
   auto issue = [&](int i, uint32_t slot) {
-    const int t = wave + i * WAVES;
+    const int k = min((wave + i * WAVES) * kStep, K - kStep);
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      uint32_t at = off[j];
-      if (t == steps - 1 && tail < kStep)
-        at = 16 * chunk[j & 1] < tail ? at : at - 16u * chunk[j & 1];
-      dma(ring + slot + 1024 * j, (j < 2 * NT ? w_base : a.x) + (int64_t)t * kStep, at);
-    }
+    for (int j = 0; j < P; ++j)
+      dma(ring + slot + 1024 * j, (j < 2 * NT ? w_base : a.x) + k, off[j]);
   };
   uint32_t at[2];
 #pragma unroll
@@ -573,10 +586,10 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) x[s][m] = lds16(at[s] + slot + 16 * kStep * (NT + m));
     }
-    if (wave + i * WAVES == steps - 1 && tail < kStep) {
+    if (wave + i * WAVES == steps - 1 && tail < kStep) {  // (K's last 128 bytes)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const bool in = 64 * s + 16 * grp < tail;
+        const bool in = 64 * s + 16 * grp >= kStep - tail;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -676,55 +689,95 @@ __global__ void __launch_bounds__(256) int8_short_rows_kernel(LinearArgs a) {
   }
 }
 
-typedef Tile<128, 128, 2, 2> Small;
-typedef Tile<256, 256, 2, 4> Large;
-
-// How a product is cut: by rows, size and alignment alone.
+// How a product is cut: by its sizes and alignment alone.  A step of a tile costs about the same
+// for few rows as for many, so small tiles finish few rows first and large ones many; `parts` of K
+// fill the CUs where tiles do not, for a second kernel's time.  The estimate below is fitted to
+// measured times (us; 64 to 16384 rows, 64 to 37888 columns, 1008 to 18944 values).
+//   512 rows, 3584 x 3584: 64 x 64 16.3, 64 x 128 14.7, 128 x 128 18.1, 256 x 256 42
+//   256 rows, 3584 columns of 18944 values: 64 x 64 55 (two parts 48), 128 x 128 83 (four 32)
+//   1003 rows of the same: 64 x 64 138, 128 x 128 87, 256 x 256 230 (four 86)
+//   128 rows, 37888 x 3584: 128 x 256 34, 128 x 128 40, 256 x 256 50
+//   4096 rows, 8192 x 8192: 256 x 256 223, 128 x 256 258, 128 x 128 280
+typedef Tile<64, 64, 2, 1, 4> Tile64;
+typedef Tile<64, 128, 2, 2, 3> Tile64x128;
+typedef Tile<128, 128, 4, 2, 4> TileDeep;     // a workgroup a CU
+typedef Tile<128, 128, 4, 2, 2> Tile128;      // two
+typedef Tile<128, 256, 2, 4, 3> Tile128x256;
+typedef Tile<256, 256, 2, 4, 2> Tile256;
+struct Shape {
+  int tm, tn, room;        // workgroups that the CUs hold
+  float one, two, fixed;   // us: a step of a workgroup alone on its CU, of two, the rest
+  bool any_rows;           // also for rows at any address
+};
+constexpr Shape kShapes[] = {
+    {64, 64, 512, 0.335f, 0.45f, 5.f, true},     {64, 128, 512, 0.40f, 0.70f, 5.f, false},
+    {128, 128, 256, 0.52f, 0.52f, 5.f, false},   {128, 128, 512, 0.83f, 1.0f, 5.f, true},
+    {128, 256, 256, 0.82f, 0.82f, 6.f, false},   {256, 256, 256, 1.42f, 1.42f, 8.f, true},
+};
 struct Plan {
-  enum { kShort, kFew, kSmall, kLarge } kind;
+  enum { kShort, kFew, kTiles } kind;
+  int shape;
   bool dma;
   int64_t tiles_m, tiles_n, parts, bytes, cols;
 };
 Plan plan_of(int64_t M, int64_t N, int64_t K, bool aligned) {
-  Plan p = {Plan::kSmall, aligned, 1, 1, 1, 0, 0};
+  Plan p = {Plan::kTiles, 0, aligned, 1, 1, 1, 0, 0};
   if (K < 16) {
     p.kind = Plan::kShort;
     return p;
   }
-  // Up to 64 rows the weights' bytes count.  Columns of a workgroup: 32 while that leaves enough
-  // workgroups (rows are then fetched half as often), else 16.
-  if (M <= 64 && !(aligned && M > 32 && N > 16384)) {
+  float best = 1e30f;
+  if (M <= 64) {
+    // Up to 64 rows the weights' bytes count, and the rows' that every workgroup fetches again.
+    // Columns of a workgroup: 32 while that leaves enough workgroups, else 16.
     p.kind = Plan::kFew;
     p.cols = aligned && N >= 32 * 144 ? 32 : 16;
     p.tiles_n = (N + p.cols - 1) / p.cols;
-    return p;
+    if (!aligned || M <= 32) return p;
+    best = 3.f + (float)N * (float)K * (1.f + 64.f / (float)p.cols) * 1e-7f;
   }
-  auto tiles = [&](int64_t tm, int64_t tn) {
-    p.tiles_m = (M + tm - 1) / tm;
-    p.tiles_n = (N + tn - 1) / tn;
-  };
-  tiles(Large::TM, Large::TN);
-  if (aligned && p.tiles_m * p.tiles_n >= 256) {
-    p.kind = Plan::kLarge;
-    return p;
+  const int64_t steps = (K + kStep - 1) / kStep;
+  for (int i = 0; i < (int)(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
+    const Shape& s = kShapes[i];
+    if (!aligned && !s.any_rows) continue;
+    const int64_t tm = (M + s.tm - 1) / s.tm, tn = (N + s.tn - 1) / s.tn;
+    for (const int parts : {1, 2, 3, 4, 6, 8}) {
+      if (parts > steps) break;
+      const int64_t items = tm * tn * parts;
+      const float rounds = items <= 4 * s.room ? (float)((items + s.room - 1) / s.room)
+                                               : (float)items / (float)s.room + 0.5f;
+      const float step = items <= 256 ? s.one : s.two;
+      const int64_t bytes = parts > 1 ? items * s.tm * s.tn * 4 : 0;
+      const float time = rounds * (s.fixed + step * (float)((steps + parts - 1) / parts)) +
+                         (parts > 1 ? 6.f + 0.27e-6f * (float)bytes : 0.f);
+      if (time < best) {
+        best = time;
+        p.kind = Plan::kTiles;
+        p.shape = i;
+        p.tiles_m = tm;
+        p.tiles_n = tn;
+        p.parts = parts;
+        p.bytes = bytes;
+      }
+    }
   }
-  tiles(128, 128);
-  const int64_t steps = (K + kStep - 1) / kStep, want = 512 / std::max<int64_t>(1, p.tiles_m * p.tiles_n);
-  p.parts = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 16), steps / 8));
-  if (p.parts > 1) p.bytes = p.tiles_m * p.tiles_n * p.parts * 128 * 128 * 4;
   return p;
 }
 bool aligned_rows(const void* p, int64_t stride, int64_t rows) {
   return (uintptr_t)p % 16 == 0 && (rows == 1 || (stride % 16 == 0 && stride < (1 << 22)));
 }
 
-template <class T>
+template <class T, bool ANY>
 void launch_tiles(const LinearArgs& a, bool dma, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.tiles_m * a.tiles_n * a.parts)), block(T::THREADS);
-  if (dma) hipLaunchKernelGGL((int8_tile_kernel<T, true>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((int8_tile_kernel<T, false>), grid, block, 0, stream, a);
+  if (dma) {
+    hipLaunchKernelGGL((int8_tile_kernel<T, true>), grid, block, 0, stream, a);
+  } else if constexpr (ANY) {
+    hipLaunchKernelGGL((int8_tile_kernel<T, false>), grid, block, 0, stream, a);
+  }
   if (a.parts > 1)
-    hipLaunchKernelGGL((int8_join_kernel<T>), dim3((unsigned)(a.tiles_m * a.tiles_n)), block, 0,
+    hipLaunchKernelGGL((int8_join_kernel<T>),
+                       dim3((unsigned)(a.tiles_m * a.tiles_n * (T::MT * T::NT / 2))), block, 0,
                        stream, a);
 }
 
@@ -775,7 +828,7 @@ extern "C" int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const
   if (((uintptr_t)x_scales | (uintptr_t)weight_scales) % 4 != 0 ||
       ((uintptr_t)bias | (uintptr_t)out) % size != 0)
     return MRSA_ERR_INVALID_ARGUMENT;
-  const bool aligned = dim % 16 == 0 && aligned_rows(x, x_row_stride, rows) &&
+  const bool aligned = dim % 16 == 0 && dim >= kStep && aligned_rows(x, x_row_stride, rows) &&
                        aligned_rows(weight, weight_row_stride, out_dim);
   const Plan p = plan_of(rows, out_dim, dim, aligned);
   const int64_t groups = p.kind == Plan::kFew ? p.tiles_n : p.tiles_m * p.tiles_n * p.parts;
@@ -796,8 +849,16 @@ extern "C" int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const
       launch_few(a, p, st);
       break;
     }
-    case Plan::kSmall: launch_tiles<Small>(a, p.dma, st); break;
-    case Plan::kLarge: launch_tiles<Large>(a, p.dma, st); break;
+    case Plan::kTiles:
+      switch (p.shape) {
+        case 0: launch_tiles<Tile64, true>(a, p.dma, st); break;
+        case 1: launch_tiles<Tile64x128, false>(a, p.dma, st); break;
+        case 2: launch_tiles<TileDeep, false>(a, p.dma, st); break;
+        case 3: launch_tiles<Tile128, true>(a, p.dma, st); break;
+        case 4: launch_tiles<Tile128x256, false>(a, p.dma, st); break;
+        default: launch_tiles<Tile256, true>(a, p.dma, st);
+      }
+      break;
   }
   return mrsa_launch_status();
 }

@@ -13,15 +13,18 @@ from test_dma_waits import HIPCC, device_assembly
 @pytest.mark.skipif(not os.path.exists(HIPCC), reason="no hipcc")
 def test_int8_tiles_wait_for_their_operands_before_the_barrier(tmp_path):
     text = device_assembly("int8_linear", tmp_path / "int8.s")
-    kernels = re.findall(r"^(_ZN\S*int8_tile_kernel\S*Lb1E\S*):(.*?)^\.Lfunc_end", text,
-                         re.S | re.M)
+    kernels = re.findall(r"^(_ZN\S*int8_tile_kernelI\S*?Li(\d+)ELi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)EEELb1E"
+                         r"\S*):(.*?)^\.Lfunc_end", text, re.S | re.M)
     assert len(kernels) >= 2  # tile sizes, rows by DMA
-    for name, body in kernels:
+    for name, tm, tn, wm, wn, slots, body in kernels:
         assert "global_load_lds_dwordx4" in body, name
-        # first step and steady state; a wave's own operands have been read, too, when their
-        # slot is given to the next rows
-        joint = re.findall(r"s_waitcnt vmcnt\(0\) lgkmcnt\(0\)\n\s*s_barrier\n\s*;;#ASMEND", body)
-        assert len(joint) >= 2, name
-        # no DMA behind the last joint wait but the loop's own
-        others = len(re.findall(r"\bs_barrier\b", body)) - len(joint)
-        assert others <= 1, name  # before the results
+        # a wave's DMA instructions of a step: its KB
+        pieces = (int(tm) + int(tn)) * 128 // 1024 // (int(wm) * int(wn))
+        # The barriers of the first step and of the steady state, each behind a wait for the
+        # wave's own rows (those of the further steps that fit the slots may be on their way) and
+        # for its reads of the slot that is filled next; and those of the last steps, behind all.
+        waits = re.findall(r"s_waitcnt vmcnt\((\d+)\) lgkmcnt\(0\)\n\s*s_barrier", body)
+        assert len(waits) == len(re.findall(r"\bs_barrier\b", body)) >= 4, name
+        ahead = pieces * (int(slots) - 2)
+        assert sorted(set(map(int, waits))) == sorted({0, ahead}), (name, waits)
+        assert ahead < 64, name   # (what the counter holds)
