@@ -744,6 +744,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, bool aligned) {
     for (const int parts : {1, 2, 3, 4, 6, 8}) {
       if (parts > steps) break;
       const int64_t items = tm * tn * parts;
+      if (parts > 1 && items > s.room) break;  // (and so the workspace stays small)
       const float rounds = items <= 4 * s.room ? (float)((items + s.room - 1) / s.room)
                                                : (float)items / (float)s.room + 0.5f;
       const float step = items <= 256 ? s.one : s.two;

@@ -16,17 +16,25 @@ sliding-window layers.  GEMMs run on hipBLASLt through ``torch.nn.functional
 .linear``; the attention stages and the elementwise glue run on the gfx950
 kernels of libmrsa (``mrsa_add_rms_norm_fwd``, ``mrsa_rope_qkv_fwd``,
 ``mrsa_swiglu_fwd``).  Weights are random-initialised (no checkpoint).
+
+``DreamWeights.int8()`` gives the same model with its layers' projections in 8-bit
+integers (a scale for each output channel), and the forward then makes each
+projection's input 8-bit rows behind the norm, the activation or the attention
+and multiplies on ``int8_linear``; embeddings, norms, lm_head and the second
+factor of the low-rank routing query stay bf16.
 """
 
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
 
 from . import _lib
+from .int8 import add_rms_norm_int8, int8_linear, quantize_rows, swiglu_int8
 from .route_layer import RouteLayerConfig, route_attention, swa_attention
 
 
@@ -121,8 +129,18 @@ def yarn_rotate_fp32(x: torch.Tensor, shape: DreamShape) -> torch.Tensor:
     return torch.cat((x1 * c - x2 * s, x2 * c + x1 * s), dim=-1)
 
 
+class Int8Rows(NamedTuple):
+    """Rows in 8 bits (``quantize_rows``): of activations, or a weight matrix's output channels."""
+
+    values: torch.Tensor              # int8 [rows, dim]
+    scales: torch.Tensor              # fp32 [rows]
+
+
 @dataclass
 class DreamLayerWeights:
+    """One layer.  ``int8()`` holds qkv_weight, o_weight, gate_up_weight, down_weight and
+    qcal_down as Int8Rows instead."""
+
     input_norm: torch.Tensor          # bf16 [hidden]
     qkv_weight: torch.Tensor          # bf16 [(Hq + 2 Hkv) * D, hidden]
     qkv_bias: torch.Tensor            # bf16 [(Hq + 2 Hkv) * D]
@@ -135,6 +153,21 @@ class DreamLayerWeights:
     qcal_norm: torch.Tensor | None = None      # fp32 [D]
     entropy_bias_scale: torch.Tensor | None = None  # fp32 [Hq]
 
+    @property
+    def is_int8(self) -> bool:
+        return isinstance(self.qkv_weight, Int8Rows)
+
+    def int8(self) -> "DreamLayerWeights":
+        if self.is_int8:
+            return self
+
+        def rows(w):
+            return None if w is None else Int8Rows(*quantize_rows(w.detach()))
+
+        return replace(self, qkv_weight=rows(self.qkv_weight), o_weight=rows(self.o_weight),
+                       gate_up_weight=rows(self.gate_up_weight),
+                       down_weight=rows(self.down_weight), qcal_down=rows(self.qcal_down))
+
 
 @dataclass
 class DreamWeights:
@@ -144,6 +177,11 @@ class DreamWeights:
     final_norm: torch.Tensor          # bf16 [hidden]
     lm_head: torch.Tensor             # bf16 [vocab, hidden]
     layers: list[DreamLayerWeights]
+
+    def int8(self) -> "DreamWeights":
+        """The model with its layers' projections in 8 bits; what stays bf16 is shared."""
+
+        return replace(self, layers=[lw.int8() for lw in self.layers])
 
     @classmethod
     def random(cls, shape: DreamShape, device, seed: int = 0, std: float = 0.02) -> "DreamWeights":
@@ -219,6 +257,23 @@ def swiglu(gate_up):
     return out
 
 
+def _norm(x, residual, weight, eps, lw):
+    """add_rms_norm for the projections of layer lw (None: the lm_head), in their form."""
+
+    if lw is None or not lw.is_int8:
+        return add_rms_norm(x, residual, weight, eps)
+    total, values, scales = add_rms_norm_int8(x, residual, weight, eps)
+    return total, Int8Rows(values, scales)
+
+
+def _project(x, weight, bias=None):
+    """x, rows in the form of the weight, times the weight."""
+
+    if isinstance(weight, Int8Rows):
+        return int8_linear(*x, *weight, bias)
+    return F.linear(x, weight, bias)
+
+
 def landmark_layout(text_ids: torch.Tensor, shape: DreamShape):
     """The physical sequence of the "mask_type" landmark mode for one
     all-valid document (dream_dllm_hils/data.py:970-1010): every chunk is
@@ -276,7 +331,7 @@ def dream_forward(w: DreamWeights, input_ids: torch.Tensor, *, position_ids=None
                   return_hidden: bool = False) -> torch.Tensor:
     """Denoising forward of one sequence: input_ids int64 [1, L] in the
     landmark layout (landmark_layout) -> logits bf16 [L, vocab] (or the final
-    normed hidden [L, hidden]).  position_ids default to the layout's
+    normed hidden [L, hidden]).  Layers of w.int8() run on 8-bit projections.  position_ids default to the layout's
     (landmark_positions); tables = (cos, sin) rows per slot, if precomputed."""
 
     shape = w.shape
@@ -295,21 +350,24 @@ def dream_forward(w: DreamWeights, input_ids: torch.Tensor, *, position_ids=None
     route = set(shape.route_layers())
     Hq, D = shape.q_heads, shape.head_dim
     h = embed_tokens(w, input_ids)
-    _, x = add_rms_norm(h, None, w.layers[0].input_norm, shape.rms_eps)
+    _, x = _norm(h, None, w.layers[0].input_norm, shape.rms_eps, w.layers[0])
     for i, lw in enumerate(w.layers):
-        qkv = F.linear(x, lw.qkv_weight, lw.qkv_bias)
+        qkv = _project(x, lw.qkv_weight, lw.qkv_bias)
         if i in route:
-            delta = F.linear(F.linear(x, lw.qcal_down), lw.qcal_up)
+            delta = F.linear(_project(x, lw.qcal_down), lw.qcal_up)
             q, k, v, rq = rope_qkv(qkv, cos, sin, shape, delta, lw.qcal_norm)
             a = route_attention(q, k, v, rq, lw.entropy_bias_scale, None, shape.route)
         else:
             q, k, v, _ = rope_qkv(qkv, cos, sin, shape)
             a = swa_attention(q, k, v, None, shape.swa_window, shape.route.chunk_size)
-        o = F.linear(a.reshape(L, Hq * D), lw.o_weight)
-        h, x = add_rms_norm(o, h, lw.post_norm, shape.rms_eps)
-        m = F.linear(swiglu(F.linear(x, lw.gate_up_weight)), lw.down_weight)
-        nxt = w.layers[i + 1].input_norm if i + 1 < len(w.layers) else w.final_norm
-        h, x = add_rms_norm(m, h, nxt, shape.rms_eps)
+        a = a.reshape(L, Hq * D)
+        o = _project(Int8Rows(*quantize_rows(a)) if lw.is_int8 else a, lw.o_weight)
+        h, x = _norm(o, h, lw.post_norm, shape.rms_eps, lw)
+        g = _project(x, lw.gate_up_weight)
+        m = _project(Int8Rows(*swiglu_int8(g)) if lw.is_int8 else swiglu(g), lw.down_weight)
+        after = w.layers[i + 1] if i + 1 < len(w.layers) else None
+        h, x = _norm(m, h, w.final_norm if after is None else after.input_norm, shape.rms_eps,
+                     after)
     if return_hidden:
         return x
     return F.linear(x, w.lm_head)

@@ -1,11 +1,10 @@
 """Linear layers in 8 bits on the GPU against their definitions in 64 bits.
 
 Tolerances, u = 2^-24 (half a step of fp32):
-  * 8-bit values: v is the whole number nearest to f * up (one fused rounding), where
-    up = 127 / top is off by u and, behind the norm, f = t * w and top by u each:
-    |v - 127 y / a| <= 1/2 + 127 * 2 u (plain rows: up alone, counted twice over), 1/2 + 127 * 4 u
-    (norm).  The gated activation: exp2 of an argument off by 1.5 u |g| (the product and the
-    constant), exp2 and reciprocal off by 2 u each, four roundings: (1.5 |g| + 8) u of y and as
+  * 8-bit values: v is the whole number nearest to the fp32 product f * up, where
+    up = (1 / top) * 127 is off by 2 u, the product by u and, behind the norm, f = t * w and top
+    by u each: |v - 127 y / a| <= 1/2 + 127 * 3 u, 1/2 + 127 * 5 u (norm).  The gated activation:
+    exp within 2 steps (4 u), a sum, a quotient and a product: below (1.5 |g| + 8) u of y and as
     much of the top.
   * scales: top / 127 off by u; the norm's also by its mean: a sum of squares along a chain of n
     additions is off by n u, and enters with its square root; six more roundings (the square, the
@@ -56,7 +55,7 @@ def check_rows(values, scales, y, value_slack, scale_slack):
 def test_quantize_rows(dim, dtype):
     x = _rows(5, dim, dtype, dim)
     values, scales = mrsa.quantize_rows(x)
-    check_rows(values, scales, x.double(), 127 * 2 * U, U)
+    check_rows(values, scales, x.double(), 127 * 3 * U, U)
     # the largest magnitude stands for 127
     top = x.double().abs().amax(dim=-1, keepdim=True) == x.double().abs()
     assert (values.abs()[top] == 127).all()
@@ -75,7 +74,7 @@ def test_quantize_rows_without_a_scale(dim, dtype):
     x[5, dim - 1] = -1.5
     values, scales = mrsa.quantize_rows(x)
     y = x.double()
-    check_rows(values, scales, y, 127 * 2 * U, U)
+    check_rows(values, scales, y, 127 * 3 * U, U)
     assert scales[0] == 0 and not values[:4].any() and scales[1:4].isnan().all()
     assert values[5, dim - 1] == -127 and values[5].abs().sum() == 127
     back = mrsa.dequantize_rows(values, scales, dtype)
@@ -89,7 +88,7 @@ def test_quantize_rows_at_the_ends_of_fp32(dim, value):
     x = (torch.rand(3, dim, generator=g, device=DEV) * 2 - 1).float() * value
     x[:, dim - 1] = value
     values, scales = mrsa.quantize_rows(x)
-    check_rows(values, scales, x.double(), 127 * 2 * U, U)
+    check_rows(values, scales, x.double(), 127 * 3 * U, U)
 
 
 def test_rounding_takes_ties_to_even():
@@ -117,7 +116,7 @@ def test_add_rms_norm_int8(dim, residual, dtype):
         assert total is None
     y = O8.norm_rows(t.double(), w.double(), 1e-6)
     chain = dim / 64 + 24
-    check_rows(values, scales, y, 127 * 4 * U, (chain / 2 + 8) * U)
+    check_rows(values, scales, y, 127 * 5 * U, (chain / 2 + 8) * U)
 
 
 @pytest.mark.parametrize("dtype,big", [(torch.bfloat16, 2e38), (torch.float32, 3e38),
@@ -133,7 +132,7 @@ def test_norm_of_values_whose_squares_leave_fp32(dim, dtype, big):
     w = (1 + 0.2 * _rows(1, dim, torch.float32, 7)[0]).to(dtype)
     _, values, scales = mrsa.add_rms_norm_int8(x, None, w, 1e-6)
     y = O8.norm_rows(x.double(), w.double(), 1e-6)
-    check_rows(values, scales, y, 127 * 4 * U, ((dim / 64 + 24) / 2 + 8) * U)
+    check_rows(values, scales, y, 127 * 5 * U, ((dim / 64 + 24) / 2 + 8) * U)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -185,7 +184,7 @@ def test_rows_of_any_strides():
         again = mrsa.quantize_rows(x.contiguous())
         assert values.is_contiguous() and values.shape == x.shape
         assert torch.equal(values, again[0]) and torch.equal(scales, again[1])
-        check_rows(values, scales, x.double(), 127 * 2 * U, U)
+        check_rows(values, scales, x.double(), 127 * 3 * U, U)
         w = torch.ones(2 * x.shape[-1], dtype=x.dtype, device=DEV)[::2]
         res = torch.ones_like(x).expand(x.shape)
         got = mrsa.add_rms_norm_int8(x, res, w, 1e-5)
@@ -409,6 +408,6 @@ def test_offsets_past_32_bits():
     f = torch.zeros(rows, K, dtype=torch.bfloat16, device=DEV)
     f[-3:] = _rows(3, K, torch.bfloat16, 9)
     values, scales = mrsa.quantize_rows(f)
-    check_rows(values[-3:], scales[-3:], f[-3:].double(), 127 * 2 * U, U)
+    check_rows(values[-3:], scales[-3:], f[-3:].double(), 127 * 3 * U, U)
     back = mrsa.dequantize_rows(values, scales)
     assert torch.equal(back[-3:], (values[-3:].float() * scales[-3:, None]).bfloat16())
