@@ -119,15 +119,17 @@ __device__ __forceinline__ void dma(uint32_t to, const int8_t* base, uint32_t at
 }
 
 // Tiles in an order that gives each XCD (workgroups go round them) a contiguous range of bands of
-// 8 tile rows, walked column by column: its concurrent tiles share operands in its L2.
+// 4 tile rows, walked column by column: its concurrent tiles share operands in its L2.  (Bands of 8:
+// 16384 x 3584 of 18944 values 984 us instead of 951, 4096 x 8192 of 8192 226 instead of 224; of
+// 16: 1007 and 234.)
 __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int tiles = tiles_m * tiles_n, each = tiles / 8, more = tiles % 8;
   const int xcd = b % 8, i = b / 8;
   const int t = xcd * each + min(xcd, more) + i;
-  const int band = t / (8 * tiles_n), rest = t - band * 8 * tiles_n;
-  const int rows = min(8, tiles_m - 8 * band);
+  const int band = t / (4 * tiles_n), rest = t - band * 4 * tiles_n;
+  const int rows = min(4, tiles_m - 4 * band);
   tn = __builtin_amdgcn_readfirstlane(rest / rows);
-  tm = __builtin_amdgcn_readfirstlane(8 * band + rest - tn * rows);
+  tm = __builtin_amdgcn_readfirstlane(4 * band + rest - tn * rows);
 }
 
 template <class T>
@@ -527,39 +529,24 @@ __device__ __forceinline__ void put4(const LinearArgs& a, int64_t m, int64_t n, 
   }
 }
 
-// Aligned rows, by DMA: consecutive lanes fetch consecutive bytes of a row, which operands loaded
-// straight from memory (16 rows side by side) do not.  A workgroup has 16 NT columns and up to 16 MT
-// rows; its waves take K's steps of 128 in turn, each through a ring of its own in LDS, RING steps
-// deep, without barriers, and add their sums in the end.
-template <int MT, int NT, int WAVES, int RING>
+// Consecutive lanes fetch consecutive bytes of a row, which operands loaded straight from memory
+// (16 rows side by side) do not.  A workgroup has 16 NT columns and up to 16 MT rows; its waves take
+// K's steps of 128 in turn, each through a ring of its own in LDS, RING steps deep, without barriers,
+// and add their sums in the end.  DMA: aligned rows, K from 128 on.  Otherwise the rows go through
+// registers, RING steps ahead, and one step of LDS.
+template <int MT, int NT, int WAVES, int RING, bool DMA>
 __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
   constexpr int P = 2 * NT + 2 * MT, SLOT = P * 1024, Q = MT * NT;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * RING * SLOT];
-  static_assert(Q * 1024 <= RING * SLOT && RING >= 2 && RING <= 4);
+  constexpr int SLOTS = DMA ? RING : 1;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * SLOTS * SLOT];
+  static_assert(Q * 1024 <= SLOTS * SLOT && RING >= 2 && RING <= 4);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
   const int r = lane & 15, grp = lane >> 4;
   const int K = (int)a.K, steps = (K + kStep - 1) / kStep, tail = K - (steps - 1) * kStep;
   const int mine = steps > wave ? (steps - wave - 1) / WAVES + 1 : 0;
-  const uint32_t ring = lds_at(lds) + wave * RING * SLOT;
-  // piece i: rows 8 i .. of W, then of X
-  uint32_t off[P];
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const bool is_w = i < 2 * NT;
-    const int row = (is_w ? i : i - 2 * NT) * 8 + (lane >> 3);
-    const int64_t last = is_w ? a.N - 1 - n0 : a.M - 1;
-    off[i] = (uint32_t)(min((int64_t)row, last) * (is_w ? a.w_stride : a.x_stride)) +
-             16u * ((lane & 7) ^ swizzle(row));
-  }
-  const int8_t* const w_base = a.w + n0 * a.w_stride;
-  auto issue = [&](int i, uint32_t slot) {
-    const int k = min((wave + i * WAVES) * kStep, K - kStep);
-#pragma unroll
-    for (int j = 0; j < P; ++j)
-      dma(ring + slot + 1024 * j, (j < 2 * NT ? w_base : a.x) + k, off[j]);
-  };
+  const uint32_t ring = lds_at(lds) + wave * SLOTS * SLOT;
   uint32_t at[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) at[s] = ring + r * kStep + 16u * ((4 * s + grp) ^ swizzle(r));
@@ -568,17 +555,7 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[m][n] = i32x4_t{0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < RING; ++i)
-    if (i < mine) issue(i, i * SLOT);
-  uint32_t slot = 0;
-  for (int i = 0; i < mine; ++i) {
-    const int later = min(RING - 1, mine - 1 - i);   // steps still on their way
-    if (later == 3) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(3 * P) : "memory");
-    else if (later == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * P) : "memory");
-    else if (later == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(P) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    u32x4_t w[2][NT], x[2][MT];
+  auto operands = [&](uint32_t slot, u32x4_t (&w)[2][NT], u32x4_t (&x)[2][MT]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
@@ -586,26 +563,102 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) x[s][m] = lds16(at[s] + slot + 16 * kStep * (NT + m));
     }
-    if (wave + i * WAVES == steps - 1 && tail < kStep) {  // (K's last 128 bytes)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const bool in = 64 * s + 16 * grp >= kStep - tail;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int d = 0; d < 4; ++d) w[s][n][d] = in ? w[s][n][d] : 0u;
-      }
-    }
-    // (read before the slot is filled again)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (i + RING < mine) issue(i + RING, slot);
+  };
+  auto products = [&](const u32x4_t (&w)[2][NT], const u32x4_t (&x)[2][MT]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[s][n], x[s][m], acc[m][n]);
-    slot = slot + SLOT == RING * SLOT ? 0 : slot + SLOT;
+  };
+  // piece i: rows 8 i .. of W, then of X; rows past the end repeat the last one
+  auto row_of = [&](int i) {
+    const int64_t r = (i < 2 * NT ? i : i - 2 * NT) * 8 + (lane >> 3);
+    return min(r, i < 2 * NT ? a.N - 1 - n0 : a.M - 1);
+  };
+  auto chunk_of = [&](int i) { return (lane & 7) ^ swizzle(8 * (i & 1) + (lane >> 3)); };
+  const int8_t* const w_base = a.w + n0 * a.w_stride;
+  if constexpr (DMA) {
+    uint32_t off[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      off[i] = (uint32_t)(row_of(i) * (i < 2 * NT ? a.w_stride : a.x_stride)) + 16u * chunk_of(i);
+    auto issue = [&](int i, uint32_t slot) {
+      const int k = min((wave + i * WAVES) * kStep, K - kStep);
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        dma(ring + slot + 1024 * j, (j < 2 * NT ? w_base : a.x) + k, off[j]);
+    };
+#pragma unroll
+    for (int i = 0; i < RING; ++i)
+      if (i < mine) issue(i, i * SLOT);
+    uint32_t slot = 0;
+    for (int i = 0; i < mine; ++i) {
+      const int later = min(RING - 1, mine - 1 - i);   // steps still on their way
+      if (later == 3) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(3 * P) : "memory");
+      else if (later == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * P) : "memory");
+      else if (later == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(P) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      u32x4_t w[2][NT], x[2][MT];
+      operands(slot, w, x);
+      if (wave + i * WAVES == steps - 1 && tail < kStep) {  // (K's last 128 bytes)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const bool in = 64 * s + 16 * grp >= kStep - tail;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) w[s][n][d] = in ? w[s][n][d] : 0u;
+        }
+      }
+      // (read before the slot is filled again)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (i + RING < mine) issue(i + RING, slot);
+      products(w, x);
+      slot = slot + SLOT == RING * SLOT ? 0 : slot + SLOT;
+    }
+  } else {
+    const int8_t* row[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      row[i] = i < 2 * NT ? w_base + row_of(i) * a.w_stride : a.x + row_of(i) * a.x_stride;
+    u32x4_t held[RING][P];
+    auto load = [&](int i, u32x4_t (&h)[P]) __attribute__((always_inline)) {
+      if (i >= mine) return;
+      const int k0 = (wave + i * WAVES) * kStep;
+      if (k0 + kStep <= K) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) h[j] = load16(row[j] + k0 + 16 * chunk_of(j));
+      } else {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          const int k = k0 + 16 * chunk_of(j), from = min(k, K - 16);
+          h[j] = load16(row[j] + from);
+          if (j < 2 * NT) h[j] = without_first(h[j], k - from);
+        }
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < RING; ++i) load(i, held[i]);
+    for (int i0 = 0; i0 < mine; i0 += RING)
+#pragma unroll
+      for (int u = 0; u < RING; ++u) {
+        if (i0 + u >= mine) break;
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          *(__attribute__((address_space(3))) u32x4_t*)(uintptr_t)(ring + 1024 * j + 16 * lane) =
+              held[u][j];
+        load(i0 + u + RING, held[u]);
+        // (a wave's LDS accesses take effect in their order)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        u32x4_t w[2][NT], x[2][MT];
+        operands(0, w, x);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        products(w, x);
+      }
   }
   i32x4_t* const sums = (i32x4_t*)lds;   // [WAVES][Q][64], once no ring is in use
   __syncthreads();
@@ -619,58 +672,6 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
     i32x4_t s = sums[q * 64 + lane];
 #pragma unroll
     for (int v = 1; v < WAVES; ++v) s += sums[(v * Q + q) * 64 + lane];
-    put4(a, m, n, s);
-  }
-}
-
-// Rows at any address: a workgroup has 16 columns and up to 16 MT rows; its waves take K's steps of 64
-// in turn, U at a time, and add their sums in LDS.  W and X go from memory to the operands'
-// registers.
-template <int MT, int WAVES, int U>
-__global__ void __launch_bounds__(64 * WAVES) int8_few_rows_kernel(LinearArgs a) {
-  constexpr int Q = MT;
-  __shared__ i32x4_t sums[WAVES][Q][64];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const int r = lane & 15, grp = lane >> 4;
-  const int8_t* x[MT];
-  const int8_t* const w = a.w + min(n0 + r, a.N - 1) * a.w_stride;
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-    x[m] = a.x + min((int64_t)(16 * m + r), a.M - 1) * a.x_stride;
-  i32x4_t acc[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m] = i32x4_t{0, 0, 0, 0};
-  const int K = (int)a.K, steps = (K + 63) / 64;
-  for (int t = wave; t < steps; t += U * WAVES) {
-    u32x4_t wf[U], xf[U][MT];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = min(64 * (t + u * WAVES) + 16 * grp, K - 16);
-      wf[u] = load16(w + k);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) xf[u][i] = load16(x[i] + k);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k0 = 64 * (t + u * WAVES);
-      if (k0 + 64 > K) {
-        const int k = k0 + 16 * grp;
-        wf[u] = without_first(wf[u], k - min(k, K - 16));
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i] = mfma(wf[u], xf[u][i], acc[i]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) sums[wave][i][lane] = acc[i];
-  __syncthreads();
-  for (int q = wave; q < Q; q += WAVES) {
-    const int64_t m = 16 * q + r, n = n0 + 4 * grp;
-    i32x4_t s = sums[0][q][lane];
-#pragma unroll
-    for (int v = 1; v < WAVES; ++v) s += sums[v][q][lane];
     put4(a, m, n, s);
   }
 }
@@ -731,9 +732,9 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, bool aligned) {
     // Up to 64 rows the weights' bytes count, and the rows' that every workgroup fetches again.
     // Columns of a workgroup: 32 while that leaves enough workgroups, else 16.
     p.kind = Plan::kFew;
-    p.cols = aligned && N >= 32 * 144 ? 32 : 16;
+    p.cols = N >= 32 * 144 ? 32 : 16;
     p.tiles_n = (N + p.cols - 1) / p.cols;
-    if (!aligned || M <= 32) return p;
+    if (M <= 32) return p;
     best = 3.f + (float)N * (float)K * (1.f + 64.f / (float)p.cols) * 1e-7f;
   }
   const int64_t steps = (K + kStep - 1) / kStep;
@@ -782,22 +783,19 @@ void launch_tiles(const LinearArgs& a, bool dma, hipStream_t stream) {
                        stream, a);
 }
 
+template <bool DMA>
 void launch_few(const LinearArgs& a, const Plan& p, hipStream_t stream) {
   const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
   void (*kern)(LinearArgs);
-  if (!p.dma)
-    kern = mt == 1   ? int8_few_rows_kernel<1, 8, 4>
-           : mt == 2 ? int8_few_rows_kernel<2, 8, 4>
-                     : int8_few_rows_kernel<4, 8, 2>;
-  else if (p.cols == 16)
-    kern = mt == 1   ? int8_stream_kernel<1, 1, 4, 4>
-           : mt == 2 ? int8_stream_kernel<2, 1, 4, 3>
-                     : int8_stream_kernel<4, 1, 4, 2>;
+  if (p.cols == 16)
+    kern = mt == 1   ? int8_stream_kernel<1, 1, 4, 4, DMA>
+           : mt == 2 ? int8_stream_kernel<2, 1, 4, 3, DMA>
+                     : int8_stream_kernel<4, 1, 4, 2, DMA>;
   else
-    kern = mt == 1   ? int8_stream_kernel<1, 2, 4, 2>
-           : mt == 2 ? int8_stream_kernel<2, 2, 4, 2>
-                     : int8_stream_kernel<4, 2, 4, 2>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)p.tiles_n), dim3(p.dma ? 256 : 512), 0, stream, a);
+    kern = mt == 1   ? int8_stream_kernel<1, 2, 4, 2, DMA>
+           : mt == 2 ? int8_stream_kernel<2, 2, 4, 2, DMA>
+                     : int8_stream_kernel<4, 2, 4, 2, DMA>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)p.tiles_n), dim3(256), 0, stream, a);
 }
 
 }  // namespace
@@ -847,7 +845,8 @@ extern "C" int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const
       break;
     }
     case Plan::kFew: {
-      launch_few(a, p, st);
+      if (p.dma) launch_few<true>(a, p, st);
+      else launch_few<false>(a, p, st);
       break;
     }
     case Plan::kTiles:

@@ -71,6 +71,10 @@ def _as_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 else dense_rows(t)
 
 
+def _row_stride(rows: torch.Tensor) -> int:
+    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]   # (a single one has any)
+
+
 def _rows_empty(t: torch.Tensor, dim: int, dtype: torch.dtype) -> torch.Tensor:
     """New rows [..., dim] for those of t.  (At few rows a call is host time: two dims, the usual
     form, go past new_empty's parsing, 0.7 against 1.4 us.)"""
@@ -96,7 +100,7 @@ def _quantize_rows_impl(x):
     rows = _as_rows(x)
     n, dim = rows.shape
     values, scales = _rows_out(x, dim)
-    status = _lib.call_on(x.device, "mrsa_quantize_rows_fwd", rows.data_ptr(), rows.stride(0), n,
+    status = _lib.call_on(x.device, "mrsa_quantize_rows_fwd", rows.data_ptr(), _row_stride(rows), n,
                           dim, DTYPES[x.dtype], values.data_ptr(), scales.data_ptr(),
                           _lib.stream_of(x))
     _lib.check(status, "quantize_rows")
@@ -122,7 +126,7 @@ def _dequantize_rows_impl(values, scales, dtype):
     n, dim = rows.shape
     out = _rows_empty(values, dim, dtype)
     status = _lib.call_on(values.device, "mrsa_dequantize_rows_fwd", rows.data_ptr(),
-                          rows.stride(0), s.data_ptr(), n, dim, DTYPES[dtype], out.data_ptr(),
+                          _row_stride(rows), s.data_ptr(), n, dim, DTYPES[dtype], out.data_ptr(),
                           _lib.stream_of(values))
     _lib.check(status, "dequantize_rows")
     return out
@@ -149,11 +153,11 @@ def _add_rms_norm_int8_impl(x, residual, weight, eps):
         rp, rs, total, tp = None, 0, x.new_empty(0), None
     else:
         res = _as_rows(residual)
-        rp, rs = res.data_ptr(), res.stride(0)
+        rp, rs = res.data_ptr(), _row_stride(res)
         total = _rows_empty(x, dim, x.dtype)
         tp = total.data_ptr()
     values, scales = _rows_out(x, dim)
-    status = _lib.call_on(x.device, "mrsa_add_rms_norm_int8_fwd", rows.data_ptr(), rows.stride(0),
+    status = _lib.call_on(x.device, "mrsa_add_rms_norm_int8_fwd", rows.data_ptr(), _row_stride(rows),
                           rp, rs, w.data_ptr(), n, dim, eps, DTYPES[x.dtype], tp,
                           values.data_ptr(), scales.data_ptr(), _lib.stream_of(x))
     _lib.check(status, "add_rms_norm_int8")
@@ -190,7 +194,7 @@ def _swiglu_int8_impl(gate_up):
     rows = _as_rows(gate_up)
     n, dim = rows.shape[0], rows.shape[1] // 2
     values, scales = _rows_out(gate_up, dim)
-    status = _lib.call_on(gate_up.device, "mrsa_swiglu_int8_fwd", rows.data_ptr(), rows.stride(0),
+    status = _lib.call_on(gate_up.device, "mrsa_swiglu_int8_fwd", rows.data_ptr(), _row_stride(rows),
                           n, dim, DTYPES[gate_up.dtype], values.data_ptr(), scales.data_ptr(),
                           _lib.stream_of(gate_up))
     _lib.check(status, "swiglu_int8")
@@ -225,8 +229,8 @@ def _int8_linear_impl(x, x_scales, weight, weight_scales, bias, dtype):
     nbytes = _workspace_bytes(n, out_dim, dim)
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
     status = _lib.call_on(
-        x.device, "mrsa_int8_linear_fwd", rows.data_ptr(), rows.stride(0), sx.data_ptr(),
-        w.data_ptr(), w.stride(0), sw.data_ptr(), _lib.ptr(b), n, out_dim, dim, DTYPES[dtype],
+        x.device, "mrsa_int8_linear_fwd", rows.data_ptr(), _row_stride(rows), sx.data_ptr(),
+        w.data_ptr(), _row_stride(w), sw.data_ptr(), _lib.ptr(b), n, out_dim, dim, DTYPES[dtype],
         _lib.ptr(ws), nbytes, out.data_ptr(), _lib.stream_of(x))
     _lib.check(status, "int8_linear")
     return out
