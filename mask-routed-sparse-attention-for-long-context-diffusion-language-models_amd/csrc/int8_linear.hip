@@ -76,7 +76,7 @@ struct Tile {
   static constexpr int ROWS = (16 * MT + 63) / 64;             // loads of a wave's rows' scales
   static constexpr int SCALES = 2 * COLS + 64 * ROWS;           // floats, of a wave
   static constexpr int LDS = SLOTS * SLOT + 4 * WAVES * SCALES;
-  static_assert(SLOT % (1024 * WAVES) == 0 && MT % 2 == 0 && NT == 4 &&
+  static_assert(SLOT % (1024 * WAVES) == 0 && NT == 4 &&
                 LDS <= 160 * 1024);
 };
 
@@ -373,32 +373,24 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
         __builtin_amdgcn_sched_barrier(0);
       }
       if (partial) cut(w[1], 1);
-      // second half: in its middle the next step has arrived for every wave, and every wave
-      // has read all of this one, whose slot the step SLOTS further on then fills
-#pragma unroll
-      for (int m = 0; m < MT / 2; ++m) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[1][n], x[m], acc[m][n]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      // in between: the next step has arrived for every wave, and every wave has read all of this
+      // one, whose slot the step SLOTS further on then fills
       if (t + SLOTS - 1 < t1) arrived(most);
       else arrived(none);
+      // second half: each row tile's operand replaced by the next step's (behind the last step:
+      // read, not used)
       const bool more = t + SLOTS < t1;
 #pragma unroll
-      for (int m = MT / 2; m < MT; ++m) {
+      for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[1][n], x[m], acc[m][n]);
-        // (behind the last step: read, not used)
-        constexpr int WR = (NT + MT / 2 - 1) / (MT / 2);
-        const int j = m - MT / 2;
+        constexpr int WR = (NT + MT - 1) / MT, EACH = (P + MT - 1) / MT;
 #pragma unroll
-        for (int n = j * WR; n < (j + 1) * WR && n < NT; ++n) w[0][n] = w_read(0, n, next);
-        x[j] = x_read(0, j, next);
+        for (int n = m * WR; n < (m + 1) * WR && n < NT; ++n) w[0][n] = w_read(0, n, next);
         x[m] = x_read(0, m, next);
         if (more) {
-          constexpr int EACH = (P + MT / 2 - 1) / (MT / 2);
 #pragma unroll
-          for (int i = j * EACH; i < (j + 1) * EACH && i < P; ++i) issue(t + SLOTS, i, slot);
+          for (int i = m * EACH; i < (m + 1) * EACH && i < P; ++i) issue(t + SLOTS, i, slot);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
