@@ -432,7 +432,8 @@ extern "C" int mrsa_swiglu_int8_fwd(const void* gate_up, int64_t row_stride, int
                                     int64_t dim, int32_t dtype, int8_t* values, float* scales,
                                     void* stream) {
   if (rows < 0 || dim < 0 || row_stride < 0) return MRSA_ERR_INVALID_ARGUMENT;
-  if (!known_dtype(dtype) || dim == 0 || too_large(rows, 2 * dim, row_stride))
+  if (!known_dtype(dtype) || dim == 0 || dim > (int64_t)1 << 30 ||
+      too_large(rows, 2 * dim, row_stride))
     return MRSA_ERR_UNSUPPORTED;
   if (rows == 0) return MRSA_OK;
   if (!gate_up || !values || !scales || misaligned(gate_up, dtype) || (uintptr_t)scales % 4 != 0)

@@ -15,16 +15,13 @@ Rounding to 8 bits has no useful derivative: the operators refuse tensors that a
 
 from __future__ import annotations
 
-import functools
 from typing import Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
 
-from . import _lib
-from .rotary import DTYPES, dense_rows, refuse_tangents
+from .rotary import DTYPES
 
-_empty_strided = torch._C._dynamo.guards._empty_strided_cuda   # on the current device
 MAX_DIM = 131071   # of int8_linear: products of 2^14, summed in 32 bits
 
 
@@ -43,15 +40,16 @@ def _no_gradient(name: str, *tensors) -> None:
 
 
 def _check_rows(t, name: str) -> None:
-    if t.ndim < 1 or t.shape[-1] < 1:
-        raise ValueError(f"{name} must have rows of at least one value, got {tuple(t.shape)}")
+    shape = t.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"{name} must have rows of at least one value, got {tuple(shape)}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in DTYPES:
         raise ValueError(f"{name} must be bf16, fp16 or fp32, got {t.dtype}")
 
 
-def _check_values(values, scales, name: str) -> None:
+def _check_values(values, scales, name: str) -> torch.Size:
     shape = values.shape
     if values.dtype != torch.int8 or not values.is_cuda or not shape:
         raise ValueError(f"{name} must be CUDA int8 rows, got {tuple(shape)} {values.dtype} on "
@@ -59,52 +57,9 @@ def _check_values(values, scales, name: str) -> None:
     if scales.shape != shape[:-1] or scales.dtype != torch.float32:
         raise ValueError(f"{name} of shape {tuple(shape)} need fp32 scales of shape "
                          f"{tuple(shape[:-1])}, got {tuple(scales.shape)} {scales.dtype}")
-    if scales.device != values.device:
+    if scales.get_device() != values.get_device():
         raise ValueError(f"{name} and their scales must be on one device")
-
-
-def _as_rows(t: torch.Tensor) -> torch.Tensor:
-    """t as rows [n, dim] whose last dim is dense (a copy only if no strides give that)."""
-
-    if t.ndim != 2:
-        t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 else dense_rows(t)
-
-
-def _row_stride(rows: torch.Tensor) -> int:
-    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]   # (a single one has any)
-
-
-def _rows_empty(t: torch.Tensor, dim: int, dtype: torch.dtype) -> torch.Tensor:
-    """New rows [..., dim] for those of t.  (At few rows a call is host time: two dims, the usual
-    form, go past new_empty's parsing, 0.7 against 1.4 us.)"""
-
-    lead = t.shape[:-1]
-    if len(lead) == 1 and torch._C._cuda_getDevice() == t.device.index:
-        return _empty_strided((lead[0], dim), (dim, 1), dtype)
-    return t.new_empty((*lead, dim), dtype=dtype)
-
-
-def _rows_out(t: torch.Tensor, dim: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    """New 8-bit rows for those of t, and their scales."""
-
-    lead = t.shape[:-1]
-    if len(lead) == 1 and torch._C._cuda_getDevice() == t.device.index:
-        return (_empty_strided((lead[0], dim), (dim, 1), torch.int8),
-                _empty_strided((lead[0],), (1,), torch.float32))
-    return (t.new_empty((*lead, dim), dtype=torch.int8), t.new_empty(lead, dtype=torch.float32))
-
-
-def _quantize_rows_impl(x):
-    refuse_tangents("mrsa::quantize_rows", x)
-    rows = _as_rows(x)
-    n, dim = rows.shape
-    values, scales = _rows_out(x, dim)
-    status = _lib.call_on(x.device, "mrsa_quantize_rows_fwd", rows.data_ptr(), _row_stride(rows), n,
-                          dim, DTYPES[x.dtype], values.data_ptr(), scales.data_ptr(),
-                          _lib.stream_of(x))
-    _lib.check(status, "quantize_rows")
-    return values, scales
+    return shape
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -120,18 +75,6 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return torch.ops.mrsa.quantize_rows.default(x)
 
 
-def _dequantize_rows_impl(values, scales, dtype):
-    refuse_tangents("mrsa::dequantize_rows", scales)
-    rows, s = _as_rows(values), scales.contiguous()
-    n, dim = rows.shape
-    out = _rows_empty(values, dim, dtype)
-    status = _lib.call_on(values.device, "mrsa_dequantize_rows_fwd", rows.data_ptr(),
-                          _row_stride(rows), s.data_ptr(), n, dim, DTYPES[dtype], out.data_ptr(),
-                          _lib.stream_of(values))
-    _lib.check(status, "dequantize_rows")
-    return out
-
-
 def dequantize_rows(values: torch.Tensor, scales: torch.Tensor,
                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """values_k * scale in ``dtype`` (bf16, fp16 or fp32): what 8-bit rows stand for."""
@@ -143,25 +86,6 @@ def dequantize_rows(values: torch.Tensor, scales: torch.Tensor,
         raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
     _no_gradient("dequantize_rows", scales)
     return torch.ops.mrsa.dequantize_rows.default(values, scales, dtype)
-
-
-def _add_rms_norm_int8_impl(x, residual, weight, eps):
-    refuse_tangents("mrsa::add_rms_norm_int8", x, residual, weight)
-    rows, w = _as_rows(x), weight.contiguous()
-    n, dim = rows.shape
-    if residual is None:
-        rp, rs, total, tp = None, 0, x.new_empty(0), None
-    else:
-        res = _as_rows(residual)
-        rp, rs = res.data_ptr(), _row_stride(res)
-        total = _rows_empty(x, dim, x.dtype)
-        tp = total.data_ptr()
-    values, scales = _rows_out(x, dim)
-    status = _lib.call_on(x.device, "mrsa_add_rms_norm_int8_fwd", rows.data_ptr(), _row_stride(rows),
-                          rp, rs, w.data_ptr(), n, dim, eps, DTYPES[x.dtype], tp,
-                          values.data_ptr(), scales.data_ptr(), _lib.stream_of(x))
-    _lib.check(status, "add_rms_norm_int8")
-    return total, values, scales
 
 
 def add_rms_norm_int8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
@@ -189,18 +113,6 @@ def add_rms_norm_int8(x: torch.Tensor, residual: Optional[torch.Tensor], weight:
     return (None if residual is None else total), values, scales
 
 
-def _swiglu_int8_impl(gate_up):
-    refuse_tangents("mrsa::swiglu_int8", gate_up)
-    rows = _as_rows(gate_up)
-    n, dim = rows.shape[0], rows.shape[1] // 2
-    values, scales = _rows_out(gate_up, dim)
-    status = _lib.call_on(gate_up.device, "mrsa_swiglu_int8_fwd", rows.data_ptr(), _row_stride(rows),
-                          n, dim, DTYPES[gate_up.dtype], values.data_ptr(), scales.data_ptr(),
-                          _lib.stream_of(gate_up))
-    _lib.check(status, "swiglu_int8")
-    return values, scales
-
-
 def swiglu_int8(gate_up: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """silu(gate) * up in 8-bit rows: gate_up [..., 2 dim] in bf16, fp16 or fp32 (gate columns
     first), any strides -> (values int8 [..., dim], scales fp32 [...]).  fp32 arithmetic, no
@@ -211,29 +123,6 @@ def swiglu_int8(gate_up: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"gate_up must have an even last dim, got {tuple(gate_up.shape)}")
     _no_gradient("swiglu_int8", gate_up)
     return torch.ops.mrsa.swiglu_int8.default(gate_up)
-
-
-@functools.lru_cache(maxsize=4096)
-def _workspace_bytes(rows: int, out_dim: int, dim: int) -> int:
-    return _lib.call("mrsa_int8_linear_workspace_bytes", rows, out_dim, dim)
-
-
-def _int8_linear_impl(x, x_scales, weight, weight_scales, bias, dtype):
-    refuse_tangents("mrsa::int8_linear", x_scales, weight_scales, bias)
-    rows, w = _as_rows(x), dense_rows(weight)
-    sx, sw = x_scales.contiguous(), weight_scales.contiguous()
-    b = None if bias is None else bias.contiguous()
-    n, dim = rows.shape
-    out_dim = w.shape[0]
-    out = _rows_empty(x, out_dim, dtype)
-    nbytes = _workspace_bytes(n, out_dim, dim)
-    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
-    status = _lib.call_on(
-        x.device, "mrsa_int8_linear_fwd", rows.data_ptr(), _row_stride(rows), sx.data_ptr(),
-        w.data_ptr(), _row_stride(w), sw.data_ptr(), _lib.ptr(b), n, out_dim, dim, DTYPES[dtype],
-        _lib.ptr(ws), nbytes, out.data_ptr(), _lib.stream_of(x))
-    _lib.check(status, "int8_linear")
-    return out
 
 
 def int8_linear(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor,
@@ -247,19 +136,19 @@ def int8_linear(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor,
     multiple of 16 are fastest.  The sum is exact in int32 (dim up to 131071); scales, bias and
     the rounding follow in fp32, so equal inputs give equal bits."""
 
-    _check_values(x, x_scales, "x")
-    _check_values(weight, weight_scales, "weight")
-    if weight.ndim != 2 or weight.shape[1] != x.shape[-1]:
-        raise ValueError(f"weight must be [out_dim, {x.shape[-1]}], got {tuple(weight.shape)}")
-    if weight.device != x.device:
+    dim = _check_values(x, x_scales, "x")[-1]
+    shape = _check_values(weight, weight_scales, "weight")
+    if len(shape) != 2 or shape[1] != dim:
+        raise ValueError(f"weight must be [out_dim, {dim}], got {tuple(shape)}")
+    if weight.get_device() != x.get_device():
         raise ValueError("x and weight must be on one device")
-    if not 1 <= x.shape[-1] <= MAX_DIM:
-        raise ValueError(f"rows of 1 to {MAX_DIM} values have a sum in 32 bits, got {x.shape[-1]}")
+    if not 1 <= dim <= MAX_DIM:
+        raise ValueError(f"rows of 1 to {MAX_DIM} values have a sum in 32 bits, got {dim}")
     if dtype not in DTYPES:
         raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
-    if bias is not None and (bias.shape != weight.shape[:1] or bias.dtype != dtype
-                             or bias.device != x.device):
-        raise ValueError(f"bias must be [{weight.shape[0]}] {dtype} on {x.device}, got "
+    if bias is not None and (bias.shape != shape[:1] or bias.dtype != dtype
+                             or bias.get_device() != x.get_device()):
+        raise ValueError(f"bias must be [{shape[0]}] {dtype} on {x.device}, got "
                          f"{tuple(bias.shape)} {bias.dtype} on {bias.device}")
     _no_gradient("int8_linear", x_scales, weight_scales, bias)
     return torch.ops.mrsa.int8_linear.default(x, x_scales, weight, weight_scales, bias, dtype)

@@ -15,14 +15,15 @@ implementation: a CPU tensor reaching an operator raises.
 
 from __future__ import annotations
 
+import os
 from typing import Optional
 
 import torch
 from torch import Tensor
 
+from ._lib import LIB_PATH, MrsaLibraryError
+
 from .fusion import _fuse_bwd_impl, _fuse_impl
-from .int8 import (_add_rms_norm_int8_impl, _dequantize_rows_impl, _int8_linear_impl,
-                   _quantize_rows_impl, _swiglu_int8_impl)
 from .kernel_utils import _drop_mask_impl, _drop_mask_rows_impl
 from .local_attention import _local_attention_impl
 from .paged_cache import _copy_pages_impl, _paged_append_impl, _paged_attention_impl
@@ -417,38 +418,69 @@ def _(k_pages, v_pages, src, dst):
 
 
 # -- linear layers in 8 bits ------------------------------------------------
+# Their CUDA implementations are C++ (csrc/torch_int8.cpp): a call of one token is host time.
+NATIVE_PATH = os.path.join(os.path.dirname(LIB_PATH), "libmrsa_torch.so")
+_native = []
+
+
+def _define_native(schema):
+    name = schema.split("(")[0]
+    _lib.define(schema)
+    _native.append(name)
+    return torch.library.register_fake(f"mrsa::{name}", lib=_lib)
+
+
+def _load_native(path):
+    """Load the C++ implementations; None, or the error that their calls then raise."""
+
+    try:
+        torch.ops.load_library(path)
+    except OSError as exc:
+        return MrsaLibraryError(
+            f"cannot load {path}: build it first (python -c 'import __graft_entry__ as g; "
+            f"g.build()' from the repository root): {exc}")
+
+
 def _rows_fake(x, dim):
     return x.new_empty((*x.shape[:-1], dim), dtype=torch.int8), x.new_empty(x.shape[:-1],
                                                                             dtype=torch.float32)
 
 
-@_define("quantize_rows(Tensor x) -> (Tensor, Tensor)", _quantize_rows_impl)
+@_define_native("quantize_rows(Tensor x) -> (Tensor, Tensor)")
 def _(x):
     return _rows_fake(x, x.shape[-1])
 
 
-@_define("dequantize_rows(Tensor values, Tensor scales, ScalarType dtype) -> Tensor",
-         _dequantize_rows_impl)
+@_define_native("dequantize_rows(Tensor values, Tensor scales, ScalarType dtype) -> Tensor")
 def _(values, scales, dtype):
     return values.new_empty(values.shape, dtype=dtype)
 
 
-@_define("add_rms_norm_int8(Tensor x, Tensor? residual, Tensor weight, float eps) "
-         "-> (Tensor, Tensor, Tensor)", _add_rms_norm_int8_impl)
+@_define_native("add_rms_norm_int8(Tensor x, Tensor? residual, Tensor weight, float eps) "
+                "-> (Tensor, Tensor, Tensor)")
 def _(x, residual, weight, eps):
     total = x.new_empty(0 if residual is None else x.shape)
     return (total, *_rows_fake(x, x.shape[-1]))
 
 
-@_define("swiglu_int8(Tensor gate_up) -> (Tensor, Tensor)", _swiglu_int8_impl)
+@_define_native("swiglu_int8(Tensor gate_up) -> (Tensor, Tensor)")
 def _(gate_up):
     return _rows_fake(gate_up, gate_up.shape[-1] // 2)
 
 
-@_define("int8_linear(Tensor x, Tensor x_scales, Tensor weight, Tensor weight_scales, "
-         "Tensor? bias, ScalarType dtype) -> Tensor", _int8_linear_impl)
+@_define_native("int8_linear(Tensor x, Tensor x_scales, Tensor weight, Tensor weight_scales, "
+                "Tensor? bias, ScalarType dtype) -> Tensor")
 def _(x, x_scales, weight, weight_scales, bias, dtype):
     return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=dtype)
+
+
+_native_error = _load_native(NATIVE_PATH)
+if _native_error is not None:
+    def _unavailable(*args):
+        raise _native_error
+
+    for _name in _native:
+        _lib.impl(_name, _unavailable, "CUDA")
 
 
 OPERATORS = (

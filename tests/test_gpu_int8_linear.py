@@ -392,6 +392,73 @@ def test_compiled_chain_gives_the_same_bits():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_direct_calls_refuse_tangents():
+    """What a compiler has traced reaches the operators past the public functions."""
+
+    from torch.autograd import forward_ad
+
+    x = torch.zeros(4, 32, device=DEV)
+    v, s = mrsa.quantize_rows(x)
+    ops = torch.ops.mrsa
+    with forward_ad.dual_level(), torch.no_grad():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        ds = forward_ad.make_dual(s, torch.ones_like(s))
+        for call in (lambda: ops.quantize_rows(dual), lambda: ops.swiglu_int8(dual),
+                     lambda: ops.add_rms_norm_int8(x, dual, x[0], 1e-6),
+                     lambda: ops.add_rms_norm_int8(dual, None, x[0], 1e-6),
+                     lambda: ops.add_rms_norm_int8(x, None, dual[0], 1e-6),
+                     lambda: ops.dequantize_rows(v, ds, torch.float32),
+                     lambda: ops.int8_linear(v, ds, v, s, None, torch.float32),
+                     lambda: ops.int8_linear(v, s, v, ds, None, torch.float32),
+                     lambda: ops.int8_linear(v, s, v, s, ds, torch.float32)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        ops.quantize_rows(x)
+
+
+def test_direct_calls_map_errors_as_the_others():
+    """The C entry points' checks behind the operators: ValueError, as through ctypes."""
+
+    x = torch.zeros(4, 32, device=DEV)
+    v, s = mrsa.quantize_rows(x)
+    ops = torch.ops.mrsa
+    with pytest.raises(ValueError):
+        ops.add_rms_norm_int8(x, None, x[0].contiguous(), 0.0)
+    with pytest.raises(ValueError):
+        ops.quantize_rows(x.double())
+    with pytest.raises(ValueError):
+        ops.dequantize_rows(v, s, torch.float64)
+    with pytest.raises(NotImplementedError):
+        ops.quantize_rows(x.cpu())
+
+
+def test_direct_calls_refuse_what_would_pass_their_memory():
+    x = torch.zeros(4, 32, device=DEV)
+    v, s = mrsa.quantize_rows(x)
+    ops = torch.ops.mrsa
+    f32, bf16 = torch.float32, torch.bfloat16
+    for call in (lambda: ops.dequantize_rows(v, s[:3], f32),
+                 lambda: ops.dequantize_rows(v, s.double(), f32),
+                 lambda: ops.dequantize_rows(v, s.cpu(), f32),
+                 lambda: ops.dequantize_rows(x, s, f32),
+                 lambda: ops.add_rms_norm_int8(x, None, x[0, :31], 1e-6),
+                 lambda: ops.add_rms_norm_int8(x, None, x[0].bfloat16(), 1e-6),
+                 lambda: ops.add_rms_norm_int8(x, x[:3], x[0], 1e-6),
+                 lambda: ops.add_rms_norm_int8(x, x.view(8, 16), x[0], 1e-6),
+                 lambda: ops.add_rms_norm_int8(x, x.bfloat16(), x[0], 1e-6),
+                 lambda: ops.swiglu_int8(x[:, :31]),
+                 lambda: ops.int8_linear(v, s[:3], v, s, None, f32),
+                 lambda: ops.int8_linear(v, s, v, s[:3], None, f32),
+                 lambda: ops.int8_linear(v, s, v[:, :16], s, None, f32),
+                 lambda: ops.int8_linear(v, s, v.float(), s, None, f32),
+                 lambda: ops.int8_linear(x, s, v, s, None, f32),
+                 lambda: ops.int8_linear(v, s, v.cpu(), s, None, f32),
+                 lambda: ops.int8_linear(v, s, v, s, x[0, :3], f32),
+                 lambda: ops.int8_linear(v, s, v, s, x[0, :4], bf16)):
+        with pytest.raises((ValueError, NotImplementedError)):
+            call()
+
+
 def test_offsets_past_32_bits():
     """The last rows of matrices of more than 2^32 elements."""
 

@@ -157,9 +157,13 @@ def test_dual_tensors_are_refused():
 
         with pytest.raises(ValueError, match="forward-mode"):
             int8._no_gradient("quantize_rows", dual)
-        with pytest.raises(ValueError, match="forward-mode"):   # what a compiler has traced
-            int8._quantize_rows_impl(dual)
         int8._no_gradient("quantize_rows", x)
+
+
+def test_a_missing_library_is_an_error_of_the_call():
+    error = mrsa.ops._load_native("/nonexistent/libmrsa_torch.so")
+    assert isinstance(error, mrsa.MrsaLibraryError) and "build" in str(error)
+    assert mrsa.ops._native_error is None   # (built for these tests)
 
 
 def test_fake_results():
@@ -220,6 +224,8 @@ def test_c_entry_points_check_before_they_launch():
     assert call("mrsa_swiglu_int8_fwd", None, 16, 0, 8, bf16, None, None, None) == 0
     assert call("mrsa_swiglu_int8_fwd", p, 16, 2, 8, bf16, None, p, None) == 1
     assert call("mrsa_swiglu_int8_fwd", p, 16, 2, 8, 7, p, p, None) == 2
+    for dim in (0, (1 << 30) + 1, 1 << 62, (1 << 63) - 1):   # (twice it may pass 63 bits)
+        assert call("mrsa_swiglu_int8_fwd", p, 16, 2, dim, bf16, p, p, None) == 2
     norm = "mrsa_add_rms_norm_int8_fwd"
     assert call(norm, None, 8, None, 0, None, 0, 8, 1e-6, bf16, None, None, None, None) == 0
     assert call(norm, p, 8, p, 8, p, 2, 8, 1e-6, bf16, None, p, p, None) == 1   # sum nowhere
