@@ -338,7 +338,19 @@ void launch_rows(const RowArgs& a, hipStream_t stream) {
                      a);
 }
 
-// A wave a row up to 1024 elements, then a block whose threads hold the row in registers.
+// A wave a row up to 1024 elements (no barriers: 16384 rows of 1024 9.6 us, by blocks of 256
+// 13.7), then a block whose threads hold the row in registers, with as few units a thread as
+// leaves no thread idle: bf16, 16384 rows,
+//                     elements   256 threads (units)   512           1024
+//   quantize              3584   28.8 (2)              34.0 (1)      56.0 (1)
+//   norm                  3584   70.3 (2)              73.2 (1)      101 (1)
+//   swiglu                3584   67.0 (2)              58.0 (1)      103 (1)
+//   swiglu                8192   136 (4)               121 (2)       121 (1)
+//   norm                 12288   278 (8)               242 (3)       284 (2)
+//   swiglu               18944   315 (10)              285 (5)       314 (3)
+//   norm                 18944   538 (10)              440 (5)       430 (3)
+// Past 20480 elements the row is read twice, by 1024 threads (8192 rows of 32768: quantize 175 us,
+// 512 threads 192; one row of them 3.9 and 5.0).
 template <class T, int OP>
 void rows_of(const RowArgs& a, hipStream_t stream) {
   const int64_t units = (a.K + 7) / 8;
@@ -346,11 +358,12 @@ void rows_of(const RowArgs& a, hipStream_t stream) {
   else if (units <= 64) launch_rows<T, OP, 64, 1>(a, stream);
   else if (units <= 128) launch_rows<T, OP, 64, 2>(a, stream);
   else if (units <= 256) launch_rows<T, OP, 256, 1>(a, stream);
+  else if (units <= 512 && OP == kSwiglu) launch_rows<T, OP, 512, 1>(a, stream);
   else if (units <= 512) launch_rows<T, OP, 256, 2>(a, stream);
-  else if (units <= 1024) launch_rows<T, OP, 256, 4>(a, stream);
+  else if (units <= 1024) launch_rows<T, OP, 512, 2>(a, stream);
   else if (units <= 1536) launch_rows<T, OP, 512, 3>(a, stream);
   else if (units <= 2560) launch_rows<T, OP, 512, 5>(a, stream);
-  else launch_rows<T, OP, 512, 0>(a, stream);
+  else launch_rows<T, OP, 1024, 0>(a, stream);
 }
 
 template <int OP>
