@@ -682,6 +682,37 @@ __global__ void __launch_bounds__(256) int8_short_rows_kernel(LinearArgs a) {
   }
 }
 
+// Rows of any stride and address to rows of `padded` bytes (a multiple of 128), zeros behind K >= 16:
+// W's N rows, then X's M.  16 bytes a thread; blocks cover chunks (x) of rows (y).
+__global__ void __launch_bounds__(256) int8_pad_kernel(LinearArgs a, int64_t padded, int8_t* to) {
+  const int64_t k = 16 * ((int64_t)blockIdx.x * blockDim.x + threadIdx.x);
+  if (k >= padded) return;
+  for (int64_t r = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r < a.N + a.M;
+       r += (int64_t)gridDim.y * blockDim.y) {
+    const int8_t* const from = r < a.N ? a.w + r * a.w_stride : a.x + (r - a.N) * a.x_stride;
+    u32x4_t v = {0, 0, 0, 0};
+    if (k + 16 <= a.K) {
+      v = load16(from + k);
+    } else if (k < a.K) {
+      // the row's last 16 bytes, the ones before k moved out
+      v = load16(from + a.K - 16);
+      const int out = 16 - (int)(a.K - k), words = out >> 2, bits = 8 * (out & 3);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        uint32_t lo = 0, hi = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (e == d + words) lo = v[e];
+          if (e == d + words + 1) hi = v[e];
+        }
+        // (d ascends and reads only what is at or above it)
+        v[d] = bits ? lo >> bits | hi << (32 - bits) : lo;
+      }
+    }
+    *(u32x4_t*)(to + r * padded + k) = v;
+  }
+}
+
 // How a product is cut: by its sizes and alignment alone.  A step of a tile costs about the same
 // for few rows as for many, so small tiles finish few rows first and large ones many; `parts` of K
 // fill the CUs where tiles do not, for a second kernel's time.  The estimate below is fitted to
@@ -712,23 +743,11 @@ struct Plan {
   int shape;
   bool dma;
   int64_t tiles_m, tiles_n, parts, bytes, cols;
+  int64_t padded;   // bytes of the padded rows that the tiles are cut from, at the workspace's end
 };
-Plan plan_of(int64_t M, int64_t N, int64_t K, bool aligned) {
-  Plan p = {Plan::kTiles, 0, aligned, 1, 1, 1, 0, 0};
-  if (K < 16) {
-    p.kind = Plan::kShort;
-    return p;
-  }
-  float best = 1e30f;
-  if (M <= 64) {
-    // Up to 64 rows the weights' bytes count, and the rows' that every workgroup fetches again.
-    // Columns of a workgroup: 32 while that leaves enough workgroups, else 16.
-    p.kind = Plan::kFew;
-    p.cols = N >= 32 * 144 ? 32 : 16;
-    p.tiles_n = (N + p.cols - 1) / p.cols;
-    if (M <= 32) return p;
-    best = 3.f + (float)N * (float)K * (1.f + 64.f / (float)p.cols) * 1e-7f;
-  }
+
+// The best cut of tiles that beats `best` us, with `more` us for all that comes before them.
+void best_tiles(int64_t M, int64_t N, int64_t K, bool aligned, float more, float& best, Plan& p) {
   const int64_t steps = (K + kStep - 1) / kStep;
   for (int i = 0; i < (int)(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
     const Shape& s = kShapes[i];
@@ -740,19 +759,51 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, bool aligned) {
       if (parts > 1 && items > s.room) break;  // (and so the workspace stays small)
       const float rounds = items <= 4 * s.room ? (float)((items + s.room - 1) / s.room)
                                                : (float)items / (float)s.room + 0.5f;
-      const float step = items <= 256 ? s.one : s.two;
+      // (through registers a step takes 1.3 to 1.9 times as long)
+      const float step = (items <= 256 ? s.one : s.two) * (aligned ? 1.f : 1.6f);
       const int64_t bytes = parts > 1 ? items * s.tm * s.tn * 4 : 0;
-      const float time = rounds * (s.fixed + step * (float)((steps + parts - 1) / parts)) +
+      const float time = more +
+                         rounds * (s.fixed + step * (float)((steps + parts - 1) / parts)) +
                          (parts > 1 ? 6.f + 0.27e-6f * (float)bytes : 0.f);
       if (time < best) {
         best = time;
-        p.kind = Plan::kTiles;
-        p.shape = i;
-        p.tiles_m = tm;
-        p.tiles_n = tn;
-        p.parts = parts;
-        p.bytes = bytes;
+        p = {Plan::kTiles, i, aligned, tm, tn, parts, bytes, 0, 0};
       }
+    }
+  }
+}
+
+Plan plan_of(int64_t M, int64_t N, int64_t K, bool aligned) {
+  Plan p = {Plan::kTiles, 0, aligned, 1, 1, 1, 0, 0, 0};
+  if (K < 16) {
+    p.kind = Plan::kShort;
+    return p;
+  }
+  float best = 1e30f;
+  if (M <= 64) {
+    // Up to 64 rows the weights' bytes count, and the rows' that every workgroup fetches again.
+    // Columns of a workgroup: 32 while that leaves half the CUs a workgroup, else 16 (us, 16 and
+    // 32: 32 rows of 3584 values, 3584 columns 5.0 and 5.3, 4608 6.8 and 5.6, 37888 39 and 31; 16
+    // rows of 4096, 4096 columns 6.9 and 5.9; 64 rows 8.1 and 8.3).
+    p.kind = Plan::kFew;
+    p.cols = N >= 32 * 128 ? 32 : 16;
+    p.tiles_n = (N + p.cols - 1) / p.cols;
+    if (M <= 32) return p;
+    best = 3.f + (float)N * (float)K * (1.f + 64.f / (float)p.cols) * 1e-7f;
+  }
+  best_tiles(M, N, K, aligned, 0.f, best, p);
+  if (K % 16 != 0) {
+    // Rows that no stride aligns: padded copies of them first where the tiles gain more than the
+    // copies' bytes cost (us, through registers and with copies: 512 x 3584 of 3583 values 27.9 and
+    // 26.3, 2000 x 2000 of 7999 70 and 51, 8192 x 4096 of 4095 161 and 139, 16384 x 3584 of 18943
+    // 1451 and 1095).
+    const int64_t padded = (K + kStep - 1) / kStep * kStep;
+    const float bytes = (float)(M + N) * (float)padded;
+    const float before = best;
+    best_tiles(M, N, padded, true, 3.f + bytes * 0.33e-6f, best, p);
+    if (best < before) {
+      p.padded = padded;
+      p.bytes += (M + N) * padded;
     }
   }
   return p;
@@ -796,8 +847,8 @@ extern "C" int64_t mrsa_int8_linear_workspace_bytes(int64_t rows, int64_t out_di
   if (rows < 0 || out_dim < 0 || dim < 0 || rows >= (int64_t)1 << 31 ||
       out_dim >= (int64_t)1 << 31 || dim > 131071)
     return -1;
-  return std::max(plan_of(rows, out_dim, dim, true).bytes,
-                  plan_of(rows, out_dim, dim, false).bytes);
+  const int64_t bytes = plan_of(rows, out_dim, dim, false).bytes;
+  return dim % 16 != 0 ? bytes : std::max(bytes, plan_of(rows, out_dim, dim, true).bytes);
 }
 
 extern "C" int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const float* x_scales,
@@ -826,10 +877,23 @@ extern "C" int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const
   if (groups >= (int64_t)1 << 23) return MRSA_ERR_UNSUPPORTED;
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16 != 0))
     return MRSA_ERR_INVALID_ARGUMENT;
-  const LinearArgs a = {x, weight, x_scales, weight_scales, bias, out, (int32_t*)workspace, rows,
+  LinearArgs a = {x, weight, x_scales, weight_scales, bias, out, (int32_t*)workspace, rows,
                         out_dim, dim, x_row_stride, weight_row_stride, dtype, (int32_t)p.parts,
                         (int32_t)p.tiles_m, (int32_t)p.tiles_n};
   const hipStream_t st = (hipStream_t)stream;
+  if (p.padded > 0) {
+    int8_t* const to = (int8_t*)workspace + (p.bytes - (rows + out_dim) * p.padded);
+    const int64_t chunks = p.padded / 16, all = rows + out_dim;
+    unsigned tx = 8;
+    while (tx < 64 && tx < chunks) tx *= 2;
+    const dim3 block(tx, 256 / tx);
+    const int64_t by = std::min<int64_t>((all + block.y - 1) / block.y, 16384);
+    hipLaunchKernelGGL(int8_pad_kernel, dim3((unsigned)((chunks + tx - 1) / tx), (unsigned)by),
+                       block, 0, st, a, p.padded, to);
+    a.w = to;
+    a.x = to + out_dim * p.padded;
+    a.K = a.x_stride = a.w_stride = p.padded;
+  }
   switch (p.kind) {
     case Plan::kShort: {
       const int64_t blocks = std::min<int64_t>((rows * out_dim + 255) / 256, 1 << 20);

@@ -17,6 +17,7 @@ import pytest
 import torch
 
 import mrsa
+from mrsa import _lib
 from oracle import int8_oracle as O8
 
 pytestmark = pytest.mark.gpu
@@ -298,6 +299,25 @@ def test_int8_linear_of_any_strides(M):
     assert one.shape == (N,) and torch.equal(one, want[0])
     same = mrsa.int8_linear(x[:1].expand(M, K), sx[:1].expand(M), w, sw, bias, dtype=torch.float32)
     assert torch.equal(same, want[:1].expand(M, N))
+
+
+@pytest.mark.parametrize("more", range(1, 16))
+def test_rows_that_are_copied_to_aligned_ones(more):
+    """Lengths that no stride aligns, at sizes where the copies pay: their last bytes, and what
+    lies behind the rows."""
+
+    M, N, K = 1301, 1403, 2032 + more
+    need = _lib.call("mrsa_int8_linear_workspace_bytes", M, N, K)
+    assert need >= (M + N) * 2048   # copied
+    x, sx, w, sw, bias = _operands(M, N, K, more, full=True)
+    want = mrsa.int8_linear(x, sx, w, sw, bias, dtype=torch.float32)
+    check_linear(want, x, sx, w, sw, bias)
+    wide = torch.full((M, K + 5 + more), 127, dtype=torch.int8, device=DEV)
+    wide[:, 2:K + 2] = x
+    heavy = torch.full((N, K + 48 - more), -128, dtype=torch.int8, device=DEV)
+    heavy[:, 1:K + 1] = w
+    got = mrsa.int8_linear(wide[:, 2:K + 2], sx, heavy[:, 1:K + 1], sw, bias, dtype=torch.float32)
+    assert torch.equal(got, want)
 
 
 @pytest.mark.parametrize("M", (3, 40, 200))
