@@ -64,20 +64,24 @@ __device__ __forceinline__ u32x4_t without_first(u32x4_t v, int64_t bytes) {
 // A step is 128 bytes of K: whole cache lines.
 constexpr int kStep = 128;
 
-template <int TM_, int TN_, int WM_, int WN_, int SLOTS_>
+// WS and XS: steps of W and of X that are in LDS at once.
+template <int TM_, int TN_, int WM_, int WN_, int WS_, int XS_>
 struct Tile {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, SLOTS = SLOTS_;
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WS = WS_, XS = XS_;
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int MT = TM / WM / 16, NT = TN / WN / 16;   // 16 x 16 products of a wave
-  static constexpr int SLOT = (TM + TN) * kStep;               // bytes of a step: W's rows, X's
-  static constexpr int PIECES = SLOT / 1024 / WAVES;           // 1 KB each, of a wave
-  static constexpr int W_PIECES = TN * kStep / 1024;
+  static constexpr int W_SLOT = TN * kStep, X_SLOT = TM * kStep;   // bytes of a step
+  static constexpr int X_LDS = WS * W_SLOT, SLOTS_END = X_LDS + XS * X_SLOT;
+  static constexpr int PW = W_SLOT / 1024 / WAVES, PX = X_SLOT / 1024 / WAVES;   // 1 KB, of a wave
   static constexpr int COLS = 16 * NT;
   static constexpr int ROWS = (16 * MT + 63) / 64;             // loads of a wave's rows' scales
   static constexpr int SCALES = 2 * COLS + 64 * ROWS;           // floats, of a wave
-  static constexpr int LDS = SLOTS * SLOT + 4 * WAVES * SCALES;
-  static_assert(SLOT % (1024 * WAVES) == 0 && NT == 4 &&
-                LDS <= 160 * 1024);
+  // One more step of W than of X: the scales have no room of their own.
+  static constexpr bool SHARED = WS > XS;
+  static constexpr int LDS = SLOTS_END + (SHARED ? 0 : 4 * WAVES * SCALES);
+  static_assert(W_SLOT % (1024 * WAVES) == 0 && X_SLOT % (1024 * WAVES) == 0 && NT == 4 &&
+                LDS <= 160 * 1024 && XS >= 2 && (WS == XS || (WS == 3 && XS == 2)) &&
+                4 * WAVES * SCALES <= W_SLOT);
 };
 
 // Chunk c (16 bytes) of row r lies in place c ^ swizzle(r) of the row: the sixteen rows of a
@@ -261,7 +265,7 @@ template <class T, bool DMA>
 __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 : 2))
     int8_tile_kernel(LinearArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
-  constexpr int P = T::PIECES, MT = T::MT, NT = T::NT;
+  constexpr int PW = T::PW, PX = T::PX, MT = T::MT, NT = T::NT;
   const int tiles = a.tiles_m * a.tiles_n;
   const int part = blockIdx.x / tiles, tile = blockIdx.x - part * tiles;
   const int steps = (int)((a.K + kStep - 1) / kStep);
@@ -269,8 +273,11 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
   const int t0 = (int)((int64_t)steps * part / a.parts);
   const int t1 = (int)((int64_t)steps * (part + 1) / a.parts);
   const Position<T> p(a, tile);
-  float* const scales = (float*)(lds + T::SLOTS * T::SLOT) + p.wave * T::SCALES;
-  if (a.parts == 1) fetch_scales<T>(a, p, scales);
+  // The scales' place.  SHARED: the slot of W that the last two steps leave free.
+  float* const scales =
+      (float*)(lds + (!T::SHARED ? T::SLOTS_END : (DMA ? (t1 + 1 - t0) % 3 : 2) * T::W_SLOT)) +
+      p.wave * T::SCALES;
+  if (a.parts == 1 && (!T::SHARED || !DMA || t1 - t0 == 1)) fetch_scales<T>(a, p, scales);
   const int lane = p.lane, wave = p.wave;
 
   // ---- operands in LDS: row lane % 16 of a product, chunk lane / 16 of its 64 bytes.  (Products
@@ -281,7 +288,7 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
   for (int s = 0; s < 2; ++s) {
     const int r = lane & 15, c = 4 * s + (lane >> 4), rw = column_of(0, r);
     w_at[s] = lds0 + (p.wn * T::COLS + rw) * kStep + 16u * (c ^ swizzle_w(rw));
-    x_at[s] = lds0 + T::TN * kStep + (p.wm * 16 * MT + r) * kStep + 16u * (c ^ swizzle(r));
+    x_at[s] = lds0 + T::X_LDS + (p.wm * 16 * MT + r) * kStep + 16u * (c ^ swizzle(r));
   }
   auto w_read = [&](int s, int n, uint32_t slot) {
     return lds16(w_at[s] + slot + kStep * column_of(n, 0));
@@ -300,58 +307,68 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
 #pragma unroll
       for (int d = 0; d < 4; ++d) f[n][d] = in ? f[n][d] : 0u;
   };
-  const uint32_t to = lds0 + wave * P * 1024;
-  auto row_of = [&](int i) {  // piece i of the wave: rows 8 at a time of W, then of X
-    const int piece = wave * P + i;
-    return (piece - (piece < T::W_PIECES ? 0 : T::W_PIECES)) * 8 + (lane >> 3);
-  };
-  auto chunk_of = [&](int i) {
-    const int r = row_of(i);
-    return (lane & 7) ^ (wave * P + i < T::W_PIECES ? swizzle_w(r) : swizzle(r));
-  };
+  // piece i of the wave, of W or of X: eight rows of a step
+  const uint32_t w_to = lds0 + wave * PW * 1024, x_to = lds0 + T::X_LDS + wave * PX * 1024;
+  auto w_row = [&](int i) { return (wave * PW + i) * 8 + (lane >> 3); };
+  auto x_row = [&](int i) { return (wave * PX + i) * 8 + (lane >> 3); };
+  auto w_chunk = [&](int i) { return (lane & 7) ^ swizzle_w(w_row(i)); };
+  auto x_chunk = [&](int i) { return (lane & 7) ^ swizzle(x_row(i)); };
 
   if constexpr (DMA) {
     // Where this wave's pieces come from: rows past the end repeat the last one.
     const int8_t* const w_from = uniform(a.w + p.n0 * a.w_stride);
     const int8_t* const x_from = uniform(a.x + p.m0 * a.x_stride);
-    uint32_t off[P];
+    uint32_t w_off[PW], x_off[PX];
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const bool is_w = wave * P + i < T::W_PIECES;
-      const int64_t last = is_w ? a.N - 1 - p.n0 : a.M - 1 - p.m0;
-      off[i] = (uint32_t)(min((int64_t)row_of(i), last) * (is_w ? a.w_stride : a.x_stride)) +
-               16u * chunk_of(i);
-    }
-    auto issue = [&](int t, int i, uint32_t slot) {
-      dma(to + slot + 1024 * i,
-          (wave * P + i < T::W_PIECES ? w_from : x_from) + min((int64_t)t * kStep, a.K - kStep),
-          off[i]);
+    for (int i = 0; i < PW; ++i)
+      w_off[i] = (uint32_t)(min((int64_t)w_row(i), a.N - 1 - p.n0) * a.w_stride) + 16u * w_chunk(i);
+#pragma unroll
+    for (int i = 0; i < PX; ++i)
+      x_off[i] = (uint32_t)(min((int64_t)x_row(i), a.M - 1 - p.m0) * a.x_stride) + 16u * x_chunk(i);
+    auto issue_w = [&](int t, int i, uint32_t slot) {
+      dma(w_to + slot + 1024 * i, w_from + min((int64_t)t * kStep, a.K - kStep), w_off[i]);
     };
-    // The wave's own pieces of a step have landed (those of the LATER steps behind it may be on
-    // their way), its reads are done, and so for every wave.
+    auto issue_x = [&](int t, int i, uint32_t slot) {
+      dma(x_to + slot + 1024 * i, x_from + min((int64_t)t * kStep, a.K - kStep), x_off[i]);
+    };
+    // The wave's own pieces of a step have landed (the LATER ones behind them may be on their
+    // way), its reads are done, and so for every wave.
     auto arrived = [&](auto later) {
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(P * later()) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(later()) : "memory");
     };
-    constexpr int SLOTS = T::SLOTS;
+    constexpr int WS = T::WS, XS = T::XS;
     auto none = [] { return 0; };
-    auto most = [] { return SLOTS - 2; };
+    auto most = [] { return WS > XS ? PW : (PW + PX) * (XS - 2); };
+    auto after = [](uint32_t slot, int slots, int bytes) {
+      return slot == (uint32_t)((slots - 1) * bytes) ? 0u : slot + (uint32_t)bytes;
+    };
+    // Pieces in the order in which steps need them, X's ahead of W's: after those of step t come
+    // at most `most` others.
 #pragma unroll
-    for (int j = 0; j < SLOTS - 1; ++j) {
+    for (int j = 0; j < WS - 1; ++j) {
       if (t0 + j >= t1) break;
+      if (j < XS - 1) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) issue(t0 + j, i, j * T::SLOT);
+        for (int i = 0; i < PX; ++i) issue_x(t0 + j, i, j * T::X_SLOT);
+      }
+#pragma unroll
+      for (int i = 0; i < PW; ++i) issue_w(t0 + j, i, j * T::W_SLOT);
     }
-    if (t0 + SLOTS - 2 < t1) arrived(most);
+    if (t0 + WS - 2 < t1) arrived(most);
     else arrived(none);
 #pragma unroll
     for (int n = 0; n < NT; ++n) w[0][n] = w_read(0, n, 0);
 #pragma unroll
     for (int m = 0; m < MT; ++m) x[m] = x_read(0, m, 0);
-    if (t0 + SLOTS - 1 < t1) {
+    if (t0 + XS - 1 < t1) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) issue(t0 + SLOTS - 1, i, (SLOTS - 1) * T::SLOT);
+      for (int i = 0; i < PX; ++i) issue_x(t0 + XS - 1, i, (XS - 1) * T::X_SLOT);
     }
-    uint32_t slot = 0;
+    if (t0 + WS - 1 < t1) {
+#pragma unroll
+      for (int i = 0; i < PW; ++i) issue_w(t0 + WS - 1, i, (WS - 1) * T::W_SLOT);
+    }
+    uint32_t w_slot = 0, x_slot = 0;
     for (int t = t0; t < t1; ++t) {
       // (in registers that the products need no copies of)
 #pragma unroll
@@ -359,7 +376,7 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
 #pragma unroll
         for (int n = 0; n < NT; ++n) asm volatile("" : "+v"(acc[m][n]));
       const bool partial = t == steps - 1 && tail < kStep;
-      const uint32_t next = slot == (SLOTS - 1) * T::SLOT ? 0 : slot + (uint32_t)T::SLOT;
+      const uint32_t w_next = after(w_slot, WS, T::W_SLOT), x_next = after(x_slot, XS, T::X_SLOT);
       // first half: its products, each row tile's operand replaced by the second half's
       if (partial) cut(w[0], 0);
 #pragma unroll
@@ -368,83 +385,94 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
         for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[0][n], x[m], acc[m][n]);
         constexpr int WR = (NT + MT - 1) / MT;
 #pragma unroll
-        for (int n = m * WR; n < (m + 1) * WR && n < NT; ++n) w[1][n] = w_read(1, n, slot);
-        x[m] = x_read(1, m, slot);
+        for (int n = m * WR; n < (m + 1) * WR && n < NT; ++n) w[1][n] = w_read(1, n, w_slot);
+        x[m] = x_read(1, m, x_slot);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (partial) cut(w[1], 1);
       // in between: the next step has arrived for every wave, and every wave has read all of this
-      // one, whose slot the step SLOTS further on then fills
-      if (t + SLOTS - 1 < t1) arrived(most);
+      // one, whose slots steps WS and XS further on then fill
+      if (t + WS - 1 < t1) arrived(most);
       else arrived(none);
       // second half: each row tile's operand replaced by the next step's (behind the last step:
       // read, not used)
-      const bool more = t + SLOTS < t1;
+      const bool more_w = t + WS < t1, more_x = t + XS < t1;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[1][n], x[m], acc[m][n]);
-        constexpr int WR = (NT + MT - 1) / MT, EACH = (P + MT - 1) / MT;
+        constexpr int WR = (NT + MT - 1) / MT, EACH = (PX + PW + MT - 1) / MT;
 #pragma unroll
-        for (int n = m * WR; n < (m + 1) * WR && n < NT; ++n) w[0][n] = w_read(0, n, next);
-        x[m] = x_read(0, m, next);
-        if (more) {
+        for (int n = m * WR; n < (m + 1) * WR && n < NT; ++n) w[0][n] = w_read(0, n, w_next);
+        x[m] = x_read(0, m, x_next);
 #pragma unroll
-          for (int i = m * EACH; i < (m + 1) * EACH && i < P; ++i) issue(t + SLOTS, i, slot);
+        for (int i = m * EACH; i < (m + 1) * EACH && i < PX + PW; ++i) {
+          if (i < PX) {
+            if (more_x) issue_x(t + XS, i, x_slot);
+          } else {
+            if (more_w) issue_w(t + WS, i - PX, w_slot);
+          }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      slot = next;
+      // (every wave has read this step, and none comes that fills its slot of W)
+      if (T::SHARED && t + 2 == t1 && a.parts == 1) fetch_scales<T>(a, p, scales);
+      w_slot = w_next;
+      x_slot = x_next;
     }
   } else {
     // Through registers; rows at any address, K from 16 on.
-    u32x4_t held[P];
-    const int8_t* row[P];
+    u32x4_t w_held[PW], x_held[PX];
+    const int8_t *w_from[PW], *x_from[PX];
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const bool is_w = wave * P + i < T::W_PIECES;
-      row[i] = (is_w ? a.w : a.x) +
-               min((is_w ? p.n0 : p.m0) + row_of(i), (is_w ? a.N : a.M) - 1) *
-                   (is_w ? a.w_stride : a.x_stride);
-    }
+    for (int i = 0; i < PW; ++i) w_from[i] = a.w + min(p.n0 + w_row(i), a.N - 1) * a.w_stride;
+#pragma unroll
+    for (int i = 0; i < PX; ++i) x_from[i] = a.x + min(p.m0 + x_row(i), a.M - 1) * a.x_stride;
     auto load = [&](int t) {
       const int64_t k0 = (int64_t)t * kStep;
       if (k0 + kStep <= a.K) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) held[i] = load16(row[i] + k0 + 16 * chunk_of(i));
+        for (int i = 0; i < PW; ++i) w_held[i] = load16(w_from[i] + k0 + 16 * w_chunk(i));
+#pragma unroll
+        for (int i = 0; i < PX; ++i) x_held[i] = load16(x_from[i] + k0 + 16 * x_chunk(i));
       } else {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-          const int64_t k = k0 + 16 * chunk_of(i), at = min(k, a.K - 16);
-          held[i] = load16(row[i] + at);
-          if (wave * P + i < T::W_PIECES) held[i] = without_first(held[i], k - at);
+        for (int i = 0; i < PW; ++i) {
+          const int64_t k = k0 + 16 * w_chunk(i), at = min(k, a.K - 16);
+          w_held[i] = without_first(load16(w_from[i] + at), k - at);
         }
+#pragma unroll
+        for (int i = 0; i < PX; ++i)
+          x_held[i] = load16(x_from[i] + min(k0 + 16 * x_chunk(i), a.K - 16));
       }
     };
-    auto store = [&](uint32_t slot) {
+    auto store = [&](int slot) {
+      auto put = [&](uint32_t at, u32x4_t v) {
+        *(__attribute__((address_space(3))) u32x4_t*)(uintptr_t)(at + 16 * lane) = v;
+      };
 #pragma unroll
-      for (int i = 0; i < P; ++i)
-        *(__attribute__((address_space(3))) u32x4_t*)(uintptr_t)(to + slot + 1024 * i + 16 * lane) =
-            held[i];
+      for (int i = 0; i < PW; ++i) put(w_to + slot * T::W_SLOT + 1024 * i, w_held[i]);
+#pragma unroll
+      for (int i = 0; i < PX; ++i) put(x_to + slot * T::X_SLOT + 1024 * i, x_held[i]);
       __syncthreads();
     };
     load(t0);
     store(0);
-    uint32_t slot = 0;
+    int slot = 0;
     for (int t = t0; t < t1; ++t) {
       if (t + 1 < t1) load(t + 1);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) w[0][n] = w_read(s, n, slot);
+        for (int n = 0; n < NT; ++n) w[0][n] = w_read(s, n, slot * T::W_SLOT);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          x[m] = x_read(s, m, slot);
+          x[m] = x_read(s, m, slot * T::X_SLOT);
 #pragma unroll
           for (int n = 0; n < NT; ++n) acc[m][n] = mfma(w[0][n], x[m], acc[m][n]);
         }
       }
-      slot ^= (uint32_t)T::SLOT;
+      slot ^= 1;
       if (t + 1 < t1) store(slot);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the scales)
@@ -722,12 +750,12 @@ __global__ void __launch_bounds__(256) int8_pad_kernel(LinearArgs a, int64_t pad
 //   1003 rows of the same: 64 x 64 138, 128 x 128 87, 256 x 256 230 (four 86)
 //   128 rows, 37888 x 3584: 128 x 256 34, 128 x 128 40, 256 x 256 50
 //   4096 rows, 8192 x 8192: 256 x 256 223, 128 x 256 258, 128 x 128 280
-typedef Tile<64, 64, 2, 1, 4> Tile64;
-typedef Tile<64, 128, 2, 2, 3> Tile64x128;
-typedef Tile<128, 128, 4, 2, 4> TileDeep;     // a workgroup a CU
-typedef Tile<128, 128, 4, 2, 2> Tile128;      // two
-typedef Tile<128, 256, 2, 4, 3> Tile128x256;
-typedef Tile<256, 256, 2, 4, 2> Tile256;
+typedef Tile<64, 64, 2, 1, 4, 4> Tile64;
+typedef Tile<64, 128, 2, 2, 3, 3> Tile64x128;
+typedef Tile<128, 128, 4, 2, 4, 4> TileDeep;     // a workgroup a CU
+typedef Tile<128, 128, 4, 2, 2, 2> Tile128;      // two
+typedef Tile<128, 256, 2, 4, 3, 3> Tile128x256;
+typedef Tile<256, 256, 2, 4, 3, 2> Tile256;
 struct Shape {
   int tm, tn, room;        // workgroups that the CUs hold
   float one, two, fixed;   // us: a step of a workgroup alone on its CU, of two, the rest
