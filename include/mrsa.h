@@ -1049,9 +1049,10 @@ int mrsa_swiglu_int8_fwd(const void* gate_up, int64_t row_stride, int64_t rows, 
  *   bias: optional [out_dim] of `dtype`; out: [rows, out_dim] of `dtype`, dense
  *   workspace: mrsa_int8_linear_workspace_bytes (16-byte aligned; may be NULL
  *     for 0 bytes), held by one call at a time
- * Rows at multiples of 16 bytes with dim a multiple of 16 are fastest.  Limits:
- * dim <= 131071, rows, out_dim and strides < 2^31, fewer than 2^23 workgroups
- * (tiles of 128 x 128 or more results, 16 columns for up to 64 rows).
+ * Rows at multiples of 16 bytes with dim a multiple of 16, from 128 on, are
+ * fastest; where dim is not a multiple of 16 the workspace may hold copies of
+ * both matrices.  Limits: dim <= 131071, rows, out_dim and strides < 2^31, fewer
+ * than 2^23 workgroups (of 256 x 256 results where there are many).
  */
 int64_t mrsa_int8_linear_workspace_bytes(int64_t rows, int64_t out_dim, int64_t dim);
 int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const float* x_scales,

@@ -259,8 +259,23 @@ __device__ __forceinline__ void finish(const LinearArgs& a, const Position<T>& p
   }
 }
 
-// A workgroup computes one part of K of a tile.  DMA: rows 16-byte aligned and K a multiple of 16,
-// from 128 on.  Otherwise rows go through registers.
+// A workgroup computes one part of K of a tile, each wave (16 MT) x 64 of it, W as the products'
+// first operand.  DMA: rows 16-byte aligned and K a multiple of 16, from 128 on.  Otherwise rows go
+// through registers, a step ahead.
+//
+// What bounds the large shapes is bringing operands from L2 to LDS: at 256 x 256 results a CU's
+// registers are full, and a step's 64 KB come in where the matrix cores need 2048 cycles for its
+// products.  16384 x 37888 of 3584 values take 1927 us (2310 TOPS, matrix cores 57% busy); the same
+// with one row of X and W read over and over 1419, with values all zero 1900 (so not the clocks).
+// Hence steps of 128 bytes (64-byte steps ask L2 twice as often: 4096 x 8192 of 8192 268 us, 223),
+// three steps of W in LDS and two of X (two and two: 2022 us, since W misses L2 and X seldom does),
+// and one barrier a step, between its halves, behind which reads and DMA have the second half's
+// products to hide under (at the step's end: 4096 x 8192 of 8192 218 us, 212).  16 x 16 x 64
+// products sustain more than 32 x 32 x 32 (random operands, nothing else running: 3966 TOPS,
+// 3284).  Slower when tried: four waves of 128 x 128 (302 us against 220: a SIMD's one wave has no
+// other to wait behind), a persistent workgroup with the next tile's DMA ahead of the epilogue
+// (2060 us against 1989), results through LDS (4090 x 4100 of 96: 27.6 us against 22.8) or past the
+// caches (2017 against 1988), W or X read as streaming data (2049, 2076 against 1979).
 template <class T, bool DMA>
 __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 : 2))
     int8_tile_kernel(LinearArgs a) {
@@ -491,7 +506,8 @@ __global__ void __launch_bounds__(T::THREADS, T::WAVES / 4 * (T::WAVES > 4 ? 1 :
 }
 
 // Sums of a tile's parts and its results, for eight columns of a row a thread: two of the
-// registers that int8_tile_kernel kept, of one of its lanes.
+// registers that int8_tile_kernel kept, of one of its lanes.  Bound by the partial sums' bytes from
+// the caches: 1024 x 3584 in two parts 9.2 us (29 MB in, 7 MB out).
 template <class T>
 __global__ void __launch_bounds__(T::THREADS) int8_join_kernel(LinearArgs a) {
   constexpr int PAIRS = T::MT * T::NT / 2, EACH = 2 * PAIRS * T::THREADS;
@@ -549,8 +565,12 @@ __device__ __forceinline__ void put4(const LinearArgs& a, int64_t m, int64_t n, 
   }
 }
 
+// Bound by W's bytes from HBM: 32 rows, 37888 x 3584 in 26.7 us (138 MB, 5.2 TB/s, a large copy's
+// rate); one row, 4608 x 3584 in 5.4 us (16.5 MB, 3.1 TB/s: 144 workgroups of seven steps, over
+// before the memory is at its rate).
+//
 // Consecutive lanes fetch consecutive bytes of a row, which operands loaded straight from memory
-// (16 rows side by side) do not.  A workgroup has 16 NT columns and up to 16 MT rows; its waves take
+// (16 rows side by side: 60 us where this takes 31) do not.  A workgroup has 16 NT columns and up to 16 MT rows; its waves take
 // K's steps of 128 in turn, each through a ring of its own in LDS, RING steps deep, without barriers,
 // and add their sums in the end.  DMA: aligned rows, K from 128 on.  Otherwise the rows go through
 // registers, RING steps ahead, and one step of LDS.
@@ -696,7 +716,7 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
   }
 }
 
-// A row of fewer than 16 values: one result a thread.
+// A row of fewer than 16 values: one result a thread.  (Bound by the launch and the results.)
 __global__ void __launch_bounds__(256) int8_short_rows_kernel(LinearArgs a) {
   for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < a.M * a.N;
        e += (int64_t)gridDim.x * 256) {
@@ -711,7 +731,8 @@ __global__ void __launch_bounds__(256) int8_short_rows_kernel(LinearArgs a) {
 }
 
 // Rows of any stride and address to rows of `padded` bytes (a multiple of 128), zeros behind K >= 16:
-// W's N rows, then X's M.  16 bytes a thread; blocks cover chunks (x) of rows (y).
+// W's N rows, then X's M.  16 bytes a thread; blocks cover chunks (x) of rows (y).  Bound by its
+// bytes: 16384 + 3584 rows of 18943, 757 MB read and written, about 130 us (5.8 TB/s).
 __global__ void __launch_bounds__(256) int8_pad_kernel(LinearArgs a, int64_t padded, int8_t* to) {
   const int64_t k = 16 * ((int64_t)blockIdx.x * blockDim.x + threadIdx.x);
   if (k >= padded) return;
