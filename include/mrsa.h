@@ -1044,7 +1044,8 @@ int mrsa_swiglu_int8_fwd(const void* gate_up, int64_t row_stride, int64_t rows, 
 
 /*
  * out[m, n] = x_scales[m] weight_scales[n] sum_k x[m, k] weight[n, k] + bias[n],
- * the sum exact in int32, the rest in fp32, rounded once to `dtype`.
+ * the sum exact in int32, the rest in fp32, rounded once to `dtype`.  (The sum
+ * times x_scales[m] comes first: where that passes fp32, so does the result.)
  *   x: int8 [rows, dim], weight: int8 [out_dim, dim], rows at strides in bytes
  *   bias: optional [out_dim] of `dtype`; out: [rows, out_dim] of `dtype`, dense
  *   workspace: mrsa_int8_linear_workspace_bytes (16-byte aligned; may be NULL

@@ -123,9 +123,9 @@ __device__ __forceinline__ void dma(uint32_t to, const int8_t* base, uint32_t at
 }
 
 // Tiles in an order that gives each XCD (workgroups go round them) a contiguous range of bands of
-// 4 tile rows, walked column by column: its concurrent tiles share operands in its L2.  (Bands of 8:
-// 16384 x 3584 of 18944 values 984 us instead of 951, 4096 x 8192 of 8192 226 instead of 224; of
-// 16: 1007 and 234.)
+// 4 tile rows, walked column by column: its concurrent tiles share operands in its L2.  (Bands of
+// 8: 16384 x 3584 of 18944 values 952 us instead of 901, 16384 x 37888 of 3584 1883 instead of
+// 1912; of 16: 1007 instead of 951, and 4096 x 8192 of 8192 234 instead of 224.)
 __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int tiles = tiles_m * tiles_n, each = tiles / 8, more = tiles % 8;
   const int xcd = b % 8, i = b / 8;
@@ -570,10 +570,10 @@ __device__ __forceinline__ void put4(const LinearArgs& a, int64_t m, int64_t n, 
 // before the memory is at its rate).
 //
 // Consecutive lanes fetch consecutive bytes of a row, which operands loaded straight from memory
-// (16 rows side by side: 60 us where this takes 31) do not.  A workgroup has 16 NT columns and up to 16 MT rows; its waves take
-// K's steps of 128 in turn, each through a ring of its own in LDS, RING steps deep, without barriers,
-// and add their sums in the end.  DMA: aligned rows, K from 128 on.  Otherwise the rows go through
-// registers, RING steps ahead, and one step of LDS.
+// (16 rows side by side: 60 us where this takes 31) do not.  A workgroup has 16 NT columns and up
+// to 16 MT rows; its waves take K's steps of 128 in turn, each through a ring of its own in LDS,
+// RING steps deep, without barriers, and add their sums in the end.  DMA: aligned rows, K from 128
+// on.  Otherwise the rows go through registers, RING steps ahead, and one step of LDS.
 template <int MT, int NT, int WAVES, int RING, bool DMA>
 __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
   constexpr int P = 2 * NT + 2 * MT, SLOT = P * 1024, Q = MT * NT;
@@ -730,9 +730,9 @@ __global__ void __launch_bounds__(256) int8_short_rows_kernel(LinearArgs a) {
   }
 }
 
-// Rows of any stride and address to rows of `padded` bytes (a multiple of 128), zeros behind K >= 16:
-// W's N rows, then X's M.  16 bytes a thread; blocks cover chunks (x) of rows (y).  Bound by its
-// bytes: 16384 + 3584 rows of 18943, 757 MB read and written, about 130 us (5.8 TB/s).
+// Rows of any stride and address to rows of `padded` bytes (a multiple of 128), zeros behind
+// K >= 16: W's N rows, then X's M.  16 bytes a thread; blocks cover chunks (x) of rows (y).  Bound
+// by its bytes: 16384 + 3584 rows of 18943, 757 MB read and written, about 130 us (5.8 TB/s).
 __global__ void __launch_bounds__(256) int8_pad_kernel(LinearArgs a, int64_t padded, int8_t* to) {
   const int64_t k = 16 * ((int64_t)blockIdx.x * blockDim.x + threadIdx.x);
   if (k >= padded) return;

@@ -407,7 +407,8 @@ void back(const int8_t* values, int64_t stride, const float* scales, int64_t row
   while (tx < 256 && tx < units) tx *= 2;
   const unsigned ty = 256 / tx;
   // (four rows a thread keep the number of blocks low where there are many)
-  const int64_t by = std::min<int64_t>((rows + ty - 1) / ty, std::max<int64_t>(2048, rows / ty / 4));
+  const int64_t by =
+      std::min<int64_t>((rows + ty - 1) / ty, std::max<int64_t>(2048, rows / ty / 4));
   const dim3 grid((unsigned)((units + tx - 1) / tx), (unsigned)std::min<int64_t>(by, 65535));
   auto kern = K < 16 ? int8_back_kernel<T, true> : int8_back_kernel<T, false>;
   hipLaunchKernelGGL(kern, grid, dim3(tx, ty), 0, stream, values, stride, scales, rows, K,

@@ -69,8 +69,11 @@ struct Launch {
   c10::hip::HIPGuard guard;
   void* stream;
   explicit Launch(const Tensor& t)
-      : guard(t.device().index()),
-        stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+      : guard(device_of(t)), stream(c10::hip::getCurrentHIPStream(device_of(t)).stream()) {}
+  static c10::DeviceIndex device_of(const Tensor& t) {
+    TORCH_CHECK_VALUE(t.is_cuda(), "8-bit operators need CUDA tensors, got one on ", t.device());
+    return t.device().index();
+  }
 };
 
 std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {

@@ -331,8 +331,9 @@ def dream_forward(w: DreamWeights, input_ids: torch.Tensor, *, position_ids=None
                   return_hidden: bool = False) -> torch.Tensor:
     """Denoising forward of one sequence: input_ids int64 [1, L] in the
     landmark layout (landmark_layout) -> logits bf16 [L, vocab] (or the final
-    normed hidden [L, hidden]).  Layers of w.int8() run on 8-bit projections.  position_ids default to the layout's
-    (landmark_positions); tables = (cos, sin) rows per slot, if precomputed."""
+    normed hidden [L, hidden]).  Layers of w.int8() run on 8-bit projections.
+    position_ids default to the layout's (landmark_positions); tables = (cos, sin)
+    rows per slot, if precomputed."""
 
     shape = w.shape
     if input_ids.ndim != 2 or input_ids.shape[0] != 1:

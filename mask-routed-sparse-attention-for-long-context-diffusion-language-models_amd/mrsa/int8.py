@@ -133,8 +133,8 @@ def int8_linear(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor,
     x int8 [..., dim] with fp32 scales [...], weight int8 [out_dim, dim] with fp32 scales
     [out_dim] (``quantize_rows`` makes both), bias [out_dim] of the result's ``dtype`` (bf16,
     fp16 or fp32).  Any row strides; rows and matrices that are 16-byte aligned with dim a
-    multiple of 16 are fastest.  The sum is exact in int32 (dim up to 131071); scales, bias and
-    the rounding follow in fp32, so equal inputs give equal bits."""
+    multiple of 16 are fastest.  The sum is exact in int32 (dim up to 131071); scales (the row's
+    first), bias and the rounding follow in fp32, so equal inputs give equal bits."""
 
     dim = _check_values(x, x_scales, "x")[-1]
     shape = _check_values(weight, weight_scales, "weight")

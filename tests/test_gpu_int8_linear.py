@@ -237,13 +237,13 @@ def check_linear(out, x, sx, w, sw, bias=None):
     assert not bad.any(), (bad.nonzero()[:4].tolist(), int(bad.sum()))
 
 
-SHAPES = [(1, 1, 1), (2, 3, 15), (70, 90, 9), (1, 5, 16), (1, 4608, 3584), (3, 17, 16), (16, 33, 64),
-          (17, 64, 80), (2, 100, 1003), (32, 3584, 1003), (33, 129, 1000), (48, 20, 31),
-          (64, 48, 4096), (64, 1, 18944), (65, 1, 16), (65, 129, 17), (100, 300, 48),
-          (128, 128, 64), (129, 257, 1008), (200, 130, 18944), (257, 511, 255), (1000, 64, 3584),
-          (517, 1001, 1003), (1, 37888, 3584), (300, 4608, 3584), (513, 8192, 1040),
-          (4097, 4097, 16), (4097, 4097, 64), (4090, 4100, 96), (4097, 4096, 112),
-          (3900, 4300, 336), (2000, 9000, 1600)]
+SHAPES = [(1, 1, 1), (2, 3, 15), (70, 90, 9), (1, 5, 16), (1, 4608, 3584), (3, 17, 16),
+          (16, 33, 64), (17, 64, 80), (2, 100, 1003), (32, 3584, 1003), (33, 129, 1000),
+          (48, 20, 31), (64, 48, 4096), (64, 1, 18944), (65, 1, 16), (65, 129, 17),
+          (100, 300, 48), (128, 128, 64), (129, 257, 1008), (200, 130, 18944), (257, 511, 255),
+          (1000, 64, 3584), (517, 1001, 1003), (1, 37888, 3584), (300, 4608, 3584),
+          (513, 8192, 1040), (4097, 4097, 16), (4097, 4097, 64), (4090, 4100, 96),
+          (4097, 4096, 112), (3900, 4300, 336), (2000, 9000, 1600)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -388,6 +388,49 @@ def test_a_chain_captured_and_replayed(rows):
         assert all(torch.equal(a, b) for a, b in zip(outs[i % 2], want))
 
 
+@pytest.mark.parametrize("M,N,K", [(256, 512, 9000), (1301, 1403, 2033), (1003, 3584, 18943)])
+def test_products_with_a_workspace_captured_and_replayed(M, N, K):
+    """Partial sums, copies of rows, or both, in two graphs of one pool."""
+
+    assert _lib.call("mrsa_int8_linear_workspace_bytes", M, N, K) > 0
+    x, sx, w, sw, bias = _operands(M, N, K, 9)
+    x0, w0 = x.clone(), w.clone()
+    mrsa.int8_linear(x, sx, w, sw, bias, dtype=torch.float32)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    pool = torch.cuda.graph_pool_handle()
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            out = mrsa.int8_linear(x, sx, w, sw, bias, dtype=torch.float32)
+        graphs.append(g)
+        outs.append(out)
+    for i in range(4):
+        x.copy_(x0.roll(i, 0))
+        w.copy_(w0.roll(i, 1))
+        want = mrsa.int8_linear(x, sx, w, sw, bias, dtype=torch.float32)
+        if i == 0:
+            check_linear(want, x, sx, w, sw, bias)
+        torch.cuda.synchronize()
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i % 2], want)
+
+
+def test_products_with_a_workspace_on_other_streams():
+    ops = [_operands(*s, 3) for s in ((256, 512, 9000), (1301, 1403, 2033), (257, 511, 9001))]
+    want = [mrsa.int8_linear(*o, dtype=torch.float32) for o in ops]
+    torch.cuda.synchronize()
+    got = []
+    for o, st in zip(ops, [torch.cuda.Stream() for _ in ops]):
+        with torch.cuda.stream(st):
+            for _ in range(5):
+                out = mrsa.int8_linear(*o, dtype=torch.float32)
+            got.append(out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_calls_on_other_streams():
     ops = [_chain_operands(rows, seed=rows) for rows in (200, 131, 33)]
     want = [_chain(*o) for o in ops]
@@ -461,6 +504,9 @@ def test_direct_calls_refuse_what_would_pass_their_memory():
                  lambda: ops.dequantize_rows(v, s.double(), f32),
                  lambda: ops.dequantize_rows(v, s.cpu(), f32),
                  lambda: ops.dequantize_rows(x, s, f32),
+                 lambda: ops.dequantize_rows(v.cpu(), s, f32),
+                 lambda: ops.add_rms_norm_int8(x.cpu(), x, x[0], 1e-6),
+                 lambda: ops.int8_linear(v.cpu(), s, v, s, None, f32),
                  lambda: ops.add_rms_norm_int8(x, None, x[0, :31], 1e-6),
                  lambda: ops.add_rms_norm_int8(x, None, x[0].bfloat16(), 1e-6),
                  lambda: ops.add_rms_norm_int8(x, x[:3], x[0], 1e-6),
