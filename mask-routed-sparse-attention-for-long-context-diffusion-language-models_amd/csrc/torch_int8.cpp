@@ -1,9 +1,10 @@
 // The CUDA implementations of the 8-bit torch.ops.mrsa operators (schemas and fake kernels:
 // mrsa/ops.py): tensors to the C entry points of libmrsa.so.  At one token a call of these
-// operators is host time, and a public call costs 2 to 4 us less with this side of it in C++ than
-// through ctypes (norm of one row 12.1 -> 8.3 us, rows 8.6 -> 6.2, product 10.9 -> 7.0).
+// operators is host time, and a public call costs half as much with this side of it and the checks
+// in C++ as through ctypes (norm of one row 12.1 -> 6.3 us, rows 8.6 -> 5.4, product 10.9 -> 5.4).
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/core/grad_mode.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -18,8 +19,6 @@ namespace {
 using at::Tensor;
 
 int32_t dtype_code(at::ScalarType t) {
-  TORCH_CHECK_VALUE(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat,
-                    "8-bit operators work on bf16, fp16 or fp32, got ", t);
   return t == at::kBFloat16 ? MRSA_DTYPE_BF16 : t == at::kHalf ? MRSA_DTYPE_FP16 : MRSA_DTYPE_FP32;
 }
 
@@ -31,17 +30,35 @@ void check(int status, const char* op) {
   TORCH_CHECK(false, op, ": ", mrsa_status_string(status), " (status ", status, ")");
 }
 
-// What a compiler has traced, or calls the operators directly, reaches them past the checks of the
-// public functions: what a kernel would read or write out of range for is refused here too.
-void refuse_tangent(const Tensor& t, const char* op) {
-  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), op, " has no forward-mode derivative here");
+// The checks of mrsa/int8.py's _check functions, in their words.
+bool float_type(at::ScalarType t) {
+  return t == at::kBFloat16 || t == at::kHalf || t == at::kFloat;
 }
-
-void need(const Tensor& t, int64_t numel, at::ScalarType dtype, const Tensor& like,
-          const char* name) {
-  TORCH_CHECK_VALUE(t.numel() == numel && t.scalar_type() == dtype && t.device() == like.device(),
-                    name, " must hold ", numel, " elements of ", dtype, " on ", like.device(),
-                    ", got ", t.sizes(), " ", t.scalar_type(), " on ", t.device());
+void check_rows(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.dim() >= 1 && t.size(-1) >= 1, name,
+                    " must have rows of at least one value, got ", t.sizes());
+  TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK_VALUE(float_type(t.scalar_type()), name, " must be bf16, fp16 or fp32, got ",
+                    t.scalar_type());
+}
+void check_values(const Tensor& values, const Tensor& scales, const char* name) {
+  TORCH_CHECK_VALUE(values.scalar_type() == at::kChar && values.is_cuda() && values.dim() >= 1,
+                    name, " must be CUDA int8 rows, got ", values.sizes(), " ",
+                    values.scalar_type(), " on ", values.device());
+  const auto want = values.sizes().slice(0, values.dim() - 1);
+  TORCH_CHECK_VALUE(scales.sizes() == want && scales.scalar_type() == at::kFloat, name,
+                    " of shape ", values.sizes(), " need fp32 scales of shape ", want, ", got ",
+                    scales.sizes(), " ", scales.scalar_type());
+  TORCH_CHECK_VALUE(scales.device() == values.device(), name,
+                    " and their scales must be on one device");
+}
+void check_dtype(at::ScalarType dtype) {
+  TORCH_CHECK_VALUE(float_type(dtype), "dtype must be bf16, fp16 or fp32, got ", dtype);
+}
+void no_gradient(const char* op, const Tensor& t) {
+  TORCH_CHECK_VALUE(!t.requires_grad() || !at::GradMode::is_enabled(), op,
+                    " has no gradient: call it under torch.no_grad()");
+  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), op, " has no forward-mode derivative");
 }
 
 // t as rows [n, dim] whose last dim is dense (a copy only if no strides give that).
@@ -57,11 +74,13 @@ at::DimVector with_dim(const Tensor& t, int64_t dim) {
   sizes.back() = dim;
   return sizes;
 }
+// (as at::empty, without another pass through the dispatcher)
 Tensor new_rows(const Tensor& t, int64_t dim, at::ScalarType dtype) {
-  return at::empty(with_dim(t, dim), t.options().dtype(dtype));
+  return at::detail::empty_cuda(with_dim(t, dim), dtype, t.device(), std::nullopt);
 }
 Tensor new_scales(const Tensor& t) {
-  return at::empty(t.sizes().slice(0, t.dim() - 1), t.options().dtype(at::kFloat));
+  return at::detail::empty_cuda(t.sizes().slice(0, t.dim() - 1), at::kFloat, t.device(),
+                                std::nullopt);
 }
 
 // The device of the tensors, current during the call, and its current stream.
@@ -69,15 +88,13 @@ struct Launch {
   c10::hip::HIPGuard guard;
   void* stream;
   explicit Launch(const Tensor& t)
-      : guard(device_of(t)), stream(c10::hip::getCurrentHIPStream(device_of(t)).stream()) {}
-  static c10::DeviceIndex device_of(const Tensor& t) {
-    TORCH_CHECK_VALUE(t.is_cuda(), "8-bit operators need CUDA tensors, got one on ", t.device());
-    return t.device().index();
-  }
+      : guard(t.device().index()),
+        stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
 
 std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
-  refuse_tangent(x, "mrsa::quantize_rows");
+  check_rows(x, "x");
+  no_gradient("quantize_rows", x);
   const Launch at(x);
   const Tensor rows = rows_of(x);
   const int64_t dim = rows.size(1);
@@ -90,12 +107,14 @@ std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
 }
 
 Tensor dequantize_rows(const Tensor& values, const Tensor& scales, at::ScalarType dtype) {
-  refuse_tangent(scales, "mrsa::dequantize_rows");
+  check_values(values, scales, "values");
+  TORCH_CHECK_VALUE(values.size(-1) >= 1, "values must have rows of at least one value, got ",
+                    values.sizes());
+  check_dtype(dtype);
+  no_gradient("dequantize_rows", scales);
   const Launch at(values);
   const Tensor rows = rows_of(values), s = scales.contiguous();
   const int64_t dim = rows.size(1);
-  need(values, values.numel(), at::kChar, values, "values");
-  need(s, rows.size(0), at::kFloat, values, "scales");
   Tensor out = new_rows(values, dim, dtype);
   check(mrsa_dequantize_rows_fwd((const int8_t*)rows.data_ptr(), row_stride(rows),
                                  (const float*)s.data_ptr(), rows.size(0), dim, dtype_code(dtype),
@@ -107,21 +126,32 @@ Tensor dequantize_rows(const Tensor& values, const Tensor& scales, at::ScalarTyp
 std::tuple<Tensor, Tensor, Tensor> add_rms_norm_int8(const Tensor& x,
                                                      const std::optional<Tensor>& residual,
                                                      const Tensor& weight, double eps) {
-  refuse_tangent(x, "mrsa::add_rms_norm_int8");
-  refuse_tangent(weight, "mrsa::add_rms_norm_int8");
+  check_rows(x, "x");
+  if (residual) {
+    TORCH_CHECK_VALUE(residual->sizes() == x.sizes() &&
+                          residual->scalar_type() == x.scalar_type() &&
+                          residual->device() == x.device(),
+                      "residual must match x, got ", residual->sizes(), " ",
+                      residual->scalar_type(), " on ", residual->device(), " for ", x.sizes(), " ",
+                      x.scalar_type(), " on ", x.device());
+    no_gradient("add_rms_norm_int8", *residual);
+  }
+  TORCH_CHECK_VALUE(weight.dim() == 1 && weight.size(0) == x.size(-1) &&
+                        weight.scalar_type() == x.scalar_type() && weight.device() == x.device(),
+                    "weight must be [", x.size(-1), "] ", x.scalar_type(), " on ", x.device(),
+                    ", got ", weight.sizes(), " ", weight.scalar_type(), " on ", weight.device());
+  TORCH_CHECK_VALUE(eps >= 1e-24 && eps <= 1e24, "eps must be in [1e-24, 1e24], got ", eps);
+  no_gradient("add_rms_norm_int8", x);
+  no_gradient("add_rms_norm_int8", weight);
   const Launch at(x);
   const Tensor rows = rows_of(x), w = weight.contiguous();
   const int64_t dim = rows.size(1);
-  need(w, dim, x.scalar_type(), x, "weight");
   Tensor res, total;
   if (residual) {
-    refuse_tangent(*residual, "mrsa::add_rms_norm_int8");
-    need(*residual, x.numel(), x.scalar_type(), x, "residual");
-    TORCH_CHECK_VALUE(residual->sizes() == x.sizes(), "residual must have the shape of x");
     res = rows_of(*residual);
     total = new_rows(x, dim, x.scalar_type());
   } else {
-    total = at::empty({0}, x.options());
+    total = at::detail::empty_cuda({0}, x.scalar_type(), x.device(), std::nullopt);
   }
   Tensor values = new_rows(x, dim, at::kChar), scales = new_scales(x);
   check(mrsa_add_rms_norm_int8_fwd(
@@ -134,11 +164,13 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_int8(const Tensor& x,
 }
 
 std::tuple<Tensor, Tensor> swiglu_int8(const Tensor& gate_up) {
-  refuse_tangent(gate_up, "mrsa::swiglu_int8");
+  check_rows(gate_up, "gate_up");
+  TORCH_CHECK_VALUE(gate_up.size(-1) % 2 == 0, "gate_up must have an even last dim, got ",
+                    gate_up.sizes());
+  no_gradient("swiglu_int8", gate_up);
   const Launch at(gate_up);
   const Tensor rows = rows_of(gate_up);
   const int64_t dim = rows.size(1) / 2;
-  TORCH_CHECK_VALUE(rows.size(1) % 2 == 0, "gate_up must be [..., 2 * dim]");
   Tensor values = new_rows(gate_up, dim, at::kChar), scales = new_scales(gate_up);
   check(mrsa_swiglu_int8_fwd(rows.data_ptr(), row_stride(rows), rows.size(0), dim,
                              dtype_code(gate_up.scalar_type()), (int8_t*)values.data_ptr(),
@@ -150,23 +182,33 @@ std::tuple<Tensor, Tensor> swiglu_int8(const Tensor& gate_up) {
 Tensor int8_linear(const Tensor& x, const Tensor& x_scales, const Tensor& weight,
                    const Tensor& weight_scales, const std::optional<Tensor>& bias,
                    at::ScalarType dtype) {
-  refuse_tangent(x_scales, "mrsa::int8_linear");
-  refuse_tangent(weight_scales, "mrsa::int8_linear");
-  if (bias) refuse_tangent(*bias, "mrsa::int8_linear");
+  check_values(x, x_scales, "x");
+  check_values(weight, weight_scales, "weight");
+  const int64_t dim = x.size(-1);
+  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(1) == dim, "weight must be [out_dim, ", dim,
+                    "], got ", weight.sizes());
+  TORCH_CHECK_VALUE(weight.device() == x.device(), "x and weight must be on one device");
+  TORCH_CHECK_VALUE(dim >= 1 && dim <= 131071,
+                    "rows of 1 to 131071 values have a sum in 32 bits, got ", dim);
+  check_dtype(dtype);
+  if (bias) {
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == weight.size(0) &&
+                          bias->scalar_type() == dtype && bias->device() == x.device(),
+                      "bias must be [", weight.size(0), "] ", dtype, " on ", x.device(), ", got ",
+                      bias->sizes(), " ", bias->scalar_type(), " on ", bias->device());
+    no_gradient("int8_linear", *bias);
+  }
+  no_gradient("int8_linear", x_scales);
+  no_gradient("int8_linear", weight_scales);
   const Launch at(x);
   const Tensor rows = rows_of(x), w = rows_of(weight);
   const Tensor sx = x_scales.contiguous(), sw = weight_scales.contiguous();
   const Tensor b = bias ? bias->contiguous() : Tensor();
-  const int64_t n = rows.size(0), dim = rows.size(1), out_dim = w.size(0);
-  need(x, x.numel(), at::kChar, x, "x");
-  need(weight, out_dim * dim, at::kChar, x, "weight");
-  need(sx, n, at::kFloat, x, "x_scales");
-  need(sw, out_dim, at::kFloat, x, "weight_scales");
-  if (bias) need(b, out_dim, dtype, x, "bias");
+  const int64_t n = rows.size(0), out_dim = w.size(0);
   Tensor out = new_rows(x, out_dim, dtype);
   const int64_t bytes = mrsa_int8_linear_workspace_bytes(n, out_dim, dim);
   Tensor space;
-  if (bytes > 0) space = at::empty({bytes}, x.options().dtype(at::kByte));
+  if (bytes > 0) space = at::detail::empty_cuda({bytes}, at::kByte, x.device(), std::nullopt);
   check(mrsa_int8_linear_fwd((const int8_t*)rows.data_ptr(), row_stride(rows),
                              (const float*)sx.data_ptr(), (const int8_t*)w.data_ptr(),
                              row_stride(w), (const float*)sw.data_ptr(),

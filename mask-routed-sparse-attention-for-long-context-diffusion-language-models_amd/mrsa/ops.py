@@ -24,6 +24,8 @@ from torch import Tensor
 from ._lib import LIB_PATH, MrsaLibraryError
 
 from .fusion import _fuse_bwd_impl, _fuse_impl
+from .int8 import (_check_dequantize, _check_linear, _check_norm, _check_quantize,
+                   _check_swiglu)
 from .kernel_utils import _drop_mask_impl, _drop_mask_rows_impl
 from .local_attention import _local_attention_impl
 from .paged_cache import _copy_pages_impl, _paged_append_impl, _paged_attention_impl
@@ -418,14 +420,16 @@ def _(k_pages, v_pages, src, dst):
 
 
 # -- linear layers in 8 bits ------------------------------------------------
-# Their CUDA implementations are C++ (csrc/torch_int8.cpp): a call of one token is host time.
+# Their CUDA implementations are C++ (csrc/torch_int8.cpp): a call of one token is host time.  They
+# check their arguments, as the _check functions do for fake tensors; on the CPU those refuse all.
 NATIVE_PATH = os.path.join(os.path.dirname(LIB_PATH), "libmrsa_torch.so")
 _native = []
 
 
-def _define_native(schema):
+def _define_native(schema, check):
     name = schema.split("(")[0]
     _lib.define(schema)
+    _lib.impl(name, check, "CPU")
     _native.append(name)
     return torch.library.register_fake(f"mrsa::{name}", lib=_lib)
 
@@ -446,31 +450,37 @@ def _rows_fake(x, dim):
                                                                             dtype=torch.float32)
 
 
-@_define_native("quantize_rows(Tensor x) -> (Tensor, Tensor)")
+@_define_native("quantize_rows(Tensor x) -> (Tensor, Tensor)", _check_quantize)
 def _(x):
+    _check_quantize(x)
     return _rows_fake(x, x.shape[-1])
 
 
-@_define_native("dequantize_rows(Tensor values, Tensor scales, ScalarType dtype) -> Tensor")
+@_define_native("dequantize_rows(Tensor values, Tensor scales, ScalarType dtype) -> Tensor",
+                _check_dequantize)
 def _(values, scales, dtype):
+    _check_dequantize(values, scales, dtype)
     return values.new_empty(values.shape, dtype=dtype)
 
 
 @_define_native("add_rms_norm_int8(Tensor x, Tensor? residual, Tensor weight, float eps) "
-                "-> (Tensor, Tensor, Tensor)")
+                "-> (Tensor, Tensor, Tensor)", _check_norm)
 def _(x, residual, weight, eps):
+    _check_norm(x, residual, weight, eps)
     total = x.new_empty(0 if residual is None else x.shape)
     return (total, *_rows_fake(x, x.shape[-1]))
 
 
-@_define_native("swiglu_int8(Tensor gate_up) -> (Tensor, Tensor)")
+@_define_native("swiglu_int8(Tensor gate_up) -> (Tensor, Tensor)", _check_swiglu)
 def _(gate_up):
+    _check_swiglu(gate_up)
     return _rows_fake(gate_up, gate_up.shape[-1] // 2)
 
 
 @_define_native("int8_linear(Tensor x, Tensor x_scales, Tensor weight, Tensor weight_scales, "
-                "Tensor? bias, ScalarType dtype) -> Tensor")
+                "Tensor? bias, ScalarType dtype) -> Tensor", _check_linear)
 def _(x, x_scales, weight, weight_scales, bias, dtype):
+    _check_linear(x, x_scales, weight, weight_scales, bias, dtype)
     return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=dtype)
 
 

@@ -491,8 +491,62 @@ def test_direct_calls_map_errors_as_the_others():
         ops.quantize_rows(x.double())
     with pytest.raises(ValueError):
         ops.dequantize_rows(v, s, torch.float64)
-    with pytest.raises(NotImplementedError):
+    with pytest.raises(ValueError, match="CUDA"):
         ops.quantize_rows(x.cpu())
+
+
+def test_calls_that_ask_for_a_derivative():
+    """Refused on the GPU as for fake tensors; without gradients the same tensors pass."""
+
+    x = torch.ones(4, 32, device=DEV).requires_grad_()
+    v, s = mrsa.quantize_rows(x.detach())
+    s.requires_grad_()
+    for call in (lambda: mrsa.quantize_rows(x), lambda: mrsa.swiglu_int8(x),
+                 lambda: mrsa.add_rms_norm_int8(x, None, x[0].detach(), 1e-6),
+                 lambda: mrsa.add_rms_norm_int8(x.detach(), x, x[0].detach(), 1e-6),
+                 lambda: mrsa.add_rms_norm_int8(x.detach(), None, x[0], 1e-6),
+                 lambda: mrsa.dequantize_rows(v, s),
+                 lambda: mrsa.int8_linear(v, s, v, s.detach()),
+                 lambda: mrsa.int8_linear(v, s.detach(), v, s),
+                 lambda: mrsa.int8_linear(v, s.detach(), v, s.detach(), s, dtype=torch.float32)):
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with torch.no_grad(), pytest.raises(Exception, match="forward-mode"):
+        torch.func.jvp(lambda t: mrsa.quantize_rows(t)[1], (x.detach(),), (torch.ones_like(x),))
+
+
+def test_refusals_of_real_tensors():
+    """The words of the fake tensors' refusals (tests/test_int8_linear.py)."""
+
+    x = torch.zeros(4, 32, device=DEV)
+    v, s = mrsa.quantize_rows(x)
+    for call, words in (
+            (lambda: mrsa.quantize_rows(x.cpu()), "CUDA"),
+            (lambda: mrsa.quantize_rows(x.double()), "bf16, fp16 or fp32"),
+            (lambda: mrsa.quantize_rows(x[0, 0]), "at least one"),
+            (lambda: mrsa.quantize_rows(x[:, :0]), "at least one"),
+            (lambda: mrsa.swiglu_int8(x[:, :7]), "even"),
+            (lambda: mrsa.add_rms_norm_int8(x, x[:3], x[0], 1e-6), "residual"),
+            (lambda: mrsa.add_rms_norm_int8(x, x.cpu(), x[0], 1e-6), "residual"),
+            (lambda: mrsa.add_rms_norm_int8(x, None, x[:1], 1e-6), "weight"),
+            (lambda: mrsa.add_rms_norm_int8(x, None, x[0].half(), 1e-6), "weight"),
+            (lambda: mrsa.add_rms_norm_int8(x, None, x[0], float("nan")), "eps"),
+            (lambda: mrsa.dequantize_rows(x, s), "int8"),
+            (lambda: mrsa.dequantize_rows(v, s[:, None]), "scales"),
+            (lambda: mrsa.dequantize_rows(v, s.cpu()), "one device"),
+            (lambda: mrsa.dequantize_rows(v, s, torch.int32), "dtype"),
+            (lambda: mrsa.dequantize_rows(v[:, :0], s), "at least one"),
+            (lambda: mrsa.int8_linear(v, s, v[:, :31], s), "weight"),
+            (lambda: mrsa.int8_linear(v, s, v[None], s[None]), "weight"),
+            (lambda: mrsa.int8_linear(v, s, x, s), "int8"),
+            (lambda: mrsa.int8_linear(v, s[:3], v, s), "scales"),
+            (lambda: mrsa.int8_linear(v, s, v, s, s), "bias"),
+            (lambda: mrsa.int8_linear(v, s, v, s, dtype=torch.int8), "dtype"),
+            (lambda: mrsa.int8_linear(v[:, :0], s, v[:, :0], s), "131071")):
+        with pytest.raises(ValueError, match=words):
+            call()
 
 
 def test_direct_calls_refuse_what_would_pass_their_memory():
