@@ -228,3 +228,11 @@ TORCH_LIBRARY_IMPL(mrsa, CUDA, m) {
   m.impl("swiglu_int8", &swiglu_int8);
   m.impl("int8_linear", &int8_linear);
 }
+
+// Tensors that ask for a derivative are refused by the operators themselves, so autograd's own
+// fallback kernel is left out of every call.
+TORCH_LIBRARY_IMPL(mrsa, Autograd, m) {
+  for (const char* op : {"quantize_rows", "dequantize_rows", "add_rms_norm_int8", "swiglu_int8",
+                         "int8_linear"})
+    m.impl(op, torch::CppFunction::makeFallthrough());
+}
