@@ -30,7 +30,7 @@ void check(int status, const char* op) {
   TORCH_CHECK(false, op, ": ", mrsa_status_string(status), " (status ", status, ")");
 }
 
-// The checks of mrsa/int8.py's _check functions, in their words.
+// The checks of mrsa/int8_checks.py, in their words.
 bool float_type(at::ScalarType t) {
   return t == at::kBFloat16 || t == at::kHalf || t == at::kFloat;
 }

@@ -25,6 +25,7 @@ hand-written HIP kernels in ../csrc (C ABI: include/mrsa.h).  Module map:
                         copy_cache_pages: several sequences' K/V in shared pages
     int8.py             quantize_rows, add_rms_norm_int8, swiglu_int8, int8_linear,
                         dequantize_rows: linear layers in 8-bit integers
+    int8_checks.py      what those refuse, for fake and CPU tensors
     ops.py              torch.ops.mrsa.* custom operators (schemas, CUDA and fake kernels)
 """
 

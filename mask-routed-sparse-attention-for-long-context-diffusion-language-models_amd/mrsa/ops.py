@@ -24,8 +24,8 @@ from torch import Tensor
 from ._lib import LIB_PATH, MrsaLibraryError
 
 from .fusion import _fuse_bwd_impl, _fuse_impl
-from .int8 import (_check_dequantize, _check_linear, _check_norm, _check_quantize,
-                   _check_swiglu)
+from .int8_checks import (_check_dequantize, _check_linear, _check_norm, _check_quantize,
+                          _check_swiglu)
 from .kernel_utils import _drop_mask_impl, _drop_mask_rows_impl
 from .local_attention import _local_attention_impl
 from .paged_cache import _copy_pages_impl, _paged_append_impl, _paged_attention_impl
