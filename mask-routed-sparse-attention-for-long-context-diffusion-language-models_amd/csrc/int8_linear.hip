@@ -573,7 +573,8 @@ __device__ __forceinline__ void put4(const LinearArgs& a, int64_t m, int64_t n, 
 // (16 rows side by side: 60 us where this takes 31) do not.  A workgroup has 16 NT columns and up
 // to 16 MT rows; its waves take K's steps of 128 in turn, each through a ring of its own in LDS,
 // RING steps deep, without barriers, and add their sums in the end.  DMA: aligned rows, K from 128
-// on.  Otherwise the rows go through registers, RING steps ahead, and one step of LDS.
+// on.  Otherwise the rows go through registers, RING steps ahead, and one step of LDS.  More rows
+// than 16 MT: blockIdx.y.
 template <int MT, int NT, int WAVES, int RING, bool DMA>
 __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
   constexpr int P = 2 * NT + 2 * MT, SLOT = P * 1024, Q = MT * NT;
@@ -582,7 +583,7 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
   static_assert(Q * 1024 <= SLOTS * SLOT && RING >= 2 && RING <= 4);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
   const int r = lane & 15, grp = lane >> 4;
   const int K = (int)a.K, steps = (K + kStep - 1) / kStep, tail = K - (steps - 1) * kStep;
   const int mine = steps > wave ? (steps - wave - 1) / WAVES + 1 : 0;
@@ -615,10 +616,11 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
   // piece i: rows 8 i .. of W, then of X; rows past the end repeat the last one
   auto row_of = [&](int i) {
     const int64_t r = (i < 2 * NT ? i : i - 2 * NT) * 8 + (lane >> 3);
-    return min(r, i < 2 * NT ? a.N - 1 - n0 : a.M - 1);
+    return min(r, (i < 2 * NT ? a.N - n0 : a.M - m0) - 1);
   };
   auto chunk_of = [&](int i) { return (lane & 7) ^ swizzle(8 * (i & 1) + (lane >> 3)); };
   const int8_t* const w_base = a.w + n0 * a.w_stride;
+  const int8_t* const x_base = a.x + m0 * a.x_stride;
   if constexpr (DMA) {
     uint32_t off[P];
 #pragma unroll
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
       const int k = min((wave + i * WAVES) * kStep, K - kStep);
 #pragma unroll
       for (int j = 0; j < P; ++j)
-        dma(ring + slot + 1024 * j, (j < 2 * NT ? w_base : a.x) + k, off[j]);
+        dma(ring + slot + 1024 * j, (j < 2 * NT ? w_base : x_base) + k, off[j]);
     };
 #pragma unroll
     for (int i = 0; i < RING; ++i)
@@ -662,7 +664,7 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
     const int8_t* row[P];
 #pragma unroll
     for (int i = 0; i < P; ++i)
-      row[i] = i < 2 * NT ? w_base + row_of(i) * a.w_stride : a.x + row_of(i) * a.x_stride;
+      row[i] = i < 2 * NT ? w_base + row_of(i) * a.w_stride : x_base + row_of(i) * a.x_stride;
     u32x4_t held[RING][P];
     auto load = [&](int i, u32x4_t (&h)[P]) __attribute__((always_inline)) {
       if (i >= mine) return;
@@ -708,7 +710,7 @@ __global__ void __launch_bounds__(64 * WAVES) int8_stream_kernel(LinearArgs a) {
     for (int n = 0; n < NT; ++n) sums[(wave * Q + m * NT + n) * 64 + lane] = acc[m][n];
   __syncthreads();
   for (int q = wave; q < Q; q += WAVES) {
-    const int64_t m = 16 * (q / NT) + r, n = n0 + 16 * (q % NT) + 4 * grp;
+    const int64_t m = m0 + 16 * (q / NT) + r, n = n0 + 16 * (q % NT) + 4 * grp;
     i32x4_t s = sums[q * 64 + lane];
 #pragma unroll
     for (int v = 1; v < WAVES; ++v) s += sums[(v * Q + q) * 64 + lane];
@@ -780,12 +782,12 @@ typedef Tile<256, 256, 2, 4, 3, 2> Tile256;
 struct Shape {
   int tm, tn, room;        // workgroups that the CUs hold
   float one, two, fixed;   // us: a step of a workgroup alone on its CU, of two, the rest
-  bool any_rows;           // also for rows at any address
+  float any_rows;          // a step's time of rows at any address over that of aligned ones (0: -)
 };
 constexpr Shape kShapes[] = {
-    {64, 64, 512, 0.335f, 0.45f, 5.f, true},     {64, 128, 512, 0.40f, 0.70f, 5.f, false},
-    {128, 128, 256, 0.52f, 0.52f, 5.f, false},   {128, 128, 512, 0.83f, 1.0f, 5.f, true},
-    {128, 256, 256, 0.82f, 0.82f, 6.f, false},   {256, 256, 256, 1.42f, 1.42f, 8.f, true},
+    {64, 64, 512, 0.335f, 0.45f, 5.f, 1.9f},  {64, 128, 512, 0.40f, 0.70f, 5.f, 0.f},
+    {128, 128, 256, 0.52f, 0.52f, 5.f, 0.f},  {128, 128, 512, 0.83f, 1.0f, 5.f, 1.6f},
+    {128, 256, 256, 0.82f, 0.82f, 6.f, 0.f},  {256, 256, 256, 1.42f, 1.42f, 8.f, 1.6f},
 };
 struct Plan {
   enum { kShort, kFew, kTiles } kind;
@@ -800,7 +802,7 @@ void best_tiles(int64_t M, int64_t N, int64_t K, bool aligned, float more, float
   const int64_t steps = (K + kStep - 1) / kStep;
   for (int i = 0; i < (int)(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
     const Shape& s = kShapes[i];
-    if (!aligned && !s.any_rows) continue;
+    if (!aligned && s.any_rows == 0.f) continue;
     const int64_t tm = (M + s.tm - 1) / s.tm, tn = (N + s.tn - 1) / s.tn;
     for (const int parts : {1, 2, 3, 4, 6, 8}) {
       if (parts > steps) break;
@@ -808,8 +810,7 @@ void best_tiles(int64_t M, int64_t N, int64_t K, bool aligned, float more, float
       if (parts > 1 && items > s.room) break;  // (and so the workspace stays small)
       const float rounds = items <= 4 * s.room ? (float)((items + s.room - 1) / s.room)
                                                : (float)items / (float)s.room + 0.5f;
-      // (through registers a step takes 1.3 to 1.9 times as long)
-      const float step = (items <= 256 ? s.one : s.two) * (aligned ? 1.f : 1.6f);
+      const float step = (items <= 256 ? s.one : s.two) * (aligned ? 1.f : s.any_rows);
       const int64_t bytes = parts > 1 ? items * s.tm * s.tn * 4 : 0;
       const float time = more +
                          rounds * (s.fixed + step * (float)((steps + parts - 1) / parts)) +
@@ -822,24 +823,57 @@ void best_tiles(int64_t M, int64_t N, int64_t K, bool aligned, float more, float
   }
 }
 
+// Rows by 64, through the kernel of few rows: as long as its workgroups are one round or two, since
+// a wave takes a quarter of K's steps and no barriers (us, its 16 and 32 columns, and tiles: 512
+// rows, 1008 x 1008 4.7, 5.5 and 6.8; 64 x 3584 5.5, 6.8 and 9.5; 128 rows, 3584 x 3584 9.4, 7.6
+// and 13.7, of 3583 values 16, 12 and 17; 192 rows 12.5, 13.1 and 13.8; 256 rows 15, 13 and 14; 128
+// rows, 4608 x 3584 12.6, 13.2 and 13.7, 8192 x 4096 21, 18 and 16).  The estimate: rounds; or the
+// bytes that all workgroups fetch, W's again for each 64 rows and the rows' for each 16 or 32
+// columns; or those of them that come from beyond the L2s, each of which sees all workgroups.
+void best_few(int64_t M, int64_t N, int64_t K, bool aligned, float& best, Plan& p) {
+  const int64_t tm = (M + 63) / 64, steps = (K + 4 * kStep - 1) / (4 * kStep);
+  if (tm > 65535) return;
+  for (const int cols : {16, 32}) {
+    const int64_t tn = (N + cols - 1) / cols, items = tm * tn;
+    float rounds, step, rate;   // rate: bytes a us
+    if (cols == 16) {
+      rounds = std::max(1.f, (float)items / 512.f);
+      step = aligned ? (items <= 256 ? 0.57f : 0.97f) : (items <= 256 ? 1.0f : 2.05f);
+      rate = aligned ? 16.5e6f : 9.4e6f;
+    } else {
+      rounds = (float)((items + 255) / 256);
+      step = aligned ? 0.72f : 1.3f;
+      rate = aligned ? 12e6f : 7.5e6f;
+    }
+    const float bytes = (float)tm * (float)N * (float)K * (1.f + 64.f / (float)cols);
+    const float far = (float)K * ((float)N * (float)std::min<int64_t>(tm, 8) +
+                                  (float)M * (float)std::min<int64_t>(tn, 8));
+    const float time = 1.2f + std::max(rounds * (2.f + step * (float)steps),
+                                       2.f + std::max(bytes / rate, far / 5.5e6f));
+    if (time < best) {
+      best = time;
+      p = {Plan::kFew, 0, aligned, tm, tn, 1, 0, cols, 0};
+    }
+  }
+}
+
 Plan plan_of(int64_t M, int64_t N, int64_t K, bool aligned) {
   Plan p = {Plan::kTiles, 0, aligned, 1, 1, 1, 0, 0, 0};
   if (K < 16) {
     p.kind = Plan::kShort;
     return p;
   }
-  float best = 1e30f;
-  if (M <= 64) {
-    // Up to 64 rows the weights' bytes count, and the rows' that every workgroup fetches again.
-    // Columns of a workgroup: 32 while that leaves half the CUs a workgroup, else 16 (us, 16 and
-    // 32: 32 rows of 3584 values, 3584 columns 5.0 and 5.3, 4608 6.8 and 5.6, 37888 39 and 31; 16
-    // rows of 4096, 4096 columns 6.9 and 5.9; 64 rows 8.1 and 8.3).
+  if (M <= 32) {
+    // The weights' bytes count.  Columns of a workgroup: 32 while that leaves half the CUs a
+    // workgroup, else 16 (us, 16 and 32: 32 rows of 3584 values, 3584 columns 5.0 and 5.3, 4608 6.8
+    // and 5.6, 37888 39 and 31; 16 rows of 4096, 4096 columns 6.9 and 5.9).
     p.kind = Plan::kFew;
     p.cols = N >= 32 * 128 ? 32 : 16;
     p.tiles_n = (N + p.cols - 1) / p.cols;
-    if (M <= 32) return p;
-    best = 3.f + (float)N * (float)K * (1.f + 64.f / (float)p.cols) * 1e-7f;
+    return p;
   }
+  float best = 1e30f;
+  best_few(M, N, K, aligned, best, p);
   best_tiles(M, N, K, aligned, 0.f, best, p);
   if (K % 16 != 0) {
     // Rows that no stride aligns: padded copies of them first where the tiles gain more than the
@@ -887,7 +921,7 @@ void launch_few(const LinearArgs& a, const Plan& p, hipStream_t stream) {
     kern = mt == 1   ? int8_stream_kernel<1, 2, 4, 2, DMA>
            : mt == 2 ? int8_stream_kernel<2, 2, 4, 2, DMA>
                      : int8_stream_kernel<4, 2, 4, 2, DMA>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)p.tiles_n), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)p.tiles_n, (unsigned)p.tiles_m), dim3(256), 0, stream, a);
 }
 
 }  // namespace
@@ -922,7 +956,7 @@ extern "C" int mrsa_int8_linear_fwd(const int8_t* x, int64_t x_row_stride, const
   const bool aligned = dim % 16 == 0 && dim >= kStep && aligned_rows(x, x_row_stride, rows) &&
                        aligned_rows(weight, weight_row_stride, out_dim);
   const Plan p = plan_of(rows, out_dim, dim, aligned);
-  const int64_t groups = p.kind == Plan::kFew ? p.tiles_n : p.tiles_m * p.tiles_n * p.parts;
+  const int64_t groups = p.tiles_m * p.tiles_n * p.parts;
   if (groups >= (int64_t)1 << 23) return MRSA_ERR_UNSUPPORTED;
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16 != 0))
     return MRSA_ERR_INVALID_ARGUMENT;
