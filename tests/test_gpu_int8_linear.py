@@ -301,6 +301,19 @@ def test_int8_linear_of_any_strides(M):
     assert torch.equal(same, want[:1].expand(M, N))
 
 
+@pytest.mark.parametrize("M,N,K", [(65, 3584, 3583), (128, 3584, 3584), (577, 33, 130),
+                                   (130, 30, 17), (4100, 20, 100), (193, 40, 2048),
+                                   (4194240, 3, 16), (4194305, 3, 16)])
+def test_many_rows_of_few_results(M, N, K):
+    """Row groups of 64 (at most 65535 of them): the last one's rows, and those behind it."""
+
+    x, sx, w, sw, bias = _operands(M, N, K, 11, full=True)
+    out = mrsa.int8_linear(x, sx, w, sw, bias, dtype=torch.float32)
+    check_linear(out, x, sx, w, sw, bias)
+    part = mrsa.int8_linear(x[-70:], sx[-70:], w, sw, bias, dtype=torch.float32)
+    assert torch.equal(out[-70:], part)
+
+
 @pytest.mark.parametrize("more", range(1, 16))
 def test_rows_that_are_copied_to_aligned_ones(more):
     """Lengths that no stride aligns, at sizes where the copies pay: their last bytes, and what
