@@ -270,9 +270,9 @@ def test_the_longest_sum_of_the_largest_products(M, N):
     assert (out.double() == exact).all()
 
 
-@pytest.mark.parametrize("M", (1, 30, 64, 150, 4200))
-def test_int8_linear_of_any_strides(M):
-    N, K = (300, 208) if M < 4000 else (4100, 80)
+@pytest.mark.parametrize("M,N,K", [(1, 300, 208), (30, 300, 208), (64, 300, 208), (150, 300, 208),
+                                   (1500, 1404, 400), (4200, 4100, 80)])
+def test_int8_linear_of_any_strides(M, N, K):
     x, sx, w, sw, bias = _operands(M, N, K, 5, full=True)
     want = mrsa.int8_linear(x, sx, w, sw, bias, dtype=torch.float32)
     check_linear(want, x, sx, w, sw, bias)
@@ -333,9 +333,10 @@ def test_rows_that_are_copied_to_aligned_ones(more):
     assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("M", (3, 40, 200))
-def test_rows_without_a_scale_stay_alone(M):
-    x, sx, w, sw, bias = _operands(M, 70, 96, 8)
+@pytest.mark.parametrize("M,N,K", [(3, 70, 96), (40, 70, 96), (200, 70, 96), (1500, 1404, 400),
+                                   (256, 512, 9000), (1301, 1403, 2033)])
+def test_rows_without_a_scale_stay_alone(M, N, K):
+    x, sx, w, sw, bias = _operands(M, N, K, 8)
     sx[1], sx[2] = float("nan"), 0.0
     out = mrsa.int8_linear(x, sx, w, sw, bias, dtype=torch.float32)
     assert out[1].isnan().all() and torch.equal(out[2], bias)
