@@ -15,6 +15,8 @@
 // gives sum t^2 and max |t w|.
 #include "mrsa_device.h"
 
+#include <type_traits>
+
 using namespace mrsa;
 
 namespace {
@@ -83,12 +85,20 @@ __device__ __forceinline__ void store8(typename T::elem* p, int64_t K, const flo
   }
 }
 
-// g / (1 + exp(-g)): the quotient by the hardware's reciprocal and one correction, which rounds it
-// as a division does (the divisor, from 1 to 2^127, needs no scaling).
+// g / (1 + exp(-g)) for g from kFarGate on: the quotient by the hardware's reciprocal and one
+// correction, which rounds it as a division does (the divisor, from 1 to 2^126, needs no scaling).
+constexpr float kFarGate = -87.f;   // exp(87) is 0.71 2^126
 __device__ __forceinline__ float silu(float g) {
-  const float d = 1.f + fminf(expf(-g), 0x1p126f), r = rcp_hw(d);
+  const float d = 1.f + expf(-g), r = rcp_hw(d);
   const float q = g * r;
   return fmaf(fmaf(-q, d, g), r, q);
+}
+// silu(g) up for g below kFarGate, where 1 + exp(-g) is exp(-g) but nears the end of fp32, whose
+// reciprocal or quotient would lose it: the exponential in two halves around the other factor, so
+// that nothing is lost before the product itself is (-inf: NaN, as -inf / inf).
+__device__ __forceinline__ float far_gate(float g, float up) {
+  const float h = expf(0.5f * g);
+  return g * h * up * h;
 }
 
 // f + 1.5 2^23, whose low byte is the whole number nearest to f, ties to even.  (The product
@@ -100,6 +110,7 @@ __device__ __forceinline__ float whole(float f) {
 }
 
 constexpr uint32_t kInfBits = 0x7f800000u;
+constexpr uint32_t kFar = 0xffffffffu;   // above all magnitudes: the row has gates below kFarGate
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
 __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
@@ -138,6 +149,12 @@ __device__ __forceinline__ void reduce(float& sum, uint32_t& top, float* red_sum
   }
 }
 
+// The same number, but one that the compiler keeps no addresses for ahead of its use.
+__device__ __forceinline__ int apart(int i) {
+  asm volatile("" : "+v"(i));
+  return i;
+}
+
 // TPR threads a row (a wave, so four rows a block; or the whole block), each with V units of
 // eight elements; V = 0: rows of any length, read twice.  The last unit of a row ends with it and
 // so may share elements with the one before: both write the same there, and the sum of squares
@@ -151,7 +168,9 @@ __device__ __forceinline__ void reduce(float& sum, uint32_t& top, float* red_sum
 // the vector unit as busy as the memory.  One row of 3584 takes 2.9 us: a launch and three
 // dependent steps (loads, reduction, stores).
 template <class T, int OP, int TPR, int V, bool SMALL>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) int8_rows_kernel(RowArgs a) {
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR,
+                                  V == 5 && OP == kSwiglu && sizeof(typename T::elem) == 2 ? 6 : 1)
+    int8_rows_kernel(RowArgs a) {
   typedef typename T::elem E;
   constexpr int THREADS = TPR < 256 ? 256 : TPR;
   constexpr int ROWS = THREADS / TPR;
@@ -174,6 +193,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) int8_rows_kernel(RowArg
     float down = 1.f;     //       a power of two that keeps it in range
     uint32_t top_t = 0;   //       largest |t|
     uint32_t top = 0;     // largest magnitude of what `unit` gives
+    float lowest = 0.f;   // swiglu: the least gate
     // What the unit at element s is made from: x or the gate, the residual or the other factor,
     // the weight.
     struct Unit {
@@ -190,7 +210,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) int8_rows_kernel(RowArg
       return n;
     };
     // Its values before the row's factor: x, t down w, or the product.
-    auto unit = [&](const Unit& n, int64_t s, int repeated, bool first, float (&y)[8]) {
+    auto unit = [&](const Unit& n, int64_t s, int repeated, bool first, auto far, float (&y)[8]) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = T::widen(n.x.e[j]);
       if constexpr (NORM) {
@@ -218,36 +238,53 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) int8_rows_kernel(RowArg
       }
       if constexpr (OP == kSwiglu) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          y[j] = silu(y[j]) * T::widen(n.other.e[j]);
+        for (int j = 0; j < 8; ++j) {
+          const float g = y[j], up = T::widen(n.other.e[j]);
+          if constexpr (far) {
+            y[j] = g < kFarGate ? far_gate(g, up) : silu(g) * up;
+          } else {
+            lowest = fminf(lowest, g);
+            y[j] = silu(g) * up;
+          }
+        }
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = max(top, magnitude(y[j]));
     };
     float y[HELD][8];
-    auto all_units = [&](bool first) {
+    auto all_units = [&](bool first, auto far) {
       square = 0.f;
       top = top_t = 0;
-      if constexpr (V > 0) {
+      if constexpr (V > 0 && !far) {
         // (threads past the row take its last unit once more: no load depends on a branch)
-        Unit n[V];
+        Unit n[HELD];
 #pragma unroll
         for (int i = 0; i < V; ++i) n[i] = load(start_of(min<int64_t>(sub + i * TPR, units - 1)));
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const int64_t u = sub + i * TPR, s = start_of(min(u, units - 1));
-          unit(n[i], s, u < units ? (int)(8 * u - s) : 8, first, y[i]);
+          unit(n[i], s, u < units ? (int)(8 * u - s) : 8, first, far, y[i]);
         }
       } else {
-        for (int64_t u = sub; u < units; u += TPR) {
+        for (int64_t u = apart(sub); u < units; u += TPR) {
           const int64_t s = start_of(u);
-          unit(load(s), s, (int)(8 * u - s), first, y[0]);
+          unit(load(s), s, (int)(8 * u - s), first, far, y[0]);
         }
       }
+      if constexpr (OP == kSwiglu && !far) top = lowest < kFarGate ? kFar : top;
       reduce<TPR, NORM>(square, top, red_sum, red_top);
     };
-    all_units(true);
+    all_units(true, std::false_type{});
     float r = 1.f;
+    bool far = false;
+    if constexpr (OP == kSwiglu) {
+      // Again, with the form for gates that far down, and unit by unit, so that the other rows
+      // keep the registers that they had (80 for 18944 values of 16 bits: three blocks a CU, 290
+      // us instead of 314).  A test of each unit in its place slows them more (3584 values: 64 us
+      // instead of 59); all rows of 18944 taken again are 620.
+      far = top == kFar;
+      if (far) all_units(false, std::true_type{});
+    }
     if constexpr (NORM) {
       // t^2 or t w past fp32 (|t| above 1.8e19): again with t times a power of two that takes
       // the largest |t| to between 1 and 2.  A row that holds an infinity or a NaN comes here,
@@ -258,7 +295,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) int8_rows_kernel(RowArg
         reduce<TPR, false>(none, top_t, red_sum, red_top);
         const int e = past ? (int)(top_t >> 23) - 127 : 0;
         down = __uint_as_float((uint32_t)(127 - max(0, min(e, 126))) << 23);
-        all_units(false);
+        all_units(false, std::false_type{});
       }
       r = rsqrtf(square / (float)a.K + a.eps * down * down);
     }
@@ -291,18 +328,23 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) int8_rows_kernel(RowArg
       }
     };
     if (there) {
-      if constexpr (V > 0) {
+      auto read_again = [&](auto far) {
+        for (int64_t u = apart(sub); u < units; u += TPR) {
+          const int64_t s = start_of(u);
+          unit(load(s), s, 0, false, far, y[0]);
+          put(s, y[0]);
+        }
+      };
+      if (OP == kSwiglu && far) {
+        read_again(std::true_type{});
+      } else if constexpr (V > 0) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const int64_t u = sub + i * TPR;
           if (u < units) put(start_of(u), y[i]);
         }
       } else {
-        for (int64_t u = sub; u < units; u += TPR) {
-          const int64_t s = start_of(u);
-          unit(load(s), s, 0, false, y[0]);
-          put(s, y[0]);
-        }
+        read_again(std::false_type{});
       }
       if (sub == 0) a.scales[row] = bad ? __builtin_nanf("") : most * r / 127.f;
     }

@@ -1,0 +1,77 @@
+"""8-bit rows at the ends of their inputs' range, against their definitions in 64 bits.
+
+Tolerances as in tests/test_gpu_int8_linear.py, u = 2^-24 (half a step of fp32).  A gate g below
+-87, whose exp(-g) nears the end of fp32, gives ((g h) up) h with h = exp(g / 2): h twice, within 2
+steps (4 u) each, and three products: 11 u of y, and half of the smallest step, 2^-150, where y is
+that small.  Both count twice for a value: in y and in the row's top.
+"""
+
+import pytest
+import torch
+
+import mrsa
+from oracle import int8_oracle as O8
+from test_gpu_int8_linear import DEV, DTYPES, U, _rows, check_rows
+
+pytestmark = pytest.mark.gpu
+DIMS = (6, 9, 700, 1001, 3584, 18944, 21000)
+
+
+def check_swiglu(x, slack):
+    values, scales = mrsa.swiglu_int8(x)
+    y = O8.swiglu_rows(x.double())
+    for i in range(x.shape[0]):
+        top = float(y[i].abs().max())
+        small = 0.0 if top == 0 else 2.0 ** -149 * 127 / top
+        check_rows(values[i], scales[i], y[i], 127 * 2 * slack + small, 2 * slack)
+    return values, scales
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", DIMS)
+def test_swiglu_int8_of_masked_gates(dim, dtype):
+    """Gates of the type's lowest value among ordinary ones are zeros."""
+
+    x = _rows(6, 2 * dim, dtype, dim, 2.0)
+    assert x[:, :dim].max() <= 16
+    low = torch.finfo(dtype).min
+    x[1, dim - 1] = low
+    x[2, ::2] = low         # (the other factor, too: of ordinary and of masked gates)
+    x[2, dim:] = 1.0
+    x[3, : dim // 2] = low
+    x[4, 0], x[4, dim] = low, 1e4
+    x[5, 1], x[5, dim + 1] = -1e4, -1e4
+    values, _ = check_swiglu(x, (1.5 * 16 + 8) * U)
+    assert not values[2, ::2][: dim // 2].any() and not values[3, : dim // 2].any()
+    assert values[4, 0] == 0 and values[5, 1] == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", DIMS)
+def test_swiglu_int8_of_gates_that_are_all_very_negative(dim, dtype):
+    g = torch.Generator(device=DEV).manual_seed(dim)
+    big = 6e4 if dtype == torch.float16 else 1e20
+    gate = torch.rand(8, dim, generator=g, device=DEV) * 33 - 120        # -120 .. -87
+    gate[1], gate[2], gate[3], gate[4] = -88.0, -100.0, -87.0, -110.0
+    gate[5] = torch.rand(dim, generator=g, device=DEV) * 4 - 89          # on both sides of -87
+    gate[6] = torch.rand(dim, generator=g, device=DEV) * 10 - 100
+    up = torch.rand(8, dim, generator=g, device=DEV) * 2 - 1
+    up[:6] *= big                                      # (the others: near the smallest numbers)
+    x = torch.cat((gate, up), dim=1).to(dtype)
+    # (gates above -87 as others: 1.5 |g| + 8; below: 11)
+    values, scales = check_swiglu(x, (1.5 * 89 + 8) * U)
+    assert (values.abs().amax(dim=1) == 127).all() and (scales > 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", DIMS)
+def test_swiglu_int8_of_gates_that_leave_nothing(dim, dtype):
+    low = torch.finfo(dtype).min
+    gates = [-1e3, -1e4, low] + ([] if dtype == torch.float16 else [-1e30])
+    x = torch.ones(len(gates) + 1, 2 * dim, dtype=dtype, device=DEV) * 1e4
+    for i, g in enumerate(gates):
+        x[i, :dim] = g
+    x[-1, :dim] = low
+    x[-1, dim // 2] = float("-inf")                    # -inf * 0
+    values, scales = mrsa.swiglu_int8(x)
+    assert not values.any() and not scales[:-1].any() and scales[-1].isnan()
