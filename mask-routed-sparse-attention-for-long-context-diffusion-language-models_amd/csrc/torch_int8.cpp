@@ -2,7 +2,9 @@
 // mrsa/ops.py): tensors to the C entry points of libmrsa.so.  At one token a call of these
 // operators is host time, and a public call costs half as much with this side of it and the checks
 // in C++ as through ctypes (norm of one row 12.1 -> 6.0 us, rows 8.6 -> 5.1, product 10.9 -> 5.1).
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPGuard.h>
@@ -10,6 +12,7 @@
 #include <torch/library.h>
 
 #include <optional>
+#include <string>
 #include <tuple>
 
 #include "mrsa.h"
@@ -55,12 +58,6 @@ void check_values(const Tensor& values, const Tensor& scales, const char* name) 
 void check_dtype(at::ScalarType dtype) {
   TORCH_CHECK_VALUE(float_type(dtype), "dtype must be bf16, fp16 or fp32, got ", dtype);
 }
-void no_gradient(const char* op, const Tensor& t) {
-  TORCH_CHECK_VALUE(!t.requires_grad() || !at::GradMode::is_enabled(), op,
-                    " has no gradient: call it under torch.no_grad()");
-  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), op, " has no forward-mode derivative");
-}
-
 // t as rows [n, dim] whose last dim is dense (a copy only if no strides give that).
 Tensor rows_of(const Tensor& t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
@@ -94,7 +91,6 @@ struct Launch {
 
 std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
   check_rows(x, "x");
-  no_gradient("quantize_rows", x);
   const Launch at(x);
   const Tensor rows = rows_of(x);
   const int64_t dim = rows.size(1);
@@ -111,7 +107,6 @@ Tensor dequantize_rows(const Tensor& values, const Tensor& scales, at::ScalarTyp
   TORCH_CHECK_VALUE(values.size(-1) >= 1, "values must have rows of at least one value, got ",
                     values.sizes());
   check_dtype(dtype);
-  no_gradient("dequantize_rows", scales);
   const Launch at(values);
   const Tensor rows = rows_of(values), s = scales.contiguous();
   const int64_t dim = rows.size(1);
@@ -134,15 +129,12 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_int8(const Tensor& x,
                       "residual must match x, got ", residual->sizes(), " ",
                       residual->scalar_type(), " on ", residual->device(), " for ", x.sizes(), " ",
                       x.scalar_type(), " on ", x.device());
-    no_gradient("add_rms_norm_int8", *residual);
   }
   TORCH_CHECK_VALUE(weight.dim() == 1 && weight.size(0) == x.size(-1) &&
                         weight.scalar_type() == x.scalar_type() && weight.device() == x.device(),
                     "weight must be [", x.size(-1), "] ", x.scalar_type(), " on ", x.device(),
                     ", got ", weight.sizes(), " ", weight.scalar_type(), " on ", weight.device());
   TORCH_CHECK_VALUE(eps >= 1e-24 && eps <= 1e24, "eps must be in [1e-24, 1e24], got ", eps);
-  no_gradient("add_rms_norm_int8", x);
-  no_gradient("add_rms_norm_int8", weight);
   const Launch at(x);
   const Tensor rows = rows_of(x), w = weight.contiguous();
   const int64_t dim = rows.size(1);
@@ -167,7 +159,6 @@ std::tuple<Tensor, Tensor> swiglu_int8(const Tensor& gate_up) {
   check_rows(gate_up, "gate_up");
   TORCH_CHECK_VALUE(gate_up.size(-1) % 2 == 0, "gate_up must have an even last dim, got ",
                     gate_up.sizes());
-  no_gradient("swiglu_int8", gate_up);
   const Launch at(gate_up);
   const Tensor rows = rows_of(gate_up);
   const int64_t dim = rows.size(1) / 2;
@@ -196,10 +187,7 @@ Tensor int8_linear(const Tensor& x, const Tensor& x_scales, const Tensor& weight
                           bias->scalar_type() == dtype && bias->device() == x.device(),
                       "bias must be [", weight.size(0), "] ", dtype, " on ", x.device(), ", got ",
                       bias->sizes(), " ", bias->scalar_type(), " on ", bias->device());
-    no_gradient("int8_linear", *bias);
   }
-  no_gradient("int8_linear", x_scales);
-  no_gradient("int8_linear", weight_scales);
   const Launch at(x);
   const Tensor rows = rows_of(x), w = rows_of(weight);
   const Tensor sx = x_scales.contiguous(), sw = weight_scales.contiguous();
@@ -219,6 +207,39 @@ Tensor int8_linear(const Tensor& x, const Tensor& x_scales, const Tensor& weight
   return out;
 }
 
+// ---- derivatives ---------------------------------------------------------------------------
+// Tensors that ask for one are refused where autograd sees the call: below it those of torch.func's
+// reverse transforms no longer ask, and a gradient of zeros would come back.
+
+void no_derivative(const char* op, const Tensor& t) {
+  TORCH_CHECK_VALUE(!t.requires_grad() || !at::GradMode::is_enabled(), op,
+                    " has no gradient: call it under torch.no_grad()");
+  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), op, " has no forward-mode derivative");
+}
+void no_derivative(const char* op, const std::optional<Tensor>& t) {
+  if (t) no_derivative(op, *t);
+}
+void no_derivative(const char*, double) {}
+void no_derivative(const char*, at::ScalarType) {}
+
+constexpr const char* kOps[] = {"quantize_rows", "dequantize_rows", "add_rms_norm_int8",
+                                "swiglu_int8", "int8_linear"};
+
+// Operator OP of kOps for autograd: the refusals, and the call below.
+template <int OP, class R, class... Args>
+R below_autograd(c10::DispatchKeySet keys, Args... args) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow((std::string("mrsa::") + kOps[OP]).c_str(), "")
+                             .template typed<R(Args...)>();
+  (no_derivative(kOps[OP], args), ...);
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  return op.redispatch(keys & c10::after_autograd_keyset, args...);
+}
+template <int OP, class R, class... Args>
+void impl_autograd(torch::Library& m, R (*)(Args...)) {
+  m.impl(kOps[OP], TORCH_FN((below_autograd<OP, R, Args...>)));
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(mrsa, CUDA, m) {
@@ -229,10 +250,10 @@ TORCH_LIBRARY_IMPL(mrsa, CUDA, m) {
   m.impl("int8_linear", &int8_linear);
 }
 
-// Tensors that ask for a derivative are refused by the operators themselves, so autograd's own
-// fallback kernel is left out of every call.
 TORCH_LIBRARY_IMPL(mrsa, Autograd, m) {
-  for (const char* op : {"quantize_rows", "dequantize_rows", "add_rms_norm_int8", "swiglu_int8",
-                         "int8_linear"})
-    m.impl(op, torch::CppFunction::makeFallthrough());
+  impl_autograd<0>(m, &quantize_rows);
+  impl_autograd<1>(m, &dequantize_rows);
+  impl_autograd<2>(m, &add_rms_norm_int8);
+  impl_autograd<3>(m, &swiglu_int8);
+  impl_autograd<4>(m, &int8_linear);
 }

@@ -11,11 +11,12 @@ A row of activations, or of a weight matrix (an output channel), is held as int8
 
 The operators check their arguments themselves: on the GPU in csrc/torch_int8.cpp, for fake and CPU
 tensors in int8_checks.py, the same checks in the same words.  (They stand there, since at one token
-the time of a call is the host's.  Only what torch.func.jvp differentiates, which no kernel sees, is
-refused here.)
+the time of a call is the host's.)
 
 ``DreamWeights.int8()`` makes a model's projections 8-bit and ``dream_forward`` runs on them.
-Rounding to 8 bits has no useful derivative: the operators refuse tensors that ask for one.
+Rounding to 8 bits has no useful derivative: the operators refuse tensors that ask for one, in
+either mode and under torch.func's transforms (the autograd kernels of csrc/torch_int8.cpp; dual
+tensors already here, before any trace).
 """
 
 from __future__ import annotations

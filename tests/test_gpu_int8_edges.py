@@ -75,3 +75,51 @@ def test_swiglu_int8_of_gates_that_leave_nothing(dim, dtype):
     x[-1, dim // 2] = float("-inf")                    # -inf * 0
     values, scales = mrsa.swiglu_int8(x)
     assert not values.any() and not scales[:-1].any() and scales[-1].isnan()
+
+
+def test_transforms_of_real_tensors():
+    """Derivatives by torch.func are refused (tests/test_int8_transforms.py has all of them); of
+    other tensors, beside the operators, they are right; vmap alone gives the rows' own results."""
+
+    from torch.func import grad, jacrev, jvp, vmap
+
+    x, w = _rows(4, 32, torch.float32, 1), _rows(1, 32, torch.float32, 2)[0]
+    v, s = mrsa.quantize_rows(x)
+    product = lambda b: mrsa.int8_linear(v, s, v, s, b, dtype=torch.float32)   # noqa: E731
+    for call in (lambda: grad(lambda b: product(b).sum())(s), lambda: jacrev(product)(s),
+                 lambda: grad(lambda t: mrsa.add_rms_norm_int8(t, x, w, 1e-6)[0].sum())(x),
+                 lambda: grad(lambda t: torch.ops.mrsa.quantize_rows(t)[1].sum())(x),
+                 lambda: vmap(grad(lambda t: mrsa.swiglu_int8(t)[1]))(x),
+                 lambda: grad(lambda t: vmap(lambda r: mrsa.quantize_rows(r)[1])(t).sum())(x),
+                 lambda: jvp(lambda t: mrsa.dequantize_rows(v, t), (s,), (s,)),
+                 lambda: jvp(lambda t: torch.ops.mrsa.quantize_rows(t)[1], (x,), (x,))):
+        with pytest.raises(ValueError, match="no gradient|forward-mode"):
+            call()
+
+    def beside(b):
+        with torch.no_grad():
+            rows = mrsa.quantize_rows(b[:, None] * x)[1]
+        return (rows * b * mrsa.quantize_rows(x)[1] * mrsa.swiglu_int8(b.detach()[:, None] * x)[1]
+                ).sum()
+
+    b = torch.tensor([1.0, 2.0, 0.5, 3.0], device=DEV)
+    rows = b[:, None] * x
+    want = mrsa.quantize_rows(rows)[1] * mrsa.quantize_rows(x)[1] * mrsa.swiglu_int8(rows)[1]
+    torch.testing.assert_close(grad(beside)(b), want, rtol=4 * U, atol=0.0)
+    batch = torch.stack((x, 2 * x, x.flip(0)))
+    for got, one in zip(vmap(mrsa.quantize_rows)(batch), zip(*map(mrsa.quantize_rows, batch))):
+        assert torch.equal(got, torch.stack(one))
+
+
+def test_gradients_of_a_graph_around_the_operators():
+    """Ordinary autograd: what runs under no_grad inside a recorded graph stays a constant of it."""
+
+    x = _rows(4, 32, torch.float32, 3).requires_grad_()
+    with torch.no_grad():
+        v, s = mrsa.quantize_rows(x)
+        back = mrsa.dequantize_rows(v, s, torch.float32)
+    (x * back).sum().backward()
+    assert torch.equal(x.grad, back)
+    with torch.inference_mode():
+        again = mrsa.quantize_rows(x)
+    assert torch.equal(again[0], v) and torch.equal(again[1], s)
