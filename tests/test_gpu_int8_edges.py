@@ -123,3 +123,23 @@ def test_gradients_of_a_graph_around_the_operators():
     with torch.inference_mode():
         again = mrsa.quantize_rows(x)
     assert torch.equal(again[0], v) and torch.equal(again[1], s)
+
+
+@pytest.mark.parametrize("rows,dim", [((1 << 22) + 5, 9), ((1 << 22) + 5, 3),
+                                      ((1 << 20) + 3, 1025)])
+def test_more_rows_than_blocks(rows, dim):
+    """Blocks that take several rows each (rows that fit a wave: four a block)."""
+
+    x = _rows(257, dim, torch.bfloat16, dim)
+    x = x.repeat(rows // 257 + 1, 1)[:rows]
+    n = torch.arange(rows, device=DEV) % 257
+    for call in (mrsa.quantize_rows,
+                 lambda t: mrsa.add_rms_norm_int8(t, None, torch.ones_like(t[0]), 1e-6)[1:],
+                 lambda t: mrsa.swiglu_int8(t[:, : dim // 2 * 2])):
+        values, scales = call(x)
+        first, its = call(x[:257])
+        assert torch.equal(values, first[n]) and torch.equal(scales, its[n])
+    values, scales = mrsa.quantize_rows(x)
+    check_rows(values[:257], scales[:257], x[:257].double(), 127 * 3 * U, U)
+    back = mrsa.dequantize_rows(values, scales)
+    assert torch.equal(back, (values.float() * scales[:, None]).bfloat16())
