@@ -1028,7 +1028,7 @@ int mrsa_dequantize_rows_fwd(const int8_t* values, int64_t row_stride, const flo
  * t = x + residual rounded to `dtype` (written to total, dense; residual and
  * total are both given or both NULL, then t = x),
  * y = t / sqrt(mean(t^2) + eps) * weight, in fp32 with no rounding before the 8
- * bits.  1e-24 <= eps <= 1e24.
+ * bits; a y past fp32 counts as an infinity.  1e-24 <= eps <= 1e24.
  */
 int mrsa_add_rms_norm_int8_fwd(const void* x, int64_t x_row_stride, const void* residual,
                                int64_t residual_row_stride, const void* weight, int64_t rows,

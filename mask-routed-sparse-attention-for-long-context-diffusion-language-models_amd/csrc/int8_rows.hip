@@ -286,21 +286,22 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR,
       if (far) all_units(false, std::true_type{});
     }
     if constexpr (NORM) {
-      // t^2 or t w past fp32 (|t| above 1.8e19): again with t times a power of two that takes
-      // the largest |t| to between 1 and 2.  A row that holds an infinity or a NaN comes here,
-      // too, and stays what it is.
+      // t^2 or t w past fp32 (|t| above 1.8e19, or above 1 beside a large weight): again with t
+      // times a power of two that takes the largest |t| to between 1/4 and 1/2, so that t w is
+      // finite.  A row that holds an infinity or a NaN comes here, too, and stays what it is.
       const bool past = !(square < __uint_as_float(kInfBits)) || top >= kInfBits;
       if (__any(past)) {  // (the same in every wave of a row)
         float none = 0.f;
         reduce<TPR, false>(none, top_t, red_sum, red_top);
-        const int e = past ? (int)(top_t >> 23) - 127 : 0;
-        down = __uint_as_float((uint32_t)(127 - max(0, min(e, 126))) << 23);
+        const int e = past ? (int)(top_t >> 23) - 127 : -2;
+        down = ldexpf(1.f, -2 - min(e, 127));
         all_units(false, std::false_type{});
       }
       r = rsqrtf(square / (float)a.K + a.eps * down * down);
     }
-    const bool bad = top >= kInfBits;
     const float most = __uint_as_float(top);
+    // (the norm's y may pass fp32 where t w does not)
+    const bool bad = top >= kInfBits || (NORM && !(most * r < __uint_as_float(kInfBits)));
     // (rows below 2^-100, whose 127 / a could pass fp32, are lifted first)
     const float lift = most < 0x1p-100f ? 0x1p100f : 1.f;
     const float up = bad || top == 0 ? 0.f : 1.f / (most * lift) * 127.f;

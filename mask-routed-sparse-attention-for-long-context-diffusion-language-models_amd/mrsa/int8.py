@@ -65,7 +65,7 @@ def add_rms_norm_int8(x: torch.Tensor, residual: Optional[torch.Tensor], weight:
 
     x, residual [..., dim] in bf16, fp16 or fp32, any strides; weight [dim] of the same type;
     eps from 1e-24 to 1e24.  The norm is that of the rounded sum, computed in fp32 with no
-    rounding before the 8 bits."""
+    rounding before the 8 bits; a result past fp32 counts as an infinity."""
 
     if forward_ad._current_level >= 0:
         _no_gradient("add_rms_norm_int8", x, residual, weight)

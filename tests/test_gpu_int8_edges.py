@@ -143,3 +143,30 @@ def test_more_rows_than_blocks(rows, dim):
     check_rows(values[:257], scales[:257], x[:257].double(), 127 * 3 * U, U)
     back = mrsa.dequantize_rows(values, scales)
     assert torch.equal(back, (values.float() * scales[:, None]).bfloat16())
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("dim", DIMS)
+def test_norm_beside_weights_near_the_end_of_fp32(dim, dtype):
+    """t * weight leaves fp32 where the normed t times the weight does not (rows 0 and 1), or the
+    other way round (row 2: counted as infinite); ordinary rows beside them."""
+
+    x = torch.where(_rows(6, dim, torch.float32, dim) < 0, -1.9, 1.9)
+    x[0] *= 64.0
+    x[1] *= 2.0 ** 126
+    x[2] = 0.0
+    x[2, dim // 2] = 0.5
+    x[3:] = 0.0                                # small weights alone meet these
+    x[3:, :2] = _rows(3, 2, torch.float32, 9)
+    g = torch.Generator(device=DEV).manual_seed(dim)
+    w = (torch.rand(dim, generator=g, device=DEV) * 2 - 1) * 2.5e38
+    w[:2] = 1.0
+    w[dim // 2] = 2.5e38
+    x, w = x.to(dtype), w.to(dtype)
+    total, values, scales = mrsa.add_rms_norm_int8(x, None, w, 1e-6)
+    y = O8.norm_rows(x.double(), w.double(), 1e-6)
+    assert y[:2].abs().max() < 3e38 and y[2].abs().max() > 3.5e38
+    assert scales[2].isnan() and not values[2].any()
+    rest = [0, 1, 3, 4, 5]
+    check_rows(values[rest], scales[rest], y[rest], 127 * 5 * U, ((dim / 64 + 24) / 2 + 8) * U)
+    assert (values[rest].abs().amax(dim=1) == 127).all()
