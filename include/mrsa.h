@@ -1008,7 +1008,9 @@ int mrsa_copy_pages(void* k_pages, int64_t k_layer_stride, int64_t k_page_stride
  * Linear layers in 8-bit integers.  A row y of `dim` values is held as int8
  * values v and one fp32 scale: with a = max |y_k|,
  *   scale = a / 127,  v_k = rint(y_k 127 / a)  (ties to even, |v_k| <= 127);
- * a = 0: scale and values 0; a not finite: scale NaN and values 0.
+ * a = 0: scale and values 0; a not finite: scale NaN and values 0.  The scale is
+ * rounded so that 127 times it is finite; what leaves fp32 at its small end, a
+ * scale or a product before it, keeps fewer digits.
  *   values (out): [rows, dim] dense; scales (out): [rows]
  *   x, gate_up, ..: `dtype` (MRSA_DTYPE_*), rows at strides in elements (0 and
  *     overlapping rows allowed), dense in the last dim, aligned to an element

@@ -110,6 +110,7 @@ __device__ __forceinline__ float whole(float f) {
 }
 
 constexpr uint32_t kInfBits = 0x7f800000u;
+constexpr float kMostScale = 0x1.020406p121f;   // 127 times the next one passes fp32
 constexpr uint32_t kFar = 0xffffffffu;   // above all magnitudes: the row has gates below kFarGate
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR,
       } else {
         read_again(std::false_type{});
       }
-      if (sub == 0) a.scales[row] = bad ? __builtin_nanf("") : most * r / 127.f;
+      if (sub == 0) a.scales[row] = bad ? __builtin_nanf("") : fminf(most * r / 127.f, kMostScale);
     }
   }
 }

@@ -1,7 +1,8 @@
 """Linear layers in 8-bit integers: rows with one scale each, and their matrix product.
 
 A row of activations, or of a weight matrix (an output channel), is held as int8 values in
-[-127, 127] and one fp32 scale: y_k is about values_k * scale, scale = max |y_k| / 127.
+[-127, 127] and one fp32 scale: y_k is about values_k * scale, scale = max |y_k| / 127 (rounded so
+that 127 * scale is finite where the row is).
 
     quantize_rows      rows in 8 bits (activations; weights, once)
     dequantize_rows    the values that 8-bit rows stand for

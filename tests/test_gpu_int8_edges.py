@@ -170,3 +170,23 @@ def test_norm_beside_weights_near_the_end_of_fp32(dim, dtype):
     rest = [0, 1, 3, 4, 5]
     check_rows(values[rest], scales[rest], y[rest], 127 * 5 * U, ((dim / 64 + 24) / 2 + 8) * U)
     assert (values[rest].abs().amax(dim=1) == 127).all()
+
+
+@pytest.mark.parametrize("dim", DIMS)
+def test_rows_of_the_largest_numbers_come_back_finite(dim):
+    """top / 127 may round up, and 127 of it past fp32: the scale is then one step (2 u) less."""
+
+    x = _rows(4, dim, torch.float32, dim)
+    most = torch.finfo(torch.float32).max
+    x[0, dim - 1], x[1, 0] = most, -most
+    x[2] = most
+    gated = torch.cat((x, torch.ones_like(x)), dim=1)      # silu(most) is most
+    ones = torch.ones(dim, device=DEV)
+    heavy = torch.where(torch.arange(dim, device=DEV) % 2 == 0, most, 1.0)
+    for y, (values, scales) in ((x, mrsa.quantize_rows(x)), (None, mrsa.swiglu_int8(gated)),
+                                (None, mrsa.add_rms_norm_int8(ones[None], None, heavy, 1e-24)[1:])):
+        if y is not None:
+            check_rows(values, scales, y.double(), 127 * 3 * U, 2 * U)
+        back = mrsa.dequantize_rows(values, scales, torch.float32)
+        assert torch.isfinite(back).all() and torch.isfinite(scales).all()
+        assert back[0].abs().max() > 0.999 * most and values[0].abs().max() == 127
