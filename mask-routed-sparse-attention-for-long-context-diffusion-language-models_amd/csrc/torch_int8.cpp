@@ -58,10 +58,16 @@ void check_values(const Tensor& values, const Tensor& scales, const char* name) 
 void check_dtype(at::ScalarType dtype) {
   TORCH_CHECK_VALUE(float_type(dtype), "dtype must be bf16, fp16 or fp32, got ", dtype);
 }
+
 // t as rows [n, dim] whose last dim is dense (a copy only if no strides give that).
 Tensor rows_of(const Tensor& t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
   return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
+}
+// As rows_of, at strides that mrsa_int8_linear_fwd takes.
+Tensor operand_rows(const Tensor& t) {
+  Tensor r = rows_of(t);
+  return r.size(0) > 1 && r.stride(0) >= (int64_t)1 << 31 ? r.contiguous() : r;
 }
 int64_t row_stride(const Tensor& rows) {  // (a single row's is arbitrary)
   return rows.size(0) > 1 ? rows.stride(0) : rows.size(1);
@@ -189,7 +195,7 @@ Tensor int8_linear(const Tensor& x, const Tensor& x_scales, const Tensor& weight
                       bias->sizes(), " ", bias->scalar_type(), " on ", bias->device());
   }
   const Launch at(x);
-  const Tensor rows = rows_of(x), w = rows_of(weight);
+  const Tensor rows = operand_rows(x), w = operand_rows(weight);
   const Tensor sx = x_scales.contiguous(), sw = weight_scales.contiguous();
   const Tensor b = bias ? bias->contiguous() : Tensor();
   const int64_t n = rows.size(0), out_dim = w.size(0);

@@ -190,3 +190,17 @@ def test_rows_of_the_largest_numbers_come_back_finite(dim):
         back = mrsa.dequantize_rows(values, scales, torch.float32)
         assert torch.isfinite(back).all() and torch.isfinite(scales).all()
         assert back[0].abs().max() > 0.999 * most and values[0].abs().max() == 127
+
+
+def test_product_of_rows_that_lie_gigabytes_apart():
+    K, apart = 144, (1 << 31) + 16
+    memory = torch.empty(2 * apart + K, dtype=torch.int8, device=DEV)
+    far = memory.as_strided((3, K), (apart, 1))
+    near = torch.randint(-127, 128, (3, K), device=DEV).to(torch.int8)
+    far.copy_(near)
+    s, many = torch.rand(3, device=DEV), torch.randint(-127, 128, (70, K), device=DEV)
+    many, its = many.to(torch.int8), torch.rand(70, device=DEV)
+    for got, want in ((mrsa.int8_linear(far, s, many, its), mrsa.int8_linear(near, s, many, its)),
+                      (mrsa.int8_linear(many, its, far, s), mrsa.int8_linear(many, its, near, s))):
+        assert torch.equal(got, want)
+    assert torch.equal(mrsa.dequantize_rows(far, s), mrsa.dequantize_rows(near, s))
