@@ -150,9 +150,10 @@ __device__ __forceinline__ void reduce(float& sum, uint32_t& top, float* red_sum
   }
 }
 
-// The same number, but one that the compiler keeps no addresses for ahead of its use.
+// The same number; if AGAIN, one that the compiler keeps no addresses for ahead of its use.
+template <bool AGAIN>
 __device__ __forceinline__ int apart(int i) {
-  asm volatile("" : "+v"(i));
+  if constexpr (AGAIN) asm volatile("" : "+v"(i));
   return i;
 }
 
@@ -164,7 +165,7 @@ __device__ __forceinline__ int apart(int i) {
 // Bound by HBM where there are many rows, since a row stays in registers between its maximum and
 // its values and so is read once (bf16, a large copy reaches 5.17 TB/s): 16384 rows of 3584
 // quantized in 31 us (176 MB, 5.7 TB/s, partly from the caches), with the norm and the residual's
-// sum in 77 us (411 MB, 5.3 TB/s); gated, of 18944, in 296 to 344 us (1552 MB, 4.5 to 5.2 TB/s),
+// sum in 77 us (411 MB, 5.3 TB/s); gated, of 18944, in 291 to 330 us (1552 MB, 4.7 to 5.3 TB/s),
 // where the exponential, the quotient and the rounding, 30 vector instructions an element, keep
 // the vector unit as busy as the memory.  One row of 3584 takes 2.9 us: a launch and three
 // dependent steps (loads, reduction, stores).
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR,
           unit(n[i], s, u < units ? (int)(8 * u - s) : 8, first, far, y[i]);
         }
       } else {
-        for (int64_t u = apart(sub); u < units; u += TPR) {
+        for (int64_t u = apart<far>(sub); u < units; u += TPR) {
           const int64_t s = start_of(u);
           unit(load(s), s, (int)(8 * u - s), first, far, y[0]);
         }
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR,
     };
     if (there) {
       auto read_again = [&](auto far) {
-        for (int64_t u = apart(sub); u < units; u += TPR) {
+        for (int64_t u = apart<far>(sub); u < units; u += TPR) {
           const int64_t s = start_of(u);
           unit(load(s), s, 0, false, far, y[0]);
           put(s, y[0]);
@@ -393,18 +394,21 @@ void launch_rows(const RowArgs& a, hipStream_t stream) {
 }
 
 // A wave a row up to 1024 elements (no barriers: 16384 rows of 1024 9.6 us, by blocks of 256
-// 13.7), then a block whose threads hold the row in registers, with as few units a thread as
-// leaves no thread idle: bf16, 16384 rows,
-//                     elements   256 threads (units)   512           1024
-//   quantize              3584   28.8 (2)              34.0 (1)      56.0 (1)
-//   norm                  3584   70.3 (2)              73.2 (1)      101 (1)
-//   swiglu                3584   67.0 (2)              58.0 (1)      103 (1)
-//   swiglu                8192   136 (4)               121 (2)       121 (1)
-//   norm                 12288   278 (8)               242 (3)       284 (2)
-//   swiglu               18944   315 (10)              285 (5)       314 (3)
-//   norm                 18944   538 (10)              440 (5)       430 (3)
-// Past 20480 elements the row is read twice, by 1024 threads (8192 rows of 32768: quantize 175 us,
-// 512 threads 192; one row of them 3.9 and 5.0).
+// 13.3), then a block whose threads hold the row in registers, with as few units a thread as
+// leaves no thread idle: us, bf16,
+//             rows    elements   256 threads (units)   512           1024
+//   quantize  16384       3584   27.4 (2)              31.4 (1)      55.3 (1)
+//   norm      16384       3584   70.5 (2)              74.7 (1)      103 (1)
+//   swiglu       32       3584   3.0 (2)               2.8 (1)
+//   swiglu    16384       3584   51.8 (2)              59.2 (1)      101 (1)
+//   swiglu    16384       8192   128 (4)               118 (2)       122 (1)
+//   norm      16384      12288   276 (8)               242 (3)       291 (2)
+//   swiglu    16384      18944   297 (10)              284 (5)       309 (3)
+//   norm      16384      18944   549 (10)              446 (5)       434 (3)
+// (Gated rows of 2049 to 4096 elements take 512 threads for the few rows of a decode block, and in
+// fp32 also for many: 16384 rows of 3584 94 us, 256 threads 98.)  Past 20480 elements the row is
+// read twice, by 1024 threads (8192 rows of 32768: quantize 176 us, 512 threads 192; one row of
+// them 3.8 and 5.0).
 template <class T, int OP>
 void rows_of(const RowArgs& a, hipStream_t stream) {
   const int64_t units = (a.K + 7) / 8;
