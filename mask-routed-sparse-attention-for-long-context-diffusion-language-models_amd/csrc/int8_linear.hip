@@ -566,8 +566,9 @@ __device__ __forceinline__ void put4(const LinearArgs& a, int64_t m, int64_t n, 
 }
 
 // Bound by W's bytes from HBM: 32 rows, 37888 x 3584 in 26.7 us (138 MB, 5.2 TB/s, a large copy's
-// rate); one row, 4608 x 3584 in 5.4 us (16.5 MB, 3.1 TB/s: 144 workgroups of seven steps, over
-// before the memory is at its rate).
+// rate); one row, 4608 x 3584 in 5.4 us (16.5 MB, 3.1 TB/s: 144 workgroups, whose waves take seven
+// steps each, two of them in flight; eight waves or deeper rings gained nothing there and cost 15%
+// at 37888 columns).
 //
 // Consecutive lanes fetch consecutive bytes of a row, which operands loaded straight from memory
 // (16 rows side by side: 60 us where this takes 31) do not.  A workgroup has 16 NT columns and up

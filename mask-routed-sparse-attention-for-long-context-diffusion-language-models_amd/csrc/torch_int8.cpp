@@ -1,7 +1,8 @@
 // The CUDA implementations of the 8-bit torch.ops.mrsa operators (schemas and fake kernels:
 // mrsa/ops.py): tensors to the C entry points of libmrsa.so.  At one token a call of these
 // operators is host time, and a public call costs half as much with this side of it and the checks
-// in C++ as through ctypes (norm of one row 12.1 -> 6.0 us, rows 8.6 -> 5.1, product 10.9 -> 5.1).
+// in C++ as through ctypes (norm of one row 12.1 -> 6.1 us, rows 8.6 -> 5.1, product 10.9 -> 5.2;
+// where the processor is faster 5.6, 4.7 and 4.8).
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/core/dispatch/Dispatcher.h>

@@ -179,7 +179,8 @@ class DreamWeights:
     layers: list[DreamLayerWeights]
 
     def int8(self) -> "DreamWeights":
-        """The model with its layers' projections in 8 bits; what stays bf16 is shared."""
+        """The model with its layers' projections in 8 bits; what stays bf16 is shared.
+        (``add_rms_norm_int8`` asks for an rms_eps of at least 1e-24.)"""
 
         return replace(self, layers=[lw.int8() for lw in self.layers])
 
