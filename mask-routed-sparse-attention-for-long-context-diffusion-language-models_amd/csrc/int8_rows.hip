@@ -165,7 +165,7 @@ __device__ __forceinline__ int apart(int i) {
 // Bound by HBM where there are many rows, since a row stays in registers between its maximum and
 // its values and so is read once (bf16, a large copy reaches 5.17 TB/s): 16384 rows of 3584
 // quantized in 31 us (176 MB, 5.7 TB/s, partly from the caches), with the norm and the residual's
-// sum in 77 us (411 MB, 5.3 TB/s); gated, of 18944, in 291 to 330 us (1552 MB, 4.7 to 5.3 TB/s),
+// sum in 77 us (411 MB, 5.3 TB/s); gated, of 18944, in 293 to 322 us (1552 MB, 4.8 to 5.3 TB/s),
 // where the exponential, the quotient and the rounding, 30 vector instructions an element, keep
 // the vector unit as busy as the memory.  One row of 3584 takes 2.9 us: a launch and three
 // dependent steps (loads, reduction, stores).
